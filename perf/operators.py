@@ -204,7 +204,7 @@ def _prepare_verify(case, s, trees, starts, normal, g):
     batch, vocab, total = case["requests"], case["vocab"], s["parents"].numel()
     logits = normal(total, vocab, std=1.5, dtype=torch.float32)
     peaks = torch.randint(0, vocab, (total, 24), generator=g, device="cuda")
-    logits.scatter_(1, peaks, 5.0 + 2.0 * torch.randn((total, 24), generator=g, device="cuda"))
+    logits.scatter_(1, peaks, 11.0 + 2.5 * torch.randn((total, 24), generator=g, device="cuda"))
     parent_row, rank = [], []
     for t, at in zip(trees, starts):
         seen = {}
