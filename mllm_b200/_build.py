@@ -7,6 +7,7 @@ The extensions live under ``mllm_b200/csrc``:
 * ``mllm_b200_A``    — latent attention;
 * ``mllm_b200_L``    — lightning attention (linear attention with a fixed decay per head);
 * ``mllm_b200_E``    — mixtures of experts;
+* ``mllm_b200_T``    — drafted token trees (speculative decoding);
 * ``mllm_b200_X``    — 4-bit weights, vision towers, tensor- and expert-parallel exchange;
 * ``mllm_b200_host`` — host-only C++ (radix tree, page allocator, ``.mllm`` file reader).
 
@@ -72,6 +73,11 @@ EXTENSIONS: Dict[str, Dict[str, List[str]]] = {
     "mllm_b200_E": {
         "sources": ["bindings_moe.cpp", "runtime.cu", "moe.cu", "moe_pair.cu"],
         "headers": _COMMON,
+        "cuda": True,
+    },
+    "mllm_b200_T": {
+        "sources": ["bindings_tree.cpp", "runtime.cu", "attention_tree.cu"],
+        "headers": _COMMON + ["tree.h", "tree.cuh"],
         "cuda": True,
     },
     "mllm_b200_X": {

@@ -1,0 +1,846 @@
+// Attention of drafted token trees over the slot-indexed KV pool: head sizes 64, 128 and 256, caches of the activation type or 8-bit
+// floats.
+//
+// Request b has prefix cached tokens and a tree of n nodes whose keys and values stand behind them (node j at slot
+// table[prefix + j]); node j continues node parents[j] < j, or the cached text where that is -1.  It sits at position
+// prefix + (its ancestors) and sees the cached tokens, its ancestors and itself:
+//   o_j = sum_k softmax_k(scale q_j . k_k) v_k      over  {cached k, k >= low_j}  and  {ancestors and self at positions >= low_j},
+// low_j the first position of the sliding window or of the chunk.
+//
+// The rows that share K and V are (node, query head of the group) pairs, n * group of them; 128 make a row tile.  Every cached key
+// and value is read once per row tile and meets 4 * 128 operations per element at most: a memory stream up to 128 rows, like decoding,
+// with products too large for warp-level instructions (128 rows x 64 keys x 128 features twice per 32 KB).  So:
+//   * work is dealt as in decoding: the 64-token tiles of all (request, kv head, row tile) units form one line, laid out on the device
+//     from the lengths, and every CTA takes an equal run of it.  A unit inside one CTA is written out directly; others leave at most
+//     two partial results per CTA, and the CTA that has a unit's last tile leaves a note for the kernel that joins them.
+//   * warps 4-6 copy rows by slot with cp.async (a page of one token costs what a page of 16 does) into a ring of 64-token K or V
+//     stages in the operand layout; the copies themselves arrive on the stage's barrier, so the whole ring is in flight.  8-bit rows
+//     pass through registers, widened.
+//   * warp 7 issues S = Q K^T (two score buffers in tensor memory) and O += P V, P from tensor memory.
+//   * warps 0-3 hold a row per thread: online maximum and sum in fp32, P over S in place.  Masks are 64-bit words per row and tile,
+//     made only in tiles that hold tree nodes or a window's edge: cached part by comparison, tree part by a walk to the root over
+//     parents in shared memory.
+// A value that is no number must not reach rows that do not see it (0 x NaN): in masked tiles such elements of V are set to zero in the
+// stage, and added at the end to the rows that see them.
+#include <algorithm>
+
+#include "common.cuh"
+#include "tree.cuh"
+
+namespace mb200 {
+namespace {
+
+constexpr int kRows = 128;                 // MMA M
+constexpr int kTile = 64;                  // tokens of a tile
+constexpr int kThreads = 256;              // 4 softmax warps, 3 copying warps, 1 issuing warp
+constexpr int kCopyWarps = 3, kCopyThreads = 32 * kCopyWarps;
+constexpr int kStart = 2;                  // units behind every (request, kv head, row tile): what it costs beside its tiles
+constexpr int kParents = 256;              // nodes whose parents are kept in shared memory
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleThreshold = 8.0f;  // the running maximum is raised when a score passes it by 2^8
+
+struct TreeParams {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  float* part_o;     // [CTAs][2][part_rows][HD]
+  float* part_lse;   // [CTAs][2][part_rows]
+  int* jobs;         // [CTAs][kJobInts]
+  TreeIndex ix;
+  const float* sink;
+  int64_t q_stride, out_stride, num_slots, kv_tok_stride, kv_head_stride;
+  int hkv, group, tpt, ctas, part_rows, window, chunk, kv_fmt, f16;
+  float scale_log2, cap_in, cap_out;    // cap_out 0: no soft cap
+  uint32_t idesc_s, idesc_o;
+};
+// What the CTA with a unit's last tile notes for the joining kernel: rows (0: nothing to join), first row of q, first head, first CTA
+// of the unit, and whether that one has it in its second partial result
+constexpr int kJobInts = 8;
+
+// first position that a node at position i sees
+__device__ __forceinline__ int first_key(const TreeParams& p, int i) {
+  if (p.window > 0) return max(0, i - p.window + 1);
+  return p.chunk > 0 ? i / p.chunk * p.chunk : 0;
+}
+// first token that is copied: the first key of the least deep position
+__device__ __forceinline__ int first_token(const TreeParams& p, const Request& r) { return first_key(p, r.prefix) & ~(kTile - 1); }
+__device__ __forceinline__ int tiles_of(const TreeParams& p, const Request& r) {
+  return r.nodes == 0 ? 0 : (r.prefix + r.nodes - first_token(p, r) + kTile - 1) / kTile;
+}
+__device__ __forceinline__ int row_tiles(const TreeParams& p, const Request& r) { return (r.nodes + p.tpt - 1) / p.tpt; }
+
+__device__ __forceinline__ int ctas_used(const TreeParams& p, int64_t line) {
+  const int64_t want = max(line / 4, min(line / 2, static_cast<int64_t>(64)));
+  return static_cast<int>(min(static_cast<int64_t>(p.ctas), max(want, static_cast<int64_t>(1))));
+}
+__device__ __forceinline__ int64_t run_begin(int64_t line, int c, int ctas) {
+  if (line < 0xFFFFFFFFll / (ctas + 1)) return static_cast<uint32_t>(line) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
+  return line * c / ctas;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+  const int sz = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz) : "memory");
+}
+// this thread's copies so far arrive on `bar` when they have landed
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// offset of 16-byte piece `ch` of row `row` in a tile of 64-feature blocks of `block` bytes, rows of 128 bytes, 128-byte swizzle
+__device__ __forceinline__ uint32_t swz(int row, int ch, int block) {
+  return (ch >> 3) * block + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+}
+
+template <int NH>
+struct Cfg {
+  static constexpr int kD = 64 * NH;
+  static constexpr int kQBlock = kRows * 128;              // a 64-feature block of Q
+  static constexpr int kQBytes = NH * kQBlock;
+  static constexpr int kBlock = kTile * 128;               // a 64-feature block of a stage
+  static constexpr int kStage = NH * kBlock;
+  static constexpr int kStages = NH == 1 ? 10 : 5;
+  static constexpr int kSmem = kQBytes + kStages * kStage;
+  static constexpr int kPerSm = NH == 4 ? 1 : 2;
+  static_assert(kPerSm * (kSmem + 2048) <= 228 * 1024, "1 KB of each CTA is the system's, 1 KB the kernel's variables");
+  static constexpr int kCols = NH == 4 ? 512 : 256;        // two score buffers of 64 columns, then O
+};
+
+// Item i of a segment of n tiles, in the order in which the products need them: K0, K1, V0, K2, V1, ..
+__device__ __forceinline__ bool item_is_key(int i, int n) { return i < 2 ? !(n == 1 && i == 1) : (i & 1) != 0 && i != 2 * n - 1; }
+__device__ __forceinline__ int item_tile(int i, int n) {
+  if (item_is_key(i, n)) return i < 2 ? i : (i + 1) / 2;
+  return i == 2 * n - 1 ? n - 1 : (i - 2) / 2;
+}
+__device__ __forceinline__ int value_item(int t, int n) { return t == n - 1 ? 2 * n - 1 : 2 + 2 * t; }
+
+struct Place {          // of a segment
+  int b, hk, rt, t0;
+  int64_t left;
+};
+
+template <int NH, bool KV8>
+__global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(const TreeParams p) {
+  using C = Cfg<NH>;
+  constexpr int kD = C::kD, kStages = C::kStages;
+  extern __shared__ __align__(1024) uint8_t tree_smem[];
+  __shared__ uint64_t bars[2 * C::kStages + 8];
+  __shared__ uint32_t tmem_holder;
+  __shared__ int fail_flag, poison;
+  __shared__ int16_t parents[kParents];
+  __shared__ int begin_of[3];
+  __shared__ int64_t line_of[3];
+  __shared__ int ctas_of;
+  uint8_t* sQ = tree_smem;
+  uint8_t* ring = sQ + C::kQBytes;
+  uint64_t* full = bars;                 // [stage] the copying threads
+  uint64_t* empty = full + kStages;      // [stage] tcgen05.commit
+  uint64_t* s_full = empty + kStages;    // [buffer] tcgen05.commit: scores of a tile
+  uint64_t* p_full = s_full + 2;         // [buffer] 128 threads: P is in tensor memory, O rescaled
+  // [buffer] tcgen05.commit: a tile's P V.  A wait tells a phase from the one before it and no more: the scores of tile t, which a
+  // thread has seen, were issued behind P V of t - 2, so one barrier would do for neither of the two products that may be out
+  uint64_t* o_done = p_full + 2;
+  uint64_t* q_full = o_done + 2;         // the copying threads
+  uint64_t* q_free = q_full + 1;         // tcgen05.commit: the segment's last scores
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait_loads();
+
+  // ---- where this CTA's run begins ----
+  if (warp == 0) {
+    const int per = (p.ix.batch + 31) / 32;
+    const int first = min(p.ix.batch, lane * per), last = min(p.ix.batch, first + per);
+    int64_t mine = 0;
+    bool bad = false;
+    for (int b = first; b < last; ++b) {
+      const Request r = request_of(p.ix, b, &bad);
+      if (r.nodes > 0) mine += static_cast<int64_t>(row_tiles(p, r)) * (tiles_of(p, r) + kStart);
+    }
+    if (bad && blockIdx.x == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const int64_t line = __shfl_sync(0xffffffffu, incl, 31) * p.hkv;
+    const int used = ctas_used(p, line);
+    const int c = blockIdx.x;
+    const int64_t begin = c < used ? run_begin(line, c, used) : line, end = c < used ? run_begin(line, c + 1, used) : line;
+    if (lane == 0) {
+      line_of[0] = begin;
+      line_of[1] = end - begin;
+      line_of[2] = line;
+      ctas_of = used;
+      fail_flag = 0;
+      poison = 0;
+    }
+    int64_t at = (incl - mine) * p.hkv;
+    if (begin < end && begin >= at && begin < incl * p.hkv) {
+      for (int b = first; b < last; ++b) {
+        const Request r = request_of(p.ix, b, nullptr);
+        const int n = r.nodes > 0 ? tiles_of(p, r) + kStart : 0;
+        const int64_t units = static_cast<int64_t>(n) * row_tiles(p, r) * p.hkv;
+        if (begin >= at && begin < at + units) {
+          const int64_t in = begin - at;
+          const int64_t unit = in / n;
+          begin_of[0] = b;
+          begin_of[1] = static_cast<int>(unit);
+          begin_of[2] = static_cast<int>(in - unit * n);
+        }
+        at += units;
+      }
+    }
+  } else if (warp == 7) {
+    if (lane == 0) {
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(&full[i], kCopyThreads);
+        mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_full[i], 128);
+        mbar_init(&o_done[i], 1);
+      }
+      mbar_init(q_full, kCopyThreads);
+      mbar_init(q_free, 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(&tmem_holder, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_holder;
+  pdl_launch_dependents();
+
+  const bool aligned = (smem_u32(tree_smem) & 1023) == 0;      // the swizzle counts from 1 KB boundaries
+  if (!aligned && tid == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusPipelineTimeout);
+
+  // Calls fn(place, request, tiles of the unit, tiles of the segment, segment begins at the run's begin) for every segment of the
+  // run; all roles walk the same way.
+  auto segments = [&](auto&& fn) {
+    Place w;
+    w.left = aligned ? line_of[1] : 0;
+    if (w.left <= 0) return;
+    w.b = begin_of[0];
+    w.t0 = begin_of[2];
+    Request r = request_of(p.ix, w.b, nullptr);
+    int rts = row_tiles(p, r), n_all = tiles_of(p, r);
+    w.hk = begin_of[1] / rts;
+    w.rt = begin_of[1] - w.hk * rts;
+    bool first = true;
+    while (w.left > 0) {
+      if (w.t0 >= n_all) {
+        if (n_all > 0) w.left -= n_all + kStart - w.t0;
+        w.t0 = 0;
+        if (n_all == 0 || ++w.rt == rts) {
+          w.rt = 0;
+          if (n_all == 0 || ++w.hk == p.hkv) {
+            w.hk = 0;
+            if (++w.b >= p.ix.batch) return;
+            r = request_of(p.ix, w.b, nullptr);
+            rts = row_tiles(p, r);
+            n_all = tiles_of(p, r);
+          }
+        }
+        first = false;
+        continue;
+      }
+      const int n = static_cast<int>(min(static_cast<int64_t>(n_all - w.t0), w.left));
+      if (!fn(w, r, n_all, n, first)) return;
+      w.left -= n;
+      w.t0 += n;
+      first = false;
+    }
+  };
+  const int g = p.group;
+  // node of a row: rows are below 128 and g is not above, where 16 bits of the reciprocal give the quotient exactly
+  const uint32_t inv_g = (65536u + g - 1) / g;
+  auto node_of = [&](int r) { return static_cast<int>((r * inv_g) >> 16); };
+
+  if (warp >= 4 && warp < 7) {
+    // =============================== copies ===============================
+    const int cw = warp - 4;
+    bool bad = false, ok = true;
+    uint32_t item = 0, seg = 0;
+    segments([&](const Place& w, const Request& r, int, int n, bool) {
+      const int* rtt = p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride;
+      const int len = r.prefix + r.nodes, base = first_token(p, r) + w.t0 * kTile;
+      const int items = 2 * n;
+      auto slots_of = [&](int i) -> int2 {        // slots of tokens lane and lane + 32 of item i; -1: none
+        int2 s = make_int2(-1, -1);
+        if (i < items) {
+          const int tok = base + item_tile(i, n) * kTile + lane;
+          if (tok < len) s.x = __ldcg(rtt + tok);
+          if (tok + 32 < len) s.y = __ldcg(rtt + tok + 32);
+          if (s.x < 0 || s.x >= p.num_slots) {
+            bad = bad || tok < len;
+            s.x = -1;
+          }
+          if (s.y < 0 || s.y >= p.num_slots) {
+            bad = bad || tok + 32 < len;
+            s.y = -1;
+          }
+        }
+        return s;
+      };
+      auto slot_in = [&](int2 s, int row) {       // row is below 64 for every lane that uses the result
+        const int a = __shfl_sync(0xffffffffu, s.x, row & 31), b = __shfl_sync(0xffffffffu, s.y, row & 31);
+        return row < 32 ? a : b;
+      };
+      auto load_q = [&]() {
+        if (seg > 0 && !mbar_wait(q_free, (seg - 1) & 1, &fail_flag)) return false;
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(r.row) * p.q_stride + static_cast<int64_t>(w.hk) * g * kD;
+        const uint32_t to = smem_u32(sQ);
+        const int n0 = w.rt * p.tpt;
+        constexpr int kCh = 8 * NH;               // 16-byte pieces of a row
+#pragma unroll 4
+        for (int c = tid - 128; c < kRows * kCh; c += kCopyThreads) {
+          const int row = c / kCh, ch = c % kCh;
+          const int node = node_of(row);
+          const bool in = node < p.tpt && n0 + node < r.nodes;
+          const uint16_t* src = q + (in ? (n0 + node) * p.q_stride + static_cast<int64_t>(row - node * g) * kD + ch * 8 : 0);
+          cp16(to + swz(row, ch, C::kQBlock), src, in);
+        }
+        cp_arrive(q_full);
+        return true;
+      };
+      constexpr int kAhead = 4;
+      int2 sl[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) sl[i] = slots_of(i);
+      if constexpr (!KV8) {
+        constexpr int kCh = 8 * NH;
+        constexpr int kRowsPer = 32 / kCh;         // rows of a warp's copy
+        constexpr int kCopies = (kTile / kRowsPer + kCopyWarps - 1) / kCopyWarps;
+        for (int i = 0; i < items; ++i) {
+          const int2 s = sl[0];
+#pragma unroll
+          for (int k = 0; k + 1 < kAhead; ++k) sl[k] = sl[k + 1];
+          sl[kAhead - 1] = slots_of(i + kAhead);
+          const uint32_t st = item % kStages;
+          if (item >= kStages && !mbar_wait(&empty[st], (item / kStages - 1) & 1, &fail_flag)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) return ok = false;
+          const uint16_t* from = static_cast<const uint16_t*>(item_is_key(i, n) ? p.k_cache : p.v_cache) + w.hk * p.kv_head_stride;
+          const uint32_t to = smem_u32(ring) + st * C::kStage;
+          const int ch = lane % kCh, r0 = lane / kCh;
+#pragma unroll
+          for (int k = 0; k < kCopies; ++k) {
+            const int row = (k * kCopyWarps + cw) * kRowsPer + r0;
+            const int rs = slot_in(s, row);
+            if (row < kTile) cp16(to + swz(row, ch, C::kBlock), from + max(rs, 0) * p.kv_tok_stride + ch * 8, rs >= 0);
+          }
+          cp_arrive(&full[st]);
+          ++item;
+          if (i == (n == 1 ? 0 : 1) && !load_q()) return ok = false;
+        }
+      } else {
+        constexpr int kCh = 4 * NH;                // 16 elements each
+        constexpr int kRowsPer = 32 / kCh;
+        constexpr int kCopies = (kTile / kRowsPer + kCopyWarps - 1) / kCopyWarps;
+        const int ch = lane % kCh, r0 = lane / kCh;
+        auto fetch = [&](int i, int2 s, uint4 (&v)[kCopies]) {
+          const uint8_t* from = static_cast<const uint8_t*>(item_is_key(i, n) ? p.k_cache : p.v_cache) + w.hk * p.kv_head_stride + ch * 16;
+#pragma unroll
+          for (int k = 0; k < kCopies; ++k) {
+            const int row = (k * kCopyWarps + cw) * kRowsPer + r0, rs = slot_in(s, row);
+            v[k] = row < kTile && rs >= 0 ? __ldcg(reinterpret_cast<const uint4*>(from + rs * p.kv_tok_stride)) : make_uint4(0, 0, 0, 0);
+          }
+        };
+        auto widen = [&](uint32_t two) -> uint32_t {     // two 8-bit values -> two 16-bit ones, exactly
+          const float2 f = unpack_fp8x2(two, p.kv_fmt);
+          if (p.f16) {
+            const __half2 h = __floats2half2_rn(f.x, f.y);
+            return *reinterpret_cast<const uint32_t*>(&h);
+          }
+          return pack_bf16x2(f.x, f.y);
+        };
+        uint4 now[kCopies], next[kCopies];
+        fetch(0, sl[0], now);
+        for (int i = 0; i < items; ++i) {
+          if (i + 1 < items) fetch(i + 1, sl[1], next);
+#pragma unroll
+          for (int k = 0; k + 1 < kAhead; ++k) sl[k] = sl[k + 1];
+          sl[kAhead - 1] = slots_of(i + kAhead);
+          const uint32_t st = item % kStages;
+          if (item >= kStages && !mbar_wait(&empty[st], (item / kStages - 1) & 1, &fail_flag)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) return ok = false;
+          const uint32_t to = smem_u32(ring) + st * C::kStage;
+#pragma unroll
+          for (int k = 0; k < kCopies; ++k) {
+            const int row = (k * kCopyWarps + cw) * kRowsPer + r0;
+            const uint32_t x[4] = {now[k].x, now[k].y, now[k].z, now[k].w};
+#pragma unroll
+            for (int h = 0; h < 2 && row < kTile; ++h)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + swz(row, ch * 2 + h, C::kBlock)), "r"(widen(x[2 * h])),
+                           "r"(widen(x[2 * h] >> 16)), "r"(widen(x[2 * h + 1])), "r"(widen(x[2 * h + 1] >> 16))
+                           : "memory");
+            now[k] = next[k];
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(&full[st]);
+          ++item;
+          if (i == (n == 1 ? 0 : 1) && !load_q()) return ok = false;
+        }
+      }
+      ++seg;
+      return true;
+    });
+    if (!ok) fail_flag = 1;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
+  } else if (warp == 7) {
+    if (elect_one()) {
+      // =============================== products ===============================
+      bool ok = true;
+      auto wait_on = [&](uint64_t* bar, uint32_t parity) {
+        if (ok && !mbar_wait(bar, parity, &fail_flag)) ok = false;
+        if (ok) {
+          fence_proxy_async_smem();       // copies by cp.async were made in the generic proxy
+          tc_fence_after_sync();
+        }
+      };
+      const uint64_t q_desc = umma_desc_k_sw128(smem_u32(sQ)), k_desc0 = umma_desc_k_sw128(smem_u32(ring));
+      const uint64_t v_desc0 = umma_desc_mn_sw128(smem_u32(ring), C::kBlock, 1024);
+      const uint32_t idesc_s = p.idesc_s, idesc_o = p.idesc_o, tmem_o = tmem + 2 * kTile;
+      uint32_t item = 0, seg = 0, tile = 0;      // tile: products of values so far
+      segments([&](const Place&, const Request&, int, int n, bool) {
+        auto scores = [&](int t) {
+          const uint32_t st = item % kStages, buf = (tile + t) & 1;
+          wait_on(&full[st], (item / kStages) & 1);
+          if (!ok) return;
+          const uint64_t k_desc = k_desc0 + st * (C::kStage >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4 * NH; ++kk)
+            umma_f16(tmem + buf * kTile, q_desc + (kk >> 2) * (C::kQBlock >> 4) + (kk & 3) * 2,
+                     k_desc + (kk >> 2) * (C::kBlock >> 4) + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
+          umma_commit(&empty[st]);
+          umma_commit(&s_full[buf]);
+          if (t == n - 1) umma_commit(q_free);
+          ++item;
+        };
+        if (ok && !mbar_wait(q_full, seg & 1, &fail_flag)) ok = false;
+        scores(0);
+        if (n > 1) scores(1);
+        for (int t = 0; t < n && ok; ++t) {
+          const uint32_t st = item % kStages, at = tile + t, buf = at & 1;
+          wait_on(&full[st], (item / kStages) & 1);
+          wait_on(&p_full[buf], (at >> 1) & 1);
+          if (!ok) break;
+          const uint64_t v_desc = v_desc0 + st * (C::kStage >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16_ts(tmem_o, tmem + buf * kTile + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
+          umma_commit(&empty[st]);
+          umma_commit(&o_done[buf]);
+          ++item;
+          if (t + 2 < n) scores(t + 2);
+        }
+        tile += n;
+        ++seg;
+        return ok;
+      });
+      if (!ok) fail_flag = 1;
+    }
+  } else {
+    // =============================== softmax ===============================
+    const int row = tid;
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t tmem_o = tmem + 2 * kTile + lane_base;
+    const int row_node = node_of(row);
+    const bool capped = p.cap_out > 0.f;
+    bool ok = true, bad = false;
+    uint32_t tile = 0, item = 0;
+    int job_rows = 0, job_row = 0, job_head = 0, job_c0 = 0, job_second = 0;
+    segments([&](const Place& w, const Request& r, int n_all, int n, bool first) {
+      const int node = w.rt * p.tpt + row_node;
+      const bool valid = row_node < p.tpt && node < r.nodes;
+      const bool warp_valid = __any_sync(0xffffffffu, valid);
+      const int key0 = first_token(p, r) + w.t0 * kTile, len = r.prefix + r.nodes;
+      // parents to shared memory; one that is no earlier node counts as none
+      asm volatile("bar.sync 1, 128;" ::: "memory");          // the segment before has read them
+      if (row == 0) poison = 0;
+      auto parent_in = [&](int i) {
+        const int up = __ldcg(p.ix.parents + r.row + i);
+        if (up < -1 || up >= i) {
+          bad = true;
+          return -1;
+        }
+        return up;
+      };
+      for (int i = row; i < min(r.nodes, kParents); i += 128) parents[i] = static_cast<int16_t>(parent_in(i));
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      auto parent_of = [&](int i) { return i < kParents ? static_cast<int>(parents[i]) : parent_in(i); };
+      const bool bounded = p.window > 0 || p.chunk > 0;
+      int pos = r.prefix, low = 0;
+      if (valid && bounded) {
+        for (int a = parent_of(node); a >= 0; a = parent_of(a)) ++pos;
+        low = first_key(p, pos);
+      }
+      // tiles below hold keys that some row may not see for the window's or chunk's sake
+      const int deepest = r.prefix + r.nodes - 1;
+      const int edge = p.window > 0 ? deepest - p.window + 1 : p.chunk > 0 ? deepest / p.chunk * p.chunk : 0;
+      // bit c: this row sees token col0 + c
+      auto visible = [&](int col0) -> uint64_t {
+        uint64_t m = 0;
+        if (!valid) return m;       // no node: nothing to walk
+        const int a = max(low, col0) - col0, e = min(r.prefix, col0 + kTile) - col0;      // [a, e) of the cached tokens
+        if (e > a) m = (e >= 64 ? ~0ull : (1ull << e) - 1) & (~0ull << a);
+        if (col0 + kTile > r.prefix) {
+          int at = pos;
+          for (int j = node; j >= 0 && at >= low; j = parent_of(j), --at) {
+            const int c = r.prefix + j - col0;
+            if (c >= 0 && c < kTile) m |= 1ull << c;
+            if (!bounded) at = low + 1;
+          }
+        }
+        return m;
+      };
+
+      float m_used = -INFINITY;   // maximum in use for the exponent (log2 domain)
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < n; ++t) {
+        const uint32_t at = tile + t, buf = at & 1;
+        const int col0 = key0 + t * kTile;
+        const bool masked = col0 + kTile > r.prefix || col0 < edge;
+        if (!mbar_wait(&s_full[buf], (at >> 1) & 1, &fail_flag)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) return ok = false;
+        tc_fence_after_sync();
+        if (masked) {
+          // values that are no numbers: rows that do not see them must not meet them
+          const uint32_t it = item + value_item(t, n), st = it % kStages;
+          if (!mbar_wait(&full[st], (it / kStages) & 1, &fail_flag)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) return ok = false;
+          uint4* stage = reinterpret_cast<uint4*>(ring + st * C::kStage);
+          const uint32_t expo = p.f16 ? 0x7c00u : 0x7f80u;
+          bool found = false;
+#pragma unroll 4
+          for (int i = row; i < C::kStage / 16; i += 128) {
+            uint4 v = stage[i];
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+            bool here = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if ((x[k] & expo) == expo) {
+                x[k] &= 0xffff0000u;
+                here = true;
+              }
+              if ((x[k] & (expo << 16)) == (expo << 16)) {
+                x[k] &= 0xffffu;
+                here = true;
+              }
+            }
+            if (here) {
+              stage[i] = v;
+              found = true;
+            }
+          }
+          if (found) poison = 1;
+          fence_proxy_async_smem();
+        }
+        if (warp_valid) {
+          uint32_t raw[kTile];
+          const uint32_t tmem_s = tmem + buf * kTile + lane_base;
+          tmem_ld_32x32(tmem_s, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
+          tmem_ld_32x32(tmem_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
+          tmem_ld_wait();
+          float mul = p.scale_log2;
+          if (capped) {        // cap tanh(x / cap), in the log2 domain; tanh(y) = 1 - 2 / (1 + e^(2 y))
+            mul = 1.f;
+#pragma unroll
+            for (int c = 0; c < kTile; ++c)
+              raw[c] = __float_as_uint(p.cap_out * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(raw[c]) * p.cap_in))));
+          }
+          if (masked) {
+            const uint64_t vis = visible(col0);
+#pragma unroll
+            for (int c = 0; c < kTile; ++c) raw[c] = (vis >> c) & 1 ? raw[c] : __float_as_uint(-INFINITY);
+          }
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(raw[i]);
+#pragma unroll
+          for (int c = 4; c < kTile; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(raw[c]));
+          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+          float factor = 1.f;
+          bool need = false;
+          if (m_used == -INFINITY) {
+            m_used = m_tile;      // no key seen so far: the row of O is zero
+          } else if (m_tile > m_used + kRescaleThreshold) {
+            factor = exp2f(m_used - m_tile);
+            m_used = m_tile;
+            need = true;
+          }
+          if (__any_sync(0xffffffffu, need)) {
+            if (!mbar_wait(&o_done[buf ^ 1], ((at - 1) >> 1) & 1, &fail_flag)) ok = false;
+            if (!__all_sync(0xffffffffu, ok)) return ok = false;
+            tc_fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[i] *= factor;
+#pragma unroll 1
+            for (int c = 0; c < kD; c += 16) {
+              uint32_t o[16];
+              tmem_ld_32x16(tmem_o + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+              tmem_st_32x16(tmem_o + c, o);
+            }
+          }
+          const float neg = m_used == -INFINITY ? 0.f : -m_used;
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float p0 = ex2(fmaf(__uint_as_float(raw[2 * i]), mul, neg)), p1 = ex2(fmaf(__uint_as_float(raw[2 * i + 1]), mul, neg));
+            sums[i & 3] += p0 + p1;
+            if (p.f16) {
+              const __half2 h = __floats2half2_rn(p0, p1);
+              pk[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+              pk[i] = pack_bf16x2(p0, p1);
+            }
+          }
+          tmem_st_32x32(tmem_s, pk);
+          tmem_st_wait();
+        }
+        tc_fence_before_sync();
+        mbar_arrive(&p_full[buf]);
+      }
+      tile += n;
+      item += 2 * n;
+      if (!mbar_wait(&o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1, &fail_flag)) ok = false;
+      if (!__all_sync(0xffffffffu, ok)) return ok = false;
+      tc_fence_after_sync();
+
+      // ---- the segment's rows ----
+      const bool whole = w.t0 == 0 && n == n_all;
+      const int head = w.hk * g + row - row_node * g;
+      float l = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      if (whole && p.sink != nullptr && valid) l += exp2f(p.sink[head] * kLog2e - m_used);
+      const float inv = l == 0.f ? 0.f : 1.f / l;       // 0: no key seen.  A sum that is no number shows
+      const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1);
+      const bool slow = poison != 0;
+      if (warp_valid) {
+#pragma unroll 1
+        for (int c = 0; c < kD; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32(tmem_o + c, o);
+          tmem_ld_wait();
+          if (valid) {
+            float f[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * inv;
+            if (slow) {       // rare: every masked tile's values once more, for those that are no numbers
+              const int* rtt = p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride;
+              for (int t = 0; t < n; ++t) {
+                const int col0 = key0 + t * kTile;
+                if (!(col0 + kTile > r.prefix || col0 < edge)) continue;
+                const uint64_t vis = visible(col0);
+                for (int k = 0; k < kTile && col0 + k < len; ++k) {
+                  if (!((vis >> k) & 1)) continue;
+                  const int s = __ldcg(rtt + col0 + k);
+                  if (s < 0 || s >= p.num_slots) continue;
+                  const int64_t from = s * p.kv_tok_stride + w.hk * p.kv_head_stride + c;
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) {
+                    float v;
+                    if constexpr (KV8) {
+                      v = unpack_fp8x2(static_cast<const uint8_t*>(p.v_cache)[from + i], p.kv_fmt).x;
+                    } else {
+                      const uint16_t bits = static_cast<const uint16_t*>(p.v_cache)[from + i];
+                      v = p.f16 ? to_f32(__ushort_as_half(bits)) : to_f32(__ushort_as_bfloat16(bits));
+                    }
+                    if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) f[i] += v;
+                  }
+                }
+              }
+            }
+            if (whole) {
+              uint16_t* to = static_cast<uint16_t*>(p.out) + (r.row + node) * p.out_stride + static_cast<int64_t>(head) * kD + c;
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                uint32_t v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  if (p.f16) {
+                    const __half2 h = __floats2half2_rn(f[i + 2 * k], f[i + 2 * k + 1]);
+                    v[k] = *reinterpret_cast<const uint32_t*>(&h);
+                  } else {
+                    v[k] = pack_bf16x2(f[i + 2 * k], f[i + 2 * k + 1]);
+                  }
+                }
+                *reinterpret_cast<uint4*>(to + i) = make_uint4(v[0], v[1], v[2], v[3]);
+              }
+            } else {
+              float* to = p.part_o + (slot * p.part_rows + row) * kD + c;
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+            }
+          }
+        }
+        if (!whole && valid) p.part_lse[slot * p.part_rows + row] = l == 0.f ? -INFINITY : m_used + log2f(l);
+      }
+      if (row == 0 && !whole && w.t0 + n == n_all) {        // the unit's last tile (it began in front of this run)
+        const int64_t line = line_of[2], begin = line_of[0] - w.t0;
+        const int used = ctas_of;
+        job_rows = min(p.tpt, r.nodes - w.rt * p.tpt) * g;
+        job_row = r.row + w.rt * p.tpt;
+        job_head = w.hk * g;
+        job_c0 = static_cast<int>(((begin + 1) * used - 1) / line);       // the last CTA whose run begins at or before it
+        job_second = run_begin(line, job_c0, used) < begin ? 1 : 0;
+      }
+      tc_fence_before_sync();
+      return true;
+    });
+    if (!ok) fail_flag = 1;
+    if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
+    if (row == 0) {
+      int* job = p.jobs + blockIdx.x * kJobInts;
+      job[0] = ok ? job_rows : 0;
+      job[1] = job_row;
+      job[2] = job_head;
+      job[3] = job_c0;
+      job[4] = job_second;
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (fail_flag) {
+    if (tid == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusPipelineTimeout);
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);      // products and copies in flight land before the memory goes
+    __syncthreads();
+  }
+  if (warp == 7) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+// Joins the partial results of the units that lie in several CTAs: out = sum_c w_c O_c with w_c = 2^(lse_c - max) / sum; a head's
+// sink is one more term of the sum, without a value.  blockIdx.x is a note, a warp takes a row at a time.
+constexpr int kJoinWarps = 4, kJoinParts = 8;
+template <typename T, int HD>
+__global__ void __launch_bounds__(32 * kJoinWarps) attn_tree_join_kernel(const TreeParams p) {
+  constexpr int V = HD / 32;
+  pdl_launch_dependents();
+  pdl_wait_loads();
+  const int* job = p.jobs + blockIdx.x * kJobInts;
+  const int rows = __ldcg(job), row0 = __ldcg(job + 1), head0 = __ldcg(job + 2), c0 = __ldcg(job + 3), second = __ldcg(job + 4);
+  const int c1 = blockIdx.x, lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); r < rows; r += kJoinWarps * kJoinParts) {
+    const int node = r / p.group, head = head0 + r - node * p.group;
+    auto at = [&](int c) { return (static_cast<int64_t>(c) * 2 + (c == c0 ? second : 0)) * p.part_rows + r; };
+    float top = p.sink != nullptr ? p.sink[head] * kLog2e : -INFINITY;
+    const float sink = top;
+    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(p.part_lse + at(c)));
+    top = warp_max(top);
+    float den = 0.f, acc[V] = {};
+    for (int b = c0; b <= c1; b += 32) {
+      const float lse = b + lane <= c1 ? __ldcg(p.part_lse + at(b + lane)) : -INFINITY;
+      const float mine = lse == -INFINITY ? 0.f : exp2f(lse - top);
+      den += mine;
+      const int m = min(32, c1 + 1 - b);
+#pragma unroll 4
+      for (int i = 0; i < m; ++i) {
+        const float w = __shfl_sync(0xffffffffu, mine, i);
+        const float* from = p.part_o + at(b + i) * HD + lane * V;
+        float x[V];
+        if constexpr (V == 2) {
+          *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(from));
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(x + k) = __ldcg(reinterpret_cast<const float4*>(from + k));
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = w == 0.f ? acc[k] : fmaf(w, x[k], acc[k]);
+      }
+    }
+    den = warp_sum(den);
+    if (p.sink != nullptr) den += exp2f(sink - top);
+    T o[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] = from_f32<T>(den == 0.f ? 0.f : acc[k] / den);
+    T* to = static_cast<T*>(p.out) + (row0 + node) * p.out_stride + static_cast<int64_t>(head) * HD + lane * V;
+    if constexpr (V == 2) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(o);
+    else if constexpr (V == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(o);
+    else *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(o);
+  }
+}
+
+template <int NH, bool KV8>
+int launch_one(const TreeParams& p, cudaStream_t s) {
+  auto kern = attn_tree_kernel<NH, KV8>;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), Cfg<NH>::kSmem) != cudaSuccess) return -3;
+  cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(kThreads), Cfg<NH>::kSmem, s, p);
+  note_launch();
+  if (err != cudaSuccess) return -4;
+  err = p.f16 ? launch_pdl(attn_tree_join_kernel<__half, 64 * NH>, dim3(p.ctas, kJoinParts), dim3(32 * kJoinWarps), 0, s, p)
+              : launch_pdl(attn_tree_join_kernel<__nv_bfloat16, 64 * NH>, dim3(p.ctas, kJoinParts), dim3(32 * kJoinWarps), 0, s, p);
+  note_launch();
+  return err == cudaSuccess ? 0 : -4;
+}
+
+}  // namespace
+
+int tree_ctas(int head_dim, int num_sms) { return head_dim == 256 ? num_sms : 2 * num_sms; }
+int tree_part_rows(int group, int64_t rows) {
+  return static_cast<int>(std::min<int64_t>(kRows / group * group, rows * group));
+}
+int64_t tree_workspace_floats(int head_dim, int group, int64_t rows, int ctas) {
+  return static_cast<int64_t>(ctas) * (2 * tree_part_rows(group, rows) * (head_dim + 1) + kJobInts);
+}
+
+int launch_attention_tree(const TreeAttnArgs& a, cudaStream_t s) {
+  const int g = a.hkv > 0 ? a.hq / a.hkv : 0;
+  if ((a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) || a.hkv <= 0 || a.hq % a.hkv != 0 || g < 1 || g > kRows) return -1;
+  if (a.index.rows <= 0 || a.index.batch <= 0) return 0;
+  TreeParams p{};
+  p.q = a.q;
+  p.k_cache = a.k_cache;
+  p.v_cache = a.v_cache;
+  p.out = a.out;
+  p.ctas = a.ctas;
+  p.part_rows = tree_part_rows(g, a.index.rows);
+  p.part_o = a.workspace;
+  p.part_lse = p.part_o + static_cast<int64_t>(p.ctas) * 2 * p.part_rows * a.head_dim;
+  p.jobs = reinterpret_cast<int*>(p.part_lse + static_cast<int64_t>(p.ctas) * 2 * p.part_rows);
+  p.ix = a.index;
+  p.sink = a.sink;
+  p.q_stride = a.q_stride;
+  p.out_stride = a.out_stride;
+  p.num_slots = a.num_slots;
+  p.kv_tok_stride = a.kv_tok_stride;
+  p.kv_head_stride = a.kv_head_stride;
+  p.hkv = a.hkv;
+  p.group = g;
+  p.tpt = kRows / g;
+  p.window = a.window > 0 ? a.window : 0;
+  p.chunk = a.chunk > 0 ? a.chunk : 0;
+  p.kv_fmt = a.kv_fmt;
+  p.f16 = a.dt == kF16 ? 1 : 0;
+  p.scale_log2 = a.scale * kLog2e;
+  if (a.logit_cap > 0.f) {
+    p.cap_in = 2.f * kLog2e * a.scale / a.logit_cap;
+    p.cap_out = a.logit_cap * kLog2e;
+  }
+  const uint32_t fmt = a.dt == kF16 ? 0u : 1u;
+  p.idesc_s = umma_idesc(kRows, kTile, 1, fmt, fmt, 0, 0);
+  p.idesc_o = umma_idesc(kRows, a.head_dim, 1, fmt, fmt, 0, 1);
+  const bool kv8 = a.kv_fmt != kKvSame;
+  switch (a.head_dim) {
+    case 64: return kv8 ? launch_one<1, true>(p, s) : launch_one<1, false>(p, s);
+    case 128: return kv8 ? launch_one<2, true>(p, s) : launch_one<2, false>(p, s);
+    default: return kv8 ? launch_one<4, true>(p, s) : launch_one<4, false>(p, s);
+  }
+}
+
+}  // namespace mb200

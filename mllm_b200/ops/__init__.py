@@ -1494,3 +1494,7 @@ def top_k_top_p_min_p_sample(logits, temperature, top_k, top_p, min_p, uniform) 
     ext().sample(l2, temperature.float().contiguous(), top_k.to(torch.int32).contiguous(), top_p.float().contiguous(),
                  None if min_p is None else min_p.float().contiguous(), uniform.float().contiguous(), out)
     return out
+
+
+# drafted token trees
+from .tree import attention_tree  # noqa: E402,F401

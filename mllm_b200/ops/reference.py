@@ -937,3 +937,58 @@ def gated_delta_rule_chunked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         state[slot] = S.to(state.dtype)
         off += n
     return out.to(v.dtype)
+
+
+# --------------------------------------------------------------------------
+# drafted token trees (speculative decoding)
+# --------------------------------------------------------------------------
+def _tree_ways(parents: torch.Tensor, first: int, n: int):
+    """The nodes on the way from the root to each of a tree's ``n`` nodes, itself last; a parent that is no earlier node counts as none."""
+    ways = []
+    for i, up in enumerate(parents[first:first + n].tolist()):
+        ways.append((ways[up] if 0 <= up < i else []) + [i])
+    return ways
+
+
+def _weighted_values(weights: torch.Tensor, visible: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    """``weights @ v`` where a value that is no finite number reaches the rows that see it and no others.  weights, visible [.., n, L],
+    v [.., L, D]."""
+    fine = torch.isfinite(v)
+    out = weights @ torch.where(fine, v, torch.zeros_like(v))
+    if not bool(fine.all()):
+        see = visible.to(v.dtype)
+        for bad, value in ((torch.isnan(v), float("nan")), (v == float("inf"), float("inf")), (v == float("-inf"), float("-inf"))):
+            out = torch.where((see @ bad.to(v.dtype)) > 0, out + value, out)
+    return out
+
+
+def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents, scale: float,
+                   out: Optional[torch.Tensor] = None, window: Optional[int] = None, logit_cap: float = 0.0,
+                   sink: Optional[torch.Tensor] = None, chunk: Optional[int] = None) -> torch.Tensor:
+    """Row ``q_start_loc[b] + j`` is node j of request b's tree, whose key and value are in slot
+    ``req_to_token[req, prefix_lens[b] + j]``; it sees the cached tokens, its ancestors and itself."""
+    out = torch.empty_like(q) if out is None else out
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    for b in range(req_pool_indices.numel()):
+        sl, pl, qs = int(seq_lens[b]), int(prefix_lens[b]), int(q_start_loc[b])
+        n = sl - pl
+        if n <= 0:
+            continue
+        slots = req_to_token[int(req_pool_indices[b]), :sl].long()
+        visible = torch.zeros((n, sl), dtype=torch.bool)
+        for i, way in enumerate(_tree_ways(parents, qs, n)):
+            at = pl + len(way) - 1
+            low = max(0, at - int(window) + 1) if window else at // int(chunk) * int(chunk) if chunk else 0
+            visible[i, low:pl] = True
+            for up, node in enumerate(way):
+                visible[i, pl + node] = pl + up >= low
+        visible = visible.to(q.device)
+        g = q.shape[1] // k_cache.shape[1]
+        k, v = (t[slots].to(acc).transpose(0, 1).repeat_interleave(g, dim=0) for t in (k_cache, v_cache))     # [Hq, L, D]
+        s = (q[qs:qs + n].to(acc).transpose(0, 1) @ k.transpose(1, 2)) * scale
+        if logit_cap and logit_cap > 0:
+            s = logit_cap * torch.tanh(s / logit_cap)
+        s = s.masked_fill(~visible, float("-inf"))
+        o = _weighted_values(sink_softmax(s, sink), visible, v)
+        out[qs:qs + n] = o.transpose(0, 1).to(out.dtype)
+    return out
