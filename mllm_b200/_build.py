@@ -76,7 +76,7 @@ EXTENSIONS: Dict[str, Dict[str, List[str]]] = {
         "cuda": True,
     },
     "mllm_b200_T": {
-        "sources": ["bindings_tree.cpp", "runtime.cu", "attention_tree.cu"],
+        "sources": ["bindings_tree.cpp", "runtime.cu", "attention_tree.cu", "tree.cu", "tree_sample.cu"],
         "headers": _COMMON + ["tree.h", "tree.cuh"],
         "cuda": True,
     },

@@ -101,9 +101,163 @@ void attention_tree(const Tensor& q, const Tensor& k_cache, const Tensor& v_cach
   TORCH_CHECK(rc == 0, "mllm_b200 attention_tree: unsupported configuration or launch failure (code ", rc, ")");
 }
 
+void check_gain(const c10::optional<Tensor>& g, const Tensor& like, int64_t n, const char* name) {
+  if (!g.has_value()) return;
+  TORCH_CHECK(g->device() == like.device() && g->scalar_type() == like.scalar_type() && g->is_contiguous() && g->numel() == n, "mllm_b200: ",
+              name, " must be a contiguous vector of ", n, " elements like the rows");
+}
+
+Tensor tree_qk_norm_rope_kv_write(const Tensor& qkv, const c10::optional<Tensor>& q_gain, const c10::optional<Tensor>& k_gain,
+                                  const Tensor& parents, const Tensor& req_to_token, const Tensor& req_pool_indices, const Tensor& seq_lens,
+                                  const Tensor& prefix_lens, const Tensor& q_start, const Tensor& inv_freq, Tensor& k_cache, Tensor& v_cache,
+                                  int64_t hq, int64_t hkv, int64_t hd, double eps, const c10::optional<Tensor>& delta) {
+  check_half(qkv, "qkv");
+  TORCH_CHECK((hd == 64 || hd == 128 || hd == 256) && qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) == (hq + 2 * hkv) * hd &&
+                  qkv.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(qkv.data_ptr()) & 15) == 0,
+              "qkv must be [T, (Hq + 2 Hkv) * D], D 64, 128 or 256, rows on 16-byte boundaries");
+  TORCH_CHECK(parents.device() == qkv.device() && inv_freq.device() == qkv.device(), "mllm_b200: tensors on different devices");
+  TORCH_CHECK(inv_freq.scalar_type() == at::kFloat && inv_freq.is_contiguous() && inv_freq.numel() * 2 <= hd && inv_freq.numel() % 8 == 0,
+              "inv_freq must be fp32, one per rotated pair, a multiple of 8");
+  check_gain(q_gain, qkv, hd, "q_weight");
+  check_gain(k_gain, qkv, hd, "k_weight");
+  c10::cuda::CUDAGuard g(qkv.device());
+  mb200::TreePrologueArgs a{};
+  a.index = tree_index(req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start, parents, qkv.size(0));
+  a.kv_fmt = check_caches(k_cache, v_cache, qkv.scalar_type(), hkv, hd, qkv);
+  if (delta.has_value()) {
+    check_int_vec(*delta, req_pool_indices.numel(), "position_delta");
+    TORCH_CHECK(delta->device() == qkv.device(), "mllm_b200: tensors on different devices");
+    a.position_delta = delta->data_ptr<int>();
+  }
+  Tensor q = torch::empty({qkv.size(0), hq, hd}, qkv.options());
+  a.qkv = qkv.data_ptr();
+  a.q_gain = q_gain.has_value() ? q_gain->data_ptr() : nullptr;
+  a.k_gain = k_gain.has_value() ? k_gain->data_ptr() : nullptr;
+  a.inv_freq = inv_freq.data_ptr<float>();
+  a.q_out = q.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.qkv_stride = qkv.stride(0);
+  a.kv_tok_stride = k_cache.stride(0);
+  a.kv_head_stride = k_cache.stride(1);
+  a.num_slots = k_cache.size(0);
+  a.hq = static_cast<int>(hq);
+  a.hkv = static_cast<int>(hkv);
+  a.head_dim = static_cast<int>(hd);
+  a.rotated = static_cast<int>(inv_freq.numel() * 2);
+  a.eps = static_cast<float>(eps);
+  a.dt = dtype_of(qkv);
+  const int rc = mb200::launch_tree_prologue(a, stream_of(qkv));
+  TORCH_CHECK(rc == 0, "mllm_b200 tree_qk_norm_rope_kv_write: launch failure (code ", rc, ")");
+  return q;
+}
+
+void tree_kv_compact(Tensor& store, const Tensor& req_to_token, const Tensor& req_pool_indices, const Tensor& prefix_lens, const Tensor& path,
+                     const Tensor& counts) {
+  const int64_t batch = req_pool_indices.numel(), row = store.size(-1) * store.element_size();
+  TORCH_CHECK(store.is_cuda() && store.dim() >= 2 && store.is_contiguous() && row % 16 == 0 &&
+                  (reinterpret_cast<uintptr_t>(store.data_ptr()) & 15) == 0,
+              "tree_kv_compact: store must be contiguous [.., slots, features] with rows of 16-byte multiples");
+  TORCH_CHECK(req_to_token.is_cuda() && req_to_token.dim() == 2 && req_to_token.scalar_type() == at::kInt && req_to_token.stride(1) == 1,
+              "mllm_b200: req_to_token must be a two-dimensional int32 device tensor with unit inner stride");
+  TORCH_CHECK(path.dim() == 2 && path.size(0) == batch, "mllm_b200: path must be [requests, steps]");
+  check_int_vec(req_pool_indices, batch, "req_pool_indices");
+  check_int_vec(prefix_lens, batch, "prefix_lens");
+  check_int_vec(path, batch * path.size(1), "path");
+  check_int_vec(counts, batch, "counts");
+  for (const Tensor* t : {&req_to_token, &req_pool_indices, &prefix_lens, &path, &counts})
+    TORCH_CHECK(t->device() == store.device(), "mllm_b200: tensors on different devices");
+  if (store.numel() == 0 || batch == 0) return;
+  c10::cuda::CUDAGuard g(store.device());
+  mb200::TreeCompactArgs a{};
+  a.store = store.data_ptr();
+  a.req_to_token = req_to_token.data_ptr<int>();
+  a.req_pool_indices = req_pool_indices.data_ptr<int>();
+  a.prefix_lens = prefix_lens.data_ptr<int>();
+  a.path = path.data_ptr<int>();
+  a.counts = counts.data_ptr<int>();
+  a.status = device_state(store.get_device()).status.data_ptr<int>();
+  a.table_stride = req_to_token.stride(0);
+  a.num_slots = store.size(-2);
+  a.batch = static_cast<int>(batch);
+  a.steps = static_cast<int>(path.size(1));
+  a.table_rows = static_cast<int>(req_to_token.size(0));
+  a.table_cols = static_cast<int>(req_to_token.size(1));
+  a.planes = static_cast<int>(store.numel() / (store.size(-2) * store.size(-1)));
+  a.row_bytes = static_cast<int>(row);
+  const int rc = mb200::launch_tree_compact(a, stream_of(store));
+  TORCH_CHECK(rc == 0, "mllm_b200 tree_kv_compact: unsupported configuration or launch failure (code ", rc, ")");
+}
+
+std::vector<Tensor> tree_speculative_sample(const Tensor& logits, const Tensor& tokens, const Tensor& parents, const Tensor& tree_lens,
+                                            const Tensor& q_start, const Tensor& temperature, const Tensor& top_k, const Tensor& top_p,
+                                            const c10::optional<Tensor>& min_p, const Tensor& uniform, const Tensor& uniform_final,
+                                            int64_t steps, const c10::optional<Tensor>& draft) {
+  check_float(logits, "logits");
+  TORCH_CHECK(logits.dim() == 2 && logits.stride(1) == 1, "logits must be [T, vocab] with unit inner stride");
+  const int64_t rows = logits.size(0), vocab = logits.size(1), batch = tree_lens.numel();
+  TORCH_CHECK(tokens.is_cuda() && tokens.scalar_type() == at::kLong && tokens.is_contiguous() && tokens.numel() == rows,
+              "tokens must be a contiguous int64 device vector, one per row");
+  check_int_vec(parents, rows, "parents");
+  check_int_vec(tree_lens, batch, "tree_lens");
+  check_int_vec(q_start, batch, "q_start_loc");
+  check_int_vec(top_k, batch, "top_k");
+  check_f32_vec(temperature, batch, "temperature");
+  check_f32_vec(top_p, batch, "top_p");
+  check_f32_vec(uniform, rows, "uniform");
+  check_f32_vec(uniform_final, batch, "uniform_final");
+  for (const Tensor* t : {&tokens, &parents, &tree_lens, &q_start, &top_k, &temperature, &top_p, &uniform, &uniform_final})
+    TORCH_CHECK(t->device() == logits.device(), "mllm_b200: tensors on different devices");
+  mb200::TreeSampleArgs a{};
+  if (min_p.has_value()) {
+    check_f32_vec(*min_p, batch, "min_p");
+    TORCH_CHECK(min_p->device() == logits.device(), "mllm_b200: tensors on different devices");
+    a.min_p = min_p->data_ptr<float>();
+  }
+  if (draft.has_value()) {
+    TORCH_CHECK(draft->device() == logits.device() && draft->scalar_type() == at::kFloat && draft->dim() == 2 && draft->stride(1) == 1 &&
+                    draft->size(0) == rows && draft->size(1) == vocab,
+                "draft_probs must be fp32 [T, vocab] with unit inner stride");
+    a.draft = draft->data_ptr<float>();
+    a.draft_stride = draft->stride(0);
+  }
+  a.dt = dtype_of(logits);
+  TORCH_CHECK(steps > 0 && steps < (int64_t(1) << 30), "max_steps must be positive");
+  TORCH_CHECK(vocab > 0 && vocab <= mb200::tree_sample_max_vocab(a.dt), "tree_speculative_sample: vocabularies of 1 to ",
+              mb200::tree_sample_max_vocab(a.dt), " tokens, not ", vocab);
+  c10::cuda::CUDAGuard g(logits.device());
+  Tensor path = torch::empty({batch, steps}, parents.options()), out = torch::empty({batch, steps}, tokens.options()),
+         counts = torch::empty({batch}, parents.options());
+  a.logits = logits.data_ptr();
+  a.tokens = tokens.data_ptr<int64_t>();
+  a.parents = parents.data_ptr<int>();
+  a.tree_lens = tree_lens.data_ptr<int>();
+  a.q_start = q_start.data_ptr<int>();
+  a.temperature = temperature.data_ptr<float>();
+  a.top_k = top_k.data_ptr<int>();
+  a.top_p = top_p.data_ptr<float>();
+  a.uniform = uniform.data_ptr<float>();
+  a.uniform_final = uniform_final.data_ptr<float>();
+  a.path = path.data_ptr<int>();
+  a.out = out.data_ptr<int64_t>();
+  a.counts = counts.data_ptr<int>();
+  a.status = device_state(logits.get_device()).status.data_ptr<int>();
+  a.logit_stride = logits.stride(0);
+  a.rows = static_cast<int>(rows);
+  a.batch = static_cast<int>(batch);
+  a.vocab = static_cast<int>(vocab);
+  a.steps = static_cast<int>(steps);
+  const int rc = mb200::launch_tree_sample(a, stream_of(logits));
+  TORCH_CHECK(rc == 0, "mllm_b200 tree_speculative_sample: unsupported configuration or launch failure (code ", rc, ")");
+  return {path, out, counts};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("tree_speculative_sample", &tree_speculative_sample);
+  m.def("tree_qk_norm_rope_kv_write", &tree_qk_norm_rope_kv_write);
+  m.def("tree_kv_compact", &tree_kv_compact);
   m.def("attention_tree", &attention_tree);
   m.def("read_status", &read_status);
   m.def("launch_count", &launch_count);

@@ -39,4 +39,61 @@ int tree_ctas(int head_dim, int num_sms);
 int64_t tree_workspace_floats(int head_dim, int group, int64_t rows, int ctas);
 int launch_attention_tree(const TreeAttnArgs& args, cudaStream_t s);
 
+// per head: norm, rotation by position * inv_freq; queries out, keys and values to the nodes' slots (tree.cu)
+struct TreePrologueArgs {
+  TreeIndex index;
+  const void* qkv;          // [rows, hq + 2 hkv heads], qkv_stride elements apart
+  const void* q_gain;       // [head_dim] or null: no norm
+  const void* k_gain;
+  const float* inv_freq;    // [rotated / 2], pairs (i, i + rotated / 2); rotated a multiple of 16
+  const int* position_delta;   // [batch] or null
+  void* q_out;              // [rows, hq, head_dim]
+  void* k_cache;
+  void* v_cache;
+  int64_t qkv_stride, kv_tok_stride, kv_head_stride, num_slots;
+  int hq, hkv, head_dim, rotated, kv_fmt;
+  float eps;
+  DType dt;
+};
+int launch_tree_prologue(const TreePrologueArgs& args, cudaStream_t s);
+
+// cache rows of accepted nodes brought together: node i's row <- node path[i]'s, i below counts[b], in every plane of `store`
+struct TreeCompactArgs {
+  void* store;              // [planes, num_slots, row_bytes]
+  const int* req_to_token;
+  const int* req_pool_indices;
+  const int* prefix_lens;
+  const int* path;          // [batch, steps]
+  const int* counts;        // [batch]
+  int* status;
+  int64_t table_stride, num_slots;
+  int batch, steps, table_rows, table_cols, planes, row_bytes;
+};
+int launch_tree_compact(const TreeCompactArgs& args, cudaStream_t s);
+
+// walks each request's tree with the target's filtered distribution (tree_sample.cu)
+struct TreeSampleArgs {
+  const void* logits;       // [rows, vocab], logit_stride elements apart, of type dt
+  const int64_t* tokens;    // [rows]
+  const int* parents;       // [rows]
+  const int* tree_lens;     // [batch]
+  const int* q_start;       // [batch]
+  const float* temperature; // [batch]
+  const int* top_k;         // [batch], <= 0 or >= vocab: off
+  const float* top_p;       // [batch], >= 1: off
+  const float* min_p;       // [batch] or null
+  const float* uniform;     // [rows]
+  const float* uniform_final;   // [batch]
+  const float* draft;       // [rows, vocab], draft_stride apart, or null
+  int* path;                // [batch, steps]
+  int64_t* out;             // [batch, steps]
+  int* counts;              // [batch]
+  int* status;
+  int64_t logit_stride, draft_stride;
+  int rows, batch, vocab, steps;
+  DType dt;
+};
+int tree_sample_max_vocab(DType dt);
+int launch_tree_sample(const TreeSampleArgs& args, cudaStream_t s);
+
 }  // namespace mb200

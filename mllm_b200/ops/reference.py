@@ -992,3 +992,100 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
         o = _weighted_values(sink_softmax(s, sink), visible, v)
         out[qs:qs + n] = o.transpose(0, 1).to(out.dtype)
     return out
+
+
+def tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, parents, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, inv_freq,
+                               k_cache, v_cache, num_q_heads: int, num_kv_heads: int, head_dim: int, eps: float, position_delta=None):
+    """Per head: RMS norm (with a weight), rotation of the first ``2 * inv_freq.numel()`` features by ``position * inv_freq`` (in 64 bits);
+    returns the queries, keys and values go to the nodes' slots."""
+    T, half = qkv.shape[0], inv_freq.numel()
+    x = qkv.to(torch.float64 if qkv.dtype == torch.float64 else torch.float32).view(T, num_q_heads + 2 * num_kv_heads, head_dim)
+    q_out = torch.zeros((T, num_q_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
+    for b in range(req_pool_indices.numel()):
+        pl, qs, n = int(prefix_lens[b]), int(q_start_loc[b]), int(seq_lens[b]) - int(prefix_lens[b])
+        if n <= 0:
+            continue
+        start = pl + (0 if position_delta is None else int(position_delta[b]))
+        pos = torch.tensor([start + len(w) - 1 for w in _tree_ways(parents, qs, n)], dtype=torch.float64, device=qkv.device)
+        angle = pos[:, None] * inv_freq.double()
+        cos, sin = torch.cos(angle).to(x.dtype)[:, None], torch.sin(angle).to(x.dtype)[:, None]
+
+        def turned(h, weight):
+            if weight is not None:
+                h = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps) * weight.to(h.dtype)
+            a, c, rest = h.split([half, half, head_dim - 2 * half], dim=-1)
+            return torch.cat([a * cos - c * sin, c * cos + a * sin, rest], dim=-1)
+
+        q, k, v = x[qs:qs + n].split([num_q_heads, num_kv_heads, num_kv_heads], dim=1)
+        loc = req_to_token[int(req_pool_indices[b]), pl:pl + n].long()
+        q_out[qs:qs + n] = turned(q, q_weight).to(qkv.dtype)
+        k_cache[loc] = turned(k, k_weight).to(k_cache.dtype)
+        v_cache[loc] = v.to(v_cache.dtype)
+    return q_out
+
+
+def tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts) -> None:
+    """Node i's row <- node ``path[b, i]``'s, one after the other."""
+    planes = store.view(-1, store.shape[-2], store.shape[-1])
+    for b in range(req_pool_indices.numel()):
+        slots = req_to_token[int(req_pool_indices[b]), int(prefix_lens[b]):].tolist()
+        for i, node in enumerate(path[b, :int(counts[b])].tolist()):
+            if node != i:
+                planes[:, slots[i]] = planes[:, slots[node]]
+
+
+def _kept_distribution(row: torch.Tensor, temperature: float, k: int, top_p: float, min_p: float) -> torch.Tensor:
+    """The filtered distribution of one row of logits, in 64 bits."""
+    x = row.double()
+    x = torch.where(torch.isnan(x), torch.full_like(x, float("-inf")), x)
+    top = x.max()
+    if temperature <= 1e-6 or top == float("-inf"):
+        return torch.zeros_like(x).index_fill_(0, torch.nonzero(x == top)[0], 1.0)
+    e = torch.where(x == top, torch.ones_like(x), torch.exp((x - top) / temperature))
+    down, cut = torch.sort(e, descending=True).values, 0.0
+    if 0 < k < x.numel():
+        cut = max(cut, float(down[k - 1]))
+    if top_p < 1.0:
+        mass = torch.cumsum(down, 0)
+        inside = int((mass - down < top_p * mass[-1]).sum())
+        cut = max(cut, float(down[max(inside, 1) - 1]))
+    e = torch.where(e >= max(cut, min(min_p, 1.0)), e, torch.zeros_like(e))
+    return e / e.sum()
+
+
+def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, temperature, top_k, top_p, min_p, uniform, uniform_final,
+                            max_steps: int, draft_probs=None):
+    """One request after the other, node by node."""
+    B, V = tree_lens.numel(), logits.shape[1]
+    path = torch.full((B, max_steps), -1, dtype=torch.int32)
+    out = torch.full((B, max_steps), -1, dtype=torch.int64)
+    counts = torch.zeros(B, dtype=torch.int32)
+    for b in range(B):
+        first, n, node = int(q_start_loc[b]), int(tree_lens[b]), 0
+        up = parents[first:first + n].tolist()
+        for step in range(max_steps if n > 0 else 0):
+            p = _kept_distribution(logits[first + node], float(temperature[b]), int(top_k[b]), float(top_p[b]),
+                                   0.0 if min_p is None else float(min_p[b]))
+            path[b, step], counts[b], taken = node, step + 1, -1
+            for c in [j for j in range(node + 1, n) if up[j] == node][:64] if step + 1 < max_steps else []:
+                x = int(tokens[first + c])
+                if not 0 <= x < V:
+                    continue
+                q = torch.zeros_like(p).index_fill_(0, torch.tensor([x], device=p.device), 1.0) if draft_probs is None \
+                    else draft_probs[first + node].double()
+                if float(uniform[first + c]) * float(q[x]) < float(p[x]):
+                    taken = c
+                    break
+                left = (p - q).clamp(min=0.0)
+                if draft_probs is None:
+                    left = torch.where(q > 0, torch.zeros_like(p), p)
+                if float(left.sum()) > 0:
+                    p = left / left.sum()
+            if taken >= 0:
+                out[b, step], node = tokens[first + taken], taken
+                continue
+            sums = torch.cumsum(p, 0)
+            passed = torch.nonzero(sums > float(uniform_final[b]) * float(sums[-1]))
+            out[b, step] = passed[0, 0] if passed.numel() else torch.nonzero(p > 0)[-1, 0]
+            break
+    return path.to(logits.device), out.to(logits.device), counts.to(logits.device)

@@ -47,6 +47,33 @@ def _check_caches(what: str, k_cache, v_cache, heads: int, dim: int, dtype, devi
         raise ValueError(f"{what}: the caches must be [slots, {heads}, {dim}] views of one layout, of {dtype} or an 8-bit float, on {device}")
 
 
+def tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, parents, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, inv_freq,
+                               k_cache, v_cache, num_q_heads: int, num_kv_heads: int, head_dim: int, eps: float,
+                               position_delta: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Prologue of :func:`attention_tree`: ``qkv`` [T, (Hq + 2 Hkv) * D] -> queries [T, Hq, D]; keys and values go to the nodes' slots.
+    Query and key heads are divided by their root mean square and multiplied by ``q_weight`` / ``k_weight`` [D] (None: left as they are), then
+    the first ``2 * inv_freq.numel()`` features turn (feature i with the one half of them on) by ``inv_freq`` (fp32) times the node's
+    position: cached tokens, ancestors, and ``position_delta`` [requests] int32 where text positions do not count from 0.  Heads of 64, 128
+    and 256 features on the GPU, a multiple of 16 of them rotated.  ``qkv`` is left as it is; results are rounded once."""
+    what = "tree_qk_norm_rope_kv_write"
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (num_q_heads + 2 * num_kv_heads) * head_dim:
+        raise ValueError(f"{what}: qkv must be [T, {(num_q_heads + 2 * num_kv_heads) * head_dim}] with unit inner stride")
+    _check_caches(what, k_cache, v_cache, num_kv_heads, head_dim, qkv.dtype, qkv.device)
+    _check_index(what, qkv.shape[0], qkv.device, req_to_token, parents, req_pool_indices, seq_lens, prefix_lens, q_start_loc,
+                 *(() if position_delta is None else (position_delta,)))
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.numel() * 2 > head_dim or inv_freq.device != qkv.device:
+        raise ValueError(f"{what}: inv_freq must be an fp32 vector, one number per rotated pair of {head_dim} features, on {qkv.device}")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (head_dim,) or w.dtype != qkv.dtype or w.device != qkv.device):
+            raise ValueError(f"{what}: weights must be vectors of {head_dim} like qkv")
+    ops = _ops()
+    args = (parents, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, inv_freq, k_cache, v_cache, num_q_heads, num_kv_heads,
+            head_dim, float(eps), position_delta)
+    if not ops.use_kernels(qkv):
+        return ref.tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, *args)
+    return ops.ext().tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, *args)
+
+
 def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents, scale: float,
                    out: Optional[torch.Tensor] = None, window: Optional[int] = None, logit_cap: float = 0.0,
                    sink: Optional[torch.Tensor] = None, chunk: Optional[int] = None) -> torch.Tensor:
@@ -77,3 +104,65 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
     ops.ext().attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents, float(scale), out,
                              int(window or 0), float(logit_cap or 0.0), None if sink is None else sink.contiguous(), int(chunk or 0))
     return out
+
+
+def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, temperature, top_k, top_p, min_p, uniform, uniform_final,
+                            max_steps: int, draft_probs: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Walks each request's tree from node 0 with the target's distribution and emits tokens that are distributed as the target's own.
+
+    ``logits`` [T, vocab] of all nodes, ``tokens`` [T] int64 and ``parents`` [T] of the ``tree_lens[b]`` nodes from row ``q_start_loc[b]`` on.
+    At a node the distribution p is that of :func:`mllm_b200.ops.top_k_top_p_min_p_sample` (temperature up to 1e-6: the most likely token;
+    ``top_k`` below 1 and ``top_p`` of 1 and more do not filter; every filter looks at the whole distribution, and ties at a cut are kept).
+    The node's children, in order, up to 64 of them: child c with token x is taken if ``uniform[c] * q(x) < p(x)``, otherwise
+    ``p <- max(p - q, 0)``, scaled to 1 (left as it is where nothing remains).  q is row ``draft_probs[node]``, the distribution that the
+    children were drawn from one by one, or without ``draft_probs`` all of x: candidates that were picked, not drawn.  Where no child is
+    taken, or ``max_steps`` nodes are reached, the walk ends with the first token whose running sum of p in the order of the ids passes
+    ``uniform_final[b]``.  Random numbers are from [0, 1).  A logit that is no number counts as minus infinity, and a row without a finite
+    logit gives its first token.
+
+    Returns ``path`` [requests, max_steps] int32, the nodes of the walk from node 0 on (whose cache rows are now valid), ``tokens``
+    [requests, max_steps] int64, the emitted tokens (those of ``path[:, 1:]`` and one more), both -1 behind ``counts`` [requests] int32."""
+    what = "tree_speculative_sample"
+    if logits.dim() != 2 or logits.stride(1) != 1 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"{what}: logits must be [T, vocab] in 16 or 32 bits with unit inner stride")
+    T, dev, batch = logits.shape[0], logits.device, tree_lens.numel()
+    if tokens.shape != (T,) or tokens.dtype != torch.int64 or tokens.device != dev or not tokens.is_contiguous():
+        raise ValueError(f"{what}: tokens must be a contiguous int64 vector of {T} on {dev}")
+    for t, n in ((parents, T), (tree_lens, batch), (q_start_loc, batch)):
+        if t.shape != (n,) or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: parents [{T}], tree_lens and q_start_loc [{batch}] must be contiguous int32 vectors on {dev}")
+    for t, n in ((temperature, batch), (top_k, batch), (top_p, batch), (min_p, batch), (uniform, T), (uniform_final, batch)):
+        if t is not None and (t.shape != (n,) or t.device != dev):
+            raise ValueError(f"{what}: temperature, top_k, top_p, min_p and uniform_final have {batch} numbers, uniform {T}, all on {dev}")
+    if draft_probs is not None and (draft_probs.shape != logits.shape or draft_probs.dtype != torch.float32 or draft_probs.device != dev
+                                    or draft_probs.stride(1) != 1):
+        raise ValueError(f"{what}: draft_probs must be fp32 [T, vocab] like logits, with unit inner stride")
+    if max_steps < 1 or logits.shape[1] < 1:
+        raise ValueError(f"{what}: max_steps and the vocabulary must be at least 1")
+    ops = _ops()
+    if not ops.use_kernels(logits):
+        return ref.tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, temperature, top_k, top_p, min_p, uniform,
+                                           uniform_final, max_steps, draft_probs)
+    f32 = lambda t: None if t is None else t.float().contiguous()  # noqa: E731
+    return tuple(ops.ext().tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, f32(temperature),
+                                                   top_k.to(torch.int32).contiguous(), f32(top_p), f32(min_p), f32(uniform),
+                                                   f32(uniform_final), int(max_steps), draft_probs))
+
+
+def tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts) -> None:
+    """Brings the cache rows of accepted nodes together, in place and in every plane of ``store`` [.., slots, features] (contiguous; a pool's
+    storage of all layers): for i below ``counts[b]``, what node ``path[b, i]`` of request b has in its slot goes to the slot of node i.
+    ``path`` [requests, steps] and ``counts`` [requests] are those of :func:`tree_speculative_sample`: a path rises from node 0 on, what
+    stands behind ``counts`` is not read.  The request then holds ``prefix_lens + counts`` tokens."""
+    what = "tree_kv_compact"
+    if store.dim() < 2 or not store.is_contiguous() or store.shape[-1] * store.element_size() % 16:
+        raise ValueError(f"{what}: store must be contiguous [.., slots, features] with rows of a multiple of 16 bytes")
+    _check_index(what, counts.numel(), store.device, req_to_token, counts, req_pool_indices, prefix_lens)
+    if path.dim() != 2 or path.shape[0] != counts.numel() or path.dtype != torch.int32 or not path.is_contiguous() or path.device != store.device:
+        raise ValueError(f"{what}: path must be a contiguous int32 tensor [{counts.numel()}, steps] on {store.device}")
+    if counts.numel() != req_pool_indices.numel():
+        raise ValueError(f"{what}: counts must have one number per request")
+    ops = _ops()
+    if not ops.use_kernels(store):
+        return ref.tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts)
+    ops.ext().tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts)

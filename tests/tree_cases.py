@@ -94,3 +94,35 @@ def exact_attention(c, window=None, logit_cap=0.0, sink=None, chunk=None, bounds
             want[qs + i] = o
             bound[qs + i] = half * (o.abs() + reach) + reach * 2 * (D * 2 ** -24 * span + 2 ** -21)
     return (want, bound) if bounds else want
+
+
+def exact_prologue(c, qkv, gains, inv_freq, hq, hkv, eps, delta=None):
+    """(q, k, v) [T, heads, D] in 64 bits; rows of no request are zero."""
+    T, D, half = qkv.shape[0], qkv.shape[1] // (hq + 2 * hkv), inv_freq.numel()
+    x = qkv.double().view(T, hq + 2 * hkv, D)
+    pos = torch.zeros(T, dtype=torch.float64)
+    known = torch.zeros(T, dtype=torch.bool)
+    for b, parents in enumerate(c["trees"]):
+        qs = int(c["start"][b])
+        for i, way in enumerate(ways_of(parents)):
+            pos[qs + i] = int(c["prefix"][b]) + len(way) - 1 + (0 if delta is None else int(delta[b]))
+            known[qs + i] = True
+    z = torch.polar(torch.ones((T, half), dtype=torch.float64), torch.outer(pos, inv_freq.double().cpu())).to(qkv.device)
+
+    def one(h, gain):
+        if gain is not None:
+            h = h / (h.pow(2).mean(-1, keepdim=True) + eps).sqrt() * gain.double()
+        y = torch.complex(h[..., :half].contiguous(), h[..., half:2 * half].contiguous()) * z[:, None]
+        return torch.cat([y.real, y.imag, h[..., 2 * half:]], dim=-1) * known.to(h.device)[:, None, None]
+
+    return one(x[:, :hq], gains[0]), one(x[:, hq:hq + hkv], gains[1]), x[:, hq + hkv:]
+
+
+def slots_of_rows(c):
+    """Slot of every row of the batch's trees, in row order (the trees' rows follow each other)."""
+    out = []
+    for b, parents in enumerate(c["trees"]):
+        pl = int(c["prefix"][b])
+        out += c["table"][int(c["req"][b]), pl:pl + len(parents)].tolist()
+    return out
+
