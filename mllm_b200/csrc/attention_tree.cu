@@ -13,10 +13,11 @@
 //   * work is dealt as in decoding: the 64-token tiles of all (request, kv head, row tile) units form one line, laid out on the device
 //     from the lengths, and every CTA takes an equal run of it.  A unit inside one CTA is written out directly; others leave at most
 //     two partial results per CTA, and the CTA that has a unit's last tile leaves a note for the kernel that joins them.
-//   * warps 4-6 copy rows by slot with cp.async (a page of one token costs what a page of 16 does) into a ring of 64-token K or V
-//     stages in the operand layout; the copies themselves arrive on the stage's barrier, so the whole ring is in flight.  8-bit rows
-//     pass through registers, widened.
-//   * warp 7 issues S = Q K^T (two score buffers in tensor memory) and O += P V, P from tensor memory.
+//   * warps 4-10 copy rows by slot with cp.async (a page of one token costs what a page of 16 does) into a ring of 64-token K or V
+//     stages in the operand layout.  A warp takes whole stages in turn: what stands between two stages (barriers, slots, shuffles) is a
+//     chain of some 2000 cycles, which all warps paid for every stage when they shared it.  8-bit rows land as they are, and the two
+//     warps that copied them widen them.  The warps left copy Q.
+//   * warp 11 issues S = Q K^T (two score buffers in tensor memory) and O += P V, P from tensor memory.
 //   * warps 0-3 hold a row per thread: online maximum and sum in fp32, P over S in place.  Masks are 64-bit words per row and tile,
 //     made only in tiles that hold tree nodes or a window's edge: cached part by comparison, tree part by a walk to the root over
 //     parents in shared memory.
@@ -32,9 +33,13 @@ namespace {
 
 constexpr int kRows = 128;                 // MMA M
 constexpr int kTile = 64;                  // tokens of a tile
-constexpr int kThreads = 256;              // 4 softmax warps, 3 copying warps, 1 issuing warp
-constexpr int kCopyWarps = 3, kCopyThreads = 32 * kCopyWarps;
+constexpr int kThreads = 384;              // 4 softmax warps, 7 copying warps, one that issues products
+constexpr int kIssueWarp = 11;
+// registers of the groups of 4 warps, of the 384 x 80 that a CTA of two per SM is launched with
+constexpr int kLaunchRegs = 80, kSoftmaxRegs = 128, kOtherRegs = 56;
+static_assert(128 * (kSoftmaxRegs + 2 * kOtherRegs) <= kThreads * kLaunchRegs, "register split");
 constexpr int kStart = 2;                  // units behind every (request, kv head, row tile): what it costs beside its tiles
+constexpr int kNoToken = -0x7fffffff;
 constexpr int kParents = 256;              // nodes whose parents are kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleThreshold = 8.0f;  // the running maximum is raised when a score passes it by 2^8
@@ -44,7 +49,7 @@ struct TreeParams {
   const void* k_cache;
   const void* v_cache;
   void* out;
-  float* part_o;     // [CTAs][2][part_rows][HD]
+  float* part_o;     // [CTAs][2][HD / 4][part_rows][4]: lanes, which hold rows, write and read neighbouring addresses
   float* part_lse;   // [CTAs][2][part_rows]
   int* jobs;         // [CTAs][kJobInts]
   TreeIndex ix;
@@ -83,10 +88,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) 
   const int sz = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz) : "memory");
 }
-// this thread's copies so far arrive on `bar` when they have landed
-__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -97,15 +98,27 @@ __device__ __forceinline__ uint32_t swz(int row, int ch, int block) {
   return (ch >> 3) * block + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
 }
 
-template <int NH>
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int NH, bool KV8>
 struct Cfg {
   static constexpr int kD = 64 * NH;
   static constexpr int kQBlock = kRows * 128;              // a 64-feature block of Q
   static constexpr int kQBytes = NH * kQBlock;
   static constexpr int kBlock = kTile * 128;               // a 64-feature block of a stage
   static constexpr int kStage = NH * kBlock;
-  static constexpr int kStages = NH == 1 ? 10 : 5;
-  static constexpr int kSmem = kQBytes + kStages * kStage;
+  static constexpr int kStages = NH == 1 ? (KV8 ? 6 : 10) : KV8 ? 3 : 5;
+  // A team of warps copies every kTeams-th item.  Never more teams than stages: a team that waits for the item kStages before its own
+  // to be used has seen its item before go to the stage of the one 2 kStages before (a barrier tells a phase from the next, no more).
+  static constexpr int kTeam = KV8 ? 2 : 1, kTeams = KV8 ? 3 : 5;
+  static constexpr int kQWarps = kIssueWarp - 4 - kTeam * kTeams;     // those that are left copy Q
+  static_assert(kTeams <= kStages && kQWarps > 0, "teams");
+  static constexpr int kRaw = KV8 ? kTile * kD : 0;        // an item as it is cached, one per team
+  static constexpr int kSmem = kQBytes + kStages * kStage + kTeams * kRaw;
   static constexpr int kPerSm = NH == 4 ? 1 : 2;
   static_assert(kPerSm * (kSmem + 2048) <= 228 * 1024, "1 KB of each CTA is the system's, 1 KB the kernel's variables");
   static constexpr int kCols = NH == 4 ? 512 : 256;        // two score buffers of 64 columns, then O
@@ -125,8 +138,8 @@ struct Place {          // of a segment
 };
 
 template <int NH, bool KV8>
-__global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(const TreeParams p) {
-  using C = Cfg<NH>;
+__global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kernel(const TreeParams p) {
+  using C = Cfg<NH, KV8>;
   constexpr int kD = C::kD, kStages = C::kStages;
   extern __shared__ __align__(1024) uint8_t tree_smem[];
   __shared__ uint64_t bars[2 * C::kStages + 8];
@@ -134,18 +147,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
   __shared__ int fail_flag, poison;
   __shared__ int16_t parents[kParents];
   __shared__ int begin_of[3];
+  __shared__ Request begin_request;
   __shared__ int64_t line_of[3];
   __shared__ int ctas_of;
   uint8_t* sQ = tree_smem;
   uint8_t* ring = sQ + C::kQBytes;
-  uint64_t* full = bars;                 // [stage] the copying threads
+  uint64_t* full = bars;                 // [stage] the warps of a team
   uint64_t* empty = full + kStages;      // [stage] tcgen05.commit
   uint64_t* s_full = empty + kStages;    // [buffer] tcgen05.commit: scores of a tile
-  uint64_t* p_full = s_full + 2;         // [buffer] 128 threads: P is in tensor memory, O rescaled
+  uint64_t* p_full = s_full + 2;         // [buffer] the softmax warps: P is in tensor memory, O rescaled
   // [buffer] tcgen05.commit: a tile's P V.  A wait tells a phase from the one before it and no more: the scores of tile t, which a
   // thread has seen, were issued behind P V of t - 2, so one barrier would do for neither of the two products that may be out
   uint64_t* o_done = p_full + 2;
-  uint64_t* q_full = o_done + 2;         // the copying threads
+  uint64_t* q_full = o_done + 2;         // the warps that copy Q
   uint64_t* q_free = q_full + 1;         // tcgen05.commit: the segment's last scores
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -157,8 +171,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
     const int first = min(p.ix.batch, lane * per), last = min(p.ix.batch, first + per);
     int64_t mine = 0;
     bool bad = false;
-    for (int b = first; b < last; ++b) {
-      const Request r = request_of(p.ix, b, &bad);
+    Request r{};                     // of the first of this lane's requests
+    for (int b = last - 1; b >= first; --b) {
+      r = request_of(p.ix, b, &bad);
       if (r.nodes > 0) mine += static_cast<int64_t>(row_tiles(p, r)) * (tiles_of(p, r) + kStart);
     }
     if (bad && blockIdx.x == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
@@ -183,31 +198,32 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
     int64_t at = (incl - mine) * p.hkv;
     if (begin < end && begin >= at && begin < incl * p.hkv) {
       for (int b = first; b < last; ++b) {
-        const Request r = request_of(p.ix, b, nullptr);
+        if (b > first) r = request_of(p.ix, b, nullptr);
         const int n = r.nodes > 0 ? tiles_of(p, r) + kStart : 0;
         const int64_t units = static_cast<int64_t>(n) * row_tiles(p, r) * p.hkv;
         if (begin >= at && begin < at + units) {
           const int64_t in = begin - at;
-          const int64_t unit = in / n;
+          const int unit = in < 0x7fffffff ? static_cast<int>(in) / n : static_cast<int>(in / n);    // 64 bits take some 500 cycles
           begin_of[0] = b;
-          begin_of[1] = static_cast<int>(unit);
-          begin_of[2] = static_cast<int>(in - unit * n);
+          begin_of[1] = unit;
+          begin_of[2] = static_cast<int>(in - static_cast<int64_t>(unit) * n);
+          begin_request = r;
         }
         at += units;
       }
     }
-  } else if (warp == 7) {
+  } else if (warp == kIssueWarp) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(&full[i], kCopyThreads);
+        mbar_init(&full[i], C::kTeam);
         mbar_init(&empty[i], 1);
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 128);
+        mbar_init(&p_full[i], 4);
         mbar_init(&o_done[i], 1);
       }
-      mbar_init(q_full, kCopyThreads);
+      mbar_init(q_full, C::kQWarps);
       mbar_init(q_free, 1);
       fence_barrier_init();
     }
@@ -232,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
     if (w.left <= 0) return;
     w.b = begin_of[0];
     w.t0 = begin_of[2];
-    Request r = request_of(p.ix, w.b, nullptr);
+    Request r = begin_request;
     int rts = row_tiles(p, r), n_all = tiles_of(p, r);
     w.hk = begin_of[1] / rts;
     w.rt = begin_of[1] - w.hk * rts;
@@ -266,192 +282,172 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
   const uint32_t inv_g = (65536u + g - 1) / g;
   auto node_of = [&](int r) { return static_cast<int>((r * inv_g) >> 16); };
 
-  if (warp >= 4 && warp < 7) {
-    // =============================== copies ===============================
-    const int cw = warp - 4;
-    bool bad = false, ok = true;
-    uint32_t item = 0, seg = 0;
-    segments([&](const Place& w, const Request& r, int, int n, bool) {
-      const int* rtt = p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride;
-      const int len = r.prefix + r.nodes, base = first_token(p, r) + w.t0 * kTile;
-      const int items = 2 * n;
-      auto slots_of = [&](int i) -> int2 {        // slots of tokens lane and lane + 32 of item i; -1: none
-        int2 s = make_int2(-1, -1);
-        if (i < items) {
-          const int tok = base + item_tile(i, n) * kTile + lane;
-          if (tok < len) s.x = __ldcg(rtt + tok);
-          if (tok + 32 < len) s.y = __ldcg(rtt + tok + 32);
-          if (s.x < 0 || s.x >= p.num_slots) {
-            bad = bad || tok < len;
-            s.x = -1;
+  if (warp >= 4) {
+    if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp < 4 + C::kTeams * C::kTeam) {
+      // =============================== keys and values ===============================
+      const int team = (warp - 4) / C::kTeam, part = (warp - 4) % C::kTeam;
+      constexpr int kPart = kTile / C::kTeam;            // rows of this warp
+      bool bad = false, ok = true;
+      uint32_t item0 = 0;                                // items of the segments before
+      segments([&](const Place& w, const Request& r, int, int n, bool) {
+        const int* rtt = p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride;
+        const int len = r.prefix + r.nodes, base = first_token(p, r) + w.t0 * kTile + part * kPart;
+        const int items = 2 * n;
+        // slots of tokens lane and lane + 32 of this warp's rows of item i; -1: nothing to read
+        auto slots_of = [&](int i) -> int2 {
+          int2 s = make_int2(kNoToken, kNoToken);
+          if (i < items) {
+            const int tok = base + item_tile(i, n) * kTile + lane;
+            if (tok < len) s.x = __ldcg(rtt + tok);
+            if (kPart > 32 && tok + 32 < len) s.y = __ldcg(rtt + tok + 32);
           }
-          if (s.y < 0 || s.y >= p.num_slots) {
-            bad = bad || tok + 32 < len;
-            s.y = -1;
+          return s;
+        };
+        auto checked = [&](int s) {
+          if (s >= 0 && s < p.num_slots) return s;
+          bad = bad || s != kNoToken;
+          return -1;
+        };
+        constexpr int kCh = KV8 ? 4 * NH : 8 * NH;  // 16-byte pieces of a cached row
+        constexpr int kRowsPer = 32 / kCh;          // rows of a warp's copy
+        const int ch = lane % kCh, r0 = lane / kCh;
+        using Elem = typename std::conditional<KV8, uint8_t, uint16_t>::type;
+        int i = (team + C::kTeams - static_cast<int>(item0 % C::kTeams)) % C::kTeams;
+        int2 sl = slots_of(i);
+        for (; i < items; i += C::kTeams) {
+          const uint32_t item = item0 + i, st = item % kStages;
+          const uint32_t stage = smem_u32(ring) + st * C::kStage, raw = smem_u32(ring) + kStages * C::kStage + team * C::kRaw;
+          auto wait_free = [&]() {
+            if (item >= kStages && !mbar_wait(&empty[st], (item / kStages - 1) & 1, &fail_flag)) ok = false;
+            return ok = __all_sync(0xffffffffu, ok);
+          };
+          if (!KV8 && !wait_free()) return false;
+          const int2 s = make_int2(checked(sl.x), checked(sl.y));
+          const Elem* from = static_cast<const Elem*>(item_is_key(i, n) ? p.k_cache : p.v_cache) + w.hk * p.kv_head_stride + ch * (16 / sizeof(Elem));
+#pragma unroll
+          for (int k = 0; k < kPart / kRowsPer; ++k) {
+            const int row = k * kRowsPer + r0;
+            const int rs = __shfl_sync(0xffffffffu, k * kRowsPer < 32 ? s.x : s.y, row & 31);
+            cp16(KV8 ? raw + (part * kPart + row) * kD + ch * 16 : stage + swz(row, ch, C::kBlock), from + max(rs, 0) * p.kv_tok_stride, rs >= 0);
           }
+          cp_commit();
+          sl = slots_of(i + C::kTeams);
+          cp_wait<0>();
+          if constexpr (KV8) {
+            // a thread widens the bytes that it copied itself
+            if (!wait_free()) return false;
+            auto widen = [&](uint32_t two) -> uint32_t {     // two 8-bit values -> two 16-bit ones, exactly
+              const float2 f = unpack_fp8x2(two, p.kv_fmt);
+              if (p.f16) {
+                const __half2 h = __floats2half2_rn(f.x, f.y);
+                return *reinterpret_cast<const uint32_t*>(&h);
+              }
+              return pack_bf16x2(f.x, f.y);
+            };
+#pragma unroll 4
+            for (int k = 0; k < kPart / kRowsPer; ++k) {
+              const int row = part * kPart + k * kRowsPer + r0;
+              uint32_t x[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(raw + row * kD + ch * 16));
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + swz(row, ch * 2 + h, C::kBlock)), "r"(widen(x[2 * h])),
+                             "r"(widen(x[2 * h] >> 16)), "r"(widen(x[2 * h + 1])), "r"(widen(x[2 * h + 1] >> 16))
+                             : "memory");
+            }
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[st]);
         }
-        return s;
-      };
-      auto slot_in = [&](int2 s, int row) {       // row is below 64 for every lane that uses the result
-        const int a = __shfl_sync(0xffffffffu, s.x, row & 31), b = __shfl_sync(0xffffffffu, s.y, row & 31);
-        return row < 32 ? a : b;
-      };
-      auto load_q = [&]() {
-        if (seg > 0 && !mbar_wait(q_free, (seg - 1) & 1, &fail_flag)) return false;
-        const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(r.row) * p.q_stride + static_cast<int64_t>(w.hk) * g * kD;
-        const uint32_t to = smem_u32(sQ);
-        const int n0 = w.rt * p.tpt;
+        item0 += items;
+        return true;
+      });
+      cp_wait<0>();
+      if (!ok) fail_flag = 1;
+      if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
+    } else if (warp < kIssueWarp) {
+      // =============================== queries ===============================
+      // Rows that hold no node keep what is there: they meet only themselves.
+      bool ok = true;
+      uint32_t seg = 0;
+      segments([&](const Place& w, const Request& r, int, int, bool) {
+        if (seg > 0 && !mbar_wait(q_free, (seg - 1) & 1, &fail_flag)) ok = false;
+        if (!(ok = __all_sync(0xffffffffu, ok))) return false;
+        const int n0 = w.rt * p.tpt, rows = min(p.tpt, r.nodes - n0) * g;
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(r.row + n0) * p.q_stride + static_cast<int64_t>(w.hk) * g * kD;
         constexpr int kCh = 8 * NH;               // 16-byte pieces of a row
 #pragma unroll 4
-        for (int c = tid - 128; c < kRows * kCh; c += kCopyThreads) {
-          const int row = c / kCh, ch = c % kCh;
-          const int node = node_of(row);
-          const bool in = node < p.tpt && n0 + node < r.nodes;
-          const uint16_t* src = q + (in ? (n0 + node) * p.q_stride + static_cast<int64_t>(row - node * g) * kD + ch * 8 : 0);
-          cp16(to + swz(row, ch, C::kQBlock), src, in);
+        for (int c = (warp - 4 - C::kTeams * C::kTeam) * 32 + lane; c < rows * kCh; c += C::kQWarps * 32) {
+          const int row = c / kCh, ch = c % kCh, node = node_of(row);
+          cp16(smem_u32(sQ) + swz(row, ch, C::kQBlock), q + node * p.q_stride + static_cast<int64_t>(row - node * g) * kD + ch * 8, true);
         }
-        cp_arrive(q_full);
-        return true;
-      };
-      constexpr int kAhead = 4;
-      int2 sl[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) sl[i] = slots_of(i);
-      if constexpr (!KV8) {
-        constexpr int kCh = 8 * NH;
-        constexpr int kRowsPer = 32 / kCh;         // rows of a warp's copy
-        constexpr int kCopies = (kTile / kRowsPer + kCopyWarps - 1) / kCopyWarps;
-        for (int i = 0; i < items; ++i) {
-          const int2 s = sl[0];
-#pragma unroll
-          for (int k = 0; k + 1 < kAhead; ++k) sl[k] = sl[k + 1];
-          sl[kAhead - 1] = slots_of(i + kAhead);
-          const uint32_t st = item % kStages;
-          if (item >= kStages && !mbar_wait(&empty[st], (item / kStages - 1) & 1, &fail_flag)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) return ok = false;
-          const uint16_t* from = static_cast<const uint16_t*>(item_is_key(i, n) ? p.k_cache : p.v_cache) + w.hk * p.kv_head_stride;
-          const uint32_t to = smem_u32(ring) + st * C::kStage;
-          const int ch = lane % kCh, r0 = lane / kCh;
-#pragma unroll
-          for (int k = 0; k < kCopies; ++k) {
-            const int row = (k * kCopyWarps + cw) * kRowsPer + r0;
-            const int rs = slot_in(s, row);
-            if (row < kTile) cp16(to + swz(row, ch, C::kBlock), from + max(rs, 0) * p.kv_tok_stride + ch * 8, rs >= 0);
-          }
-          cp_arrive(&full[st]);
-          ++item;
-          if (i == (n == 1 ? 0 : 1) && !load_q()) return ok = false;
-        }
-      } else {
-        constexpr int kCh = 4 * NH;                // 16 elements each
-        constexpr int kRowsPer = 32 / kCh;
-        constexpr int kCopies = (kTile / kRowsPer + kCopyWarps - 1) / kCopyWarps;
-        const int ch = lane % kCh, r0 = lane / kCh;
-        auto fetch = [&](int i, int2 s, uint4 (&v)[kCopies]) {
-          const uint8_t* from = static_cast<const uint8_t*>(item_is_key(i, n) ? p.k_cache : p.v_cache) + w.hk * p.kv_head_stride + ch * 16;
-#pragma unroll
-          for (int k = 0; k < kCopies; ++k) {
-            const int row = (k * kCopyWarps + cw) * kRowsPer + r0, rs = slot_in(s, row);
-            v[k] = row < kTile && rs >= 0 ? __ldcg(reinterpret_cast<const uint4*>(from + rs * p.kv_tok_stride)) : make_uint4(0, 0, 0, 0);
-          }
-        };
-        auto widen = [&](uint32_t two) -> uint32_t {     // two 8-bit values -> two 16-bit ones, exactly
-          const float2 f = unpack_fp8x2(two, p.kv_fmt);
-          if (p.f16) {
-            const __half2 h = __floats2half2_rn(f.x, f.y);
-            return *reinterpret_cast<const uint32_t*>(&h);
-          }
-          return pack_bf16x2(f.x, f.y);
-        };
-        uint4 now[kCopies], next[kCopies];
-        fetch(0, sl[0], now);
-        for (int i = 0; i < items; ++i) {
-          if (i + 1 < items) fetch(i + 1, sl[1], next);
-#pragma unroll
-          for (int k = 0; k + 1 < kAhead; ++k) sl[k] = sl[k + 1];
-          sl[kAhead - 1] = slots_of(i + kAhead);
-          const uint32_t st = item % kStages;
-          if (item >= kStages && !mbar_wait(&empty[st], (item / kStages - 1) & 1, &fail_flag)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) return ok = false;
-          const uint32_t to = smem_u32(ring) + st * C::kStage;
-#pragma unroll
-          for (int k = 0; k < kCopies; ++k) {
-            const int row = (k * kCopyWarps + cw) * kRowsPer + r0;
-            const uint32_t x[4] = {now[k].x, now[k].y, now[k].z, now[k].w};
-#pragma unroll
-            for (int h = 0; h < 2 && row < kTile; ++h)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + swz(row, ch * 2 + h, C::kBlock)), "r"(widen(x[2 * h])),
-                           "r"(widen(x[2 * h] >> 16)), "r"(widen(x[2 * h + 1])), "r"(widen(x[2 * h + 1] >> 16))
-                           : "memory");
-            now[k] = next[k];
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(&full[st]);
-          ++item;
-          if (i == (n == 1 ? 0 : 1) && !load_q()) return ok = false;
-        }
-      }
-      ++seg;
-      return true;
-    });
-    if (!ok) fail_flag = 1;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
-  } else if (warp == 7) {
-    if (elect_one()) {
-      // =============================== products ===============================
-      bool ok = true;
-      auto wait_on = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait(bar, parity, &fail_flag)) ok = false;
-        if (ok) {
-          fence_proxy_async_smem();       // copies by cp.async were made in the generic proxy
-          tc_fence_after_sync();
-        }
-      };
-      const uint64_t q_desc = umma_desc_k_sw128(smem_u32(sQ)), k_desc0 = umma_desc_k_sw128(smem_u32(ring));
-      const uint64_t v_desc0 = umma_desc_mn_sw128(smem_u32(ring), C::kBlock, 1024);
-      const uint32_t idesc_s = p.idesc_s, idesc_o = p.idesc_o, tmem_o = tmem + 2 * kTile;
-      uint32_t item = 0, seg = 0, tile = 0;      // tile: products of values so far
-      segments([&](const Place&, const Request&, int, int n, bool) {
-        auto scores = [&](int t) {
-          const uint32_t st = item % kStages, buf = (tile + t) & 1;
-          wait_on(&full[st], (item / kStages) & 1);
-          if (!ok) return;
-          const uint64_t k_desc = k_desc0 + st * (C::kStage >> 4);
-#pragma unroll
-          for (int kk = 0; kk < 4 * NH; ++kk)
-            umma_f16(tmem + buf * kTile, q_desc + (kk >> 2) * (C::kQBlock >> 4) + (kk & 3) * 2,
-                     k_desc + (kk >> 2) * (C::kBlock >> 4) + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
-          umma_commit(&empty[st]);
-          umma_commit(&s_full[buf]);
-          if (t == n - 1) umma_commit(q_free);
-          ++item;
-        };
-        if (ok && !mbar_wait(q_full, seg & 1, &fail_flag)) ok = false;
-        scores(0);
-        if (n > 1) scores(1);
-        for (int t = 0; t < n && ok; ++t) {
-          const uint32_t st = item % kStages, at = tile + t, buf = at & 1;
-          wait_on(&full[st], (item / kStages) & 1);
-          wait_on(&p_full[buf], (at >> 1) & 1);
-          if (!ok) break;
-          const uint64_t v_desc = v_desc0 + st * (C::kStage >> 4);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f16_ts(tmem_o, tmem + buf * kTile + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
-          umma_commit(&empty[st]);
-          umma_commit(&o_done[buf]);
-          ++item;
-          if (t + 2 < n) scores(t + 2);
-        }
-        tile += n;
+        cp_commit();
+        cp_wait<0>();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
         ++seg;
-        return ok;
+        return true;
       });
       if (!ok) fail_flag = 1;
+    } else if (warp == kIssueWarp) {
+      if (elect_one()) {
+        // =============================== products ===============================
+        bool ok = true;
+        auto wait_on = [&](uint64_t* bar, uint32_t parity) {
+          if (ok && !mbar_wait(bar, parity, &fail_flag)) ok = false;
+          if (ok) {
+            fence_proxy_async_smem();       // copies by cp.async were made in the generic proxy
+            tc_fence_after_sync();
+          }
+        };
+        const uint64_t q_desc = umma_desc_k_sw128(smem_u32(sQ)), k_desc0 = umma_desc_k_sw128(smem_u32(ring));
+        const uint64_t v_desc0 = umma_desc_mn_sw128(smem_u32(ring), C::kBlock, 1024);
+        const uint32_t idesc_s = p.idesc_s, idesc_o = p.idesc_o, tmem_o = tmem + 2 * kTile;
+        uint32_t item = 0, seg = 0, tile = 0;      // tile: products of values so far
+        segments([&](const Place&, const Request&, int, int n, bool) {
+          auto scores = [&](int t) {
+            const uint32_t st = item % kStages, buf = (tile + t) & 1;
+            wait_on(&full[st], (item / kStages) & 1);
+            if (!ok) return;
+            const uint64_t k_desc = k_desc0 + st * (C::kStage >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 4 * NH; ++kk)
+              umma_f16(tmem + buf * kTile, q_desc + (kk >> 2) * (C::kQBlock >> 4) + (kk & 3) * 2,
+                       k_desc + (kk >> 2) * (C::kBlock >> 4) + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
+            umma_commit(&empty[st]);
+            umma_commit(&s_full[buf]);
+            if (t == n - 1) umma_commit(q_free);
+            ++item;
+          };
+          if (ok && !mbar_wait(q_full, seg & 1, &fail_flag)) ok = false;
+          scores(0);
+          if (n > 1) scores(1);
+          for (int t = 0; t < n && ok; ++t) {
+            const uint32_t st = item % kStages, at = tile + t, buf = at & 1;
+            wait_on(&full[st], (item / kStages) & 1);
+            wait_on(&p_full[buf], (at >> 1) & 1);
+            if (!ok) break;
+            const uint64_t v_desc = v_desc0 + st * (C::kStage >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ts(tmem_o, tmem + buf * kTile + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
+            umma_commit(&empty[st]);
+            umma_commit(&o_done[buf]);
+            ++item;
+            if (t + 2 < n) scores(t + 2);
+          }
+          tile += n;
+          ++seg;
+          return ok;
+        });
+        if (!ok) fail_flag = 1;
+      }
     }
   } else {
     // =============================== softmax ===============================
+    if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int row = tid;
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t tmem_o = tmem + 2 * kTile + lane_base;
@@ -572,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
           const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
           float factor = 1.f;
           bool need = false;
-          if (m_used == -INFINITY) {
+          if (!valid || m_used == -INFINITY) {
             m_used = m_tile;      // no key seen so far: the row of O is zero
           } else if (m_tile > m_used + kRescaleThreshold) {
             factor = exp2f(m_used - m_tile);
@@ -612,7 +608,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
           tmem_st_wait();
         }
         tc_fence_before_sync();
-        mbar_arrive(&p_full[buf]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
       }
       tile += n;
       item += 2 * n;
@@ -680,9 +677,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
                 *reinterpret_cast<uint4*>(to + i) = make_uint4(v[0], v[1], v[2], v[3]);
               }
             } else {
-              float* to = p.part_o + (slot * p.part_rows + row) * kD + c;
+              float* to = p.part_o + slot * p.part_rows * kD + (static_cast<int64_t>(c / 4) * p.part_rows + row) * 4;
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(to + static_cast<int64_t>(i) * p.part_rows) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
             }
           }
         }
@@ -719,68 +717,65 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH>::kPerSm) attn_tree_kernel(co
     for (int i = 0; i < 64; ++i) __nanosleep(1000);      // products and copies in flight land before the memory goes
     __syncthreads();
   }
-  if (warp == 7) {
+  if (warp == kIssueWarp) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, C::kCols);
   }
 }
 
 // Joins the partial results of the units that lie in several CTAs: out = sum_c w_c O_c with w_c = 2^(lse_c - max) / sum; a head's
-// sink is one more term of the sum, without a value.  blockIdx.x is a note, a warp takes a row at a time.
+// sink is one more term of the sum, without a value.  blockIdx.x is a note; a warp takes 32 rows (a lane each) and 16 features at a time.
 constexpr int kJoinWarps = 4, kJoinParts = 8;
 template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kJoinWarps) attn_tree_join_kernel(const TreeParams p) {
-  constexpr int V = HD / 32;
   pdl_launch_dependents();
   pdl_wait_loads();
   const int* job = p.jobs + blockIdx.x * kJobInts;
   const int rows = __ldcg(job), row0 = __ldcg(job + 1), head0 = __ldcg(job + 2), c0 = __ldcg(job + 3), second = __ldcg(job + 4);
   const int c1 = blockIdx.x, lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); r < rows; r += kJoinWarps * kJoinParts) {
+  const int groups = (rows + 31) / 32;
+  for (int task = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); task < groups * (HD / 16); task += kJoinWarps * kJoinParts) {
+    const int r = task % groups * 32 + lane, d = task / groups * 16;
+    if (r >= rows) continue;
     const int node = r / p.group, head = head0 + r - node * p.group;
-    auto at = [&](int c) { return (static_cast<int64_t>(c) * 2 + (c == c0 ? second : 0)) * p.part_rows + r; };
-    float top = p.sink != nullptr ? p.sink[head] * kLog2e : -INFINITY;
-    const float sink = top;
-    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(p.part_lse + at(c)));
-    top = warp_max(top);
-    float den = 0.f, acc[V] = {};
-    for (int b = c0; b <= c1; b += 32) {
-      const float lse = b + lane <= c1 ? __ldcg(p.part_lse + at(b + lane)) : -INFINITY;
-      const float mine = lse == -INFINITY ? 0.f : exp2f(lse - top);
-      den += mine;
-      const int m = min(32, c1 + 1 - b);
-#pragma unroll 4
-      for (int i = 0; i < m; ++i) {
-        const float w = __shfl_sync(0xffffffffu, mine, i);
-        const float* from = p.part_o + at(b + i) * HD + lane * V;
-        float x[V];
-        if constexpr (V == 2) {
-          *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(from));
-        } else {
+    auto slot = [&](int c) { return static_cast<int64_t>(c) * 2 + (c == c0 ? second : 0); };
+    const float sink = p.sink != nullptr ? p.sink[head] * kLog2e : -INFINITY;
+    float top = sink;
+    for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(p.part_lse + slot(c) * p.part_rows + r));
+    float den = p.sink != nullptr ? exp2f(sink - top) : 0.f, acc[16] = {};
+#pragma unroll 2
+    for (int c = c0; c <= c1; ++c) {
+      const float lse = __ldcg(p.part_lse + slot(c) * p.part_rows + r);
+      const float4* from = reinterpret_cast<const float4*>(p.part_o + slot(c) * p.part_rows * HD) + (d / 4) * p.part_rows + r;
+      float4 x[4];
 #pragma unroll
-          for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(x + k) = __ldcg(reinterpret_cast<const float4*>(from + k));
-        }
+      for (int k = 0; k < 4; ++k) x[k] = __ldcg(from + k * p.part_rows);
+      if (lse == -INFINITY) continue;           // saw no key
+      const float w = exp2f(lse - top);
+      den += w;
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] = w == 0.f ? acc[k] : fmaf(w, x[k], acc[k]);
+      for (int k = 0; k < 4; ++k) {
+        acc[4 * k] = fmaf(w, x[k].x, acc[4 * k]);
+        acc[4 * k + 1] = fmaf(w, x[k].y, acc[4 * k + 1]);
+        acc[4 * k + 2] = fmaf(w, x[k].z, acc[4 * k + 2]);
+        acc[4 * k + 3] = fmaf(w, x[k].w, acc[4 * k + 3]);
       }
     }
-    den = warp_sum(den);
-    if (p.sink != nullptr) den += exp2f(sink - top);
-    T o[V];
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    T o[16];
 #pragma unroll
-    for (int k = 0; k < V; ++k) o[k] = from_f32<T>(den == 0.f ? 0.f : acc[k] / den);
-    T* to = static_cast<T*>(p.out) + (row0 + node) * p.out_stride + static_cast<int64_t>(head) * HD + lane * V;
-    if constexpr (V == 2) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(o);
-    else if constexpr (V == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(o);
-    else *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(o);
+    for (int k = 0; k < 16; ++k) o[k] = from_f32<T>(acc[k] * inv);
+    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + node) * p.out_stride + static_cast<int64_t>(head) * HD + d);
+    to[0] = reinterpret_cast<const uint4*>(o)[0];
+    to[1] = reinterpret_cast<const uint4*>(o)[1];
   }
 }
 
 template <int NH, bool KV8>
 int launch_one(const TreeParams& p, cudaStream_t s) {
   auto kern = attn_tree_kernel<NH, KV8>;
-  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), Cfg<NH>::kSmem) != cudaSuccess) return -3;
-  cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(kThreads), Cfg<NH>::kSmem, s, p);
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), Cfg<NH, KV8>::kSmem) != cudaSuccess) return -3;
+  cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(kThreads), Cfg<NH, KV8>::kSmem, s, p);
   note_launch();
   if (err != cudaSuccess) return -4;
   err = p.f16 ? launch_pdl(attn_tree_join_kernel<__half, 64 * NH>, dim3(p.ctas, kJoinParts), dim3(32 * kJoinWarps), 0, s, p)
