@@ -55,7 +55,7 @@ struct TreeParams {
   TreeIndex ix;
   const float* sink;
   int64_t q_stride, out_stride, num_slots, kv_tok_stride, kv_head_stride;
-  int hkv, group, tpt, ctas, part_rows, window, chunk, kv_fmt, f16;
+  int hkv, group, tpt, ctas, part_rows, window, chunk;
   float scale_log2, cap_in, cap_out;    // cap_out 0: no soft cap
   uint32_t idesc_s, idesc_o;
 };
@@ -92,6 +92,41 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two 32-bit operations an instruction
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(a, b);
+  }
 }
 // offset of 16-byte piece `ch` of row `row` in a tile of 64-feature blocks of `block` bytes, rows of 128 bytes, 128-byte swizzle
 __device__ __forceinline__ uint32_t swz(int row, int ch, int block) {
@@ -137,8 +172,10 @@ struct Place {          // of a segment
   int64_t left;
 };
 
-template <int NH, bool KV8>
-__global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kernel(const TreeParams p) {
+// FMT: what the caches hold (kKvSame, kKvE4M3, kKvE5M2)
+template <typename T, int NH, int FMT>
+__global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) attn_tree_kernel(const TreeParams p) {
+  constexpr bool KV8 = FMT != kKvSame, kF16 = std::is_same<T, __half>::value;
   using C = Cfg<NH, KV8>;
   constexpr int kD = C::kD, kStages = C::kStages;
   extern __shared__ __align__(1024) uint8_t tree_smem[];
@@ -338,11 +375,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
             // a thread widens the bytes that it copied itself
             if (!wait_free()) return false;
             auto widen = [&](uint32_t two) -> uint32_t {     // two 8-bit values -> two 16-bit ones, exactly
-              const float2 f = unpack_fp8x2(two, p.kv_fmt);
-              if (p.f16) {
-                const __half2 h = __floats2half2_rn(f.x, f.y);
-                return *reinterpret_cast<const uint32_t*>(&h);
-              }
+              const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu),
+                                                               FMT == kKvE5M2 ? __NV_E5M2 : __NV_E4M3);
+              if constexpr (kF16) return *reinterpret_cast<const uint32_t*>(&h);
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
               return pack_bf16x2(f.x, f.y);
             };
 #pragma unroll 4
@@ -461,9 +497,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
       const bool valid = row_node < p.tpt && node < r.nodes;
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       const int key0 = first_token(p, r) + w.t0 * kTile, len = r.prefix + r.nodes;
-      // parents to shared memory; one that is no earlier node counts as none
-      asm volatile("bar.sync 1, 128;" ::: "memory");          // the segment before has read them
-      if (row == 0) poison = 0;
+      const bool bounded = p.window > 0 || p.chunk > 0;
+      const bool masks = bounded || key0 + n * kTile > r.prefix;      // the segment has masked tiles
       auto parent_in = [&](int i) {
         const int up = __ldcg(p.ix.parents + r.row + i);
         if (up < -1 || up >= i) {
@@ -472,10 +507,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
         }
         return up;
       };
-      for (int i = row; i < min(r.nodes, kParents); i += 128) parents[i] = static_cast<int16_t>(parent_in(i));
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (masks) {        // parents to shared memory; one that is no earlier node counts as none
+        asm volatile("bar.sync 1, 128;" ::: "memory");          // the segment before has read them
+        if (row == 0) poison = 0;
+        for (int i = row; i < min(r.nodes, kParents); i += 128) parents[i] = static_cast<int16_t>(parent_in(i));
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
       auto parent_of = [&](int i) { return i < kParents ? static_cast<int>(parents[i]) : parent_in(i); };
-      const bool bounded = p.window > 0 || p.chunk > 0;
       int pos = r.prefix, low = 0;
       if (valid && bounded) {
         for (int a = parent_of(node); a >= 0; a = parent_of(a)) ++pos;
@@ -502,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
       };
 
       float m_used = -INFINITY;   // maximum in use for the exponent (log2 domain)
-      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+      uint64_t sums[4] = {0, 0, 0, 0};      // pairs of fp32
       for (int t = 0; t < n; ++t) {
         const uint32_t at = tile + t, buf = at & 1;
         const int col0 = key0 + t * kTile;
@@ -516,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
           if (!mbar_wait(&full[st], (it / kStages) & 1, &fail_flag)) ok = false;
           if (!__all_sync(0xffffffffu, ok)) return ok = false;
           uint4* stage = reinterpret_cast<uint4*>(ring + st * C::kStage);
-          const uint32_t expo = p.f16 ? 0x7c00u : 0x7f80u;
+          const uint32_t expo = kF16 ? 0x7c00u : 0x7f80u;
           bool found = false;
 #pragma unroll 4
           for (int i = row; i < C::kStage / 16; i += 128) {
@@ -562,9 +600,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
           }
           float mx[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(raw[i]);
+          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
 #pragma unroll
-          for (int c = 4; c < kTile; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(raw[c]));
+          for (int c = 8; c < kTile; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(raw[c]), __uint_as_float(raw[c + 1]));
           const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
           float factor = 1.f;
           bool need = false;
@@ -580,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
             if (!__all_sync(0xffffffffu, ok)) return ok = false;
             tc_fence_after_sync();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums[i] *= factor;
+            for (int i = 0; i < 4; ++i) sums[i] = fma2(sums[i], pair_of(factor, factor), 0);
 #pragma unroll 1
             for (int c = 0; c < kD; c += 16) {
               uint32_t o[16];
@@ -592,17 +630,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
             }
           }
           const float neg = m_used == -INFINITY ? 0.f : -m_used;
+          const uint64_t mul2 = pair_of(mul, mul), neg2 = pair_of(neg, neg);
           uint32_t pk[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float p0 = ex2(fmaf(__uint_as_float(raw[2 * i]), mul, neg)), p1 = ex2(fmaf(__uint_as_float(raw[2 * i + 1]), mul, neg));
-            sums[i & 3] += p0 + p1;
-            if (p.f16) {
-              const __half2 h = __floats2half2_rn(p0, p1);
-              pk[i] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-              pk[i] = pack_bf16x2(p0, p1);
-            }
+            const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), mul2, neg2));
+            const float p0 = ex2(x.x), p1 = ex2(x.y);
+            sums[i & 3] = add2(sums[i & 3], pair_of(p0, p1));
+            pk[i] = pack2<T>(p0, p1);
           }
           tmem_st_32x32(tmem_s, pk);
           tmem_st_wait();
@@ -620,11 +655,43 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
       // ---- the segment's rows ----
       const bool whole = w.t0 == 0 && n == n_all;
       const int head = w.hk * g + row - row_node * g;
-      float l = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+      float l = both.x + both.y;
       if (whole && p.sink != nullptr && valid) l += exp2f(p.sink[head] * kLog2e - m_used);
       const float inv = l == 0.f ? 0.f : 1.f / l;       // 0: no key seen.  A sum that is no number shows
       const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1);
-      const bool slow = poison != 0;
+      if (masks && poison != 0) {       // rare: every masked tile's values once more, for those that are no numbers
+        const int* rtt = p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride;
+#pragma unroll 1
+        for (int c = 0; c < kD; c += 16) {
+          uint32_t o[16];
+          tmem_ld_32x16(tmem_o + c, o);
+          tmem_ld_wait();
+#pragma unroll 1
+          for (int t = 0; t < n; ++t) {
+            const int col0 = key0 + t * kTile;
+            if (!(col0 + kTile > r.prefix || col0 < edge)) continue;
+            const uint64_t vis = visible(col0);
+#pragma unroll 1
+            for (int k = 0; k < kTile && col0 + k < len; ++k) {
+              if (!((vis >> k) & 1)) continue;
+              const int s = __ldcg(rtt + col0 + k);
+              if (s < 0 || s >= p.num_slots) continue;
+              const int64_t from = s * p.kv_tok_stride + w.hk * p.kv_head_stride + c;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float v;
+                if constexpr (KV8) v = unpack_fp8x2(static_cast<const uint8_t*>(p.v_cache)[from + i], FMT).x;
+                else v = to_f32(static_cast<const T*>(p.v_cache)[from + i]);
+                if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[i] = __float_as_uint(__uint_as_float(o[i]) + v);
+              }
+            }
+          }
+          __syncwarp();
+          tmem_st_32x16(tmem_o + c, o);
+        }
+        tmem_st_wait();
+      }
       if (warp_valid) {
 #pragma unroll 1
         for (int c = 0; c < kD; c += 32) {
@@ -635,45 +702,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
             float f[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * inv;
-            if (slow) {       // rare: every masked tile's values once more, for those that are no numbers
-              const int* rtt = p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride;
-              for (int t = 0; t < n; ++t) {
-                const int col0 = key0 + t * kTile;
-                if (!(col0 + kTile > r.prefix || col0 < edge)) continue;
-                const uint64_t vis = visible(col0);
-                for (int k = 0; k < kTile && col0 + k < len; ++k) {
-                  if (!((vis >> k) & 1)) continue;
-                  const int s = __ldcg(rtt + col0 + k);
-                  if (s < 0 || s >= p.num_slots) continue;
-                  const int64_t from = s * p.kv_tok_stride + w.hk * p.kv_head_stride + c;
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) {
-                    float v;
-                    if constexpr (KV8) {
-                      v = unpack_fp8x2(static_cast<const uint8_t*>(p.v_cache)[from + i], p.kv_fmt).x;
-                    } else {
-                      const uint16_t bits = static_cast<const uint16_t*>(p.v_cache)[from + i];
-                      v = p.f16 ? to_f32(__ushort_as_half(bits)) : to_f32(__ushort_as_bfloat16(bits));
-                    }
-                    if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) f[i] += v;
-                  }
-                }
-              }
-            }
             if (whole) {
               uint16_t* to = static_cast<uint16_t*>(p.out) + (r.row + node) * p.out_stride + static_cast<int64_t>(head) * kD + c;
 #pragma unroll
               for (int i = 0; i < 32; i += 8) {
                 uint32_t v[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  if (p.f16) {
-                    const __half2 h = __floats2half2_rn(f[i + 2 * k], f[i + 2 * k + 1]);
-                    v[k] = *reinterpret_cast<const uint32_t*>(&h);
-                  } else {
-                    v[k] = pack_bf16x2(f[i + 2 * k], f[i + 2 * k + 1]);
-                  }
-                }
+                for (int k = 0; k < 4; ++k) v[k] = pack2<T>(f[i + 2 * k], f[i + 2 * k + 1]);
                 *reinterpret_cast<uint4*>(to + i) = make_uint4(v[0], v[1], v[2], v[3]);
               }
             } else {
@@ -692,7 +727,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, KV8>::kPerSm) attn_tree_kern
         job_rows = min(p.tpt, r.nodes - w.rt * p.tpt) * g;
         job_row = r.row + w.rt * p.tpt;
         job_head = w.hk * g;
-        job_c0 = static_cast<int>(((begin + 1) * used - 1) / line);       // the last CTA whose run begins at or before it
+        // the last CTA whose run begins at or before the unit
+        job_c0 = line < 0xFFFFFFFFll / (used + 1) ? static_cast<int>((static_cast<uint32_t>(begin + 1) * used - 1u) / static_cast<uint32_t>(line))
+                                                  : static_cast<int>(((begin + 1) * used - 1) / line);
         job_second = run_begin(line, job_c0, used) < begin ? 1 : 0;
       }
       tc_fence_before_sync();
@@ -771,17 +808,41 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_tree_join_kernel(const T
   }
 }
 
-template <int NH, bool KV8>
+template <typename T, int NH, int FMT>
 int launch_one(const TreeParams& p, cudaStream_t s) {
-  auto kern = attn_tree_kernel<NH, KV8>;
-  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), Cfg<NH, KV8>::kSmem) != cudaSuccess) return -3;
-  cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(kThreads), Cfg<NH, KV8>::kSmem, s, p);
+  using C = Cfg<NH, FMT != kKvSame>;
+  auto kern = attn_tree_kernel<T, NH, FMT>;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem) != cudaSuccess) return -3;
+  if constexpr (C::kPerSm == 2) {
+    // the softmax warps take registers that the others give back: together no more than the kernel is launched with
+    static const int regs = [kern] {
+      cudaFuncAttributes at{};
+      return cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(kern)) == cudaSuccess ? at.numRegs : 0;
+    }();
+    if (regs < kLaunchRegs) return -5;
+  }
+  cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(kThreads), C::kSmem, s, p);
   note_launch();
   if (err != cudaSuccess) return -4;
-  err = p.f16 ? launch_pdl(attn_tree_join_kernel<__half, 64 * NH>, dim3(p.ctas, kJoinParts), dim3(32 * kJoinWarps), 0, s, p)
-              : launch_pdl(attn_tree_join_kernel<__nv_bfloat16, 64 * NH>, dim3(p.ctas, kJoinParts), dim3(32 * kJoinWarps), 0, s, p);
+  err = launch_pdl(attn_tree_join_kernel<T, 64 * NH>, dim3(p.ctas, kJoinParts), dim3(32 * kJoinWarps), 0, s, p);
   note_launch();
   return err == cudaSuccess ? 0 : -4;
+}
+template <typename T, int NH>
+int launch_format(const TreeParams& p, int fmt, cudaStream_t s) {
+  switch (fmt) {
+    case kKvSame: return launch_one<T, NH, kKvSame>(p, s);
+    case kKvE4M3: return launch_one<T, NH, kKvE4M3>(p, s);
+    default: return launch_one<T, NH, kKvE5M2>(p, s);
+  }
+}
+template <typename T>
+int launch_type(const TreeParams& p, int head_dim, int fmt, cudaStream_t s) {
+  switch (head_dim) {
+    case 64: return launch_format<T, 1>(p, fmt, s);
+    case 128: return launch_format<T, 2>(p, fmt, s);
+    default: return launch_format<T, 4>(p, fmt, s);
+  }
 }
 
 }  // namespace
@@ -820,8 +881,6 @@ int launch_attention_tree(const TreeAttnArgs& a, cudaStream_t s) {
   p.tpt = kRows / g;
   p.window = a.window > 0 ? a.window : 0;
   p.chunk = a.chunk > 0 ? a.chunk : 0;
-  p.kv_fmt = a.kv_fmt;
-  p.f16 = a.dt == kF16 ? 1 : 0;
   p.scale_log2 = a.scale * kLog2e;
   if (a.logit_cap > 0.f) {
     p.cap_in = 2.f * kLog2e * a.scale / a.logit_cap;
@@ -830,12 +889,7 @@ int launch_attention_tree(const TreeAttnArgs& a, cudaStream_t s) {
   const uint32_t fmt = a.dt == kF16 ? 0u : 1u;
   p.idesc_s = umma_idesc(kRows, kTile, 1, fmt, fmt, 0, 0);
   p.idesc_o = umma_idesc(kRows, a.head_dim, 1, fmt, fmt, 0, 1);
-  const bool kv8 = a.kv_fmt != kKvSame;
-  switch (a.head_dim) {
-    case 64: return kv8 ? launch_one<1, true>(p, s) : launch_one<1, false>(p, s);
-    case 128: return kv8 ? launch_one<2, true>(p, s) : launch_one<2, false>(p, s);
-    default: return kv8 ? launch_one<4, true>(p, s) : launch_one<4, false>(p, s);
-  }
+  return a.dt == kF16 ? launch_type<__half>(p, a.head_dim, a.kv_fmt, s) : launch_type<__nv_bfloat16>(p, a.head_dim, a.kv_fmt, s);
 }
 
 }  // namespace mb200
