@@ -21,8 +21,8 @@
 //   * warps 0-3 hold a row per thread: online maximum and sum in fp32, P over S in place.  Masks are 64-bit words per row and tile,
 //     made only in tiles that hold tree nodes or a window's edge: cached part by comparison, tree part by a walk to the root over
 //     parents in shared memory.
-// A value that is no number must not reach rows that do not see it (0 x NaN): in masked tiles such elements of V are set to zero in the
-// stage, and added at the end to the rows that see them.
+// A value that is no number must not reach rows that do not see it (0 x NaN): in masked tiles the warps that copied V set such elements to
+// zero, and they are added at the end to the rows that see them.
 #include <algorithm>
 
 #include "common.cuh"
@@ -38,7 +38,7 @@ constexpr int kIssueWarp = 11;
 // registers of the groups of 4 warps, of the 384 x 80 that a CTA of two per SM is launched with
 constexpr int kLaunchRegs = 80, kSoftmaxRegs = 128, kOtherRegs = 56;
 static_assert(128 * (kSoftmaxRegs + 2 * kOtherRegs) <= kThreads * kLaunchRegs, "register split");
-constexpr int kStart = 2;                  // units behind every (request, kv head, row tile): what it costs beside its tiles
+constexpr int kStart = 4;                  // units behind every (request, kv head, row tile): what it costs beside its tiles
 constexpr int kNoToken = -0x7fffffff;
 constexpr int kParents = 256;              // nodes whose parents are kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
@@ -70,6 +70,8 @@ __device__ __forceinline__ int first_key(const TreeParams& p, int i) {
 }
 // first token that is copied: the first key of the least deep position
 __device__ __forceinline__ int first_token(const TreeParams& p, const Request& r) { return first_key(p, r.prefix) & ~(kTile - 1); }
+// Tokens below hold keys that some node of the request may not see for the window's or the chunk's sake.
+__device__ __forceinline__ int edge_of(const TreeParams& p, const Request& r) { return first_key(p, r.prefix + r.nodes - 1); }
 __device__ __forceinline__ int tiles_of(const TreeParams& p, const Request& r) {
   return r.nodes == 0 ? 0 : (r.prefix + r.nodes - first_token(p, r) + kTile - 1) / kTile;
 }
@@ -165,7 +167,6 @@ __device__ __forceinline__ int item_tile(int i, int n) {
   if (item_is_key(i, n)) return i < 2 ? i : (i + 1) / 2;
   return i == 2 * n - 1 ? n - 1 : (i - 2) / 2;
 }
-__device__ __forceinline__ int value_item(int t, int n) { return t == n - 1 ? 2 * n - 1 : 2 + 2 * t; }
 
 struct Place {          // of a segment
   int b, hk, rt, t0;
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
       segments([&](const Place& w, const Request& r, int, int n, bool) {
         const int* rtt = p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride;
         const int len = r.prefix + r.nodes, base = first_token(p, r) + w.t0 * kTile + part * kPart;
-        const int items = 2 * n;
+        const int items = 2 * n, edge = edge_of(p, r);
         // slots of tokens lane and lane + 32 of this warp's rows of item i; -1: nothing to read
         auto slots_of = [&](int i) -> int2 {
           int2 s = make_int2(kNoToken, kNoToken);
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
           if (!KV8 && !wait_free()) return false;
           const int2 s = make_int2(checked(sl.x), checked(sl.y));
           const Elem* from = static_cast<const Elem*>(item_is_key(i, n) ? p.k_cache : p.v_cache) + w.hk * p.kv_head_stride + ch * (16 / sizeof(Elem));
-#pragma unroll
+#pragma unroll 8
           for (int k = 0; k < kPart / kRowsPer; ++k) {
             const int row = k * kRowsPer + r0;
             const int rs = __shfl_sync(0xffffffffu, k * kRowsPer < 32 ? s.x : s.y, row & 31);
@@ -370,7 +371,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
           }
           cp_commit();
           sl = slots_of(i + C::kTeams);
+          // values of a tile that some rows do not see all of
+          const int col0 = first_token(p, r) + (w.t0 + item_tile(i, n)) * kTile;
+          const bool look = !item_is_key(i, n) && (col0 + kTile > r.prefix || col0 < edge);
+          bool found = false;
+          auto cleaned = [&](uint32_t two) -> uint32_t {       // elements that are no numbers: 0
+            constexpr uint32_t kExpo = kF16 ? 0x7c00u : 0x7f80u;
+            const uint32_t off = ((two & kExpo) == kExpo ? 0xffffu : 0u) | ((two & (kExpo << 16)) == (kExpo << 16) ? 0xffff0000u : 0u);
+            found = found || off != 0;
+            return two & ~off;
+          };
           cp_wait<0>();
+          if (!KV8 && look) {
+#pragma unroll 1
+            for (int k = 0; k < kPart / kRowsPer; ++k) {        // what this thread copied itself
+              const uint32_t at = stage + swz(k * kRowsPer + r0, ch, C::kBlock);
+              uint32_t x[4], y[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
+#pragma unroll
+              for (int h = 0; h < 4; ++h) y[h] = cleaned(x[h]);
+              if ((x[0] ^ y[0]) | (x[1] ^ y[1]) | (x[2] ^ y[2]) | (x[3] ^ y[3]))
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+            }
+          }
           if constexpr (KV8) {
             // a thread widens the bytes that it copied itself
             if (!wait_free()) return false;
@@ -381,19 +404,37 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
               const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
               return pack_bf16x2(f.x, f.y);
             };
-#pragma unroll 4
-            for (int k = 0; k < kPart / kRowsPer; ++k) {
-              const int row = part * kPart + k * kRowsPer + r0;
-              uint32_t x[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(raw + row * kD + ch * 16));
+            // four loads side by side, then their work
+            constexpr int kBatch = 4;
+            static_assert(kPart / kRowsPer % kBatch == 0, "batches of rows");
+#pragma unroll 1
+            for (int k0 = 0; k0 < kPart / kRowsPer; k0 += kBatch) {
+              uint32_t x[kBatch][4];
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + swz(row, ch * 2 + h, C::kBlock)), "r"(widen(x[2 * h])),
-                             "r"(widen(x[2 * h] >> 16)), "r"(widen(x[2 * h + 1])), "r"(widen(x[2 * h + 1] >> 16))
-                             : "memory");
+              for (int k = 0; k < kBatch; ++k) {
+                const int row = part * kPart + (k0 + k) * kRowsPer + r0;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(x[k][0]), "=r"(x[k][1]), "=r"(x[k][2]), "=r"(x[k][3])
+                             : "r"(raw + row * kD + ch * 16));
+              }
+#pragma unroll
+              for (int k = 0; k < kBatch; ++k) {
+                const int row = part * kPart + (k0 + k) * kRowsPer + r0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  uint32_t y[4] = {widen(x[k][2 * h]), widen(x[k][2 * h] >> 16), widen(x[k][2 * h + 1]), widen(x[k][2 * h + 1] >> 16)};
+                  if (look)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = cleaned(y[e]);
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + swz(row, ch * 2 + h, C::kBlock)), "r"(y[0]), "r"(y[1]),
+                               "r"(y[2]), "r"(y[3])
+                               : "memory");
+                }
+              }
             }
-            fence_proxy_async_smem();
           }
+          if (KV8 || look) fence_proxy_async_smem();
+          if (found) poison = 1;            // for the rest of the run: the rows' ends look for themselves
           __syncwarp();
           if (lane == 0) mbar_arrive(&full[st]);
         }
@@ -490,8 +531,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
     const int row_node = node_of(row);
     const bool capped = p.cap_out > 0.f;
     bool ok = true, bad = false;
-    uint32_t tile = 0, item = 0;
-    int job_rows = 0, job_row = 0, job_head = 0, job_c0 = 0, job_second = 0;
+    uint32_t tile = 0;
+    int job_rows = 0, job_row = 0, job_head = 0, job_tiles = 0;
     segments([&](const Place& w, const Request& r, int n_all, int n, bool first) {
       const int node = w.rt * p.tpt + row_node;
       const bool valid = row_node < p.tpt && node < r.nodes;
@@ -509,7 +550,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
       };
       if (masks) {        // parents to shared memory; one that is no earlier node counts as none
         asm volatile("bar.sync 1, 128;" ::: "memory");          // the segment before has read them
-        if (row == 0) poison = 0;
         for (int i = row; i < min(r.nodes, kParents); i += 128) parents[i] = static_cast<int16_t>(parent_in(i));
         asm volatile("bar.sync 1, 128;" ::: "memory");
       }
@@ -519,9 +559,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         for (int a = parent_of(node); a >= 0; a = parent_of(a)) ++pos;
         low = first_key(p, pos);
       }
-      // tiles below hold keys that some row may not see for the window's or chunk's sake
-      const int deepest = r.prefix + r.nodes - 1;
-      const int edge = p.window > 0 ? deepest - p.window + 1 : p.chunk > 0 ? deepest / p.chunk * p.chunk : 0;
+      const int edge = edge_of(p, r);
       // bit c: this row sees token col0 + c
       auto visible = [&](int col0) -> uint64_t {
         uint64_t m = 0;
@@ -530,10 +568,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         if (e > a) m = (e >= 64 ? ~0ull : (1ull << e) - 1) & (~0ull << a);
         if (col0 + kTile > r.prefix) {
           int at = pos;
-          for (int j = node; j >= 0 && at >= low; j = parent_of(j), --at) {
-            const int c = r.prefix + j - col0;
+          const int shift = r.prefix - col0;
+          auto see = [&](int j) {
+            const int c = shift + j;
             if (c >= 0 && c < kTile) m |= 1ull << c;
-            if (!bounded) at = low + 1;
+          };
+          if (!bounded && r.nodes <= kParents) {
+            for (int j = node; j >= 0; j = parents[j]) see(j);
+          } else {
+            for (int j = node; j >= 0 && at >= low; j = parent_of(j), --at) {
+              see(j);
+              if (!bounded) at = low + 1;
+            }
           }
         }
         return m;
@@ -548,38 +594,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         if (!mbar_wait(&s_full[buf], (at >> 1) & 1, &fail_flag)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) return ok = false;
         tc_fence_after_sync();
-        if (masked) {
-          // values that are no numbers: rows that do not see them must not meet them
-          const uint32_t it = item + value_item(t, n), st = it % kStages;
-          if (!mbar_wait(&full[st], (it / kStages) & 1, &fail_flag)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) return ok = false;
-          uint4* stage = reinterpret_cast<uint4*>(ring + st * C::kStage);
-          const uint32_t expo = kF16 ? 0x7c00u : 0x7f80u;
-          bool found = false;
-#pragma unroll 4
-          for (int i = row; i < C::kStage / 16; i += 128) {
-            uint4 v = stage[i];
-            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-            bool here = false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if ((x[k] & expo) == expo) {
-                x[k] &= 0xffff0000u;
-                here = true;
-              }
-              if ((x[k] & (expo << 16)) == (expo << 16)) {
-                x[k] &= 0xffffu;
-                here = true;
-              }
-            }
-            if (here) {
-              stage[i] = v;
-              found = true;
-            }
-          }
-          if (found) poison = 1;
-          fence_proxy_async_smem();
-        }
         if (warp_valid) {
           uint32_t raw[kTile];
           const uint32_t tmem_s = tmem + buf * kTile + lane_base;
@@ -647,7 +661,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         if (lane == 0) mbar_arrive(&p_full[buf]);
       }
       tile += n;
-      item += 2 * n;
       if (!mbar_wait(&o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1, &fail_flag)) ok = false;
       if (!__all_sync(0xffffffffu, ok)) return ok = false;
       tc_fence_after_sync();
@@ -721,16 +734,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         }
         if (!whole && valid) p.part_lse[slot * p.part_rows + row] = l == 0.f ? -INFINITY : m_used + log2f(l);
       }
-      if (row == 0 && !whole && w.t0 + n == n_all) {        // the unit's last tile (it began in front of this run)
-        const int64_t line = line_of[2], begin = line_of[0] - w.t0;
-        const int used = ctas_of;
+      if (!whole && w.t0 + n == n_all) {        // the unit's last tile: it began in front of this run
         job_rows = min(p.tpt, r.nodes - w.rt * p.tpt) * g;
         job_row = r.row + w.rt * p.tpt;
         job_head = w.hk * g;
-        // the last CTA whose run begins at or before the unit
-        job_c0 = line < 0xFFFFFFFFll / (used + 1) ? static_cast<int>((static_cast<uint32_t>(begin + 1) * used - 1u) / static_cast<uint32_t>(line))
-                                                  : static_cast<int>(((begin + 1) * used - 1) / line);
-        job_second = run_begin(line, job_c0, used) < begin ? 1 : 0;
+        job_tiles = w.t0;
       }
       tc_fence_before_sync();
       return true;
@@ -740,10 +748,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
     if (row == 0) {
       int* job = p.jobs + blockIdx.x * kJobInts;
       job[0] = ok ? job_rows : 0;
-      job[1] = job_row;
-      job[2] = job_head;
-      job[3] = job_c0;
-      job[4] = job_second;
+      if (ok && job_rows > 0) {
+        const int64_t line = line_of[2], begin = line_of[0] - job_tiles;
+        const int used = ctas_of;
+        // the last CTA whose run begins at or before the unit
+        const int c0 = line < 0xFFFFFFFFll / (used + 1) ? static_cast<int>((static_cast<uint32_t>(begin + 1) * used - 1u) / static_cast<uint32_t>(line))
+                                                        : static_cast<int>(((begin + 1) * used - 1) / line);
+        job[1] = job_row;
+        job[2] = job_head;
+        job[3] = c0;
+        job[4] = run_begin(line, c0, used) < begin ? 1 : 0;
+      }
     }
   }
 
