@@ -247,6 +247,7 @@ std::vector<Tensor> tree_speculative_sample(const Tensor& logits, const Tensor& 
   a.batch = static_cast<int>(batch);
   a.vocab = static_cast<int>(vocab);
   a.steps = static_cast<int>(steps);
+  a.num_sms = device_state(logits.get_device()).num_sms;
   const int rc = mb200::launch_tree_sample(a, stream_of(logits));
   TORCH_CHECK(rc == 0, "mllm_b200 tree_speculative_sample: unsupported configuration or launch failure (code ", rc, ")");
   return {path, out, counts};

@@ -90,7 +90,7 @@ struct TreeSampleArgs {
   int* counts;              // [batch]
   int* status;
   int64_t logit_stride, draft_stride;
-  int rows, batch, vocab, steps;
+  int rows, batch, vocab, steps, num_sms;
   DType dt;
 };
 int tree_sample_max_vocab(DType dt);

@@ -10,13 +10,14 @@
 //
 // What a step reads is known when the step before is done, so a walk is a chain: row, maximum, sum, cut, children, row.  A cluster of up
 // to 8 CTAs takes a request; each holds its part of the row in shared memory, and what they share goes through one exchange (a slot per
-// CTA, one cluster barrier) per stage.  The cut needs no sort of the row and no histogram: a lower bound on it (the smallest of the
-// warps' maxima for top-k, the mass that V tokens can hide below it for top-p, min_p itself) leaves a few hundred tokens, which every
-// CTA collects and sorts for itself.  Where more than kList are left (flat distributions) the cut is found bit by bit, an exchange each.
+// CTA, one cluster barrier) per stage.  The cut needs no sort of the row and no histogram: a lower bound on it (the k-th largest of the
+// warps' maxima for top-k, a level that holds the wanted mass for top-p, min_p itself) leaves a few tokens, which every CTA collects and
+// sorts for itself.  Where more than kList are left (flat distributions) the cut is closed in on, seven parts of its range an exchange.
 //
 // Whole tokens hang on sums: e is taken in 64 bits where it is above 2^-12 and sums are joined in 64 bits, so that the border of a token
 // is off by some 10^-9 of the whole.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tree.h"
@@ -28,6 +29,8 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kList = 4096;               // candidates that are sorted
 constexpr int kChildren = 64;             // of a node that are looked at
+constexpr int kMore = 6;                  // further sums of an exchange
+constexpr float kLevelStep = 2.f;         // first guesses at the cut: so much apart below the largest logit, in units of T
 
 struct SampleParams {
   const void* logits;
@@ -83,25 +86,45 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x);
   return x != x ? 0u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k); }
+// The same for values of T: numbers without the bits that T does not have, and back.
+template <typename T>
+struct Keys {
+  static constexpr int kDrop = std::is_same<T, __nv_bfloat16>::value ? 16 : std::is_same<T, __half>::value ? 13 : 0;
+  static __device__ __forceinline__ uint32_t of(float x) { return key_of(x) >> kDrop; }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    uint32_t u = k << kDrop;
+    if (u & 0x80000000u) return __uint_as_float(u & 0x7fffffffu);
+    return __uint_as_float(~(u | ((1u << kDrop) - 1)));
+  }
+};
 __device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
 
-// what the weight of a token is made of
+// The weight e of a token: above 2^-12 in 64 bits, below in 32.
 struct Scale {
   float mx, c_hi, c_lo;     // log2(e) / T as two floats
   double inv_t, mx_d;
+  __device__ __forceinline__ float log2_of(float x) const {
+    const float d = fmaxf(x - mx, -1e30f);      // a value that is no number, or minus infinity: no weight
+    return fmaf(d, c_hi, d * c_lo);
+  }
+  __device__ __forceinline__ double large(float x) const { return x == mx ? 1.0 : exp((static_cast<double>(x) - mx_d) * inv_t); }
   __device__ __forceinline__ double operator()(float x) const {
     if (!(x == x)) return 0.0;
-    if (x == mx) return 1.0;
-    const float d = x - mx, t = fmaf(d, c_hi, d * c_lo);
-    if (t > -12.f) return exp((static_cast<double>(x) - mx_d) * inv_t);
-    return static_cast<double>(fast_exp2(t));
+    const float t = log2_of(x);
+    return t > -12.f || x == mx ? large(x) : static_cast<double>(fast_exp2(t));
+  }
+  // adds it to a sum of two parts, for loops over all tokens
+  __device__ __forceinline__ void add(float x, double& big, float& small) const {
+    const float t = log2_of(x);
+    if (t > -12.f || x == mx) big += large(x);
+    else small += fast_exp2(t);
   }
 };
 
 struct Shared {
-  uint64_t slot[2][4];          // what this CTA tells the others, alternating
+  uint64_t slot[2][8];          // what this CTA tells the others, alternating
   double red[kWarps][2];
+  double red_more[kWarps][kMore];
   uint64_t red_key[kWarps];
   float red_min[kWarps];
   int list_n;
@@ -112,16 +135,20 @@ struct Shared {
   double child_w[kChildren];    // e of the token, 0 where it is filtered out
   double scale[kChildren];      // rejections so far: p <- p * scale - q
   int removed[kChildren];       // tokens taken out (candidates without probabilities)
-  int children, owner;
+  int children, owner, found;
   double scan[kWarps];
+  float group_max[kWarps];      // the warps' largest values, for the others
+  alignas(16) float all_max[kMaxCluster * kWarps];
+  float low;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 1) tree_sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ Shared sh;
   float* list = reinterpret_cast<float*>(dyn);              // this CTA's candidates
-  float* sorted = list + kList;                             // all candidates
+  float* gathered = list + kList;                           // all candidates
+  float* sorted = gathered + kList;
   T* xs = reinterpret_cast<T*>(sorted + kList);             // this CTA's part of the row
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
@@ -153,12 +180,22 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
     return;
   }
 
-  // Sums over the cluster, the same bits for every thread.
-  auto sum_all = [&](double& a, double& c) {
+  // Sums over the cluster, the same bits for every thread: two, and kMore others where `more` is given (lane i of every warp gets the i-th).
+  // `count`: a number of this CTA's (thread 0's counts), its sum in return.
+  auto sum_all = [&](double& a, double& c, double (*more)[kMore] = nullptr, int* count = nullptr) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       a += shfl_xor_d(a, o);
       c += shfl_xor_d(c, o);
+    }
+    if (more != nullptr) {
+#pragma unroll
+      for (int i = 0; i < kMore; ++i) {
+        double v = (*more)[i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += shfl_xor_d(v, o);
+        if (lane == 0) sh.red_more[warp][i] = v;
+      }
     }
     if (lane == 0) {
       sh.red[warp][0] = a;
@@ -176,6 +213,13 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
       if (lane == 0) {
         sh.slot[turn & 1][0] = static_cast<uint64_t>(__double_as_longlong(a));
         sh.slot[turn & 1][1] = static_cast<uint64_t>(__double_as_longlong(c));
+        if (count != nullptr) sh.slot[turn & 1][2 + kMore - 1] = static_cast<uint64_t>(*count);
+      }
+      if (more != nullptr && lane < kMore) {
+        double v = 0.0;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) v += sh.red_more[i][lane];
+        sh.slot[turn & 1][2 + lane] = static_cast<uint64_t>(__double_as_longlong(v));
       }
     }
     cluster_sync();
@@ -185,6 +229,18 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
       x = __longlong_as_double(static_cast<long long>(ld_cluster64(from)));
       y = __longlong_as_double(static_cast<long long>(ld_cluster64(from + 8)));
     }
+    if (more != nullptr) {
+      double v = 0.0;
+      if (lane < kMore) {
+        double from[kMaxCluster];
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxCluster; ++r)
+          from[r] = r < ranks ? __longlong_as_double(static_cast<long long>(ld_cluster64(at_rank(&sh.slot[turn & 1][2 + lane], r)))) : 0.0;
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxCluster; ++r) v += from[r];
+      }
+      (*more)[0] = v;
+    }
 #pragma unroll
     for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
       x += shfl_xor_d(x, o);
@@ -192,6 +248,10 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
     }
     a = __shfl_sync(0xffffffffu, x, 0);
     c = __shfl_sync(0xffffffffu, y, 0);
+    if (count != nullptr) {
+      int v = lane < static_cast<int>(ranks) ? static_cast<int>(ld_cluster64(at_rank(&sh.slot[turn & 1][2 + kMore - 1], lane))) : 0;
+      *count = __reduce_add_sync(0xffffffffu, v);
+    }
     ++turn;
   };
 
@@ -229,25 +289,29 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
         see(to_f32(xs[i]), i);
       }
     }
-    // groups of 32 lanes (or 8, for a larger k): that many tokens are at least as large as the smallest of their maxima
+    if (tid < 8 && n + tid < (n + 7) / 8 * 8) xs[n + tid] = from_f32<T>(-INFINITY);
+    // Groups of 32 lanes (or 8, for a larger k): that many tokens are at least as large as the smallest of their maxima, and k as the k-th
+    // largest.
     const bool by_warps = top_k <= static_cast<int>(ranks) * kWarps;
     float g_max = best;
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) g_max = fmaxf(g_max, __shfl_xor_sync(0xffffffffu, g_max, o));
-    if (by_warps) g_max = warp_max(g_max);
     float low = g_max;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+      g_max = fmaxf(g_max, __shfl_xor_sync(0xffffffffu, g_max, o));
       const uint64_t k = __shfl_xor_sync(0xffffffffu, top, o);
       top = k > top ? k : top;
     }
+    if (lane == 0) sh.group_max[warp] = g_max;
     if (lane == 0) {
       sh.red_key[warp] = top;
       sh.red_min[warp] = low;
     }
     if (tid == 0) {
       sh.list_n = 0;
+      sh.found = 0;
       sh.children = 0;
     }
     __syncthreads();
@@ -297,7 +361,27 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
       low = __shfl_sync(0xffffffffu, m, 0);
       ++turn;
     }
-    const float mx = of_key(static_cast<uint32_t>(top >> 32));
+    if (cut_k && by_warps && temp > 1e-6f) {
+      // up to 128 maxima: the one that k - 1 others precede
+      if (tid < kMaxCluster * kWarps)
+        sh.all_max[tid] = tid < static_cast<int>(ranks) * kWarps ? __uint_as_float(ld_cluster32(at_rank(&sh.group_max[tid % kWarps], tid / kWarps)))
+                                                                 : -INFINITY;
+      __syncthreads();
+      if (tid < kMaxCluster * kWarps) {
+        const float mine = sh.all_max[tid];
+        int before = 0;
+#pragma unroll 8
+        for (int j = 0; j < kMaxCluster * kWarps; j += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(sh.all_max + j);
+          before += (y.x > mine || (y.x == mine && j < tid)) + (y.y > mine || (y.y == mine && j + 1 < tid)) +
+                    (y.z > mine || (y.z == mine && j + 2 < tid)) + (y.w > mine || (y.w == mine && j + 3 < tid));
+        }
+        if (before == top_k - 1) sh.low = mine;
+      }
+      __syncthreads();
+      low = sh.low;
+    }
+    const float mx = Keys<float>::value(static_cast<uint32_t>(top >> 32));
     const int first_best = static_cast<int>(0xffffffffu - static_cast<uint32_t>(top));
     const int children = sh.children;
     // the children's numbers, read side by side
@@ -335,94 +419,189 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
     const double c = 1.4426950408889634 * w.inv_t;
     w.c_hi = static_cast<float>(c);
     w.c_lo = static_cast<float>(c - static_cast<double>(w.c_hi));
-    constexpr int kPair = sizeof(T) == 2 ? 2 : 1;
-    auto each = [&](auto&& fn) {             // fn(value, id within this part), ids far apart
-      if constexpr (kPair == 2) {
-        for (int i = tid; i < (n + 1) / 2; i += kThreads) {
-          const uint32_t two = reinterpret_cast<const uint32_t*>(xs)[i];
-          const T* e = reinterpret_cast<const T*>(&two);
-          fn(to_f32(e[0]), 2 * i);
-          if (2 * i + 1 < n) fn(to_f32(e[1]), 2 * i + 1);
-        }
+    const int groups = (n + 7) / 8;          // of eight tokens; minus infinity behind the last token
+    auto eight = [&](int i, float (&x)[8]) {
+      if constexpr (sizeof(T) == 2) {
+        const uint4 v = reinterpret_cast<const uint4*>(xs)[i];
+        const T* h = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = to_f32(h[k]);
       } else {
-        for (int i = tid; i < n; i += kThreads) fn(to_f32(xs[i]), i);
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) *reinterpret_cast<float4*>(x + k) = reinterpret_cast<const float4*>(xs)[2 * i + k / 4];
       }
     };
-    auto sum_over = [&](auto&& weight) {     // over the cluster
-      double big = 0.0, none = 0.0;
-      float small = 0.f;
-      each([&](float x, int i) {
-        const double v = weight(x, i);
-        if (v > 2.44140625e-4) big += v;
-        else small += static_cast<float>(v);
-      });
-      big += static_cast<double>(small);
-      sum_all(big, none);
-      return big;
+    // x >= bound (in 64 bits) for all x of 32: x >= the next float up
+    auto up = [](double v) { return __double2float_ru(v); };
+    // One way through this CTA's part, eight tokens at a time: a list of the tokens from `least` on, the weights of those from `from` on and
+    // of the listed ones (least >= from).
+    auto sweep = [&](bool summed, float from, bool listed, float least) {
+      double big = 0.0, in_list = 0.0;
+      float small[4] = {};
+      for (int i = tid; i < groups; i += kThreads) {
+        float x[8];
+        eight(i, x);
+        unsigned apart = 0;            // tokens with a large weight, and those for the list
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float t = w.log2_of(x[k]);
+          const bool special = (summed && t > -12.f) || (listed && x[k] >= least);
+          apart |= special ? 1u << k : 0u;
+          if (summed) small[k & 3] += x[k] >= from && !special ? fast_exp2(t) : 0.f;
+        }
+        while (apart != 0) {
+          const float v = to_f32(xs[8 * i + __ffs(apart) - 1]);
+          apart &= apart - 1;
+          if (listed && v >= least) {
+            const int at = atomicAdd(&sh.list_n, 1);
+            if (at < kList) list[at] = v;
+            if (summed) in_list += w(v);
+          } else if (v >= from) {
+            w.add(v, big, small[0]);
+          }
+        }
+      }
+      return make_double2(big + in_list + static_cast<double>((small[0] + small[1]) + (small[2] + small[3])), in_list);
+    };
+    auto sum_kept = [&](float from) {        // over the cluster
+      double a = sweep(true, from, false, 0.f).x, none = 0.0;
+      sum_all(a, none);
+      return a;
+    };
+    // below this, all tokens of the vocabulary together hold less than top_p leaves out (and a little, for the roundings)
+    auto surely_inside = [&](double total) {
+      const double share = fmax((1.0 - static_cast<double>(top_p)) * total / p.vocab, 1e-300);
+      return up(static_cast<double>(mx) + static_cast<double>(temp) * (log(share) - 1e-6)) - 1e-6f * fabsf(mx);
     };
 
     // ---- the cut: tokens from x_cut on are kept ----
-    double x_cut = -INFINITY, kept = 0.0;
-    if (min_p > 0.f) x_cut = static_cast<double>(mx) + static_cast<double>(temp) * log(static_cast<double>(fminf(min_p, 1.f)));
+    float x_cut = -INFINITY;
+    double kept = 0.0;
+    if (min_p > 0.f) x_cut = up(static_cast<double>(mx) + static_cast<double>(temp) * log(static_cast<double>(fminf(min_p, 1.f))));
     if (!cut_k && !cut_p) {
-      kept = sum_over([&](float x, int) { return static_cast<double>(x) >= x_cut ? w(x) : 0.0; });
+      kept = sum_kept(x_cut);
     } else {
-      const double total = cut_p ? sum_over([&](float x, int) { return w(x); }) : 0.0;
-      const double want = static_cast<double>(top_p) * total;
-      double bound = x_cut;
-      if (cut_k && top_k <= static_cast<int>(ranks) * (by_warps ? kWarps : 4 * kWarps)) bound = fmax(bound, static_cast<double>(low));
-      // below this, all tokens of the vocabulary together hold less than what top_p leaves out (and a little, for the roundings)
-      if (cut_p) bound = fmax(bound, static_cast<double>(mx) + static_cast<double>(temp) * (log(fmax((1.0 - static_cast<double>(top_p)) * total / p.vocab, 1e-300)) - 1e-6));
-      each([&](float x, int) {
-        if (static_cast<double>(x) >= bound) {
-          const int at = atomicAdd(&sh.list_n, 1);
-          if (at < kList) list[at] = x;
-        }
-      });
+      // Candidates: tokens from a bound on the cut upwards, listed on the way through the row that forms the sum.  For top_p the bound
+      // is a guess, 14 T below the largest logit.
+      float bound = x_cut;
+      if (cut_k && top_k <= static_cast<int>(ranks) * (by_warps ? kWarps : 4 * kWarps)) bound = fmaxf(bound, low);
+      const float from = fmaxf(bound, cut_p ? mx - (kMore + 1) * kLevelStep * temp : -INFINITY);
+      const double2 sums = sweep(cut_p, -INFINITY, true, from);
       __syncthreads();
-      if (tid == 0) sh.slot[turn & 1][0] = static_cast<uint64_t>(sh.list_n);
-      cluster_sync();
-      int have = 0;
-      if (lane < static_cast<int>(ranks)) have = static_cast<int>(min(ld_cluster64(at_rank(&sh.slot[turn & 1][0], lane)), static_cast<uint64_t>(1) << 30));
-      int upto = have;          // candidates of the ranks up to this lane's
+      double total = sums.x, mass = sums.y;
+      int listed = sh.list_n > kList ? 1 << 24 : sh.list_n;
+      int told = turn;            // the exchange that says how long the lists are
+      sum_all(total, mass, nullptr, &listed);
+      const double want = static_cast<double>(top_p) * total;
+      bool have = listed <= kList;
+      if (cut_p && have && listed <= 2 * kThreads && mass >= want) {
+        bound = from;
+      } else if (cut_p) {
+        // the mass above some levels: the highest that holds what top_p wants is a better bound
+        double above[kMore] = {}, none = 0.0, none2 = 0.0;
+        for (int i = tid; i < min(sh.list_n, kList); i += kThreads) {
+          const float x = list[i];
+          const double v = w(x);
 #pragma unroll
-      for (int o = 1; o < kMaxCluster; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto = min(upto + v, 1 << 30);
-      }
-      const int m = __shfl_sync(0xffffffffu, upto, static_cast<int>(ranks) - 1);
-      ++turn;
-      if (m <= kList) {
-        // every CTA sorts all candidates, largest first
-        int size = 32;
-        while (size < m) size <<= 1;
-        int at = 0;
-        for (uint32_t r = 0; r < ranks; ++r) {
-          const int c_n = __shfl_sync(0xffffffffu, have, r);
-          const uint32_t from = at_rank(list, r);
-          for (int i = tid; i < c_n; i += kThreads) sorted[at + i] = __uint_as_float(ld_cluster32(from + 4 * i));
-          at += c_n;
+          for (int l = 0; l < kMore; ++l)
+            if (x >= mx - (l + 1) * kLevelStep * temp) above[l] += v;
         }
-        for (int i = m + tid; i < size; i += kThreads) sorted[i] = -INFINITY;
+        sum_all(none, none2, &above);
+        const unsigned enough = __ballot_sync(0xffffffffu, lane < kMore && above[0] >= want);
+        if (enough != 0) {
+          bound = fmaxf(bound, mx - __ffs(enough) * kLevelStep * temp);
+        } else if (have && mass >= want) {
+          bound = from;
+        } else {
+          bound = fmaxf(bound, surely_inside(total));
+          have = have && bound >= from;
+        }
+      }
+      int m = 0;
+      if (!have) {            // once more, from the better bound
         __syncthreads();
-        for (int span = 2; span <= size; span <<= 1) {
-          for (int step = span >> 1; step > 0; step >>= 1) {
-            for (int i = tid; i < size / 2; i += kThreads) {
-              const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-              const float a = sorted[lo], c2 = sorted[hi];
-              const bool down = (lo & span) == 0;
-              if (down ? a < c2 : a > c2) {
-                sorted[lo] = c2;
-                sorted[hi] = a;
-              }
+        if (tid == 0) sh.list_n = 0;
+        __syncthreads();
+        sweep(false, 0.f, true, bound);
+        __syncthreads();
+        double none = 0.0, none2 = 0.0;
+        int all = sh.list_n > kList ? 1 << 24 : sh.list_n;
+        told = turn;
+        sum_all(none, none2, nullptr, &all);
+        have = all <= kList;
+      }
+      if (have) {
+        // every CTA gathers all candidates from the bound on; how many each has was told with the sums
+        int upto = 0;
+        if (lane < static_cast<int>(ranks)) upto = static_cast<int>(ld_cluster64(at_rank(&sh.slot[told & 1][2 + kMore - 1], lane)));
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const int everything = __shfl_sync(0xffffffffu, upto, static_cast<int>(ranks) - 1);
+        for (int i0 = warp * 32; i0 < everything; i0 += kThreads) {
+          const int i = i0 + lane;
+          int r = 0, front = 0;
+          for (uint32_t q = 0; q + 1 < ranks; ++q) {
+            const int end = __shfl_sync(0xffffffffu, upto, q);
+            if (i >= end) {
+              r = q + 1;
+              front = end;
             }
-            __syncthreads();
+          }
+          const float x = i < everything ? __uint_as_float(ld_cluster32(at_rank(list, r) + 4 * (i - front))) : -INFINITY;
+          const bool in = i < everything && x >= bound;
+          const unsigned votes = __ballot_sync(0xffffffffu, in);
+          int at = 0;
+          if (lane == 0 && votes != 0) at = atomicAdd(&sh.found, __popc(votes));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(votes & ((1u << lane) - 1));
+          if (in) gathered[at] = x;
+        }
+        __syncthreads();
+        m = sh.found;
+        // ---- largest first ----
+        if (m <= 2 * kThreads) {
+          // an element's place is the number of those in front of it
+          for (int i = m + tid; i < (m + 3) / 4 * 4; i += kThreads) gathered[i] = -INFINITY;
+          __syncthreads();
+          for (int i = tid; i < m; i += kThreads) {
+            const float x = gathered[i];
+            int place = 0;
+            for (int j = 0; j < m; j += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(gathered + j);
+              place += (y.x > x || (y.x == x && j < i)) + (y.y > x || (y.y == x && j + 1 < i)) + (y.z > x || (y.z == x && j + 2 < i)) +
+                       (y.w > x || (y.w == x && j + 3 < i));
+            }
+            sorted[place] = x;
+          }
+          __syncthreads();
+        } else {
+          int size = 2 * kThreads;
+          while (size < m) size <<= 1;
+          for (int i = tid; i < size; i += kThreads) sorted[i] = i < m ? gathered[i] : -INFINITY;
+          __syncthreads();
+          for (int span = 2; span <= size; span <<= 1) {
+            for (int step = span >> 1; step > 0; step >>= 1) {
+              for (int i = tid; i < size / 2; i += kThreads) {
+                const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+                const float a = sorted[lo], c2 = sorted[hi];
+                const bool down = (lo & span) == 0;
+                if (down ? a < c2 : a > c2) {
+                  sorted[lo] = c2;
+                  sorted[hi] = a;
+                }
+              }
+              __syncthreads();
+            }
           }
         }
-        // running mass, largest first: a thread has m / kThreads neighbours
+        // running mass: a thread has m / kThreads neighbours
         const int per = (m + kThreads - 1) / kThreads, i0 = min(m, tid * per), i1 = min(m, i0 + per);
+        const double w0 = i0 < i1 ? w(sorted[i0]) : 0.0;
+        auto weight_at = [&](int i) { return i == i0 ? w0 : w(sorted[i]); };
         double mine = 0.0;
-        for (int i = i0; i < i1; ++i) mine += w(sorted[i]);
+        for (int i = i0; i < i1; ++i) mine += weight_at(i);
         double incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -432,64 +611,117 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
         if (lane == 31) sh.scan[warp] = incl;
         if (tid == 0) sh.owner = 0;
         __syncthreads();
-        double before = incl - mine;
-        for (int i = 0; i < warp; ++i) before += sh.scan[i];
         if (cut_p) {            // tokens with less than `want` in front of them are inside
+          double run = incl - mine;
+          for (int i = 0; i < warp; ++i) run += sh.scan[i];
           int inside = 0;
-          double run = before;
           for (int i = i0; i < i1; ++i) {
             if (run < want) inside = i + 1;
-            run += w(sorted[i]);
+            run += weight_at(i);
           }
-          if (inside > 0) atomicMax(&sh.owner, inside);
+          inside = __reduce_max_sync(0xffffffffu, inside);
+          if (lane == 0 && inside > 0) atomicMax(&sh.owner, inside);
+          __syncthreads();
         }
-        __syncthreads();
         // fewer candidates (less mass) than asked for: the other filter's bound was higher, and so is its cut
-        if (cut_k && top_k <= m) x_cut = fmax(x_cut, static_cast<double>(sorted[top_k - 1]));
-        const int inside = max(sh.owner, 1);
-        if (cut_p && m > 0) x_cut = fmax(x_cut, static_cast<double>(sorted[min(inside, m) - 1]));
-        double sum = 0.0, none = 0.0;
-        for (int i = i0; i < i1; ++i) sum += static_cast<double>(sorted[i]) >= x_cut ? w(sorted[i]) : 0.0;
+        if (cut_k && top_k <= m) x_cut = fmaxf(x_cut, sorted[top_k - 1]);
+        if (cut_p && m > 0) x_cut = fmaxf(x_cut, sorted[min(max(sh.owner, 1), m) - 1]);
+        double sum = 0.0;
+        for (int i = i0; i < i1; ++i) sum += sorted[i] >= x_cut ? weight_at(i) : 0.0;
         // the same sums in every CTA: no exchange
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += shfl_xor_d(sum, o);
         if (lane == 0) sh.red[warp][0] = sum;
         __syncthreads();
-        for (int i = 0; i < kWarps; ++i) none += sh.red[i][0];
-        kept = none;
+        for (int i = 0; i < kWarps; ++i) kept += sh.red[i][0];
         __syncthreads();
       } else {
-        // flat rows: the largest key with k tokens (with the wanted mass) at or above it, bit by bit
-        uint32_t at_k = 0, at_p = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-          const uint32_t try_k = at_k | 1u << bit, try_p = at_p | 1u << bit;
-          double tokens = 0.0, mass = 0.0;
-          float small = 0.f;
-          each([&](float x, int) {
-            const uint32_t k = key_of(x);
-            if (cut_k && k >= try_k) tokens += 1.0;
-            if (cut_p && k >= try_p) {
-              const double v = w(x);
-              if (v > 2.44140625e-4) mass += v;
-              else small += static_cast<float>(v);
+        // Flat rows: the largest value with k tokens (with the wanted mass) at or above it, among the type's values between the bound and
+        // the largest logit; six of them a sweep and an exchange.
+        auto largest = [&](bool by_mass, double goal) {
+          uint32_t at = Keys<T>::of(bound), span = Keys<T>::of(mx) + 1 - at;
+          while (span > 1) {
+            const uint32_t step = (span + kMore) / (kMore + 1);
+            float test[kMore], small[kMore] = {};
+            double sums[kMore] = {}, none = 0.0, none2 = 0.0;
+#pragma unroll
+            for (int j = 0; j < kMore; ++j) test[j] = (j + 1) * step < span ? Keys<T>::value(at + (j + 1) * step) : INFINITY;
+            for (int i = tid; i < groups; i += kThreads) {
+              float x[8], x_top = -INFINITY;
+              eight(i, x);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x_top = fmaxf(x_top, x[k]);
+              if (!(x_top >= test[0])) continue;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float lg = w.log2_of(x[k]);
+                if (by_mass && lg > -12.f) {
+                  const double v = w.large(x[k]);
+#pragma unroll
+                  for (int j = 0; j < kMore; ++j) sums[j] += x[k] >= test[j] ? v : 0.0;
+                } else {
+                  const float v = by_mass ? fast_exp2(lg) : 1.f;
+#pragma unroll
+                  for (int j = 0; j < kMore; ++j) small[j] += x[k] >= test[j] ? v : 0.f;
+                }
+              }
             }
-          });
-          mass += static_cast<double>(small);
-          sum_all(tokens, mass);
-          if (cut_k && tokens >= static_cast<double>(top_k)) at_k = try_k;
-          if (cut_p && mass >= want && mass > 0.0) at_p = try_p;
-        }
-        if (cut_k && at_k != 0) x_cut = fmax(x_cut, static_cast<double>(of_key(at_k)));
-        if (cut_p && at_p != 0) x_cut = fmax(x_cut, static_cast<double>(of_key(at_p)));
-        kept = sum_over([&](float x, int) { return static_cast<double>(x) >= x_cut ? w(x) : 0.0; });
+#pragma unroll
+            for (int j = 0; j < kMore; ++j) sums[j] += static_cast<double>(small[j]);
+            sum_all(none, none2, &sums);
+            const uint32_t steps = __popc(__ballot_sync(0xffffffffu, lane < kMore && sums[0] >= goal && sums[0] > 0.0));
+            at += steps * step;
+            span = min(step, span - steps * step);
+          }
+          return Keys<T>::value(at);
+        };
+        if (cut_k) x_cut = fmaxf(x_cut, largest(false, static_cast<double>(top_k)));
+        if (cut_p) x_cut = fmaxf(x_cut, largest(true, want));
+        kept = sum_kept(x_cut);
       }
     }
+
+    // What eight kept tokens have left after k rejections (with probabilities), added to `sum`.  In 64 bits where the weight or the
+    // draft's probability is above 2^-12.
+    const float* draft = p.draft != nullptr ? p.draft + row * p.draft_stride + v0 : nullptr;
+    const bool wide = (reinterpret_cast<uintptr_t>(draft) & 15) == 0;
+    auto left_of_eight = [&](int g, int k, double& sum) {
+      float x[8], x_top = -INFINITY;
+      eight(g, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x_top = fmaxf(x_top, x[e]);
+      if (!(x_top >= x_cut) || x_top == -INFINITY) return;
+      float q[8];
+      if (wide && 8 * g + 8 <= n) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4*>(q + e) = __ldcg(reinterpret_cast<const float4*>(draft + 8 * g + e));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = 8 * g + e < n ? __ldcg(draft + 8 * g + e) : 0.f;
+      }
+      float small = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!(x[e] >= x_cut)) continue;
+        const float t = w.log2_of(x[e]);
+        if (t > -12.f || q[e] > 2.44140625e-4f) {
+          double v = w(x[e]);
+          for (int j = 0; j < k && v > 0.0; ++j) v = fmax(v * sh.scale[j] - q[e], 0.0);
+          sum += v;
+        } else {
+          float v = fast_exp2(t);
+          for (int j = 0; j < k && v > 0.f; ++j) v = fmaxf(fmaf(v, static_cast<float>(sh.scale[j]), -q[e]), 0.f);
+          small += v;
+        }
+      }
+      sum += static_cast<double>(small);
+    };
 
     // ---- the children in turn ----
     __syncthreads();
     if (tid < children) {
       const float x = static_cast<float>(sh.child_w[tid]);
-      sh.child_w[tid] = sh.child_token[tid] >= 0 && static_cast<double>(x) >= x_cut ? w(x) : 0.0;
+      sh.child_w[tid] = sh.child_token[tid] >= 0 && x >= x_cut ? w(x) : 0.0;
     }
     __syncthreads();
     int rejected = 0;           // rejections that changed p (with probabilities), or tokens taken out
@@ -512,7 +744,6 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
         }
       }
     } else {
-      const float* draft = p.draft + row * p.draft_stride;
       // p after k rejections, of the token with weight v and draft probability q
       auto left = [&](double v, double q, int k) {
         for (int j = 0; j < k && v > 0.0; ++j) v = fmax(v * sh.scale[j] - q, 0.0);
@@ -527,16 +758,14 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
         }
         if (sh.child_token[i] < 0) continue;
         const double scale = 1.0 / mass;
-        const double rest = sum_over([&](float x, int id) {
-          if (!(static_cast<double>(x) >= x_cut)) return 0.0;
-          const double q_id = __ldcg(draft + v0 + id);
-          return fmax(left(w(x), q_id, rejected) * scale - q_id, 0.0);
-        });
+        if (tid == 0) sh.scale[rejected] = scale;
+        __syncthreads();
+        double rest = 0.0, none = 0.0;
+        for (int g = tid; g < groups; g += kThreads) left_of_eight(g, rejected + 1, rest);
+        sum_all(rest, none);
         if (rest > 0.0) {
-          if (tid == 0) sh.scale[rejected] = scale;
           ++rejected;
           mass = rest;
-          __syncthreads();
         }
       }
     }
@@ -552,10 +781,9 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
 
     // ---- the walk's last token: the first whose running sum passes u times all ----
     {
-      const float* draft = p.draft != nullptr ? p.draft + row * p.draft_stride + v0 : nullptr;
       auto weight = [&](int i) {
         const float x = to_f32(xs[i]);
-        if (!(static_cast<double>(x) >= x_cut)) return 0.0;
+        if (!(x >= x_cut)) return 0.0;
         double v = w(x);
         if (draft != nullptr) {
           if (rejected > 0) {
@@ -568,15 +796,25 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
         }
         return v;
       };
-      const int per = (n + kThreads - 1) / kThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+      // neighbouring tokens, a thread's share of them
+      const int per = (groups + kThreads - 1) / kThreads, g0 = min(groups, tid * per), g1 = min(groups, g0 + per);
+      const int i0 = g0 * 8, i1 = min(n, g1 * 8);
       double mine = 0.0;
-      {
-        float small = 0.f;
-        for (int i = i0; i < i1; ++i) {
-          const double v = weight(i);
-          if (v > 2.44140625e-4) mine += v;
-          else small += static_cast<float>(v);
+      for (int g = g0; g < g1; ++g) {
+        if (draft != nullptr && rejected > 0) {
+          left_of_eight(g, rejected, mine);
+          continue;
         }
+        float x[8], small = 0.f;
+        eight(g, x);
+        unsigned out = 0;       // candidates that were taken out
+        for (int k = 0; k < rejected; ++k) {
+          const int d = sh.removed[k] - v0 - 8 * g;
+          out |= d >= 0 && d < 8 ? 1u << d : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (x[e] >= x_cut && !((out >> e) & 1)) w.add(x[e], mine, small);
         mine += static_cast<double>(small);
       }
       double incl = mine;
@@ -649,7 +887,7 @@ __global__ void __launch_bounds__(kThreads) tree_sample_kernel(const SampleParam
 template <typename T>
 int launch_type(const SampleParams& p, int cluster, int batch, cudaStream_t s) {
   auto kernel = tree_sample_kernel<T>;
-  const int smem = 2 * kList * 4 + p.chunk * static_cast<int>(sizeof(T));
+  const int smem = 3 * kList * 4 + p.chunk * static_cast<int>(sizeof(T));
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem) != cudaSuccess) return -3;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(cluster * batch));
@@ -673,7 +911,7 @@ int launch_type(const SampleParams& p, int cluster, int batch, cudaStream_t s) {
 }  // namespace
 
 // Bytes of shared memory that a CTA may use for its part of a row: 227 KB less the candidates and the kernel's variables.
-constexpr int kPartBytes = 184 * 1024;
+constexpr int kPartBytes = 168 * 1024;
 
 int tree_sample_max_vocab(DType dt) { return kMaxCluster * (kPartBytes / (dt == kF32 ? 4 : 2)); }
 
@@ -702,10 +940,11 @@ int launch_tree_sample(const TreeSampleArgs& a, cudaStream_t s) {
   p.rows = a.rows;
   p.vocab = a.vocab;
   p.steps = a.steps;
-  // CTAs per request: about 16384 tokens each
+  // CTAs per request: about 16384 tokens each, fewer CTAs where there are more requests than places for them (one CTA per SM)
+  const int item = a.dt == kF32 ? 4 : 2;
   int cluster = 1;
   while (cluster < kMaxCluster && cluster * 16384 < a.vocab) cluster *= 2;
-  const int item = a.dt == kF32 ? 4 : 2;
+  while (cluster > 1 && cluster * a.batch > a.num_sms && (a.vocab / (cluster / 2) + 8) * item <= kPartBytes) cluster /= 2;
   p.chunk = ((a.vocab + cluster - 1) / cluster + 7) / 8 * 8;
   if (p.chunk * item > kPartBytes) return -1;
   p.vec = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.logit_stride * item % 16 == 0 ? 1 : 0;
