@@ -24,10 +24,15 @@ import torch
 from . import reference as ref
 
 
-def _ops():
-    from .. import ops
+_front = None
 
-    return ops
+
+def _ops():
+    """The package that this module is part of; it is not complete while this one is imported."""
+    global _front
+    if _front is None:
+        from .. import ops as _front
+    return _front
 
 
 def _check_index(what: str, rows: int, device, req_to_token, parents, *per_request) -> None:
@@ -55,6 +60,11 @@ def tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, parents, req_to_token, r
     the first ``2 * inv_freq.numel()`` features turn (feature i with the one half of them on) by ``inv_freq`` (fp32) times the node's
     position: cached tokens, ancestors, and ``position_delta`` [requests] int32 where text positions do not count from 0.  Heads of 64, 128
     and 256 features on the GPU, a multiple of 16 of them rotated.  ``qkv`` is left as it is; results are rounded once."""
+    args = (parents, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, inv_freq, k_cache, v_cache, num_q_heads, num_kv_heads,
+            head_dim, float(eps), position_delta)
+    ops = _ops()
+    if ops.use_kernels(qkv):        # the binding makes the same checks
+        return ops.ext().tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, *args)
     what = "tree_qk_norm_rope_kv_write"
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (num_q_heads + 2 * num_kv_heads) * head_dim:
         raise ValueError(f"{what}: qkv must be [T, {(num_q_heads + 2 * num_kv_heads) * head_dim}] with unit inner stride")
@@ -66,12 +76,7 @@ def tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, parents, req_to_token, r
     for w in (q_weight, k_weight):
         if w is not None and (w.shape != (head_dim,) or w.dtype != qkv.dtype or w.device != qkv.device):
             raise ValueError(f"{what}: weights must be vectors of {head_dim} like qkv")
-    ops = _ops()
-    args = (parents, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, inv_freq, k_cache, v_cache, num_q_heads, num_kv_heads,
-            head_dim, float(eps), position_delta)
-    if not ops.use_kernels(qkv):
-        return ref.tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, *args)
-    return ops.ext().tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, *args)
+    return ref.tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, *args)
 
 
 def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents, scale: float,
@@ -81,6 +86,10 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
     ``window``, ``logit_cap``, ``sink`` and ``chunk`` as for :func:`mllm_b200.ops.attention_prefill`, by positions: siblings share theirs.
     Heads of 64, 128 and 256 features, 16-bit, over caches of their type or of unscaled 8-bit floats.  Rows of ``out`` that belong to no
     request keep what they hold.  A value in the cache that is no number reaches the nodes that see it and no others."""
+    ops = _ops()
+    if ops.use_kernels(q):          # the binding makes the same checks
+        return ops.ext().attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents,
+                                        float(scale), out, int(window or 0), float(logit_cap or 0.0), sink, int(chunk or 0))
     if q.dim() != 3 or k_cache.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
         raise ValueError("attention_tree: q must be [T, heads, features] with the heads of a node contiguous")
     hkv = k_cache.shape[1]
@@ -95,15 +104,8 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1
                             or out.stride(1) != out.shape[2]):
         raise ValueError("attention_tree: out must be like q, with the heads of a node contiguous")
-    ops = _ops()
-    if not ops.use_kernels(q):
-        return ref.attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents, scale, out,
-                                  window, logit_cap, sink, chunk)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ops.ext().attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents, float(scale), out,
-                             int(window or 0), float(logit_cap or 0.0), None if sink is None else sink.contiguous(), int(chunk or 0))
-    return out
+    return ref.attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents, scale, out,
+                              window, logit_cap, sink, chunk)
 
 
 def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, temperature, top_k, top_p, min_p, uniform, uniform_final,
@@ -122,6 +124,13 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
 
     Returns ``path`` [requests, max_steps] int32, the nodes of the walk from node 0 on (whose cache rows are now valid), ``tokens``
     [requests, max_steps] int64, the emitted tokens (those of ``path[:, 1:]`` and one more), both -1 behind ``counts`` [requests] int32."""
+    ops = _ops()
+    if ops.use_kernels(logits):     # the binding makes the same checks
+        f32 = lambda x: x if x is None or x.dtype == torch.float32 else x.float()  # noqa: E731
+        if top_k.dtype != torch.int32:
+            top_k = top_k.to(torch.int32)
+        return ops.ext().tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, f32(temperature), top_k, f32(top_p), f32(min_p),
+                                                 f32(uniform), f32(uniform_final), int(max_steps), draft_probs)
     what = "tree_speculative_sample"
     if logits.dim() != 2 or logits.stride(1) != 1 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError(f"{what}: logits must be [T, vocab] in 16 or 32 bits with unit inner stride")
@@ -139,14 +148,8 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
         raise ValueError(f"{what}: draft_probs must be fp32 [T, vocab] like logits, with unit inner stride")
     if max_steps < 1 or logits.shape[1] < 1:
         raise ValueError(f"{what}: max_steps and the vocabulary must be at least 1")
-    ops = _ops()
-    if not ops.use_kernels(logits):
-        return ref.tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, temperature, top_k, top_p, min_p, uniform,
-                                           uniform_final, max_steps, draft_probs)
-    f32 = lambda t: None if t is None else t.float().contiguous()  # noqa: E731
-    return tuple(ops.ext().tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, f32(temperature),
-                                                   top_k.to(torch.int32).contiguous(), f32(top_p), f32(min_p), f32(uniform),
-                                                   f32(uniform_final), int(max_steps), draft_probs))
+    return ref.tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, temperature, top_k, top_p, min_p, uniform, uniform_final,
+                                       max_steps, draft_probs)
 
 
 def tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts) -> None:
@@ -154,6 +157,9 @@ def tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, co
     storage of all layers): for i below ``counts[b]``, what node ``path[b, i]`` of request b has in its slot goes to the slot of node i.
     ``path`` [requests, steps] and ``counts`` [requests] are those of :func:`tree_speculative_sample`: a path rises from node 0 on, what
     stands behind ``counts`` is not read.  The request then holds ``prefix_lens + counts`` tokens."""
+    ops = _ops()
+    if ops.use_kernels(store):      # the binding makes the same checks
+        return ops.ext().tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts)
     what = "tree_kv_compact"
     if store.dim() < 2 or not store.is_contiguous() or store.shape[-1] * store.element_size() % 16:
         raise ValueError(f"{what}: store must be contiguous [.., slots, features] with rows of a multiple of 16 bytes")
@@ -162,7 +168,4 @@ def tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, co
         raise ValueError(f"{what}: path must be a contiguous int32 tensor [{counts.numel()}, steps] on {store.device}")
     if counts.numel() != req_pool_indices.numel():
         raise ValueError(f"{what}: counts must have one number per request")
-    ops = _ops()
-    if not ops.use_kernels(store):
-        return ref.tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts)
-    ops.ext().tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts)
+    ref.tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts)
