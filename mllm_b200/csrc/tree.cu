@@ -33,6 +33,7 @@ struct PrologueParams {
 template <typename T, int D>
 __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams p) {
   constexpr int V = 8, kLanes = D / V, kHeads = 32 / kLanes, kFreq = D / 64;      // frequencies of a lane
+  constexpr int kSteps = 4;
   pdl_launch_dependents();
   pdl_wait_loads();
   const int64_t warp = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
@@ -40,10 +41,24 @@ __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams
   const int t = static_cast<int>(warp / p.hsplit), part = static_cast<int>(warp - static_cast<int64_t>(t) * p.hsplit);
   const int lane = lane_id(), l = lane % kLanes;
   const int heads = p.hq + 2 * p.hkv, step = p.hsplit * kHeads;
-  int h = part * kHeads + lane / kLanes;
   const T* row = static_cast<const T*>(p.qkv) + t * p.qkv_stride + l * V;
-  uint4 next{};
-  if (h < heads) next = __ldcg(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D));
+  // four steps' heads at a time, those of the next four on their way meanwhile
+  uint4 next[kSteps];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const int h = h0 + k * step + lane / kLanes;
+      next[k] = h < heads ? __ldcg(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  fetch(part * kHeads);
+  const int at = l * V;                                     // the lane's first feature
+  float freq[kFreq];          // lane i has those of pairs i, i + 32, ..
+#pragma unroll
+  for (int i = 0; i < kFreq; ++i) freq[i] = lane + 32 * i < p.half ? __ldcg(p.inv_freq + lane + 32 * i) : 0.f;
+  uint4 gains[2]{};           // of queries and of keys
+  if (p.q_gain != nullptr) gains[0] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q_gain) + at));
+  if (p.k_gain != nullptr) gains[1] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_gain) + at));
 
   // ---- whose node ----
   int b = -1;
@@ -97,22 +112,15 @@ __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams
   }
   if ((!slot_ok || !tree_ok) && part == 0 && lane == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
 
-  // ---- sines and cosines: lane i has those of frequencies i, i + 32, .. ----
+  // ---- sines and cosines of the part of a turn that is left of pos * freq, in half turns ----
   float c[kFreq], s[kFreq];
   const double pos = static_cast<double>(r.prefix) + depth + delta;
 #pragma unroll
   for (int i = 0; i < kFreq; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
-    const int f = lane + 32 * i;
-    if (f < p.half) {
-      const double angle = pos * static_cast<double>(__ldcg(p.inv_freq + f));
-      const double turns = rint(angle * 0.15915494309189535);         // 1 / (2 pi)
-      sincosf(static_cast<float>(fma(turns, -6.283185307179586, angle)), &s[i], &c[i]);
-    }
+    const double angle = pos * static_cast<double>(freq[i]) * 0.15915494309189535;         // in turns: 1 / (2 pi)
+    sincospif(2.f * static_cast<float>(angle - rint(angle)), &s[i], &c[i]);
   }
   float cs[V], sn[V];
-  const int at = l * V;                                     // the lane's first feature
   const bool turns = at < 2 * p.half, second = at >= p.half;
   const int f0 = second ? at - p.half : at;
 #pragma unroll
@@ -129,53 +137,56 @@ __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams
     }
   }
   const int partner = turns ? (second ? lane - p.half / V : lane + p.half / V) : lane;
-  float gq[V], gk[V];
+  for (int first = part * kHeads; first < heads; first += kSteps * step) {
+    uint4 now[kSteps];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    gq[i] = p.q_gain != nullptr ? to_f32(static_cast<const T*>(p.q_gain)[at + i]) : 1.f;
-    gk[i] = p.k_gain != nullptr ? to_f32(static_cast<const T*>(p.k_gain)[at + i]) : 1.f;
-  }
-
-  for (int h0 = part * kHeads; h0 < heads; h0 += step, h += step) {
-    uint4 raw = next;
-    if (h + step < heads) next = __ldcg(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h + step) * D));
-    const bool is_q = h < p.hq, is_k = !is_q && h < p.hq + p.hkv;
-    T* e = reinterpret_cast<T*>(&raw);
-    float y[V];
+    for (int k = 0; k < kSteps; ++k) now[k] = next[k];
+    if (first + kSteps * step < heads) fetch(first + kSteps * step);
 #pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = to_f32(e[i]);
-    if (h0 < p.hq + p.hkv) {             // the warp has a head to norm and turn
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) ss += y[i] * y[i];
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const bool normed = (is_q ? p.q_gain : p.k_gain) != nullptr && (is_q || is_k);
-      const float rstd = normed ? rsqrtf(ss / static_cast<float>(D) + p.eps) : 1.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float x = normed ? y[i] * rstd * (is_q ? gq[i] : gk[i]) : y[i];
-        const float other = __shfl_sync(0xffffffffu, x, partner);
-        if (is_q || is_k) y[i] = turns ? x * cs[i] + other * sn[i] : x;
+    for (int k = 0; k < kSteps; ++k) {
+      const int h0 = first + k * step, h = h0 + lane / kLanes;
+      if (h0 >= heads) break;
+      uint4 raw = now[k];
+      const bool is_q = h < p.hq, is_k = !is_q && h < p.hq + p.hkv;
+      T* e = reinterpret_cast<T*>(&raw);
+      float y[V];
+  #pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = to_f32(e[i]);
+      if (h0 < p.hq + p.hkv) {             // the warp has a head to norm and turn
+        float ss = 0.f;
+  #pragma unroll
+        for (int i = 0; i < V; ++i) ss += y[i] * y[i];
+  #pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const bool normed = (is_q ? p.q_gain : p.k_gain) != nullptr && (is_q || is_k);
+        const uint4 gain = is_q ? gains[0] : gains[1];
+        const T* g = reinterpret_cast<const T*>(&gain);
+        const float rstd = normed ? rsqrtf(ss / static_cast<float>(D) + p.eps) : 1.f;
+  #pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float x = normed ? y[i] * rstd * to_f32(g[i]) : y[i];
+          const float other = __shfl_sync(0xffffffffu, x, partner);
+          if (is_q || is_k) y[i] = turns ? x * cs[i] + other * sn[i] : x;
+        }
       }
-    }
-    if (is_q) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) e[i] = from_f32<T>(y[i]);
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.hq + h) * D + at) = raw;
-    } else if (h < heads && slot_ok) {
-      void* cache = is_k ? p.k_cache : p.v_cache;
-      const int kvh = is_k ? h - p.hq : h - p.hq - p.hkv;
-      const int64_t to = slot * p.kv_tok_stride + kvh * p.kv_head_stride + at;
-      if (p.kv_fmt == kKvSame) {
-#pragma unroll
+      if (is_q) {
+  #pragma unroll
         for (int i = 0; i < V; ++i) e[i] = from_f32<T>(y[i]);
-        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + to) = raw;
-      } else {
-        uint2 o;
-        o.x = pack_fp8x2(y[0], y[1], p.kv_fmt) | (pack_fp8x2(y[2], y[3], p.kv_fmt) << 16);
-        o.y = pack_fp8x2(y[4], y[5], p.kv_fmt) | (pack_fp8x2(y[6], y[7], p.kv_fmt) << 16);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + to) = o;
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.hq + h) * D + at) = raw;
+      } else if (h < heads && slot_ok) {
+        void* cache = is_k ? p.k_cache : p.v_cache;
+        const int kvh = is_k ? h - p.hq : h - p.hq - p.hkv;
+        const int64_t to = slot * p.kv_tok_stride + kvh * p.kv_head_stride + at;
+        if (p.kv_fmt == kKvSame) {
+  #pragma unroll
+          for (int i = 0; i < V; ++i) e[i] = from_f32<T>(y[i]);
+          *reinterpret_cast<uint4*>(static_cast<T*>(cache) + to) = raw;
+        } else {
+          uint2 o;
+          o.x = pack_fp8x2(y[0], y[1], p.kv_fmt) | (pack_fp8x2(y[2], y[3], p.kv_fmt) << 16);
+          o.y = pack_fp8x2(y[4], y[5], p.kv_fmt) | (pack_fp8x2(y[6], y[7], p.kv_fmt) << 16);
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + to) = o;
+        }
       }
     }
   }
@@ -183,9 +194,11 @@ __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams
 
 // ---------------------------------------------------------------------------
 // Accepted nodes: row of node i of the request <- row of node path[i], for i below count, in every plane (layer, k or v, head) of the
-// storage.  The path rises (path[i] >= i), so a thread that has its 16 bytes of all planes' rows in the order of i reads every row before
+// storage.  The path rises (path[i] >= i), so a thread that has its 16 bytes of a plane's rows in the order of i reads every row before
 // it is overwritten: rows are read eight at a time, written behind that, and a later read is of a later node than all written so far.
-// Bound by the chain lengths -> path -> table -> rows for few requests, by the rows' bytes for many.
+// Bound by the chain lengths -> path -> table -> rows for few requests, by the rows' bytes for many; a thread goes through the chain once
+// and then through many planes (with a thread per plane and piece, three waves of blocks went through it: 32 requests of 3.5 accepted
+// nodes, 36 layers of 8 heads of 128, 11.9 us).
 // ---------------------------------------------------------------------------
 struct CompactParams {
   uint8_t* store;
@@ -206,6 +219,10 @@ __global__ void __launch_bounds__(kCompactThreads) tree_compact_kernel(const Com
   pdl_launch_dependents();
   pdl_wait_loads();
   const int b = blockIdx.y;
+  const int* path = p.path + static_cast<int64_t>(b) * p.steps;
+  int node[kMoves];
+#pragma unroll
+  for (int k = 0; k < kMoves; ++k) node[k] = k < p.steps ? __ldcg(path + k) : -1;
   const int count = min(__ldcg(p.counts + b), p.steps);
   const int prefix = __ldcg(p.prefix_lens + b), req = __ldcg(p.req_pool_indices + b);
   if (count <= 0) return;
@@ -214,20 +231,17 @@ __global__ void __launch_bounds__(kCompactThreads) tree_compact_kernel(const Com
     return;
   }
   const int lanes = p.row_bytes >> 4;
-  const int64_t item = blockIdx.x * static_cast<int64_t>(kCompactThreads) + threadIdx.x;
-  const int64_t plane = item / lanes;
-  const bool mine = plane < p.planes;
-  uint8_t* base = p.store + (mine ? plane * p.plane_bytes + (item - plane * lanes) * 16 : 0);
+  const int items = p.planes * lanes;               // below 2^31: checked by the launcher
   const int* table = p.req_to_token + req * p.table_stride;
-  const int* path = p.path + static_cast<int64_t>(b) * p.steps;
   bool bad = false;
   int before = -1;
   for (int i0 = 0; i0 < count; i0 += kMoves) {
-    uint4 v[kMoves];
-    int to[kMoves], node[kMoves];
+    if (i0 > 0) {
+      // the rows of a later part may be those that an earlier part of this thread read: all planes of a part come first
 #pragma unroll
-    for (int k = 0; k < kMoves; ++k) node[k] = i0 + k < count ? __ldcg(path + i0 + k) : -1;
-    int from[kMoves];
+      for (int k = 0; k < kMoves; ++k) node[k] = i0 + k < count ? __ldcg(path + i0 + k) : -1;
+    }
+    int from[kMoves], to[kMoves];
 #pragma unroll
     for (int k = 0; k < kMoves; ++k) {
       from[k] = to[k] = -1;
@@ -243,17 +257,25 @@ __global__ void __launch_bounds__(kCompactThreads) tree_compact_kernel(const Com
       from[k] = __ldcg(table + prefix + n);
       to[k] = __ldcg(table + prefix + i0 + k);
     }
+    bool any = false;
 #pragma unroll
     for (int k = 0; k < kMoves; ++k) {
       if (to[k] == -1 && from[k] == -1) continue;
       if (from[k] < 0 || from[k] >= p.num_slots || to[k] < 0 || to[k] >= p.num_slots) {
         bad = true;
         to[k] = -1;
-      } else if (mine) {
-        v[k] = __ldcg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(from[k]) * p.row_bytes));
+      } else {
+        any = true;
       }
     }
-    if (mine) {
+    if (!any) continue;
+    for (int item = blockIdx.x * kCompactThreads + threadIdx.x; item < items; item += gridDim.x * kCompactThreads) {
+      const int plane = item / lanes;
+      uint8_t* base = p.store + plane * p.plane_bytes + (item - plane * lanes) * 16;
+      uint4 v[kMoves];
+#pragma unroll
+      for (int k = 0; k < kMoves; ++k)
+        if (to[k] >= 0) v[k] = __ldcg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(from[k]) * p.row_bytes));
 #pragma unroll
       for (int k = 0; k < kMoves; ++k)
         if (to[k] >= 0) *reinterpret_cast<uint4*>(base + static_cast<int64_t>(to[k]) * p.row_bytes) = v[k];
@@ -286,7 +308,7 @@ int launch_tree_prologue(const TreePrologueArgs& a, cudaStream_t s) {
   p.kv_fmt = a.kv_fmt;
   p.eps = a.eps;
   const int heads = a.hq + 2 * a.hkv, per = 256 / a.head_dim, steps = (heads + per - 1) / per;
-  p.hsplit = static_cast<int>(std::min<int64_t>(steps, std::max<int64_t>(1, 4096 / a.index.rows)));
+  p.hsplit = static_cast<int>(std::min<int64_t>(steps, std::max<int64_t>(1, 2048 / a.index.rows)));
   const int64_t warps = static_cast<int64_t>(a.index.rows) * p.hsplit;
   const dim3 grid(static_cast<unsigned>((warps + 3) / 4));
   cudaError_t err = cudaErrorInvalidValue;
@@ -320,7 +342,10 @@ int launch_tree_compact(const TreeCompactArgs& a, cudaStream_t s) {
   p.planes = a.planes;
   p.row_bytes = a.row_bytes;
   const int64_t items = static_cast<int64_t>(a.planes) * (a.row_bytes / 16);
-  const dim3 grid(static_cast<unsigned>((items + kCompactThreads - 1) / kCompactThreads), static_cast<unsigned>(a.batch));
+  if (items >= (int64_t(1) << 31) - (int64_t(1) << 24)) return -1;
+  // about two blocks per SM in all
+  const int64_t blocks = std::min<int64_t>((items + kCompactThreads - 1) / kCompactThreads, std::max<int64_t>(1, 2 * 148 / a.batch));
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.batch));
   const cudaError_t err = launch_pdl(tree_compact_kernel, grid, dim3(kCompactThreads), 0, s, p);
   note_launch();
   return err == cudaSuccess ? 0 : -4;
