@@ -571,6 +571,22 @@ class ModelRunner:
             attn_backend=self.attn_backend, **extra,
         )
 
+    def prepare_forward_batch_tree(
+        self, input_ids: torch.Tensor, parents: torch.Tensor, req_pool_indices: torch.Tensor, tree_lens_cpu: List[int],
+        prefix_lens_cpu: List[int], **extra,
+    ) -> ForwardBatch:
+        """Batch of drafted token trees, one per request: ``input_ids`` and ``parents`` (int32, see :func:`ops.attention_tree`) of all nodes,
+        request by request; node j of a request goes to the slot that the request table has behind its cached tokens.  The forward pass
+        returns the logits of every node.  For models whose layers are all :class:`RadixAttention` (``draft_trees``)."""
+        if not getattr(self.model, "draft_trees", False):
+            raise ValueError(f"{type(self.model).__name__} does not run drafted token trees")
+        if len(tree_lens_cpu) != len(prefix_lens_cpu) or sum(tree_lens_cpu) != input_ids.shape[0] or parents.shape != input_ids.shape:
+            raise ValueError("a tree batch has a tree length and a prefix length per request, and a parent per node")
+        tree, prefix = (torch.tensor(x, dtype=torch.int32).to(self.device, non_blocking=True) for x in (tree_lens_cpu, prefix_lens_cpu))
+        rows = torch.arange(input_ids.shape[0], device=self.device)
+        return self.prepare_forward_batch_extend(input_ids, req_pool_indices, tree + prefix, tree, prefix, rows, list(tree_lens_cpu),
+                                                 list(prefix_lens_cpu), tree_parents=parents.to(torch.int32).contiguous(), logit_rows=rows, **extra)
+
     # ------------------------------------------------------------------ forward / sample
     @torch.no_grad()
     def forward(self, forward_batch: ForwardBatch) -> LogitsProcessorOutput:

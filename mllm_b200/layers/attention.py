@@ -50,6 +50,8 @@ class RadixAttention(nn.Module):
             return qkv.new_zeros((T, self.num_heads * self.head_dim))
         k_cache, v_cache = fb.token_to_kv_pool.get_kv_buffer(self.layer_id)
         inv_freq, axis_map = self._tables(qkv.device)
+        if fb.tree_parents is not None:
+            return self._forward_tree(qkv, q_norm_w, k_norm_w, fb, inv_freq, k_cache, v_cache)
         use_mrope = self.mrope_sections is not None and fb.mrope_positions is not None
         ops.qk_norm_rope_kv_write(
             qkv, q_norm_w, k_norm_w, fb.mrope_positions if use_mrope else fb.positions, fb.out_cache_loc,
@@ -68,6 +70,14 @@ class RadixAttention(nn.Module):
                                   fb.seq_lens, fb.extend_prefix_lens, fb.extend_start_loc, self.scaling, out=out,
                                   max_q_len=fb.max_extend_len, window=self.sliding_window, logit_cap=self.logit_cap)
         return out.view(T, self.num_heads * self.head_dim)
+
+    def _forward_tree(self, qkv, q_norm_w, k_norm_w, fb, inv_freq, k_cache, v_cache) -> torch.Tensor:
+        """Drafted token trees: positions follow from the parents, slots from the request table."""
+        index = (fb.req_to_token_pool.req_to_token, fb.req_pool_indices, fb.seq_lens, fb.extend_prefix_lens, fb.extend_start_loc)
+        q = ops.tree_qk_norm_rope_kv_write(qkv, q_norm_w, k_norm_w, fb.tree_parents, *index, inv_freq, k_cache, v_cache, self.num_heads,
+                                           self.num_kv_heads, self.head_dim, self.rms_eps)
+        out = ops.attention_tree(q, k_cache, v_cache, *index, fb.tree_parents, self.scaling, window=self.sliding_window, logit_cap=self.logit_cap)
+        return out.view(qkv.shape[0], self.num_heads * self.head_dim)
 
 
 def query_rows(fb):

@@ -177,3 +177,20 @@ def chain_speculative_sampling(draft_probs: torch.Tensor, draft_token_ids: torch
         maybe_output_emitted_draft_token_num += first_rej.to(maybe_output_emitted_draft_token_num.dtype)
         first_rej = maybe_output_emitted_draft_token_num
     return out, accepted_all, first_rej
+
+
+def tree_speculative_sampling(logits: torch.Tensor, token_ids: torch.Tensor, parents: torch.Tensor, tree_lens: torch.Tensor,
+                              start_loc: torch.Tensor, max_steps: int, temperature: Scalar = 1.0, top_k: Scalar = 0, top_p: Scalar = 1.0,
+                              min_p: Optional[Scalar] = None, draft_probs: Optional[torch.Tensor] = None,
+                              generator: Optional[torch.Generator] = None, seed: Optional[int] = None
+                              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`chain_speculative_sampling` for a tree of drafted tokens per request, from the target's logits and the request's filters:
+    ``(nodes of the walk, emitted tokens, how many)``.  See :func:`ops.tree_speculative_sample`, which runs it in one kernel."""
+    b, dev = tree_lens.numel(), logits.device
+    if generator is None and seed is not None:
+        generator = torch.Generator(device=dev)
+        generator.manual_seed(int(seed))
+    return ops.tree_speculative_sample(
+        logits, token_ids.to(torch.int64), parents, tree_lens, start_loc, _per_row(temperature, b, dev), _per_row(top_k, b, dev, torch.int32),
+        _per_row(top_p, b, dev), None if min_p is None else _per_row(min_p, b, dev), torch.rand(logits.shape[0], device=dev, generator=generator),
+        torch.rand(b, device=dev, generator=generator), max_steps, draft_probs)

@@ -97,6 +97,12 @@ class KVPool:
             self.v_buffer[layer_id - self.layer_offset],
         )
 
+    def keep_accepted(self, req_to_token, req_pool_indices, prefix_lens, path, counts) -> None:
+        """Brings the rows of accepted draft nodes together, in all layers (see :func:`ops.tree_kv_compact`)."""
+        from ..ops import tree_kv_compact
+
+        tree_kv_compact(self.store, req_to_token, req_pool_indices, prefix_lens, path, counts)
+
     def clear(self) -> None:
         self.store.zero_()
 

@@ -299,6 +299,7 @@ class VisionLanguageMixin:
     prompt with image blocks, and image features written over the image-token rows of the input
     embeddings.  The host class provides ``visual``, ``image_token_id``, ``vision_start_token_id``,
     ``spatial_merge_size``, ``hidden_size``, ``num_deepstack`` and ``model.embed_tokens``."""
+    draft_trees = False     # positions of an image prompt are not those of a tree
 
     uses_mrope = True
     # videos: rows that carry this token take features like image rows.  Qwen3-VL prompts hold one block per

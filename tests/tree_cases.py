@@ -126,3 +126,96 @@ def slots_of_rows(c):
         out += c["table"][int(c["req"][b]), pl:pl + len(parents)].tolist()
     return out
 
+
+
+class Round:
+    """A tiny model that runs prompts and drafted trees, and the same tokens as plain prompts for comparison."""
+
+    def __init__(self, preset, device, dtype, kv_cache_dtype="auto"):
+        from mllm_b200.configs import ServerConfig
+        from mllm_b200.executor import ModelRunner
+
+        self.mr = ModelRunner(ServerConfig(model_path=f"preset:{preset}", dtype=dtype, max_running_requests=24, max_total_tokens=4096),
+                              kv_cache_dtype=kv_cache_dtype, device=device)
+        self.mr.initialize()
+        self.dev = torch.device(device)
+
+    def _alloc(self, n):
+        return self.mr.token_to_kv_pool_allocator.alloc(n)
+
+    def prompt(self, ids):
+        """Runs a prompt; (request row, logits of its last token)."""
+        mr = self.mr
+        row = mr.req_to_token_pool.alloc(1)[0]
+        loc = self._alloc(len(ids))
+        mr.req_to_token_pool.req_to_token[row, :len(ids)] = loc.to(torch.int32)
+        one = lambda x: torch.tensor([x], dtype=torch.int32, device=self.dev)  # noqa: E731
+        fb = mr.prepare_forward_batch_extend(torch.tensor(ids, device=self.dev), one(row), one(len(ids)), one(len(ids)), one(0), loc, [len(ids)], [0])
+        return row, mr.forward(fb).next_token_logits[0]
+
+    def free(self, row):
+        self.mr.req_to_token_pool.free(row)
+
+    def plain(self, ids):
+        """Logits behind `ids` as a prompt of its own."""
+        row, logits = self.prompt(ids)
+        self.free(row)
+        return logits
+
+    def tree(self, rows, lens, tokens, trees):
+        """Runs a tree per request behind its cached tokens; the logits of all nodes."""
+        mr = self.mr
+        for row, n, t in zip(rows, lens, trees):
+            mr.req_to_token_pool.req_to_token[row, n:n + len(t)] = self._alloc(len(t)).to(torch.int32)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=self.dev)  # noqa: E731
+        fb = mr.prepare_forward_batch_tree(torch.tensor([x for t in tokens for x in t], device=self.dev), ints([p for t in trees for p in t]),
+                                           ints(rows), [len(t) for t in trees], list(lens))
+        return fb, mr.forward(fb).next_token_logits
+
+    def check(self, close):
+        """A round of speculative decoding: logits of nodes, greedy verification, accepted rows, the next step."""
+        from mllm_b200 import ops
+
+        g = random.Random(5)
+        vocab = self.mr.vocab_size
+        prompts = [[g.randrange(vocab) for _ in range(n)] for n in (19, 70, 1)]
+        rows, seen = [], []
+        for p in prompts:
+            row, logits = self.prompt(p)
+            rows.append(row)
+            seen.append(p + [int(logits.float().argmax())])             # the root: the request's last token
+        for _ in range(2):                                              # two rounds in a row
+            trees = [[-1, 0, 0, 1, 1, 3, 2], [-1, 0, 1, 2, 0, 4, 3, 3], [-1, 0, 0]]
+            tokens = [[s[-1]] + [g.randrange(vocab) for _ in t[1:]] for s, t in zip(seen, trees)]
+            # one way through each tree is what the model itself would say, for a while
+            ways = [[2, 6], [1, 2, 3], []]
+            for s, t, tok, way in zip(seen, trees, tokens, ways):
+                said = list(s)
+                for node in way:
+                    said.append(int(self.plain(said).float().argmax()))
+                    tok[node] = said[-1]
+            lens = [len(s) - 1 for s in seen]
+            fb, logits = self.tree(rows, lens, tokens, trees)
+            at = 0
+            for s, t, tok in zip(seen, trees, tokens):
+                for j, way in enumerate(ways_of(t)):
+                    close(logits[at + j], self.plain(s[:-1] + [tok[i] for i in way]))
+                at += len(t)
+            B, T = len(rows), logits.shape[0]
+            f = lambda x, n: torch.full((n,), x, device=self.dev)  # noqa: E731
+            path, out, counts = ops.tree_speculative_sample(
+                logits, torch.tensor([x for t in tokens for x in t], device=self.dev), fb.tree_parents, fb.extend_seq_lens, fb.extend_start_loc,
+                f(0.0, B), torch.zeros(B, dtype=torch.int32, device=self.dev), f(1.0, B), None, f(0.5, T), f(0.5, B), 5)
+            self.mr.token_to_kv_pool.keep_accepted(self.mr.req_to_token_pool.req_to_token, fb.req_pool_indices, fb.extend_prefix_lens, path, counts)
+            for b, way in enumerate(ways):
+                n = int(counts[b])
+                assert path[b, :len(way) + 1].tolist() == [0] + way[:n - 1] + [-1] * (len(way) + 1 - n) or n >= len(way) + 1
+                assert out[b, :n - 1].tolist() == [tokens[b][i] for i in path[b, 1:n].tolist()]
+                assert n >= len(way) + 1, "greedy verification takes what the model itself would say"
+                seen[b] = seen[b] + out[b, :n].tolist()
+        # behind it the requests go on as if they had been decoded token by token
+        lens = [len(s) - 1 for s in seen]
+        _, logits = self.tree(rows, lens, [[s[-1]] for s in seen], [[-1]] * len(seen))
+        for b, s in enumerate(seen):
+            close(logits[b], self.plain(s))
+        ops.check_status()
