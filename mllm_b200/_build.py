@@ -4,10 +4,9 @@ The extensions live under ``mllm_b200/csrc``:
 
 * ``mllm_b200_C``    — the sm_100a CUDA kernels of every decoder plus their PyTorch binding;
 * ``mllm_b200_R``    — gated delta rule;
-* ``mllm_b200_A``    — latent attention;
+* ``mllm_b200_A``    — latent attention, drafted token trees (speculative decoding);
 * ``mllm_b200_L``    — lightning attention (linear attention with a fixed decay per head);
 * ``mllm_b200_E``    — mixtures of experts;
-* ``mllm_b200_T``    — drafted token trees (speculative decoding);
 * ``mllm_b200_X``    — 4-bit weights, vision towers, tensor- and expert-parallel exchange;
 * ``mllm_b200_host`` — host-only C++ (radix tree, page allocator, ``.mllm`` file reader).
 
@@ -61,8 +60,8 @@ EXTENSIONS: Dict[str, Dict[str, List[str]]] = {
         "cuda": True,
     },
     "mllm_b200_A": {
-        "sources": ["bindings_latent.cpp", "runtime.cu", "latent.cu"],
-        "headers": _COMMON,
+        "sources": ["bindings_latent.cpp", "runtime.cu", "latent.cu", "attention_tree.cu", "tree.cu", "tree_sample.cu"],
+        "headers": _COMMON + ["bindings_tree.h", "tree.h", "tree.cuh"],
         "cuda": True,
     },
     "mllm_b200_L": {
@@ -73,11 +72,6 @@ EXTENSIONS: Dict[str, Dict[str, List[str]]] = {
     "mllm_b200_E": {
         "sources": ["bindings_moe.cpp", "runtime.cu", "moe.cu", "moe_pair.cu"],
         "headers": _COMMON,
-        "cuda": True,
-    },
-    "mllm_b200_T": {
-        "sources": ["bindings_tree.cpp", "runtime.cu", "attention_tree.cu", "tree.cu", "tree_sample.cu"],
-        "headers": _COMMON + ["tree.h", "tree.cuh"],
         "cuda": True,
     },
     "mllm_b200_X": {

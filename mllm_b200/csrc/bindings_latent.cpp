@@ -1,5 +1,6 @@
 // PyTorch binding of latent attention (module mllm_b200_A).
 #include "bindings_common.h"
+#include "bindings_tree.h"
 
 namespace {
 
@@ -211,6 +212,10 @@ void latent_attention(const Tensor& q, const Tensor& cache, const Tensor& req_to
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("attention_tree", &attention_tree);
+  m.def("tree_qk_norm_rope_kv_write", &tree_qk_norm_rope_kv_write);
+  m.def("tree_speculative_sample", &tree_speculative_sample);
+  m.def("tree_kv_compact", &tree_kv_compact);
   m.def("latent_prologue", &latent_prologue, py::arg("y"), py::arg("q_w"), py::arg("kv_w"), py::arg("eps"), py::arg("cq"), py::arg("loc"),
         py::arg("cache"), py::arg("positions") = py::none(), py::arg("inv_freq") = py::none(), py::arg("turns") = py::none(),
         py::arg("halves") = false);

@@ -1,4 +1,6 @@
-// PyTorch binding of the kernels for drafted token trees.
+// PyTorch binding of the kernels for drafted token trees, part of the module of latent attention.
+#pragma once
+
 #include "bindings_common.h"
 #include "tree.h"
 
@@ -271,12 +273,3 @@ std::vector<Tensor> tree_speculative_sample(const Tensor& logits, const Tensor& 
 }
 
 }  // namespace
-
-PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("tree_speculative_sample", &tree_speculative_sample);
-  m.def("tree_qk_norm_rope_kv_write", &tree_qk_norm_rope_kv_write);
-  m.def("tree_kv_compact", &tree_kv_compact);
-  m.def("attention_tree", &attention_tree);
-  m.def("read_status", &read_status);
-  m.def("launch_count", &launch_count);
-}

@@ -50,7 +50,7 @@ class RadixAttention(nn.Module):
             return qkv.new_zeros((T, self.num_heads * self.head_dim))
         k_cache, v_cache = fb.token_to_kv_pool.get_kv_buffer(self.layer_id)
         inv_freq, axis_map = self._tables(qkv.device)
-        if fb.tree_parents is not None:
+        if getattr(fb, "tree_parents", None) is not None:
             return self._forward_tree(qkv, q_norm_w, k_norm_w, fb, inv_freq, k_cache, v_cache)
         use_mrope = self.mrope_sections is not None and fb.mrope_positions is not None
         ops.qk_norm_rope_kv_write(

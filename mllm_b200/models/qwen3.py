@@ -205,7 +205,7 @@ class Qwen3DecoderLayer(nn.Module):
     def _forward_native(self, hidden, residual, fb):
         """New tokens of prompts on one GPU with 16-bit weights: the layer as one native call, since the host's work for eight calls
         takes longer than the kernels of a short prompt.  None for everything else, and where a part has been replaced or hooked."""
-        if fb.forward_mode.is_decode() or fb.forward_mode.is_idle() or fb.tree_parents is not None or not hidden.is_cuda or hidden.shape[0] == 0:
+        if fb.forward_mode.is_decode() or fb.forward_mode.is_idle() or getattr(fb, "tree_parents", None) is not None or not hidden.is_cuda or hidden.shape[0] == 0:
             return None
         mods = self._modules
         attn, mlp, norm1, norm2 = mods["self_attn"], mods["mlp"], mods["input_layernorm"], mods["post_attention_layernorm"]
