@@ -8,21 +8,26 @@
 // low_j the first position of the sliding window or of the chunk.
 //
 // The rows that share K and V are (node, query head of the group) pairs, n * group of them; 128 make a row tile.  Every cached key
-// and value is read once per row tile and meets 4 * 128 operations per element at most: a memory stream up to 128 rows, like decoding,
-// with products too large for warp-level instructions (128 rows x 64 keys x 128 features twice per 32 KB).  So:
-//   * work is dealt as in decoding: the 64-token tiles of all (request, kv head, row tile) units form one line, laid out on the device
+// and value is read once per unit of one or two row tiles and meets 4 * 128 operations per element and tile: a memory stream up to 128
+// rows, like decoding, with products too large for warp-level instructions (128 rows x 64 keys x 128 features twice per 32 KB).  So:
+//   * work is dealt as in decoding: the 64-token tiles of all (request, kv head, rows) units form one line, laid out on the device
 //     from the lengths, and every CTA takes an equal run of it.  A unit inside one CTA is written out directly; others leave at most
 //     two partial results per CTA, and the CTA that has a unit's last tile leaves a note for the kernel that joins them.
-//   * warps 4-10 copy rows by slot with cp.async (a page of one token costs what a page of 16 does) into a ring of 64-token K or V
-//     stages in the operand layout.  A warp takes whole stages in turn: what stands between two stages (barriers, slots, shuffles) is a
-//     chain of some 2000 cycles, which all warps paid for every stage when they shared it.  8-bit rows land as they are, and the two
-//     warps that copied them widen them.  The warps left copy Q.
-//   * warp 11 issues S = Q K^T (two score buffers in tensor memory) and O += P V, P from tensor memory.
-//   * warps 0-3 hold a row per thread: online maximum and sum in fp32, P over S in place.  Masks are 64-bit words per row and tile,
-//     made only in tiles that hold tree nodes or a window's edge: cached part by comparison, tree part by a walk to the root over
-//     parents in shared memory.
+//   * copying warps (4-10; 8-18 beside two row tiles) bring rows by slot with cp.async (a page of one token costs what a page of 16 does)
+//     into a ring of 64-token K or V stages in the operand layout.  A warp takes whole stages in turn: what stands between two stages
+//     (barriers, slots, shuffles) is a chain of some 2000 cycles, which all warps paid for every stage when they shared it.  8-bit rows
+//     land as they are, and the two warps that copied them widen them.  The warps left copy Q.
+//   * the last warp issues S = Q K^T (two score buffers a row tile in tensor memory) and O += P V, P from tensor memory.
+//   * the first four warps (eight) hold a row per thread: online maximum and sum in fp32, P over S in place.  Masks are 64-bit words per
+//     row and tile, made only in tiles that hold tree nodes or a window's edge: cached part by comparison, tree part by a walk to the
+//     root over parents in shared memory.
 // A value that is no number must not reach rows that do not see it (0 x NaN): in masked tiles the warps that copied V set such elements to
 // zero, and they are added at the end to the rows that see them.
+//
+// Where the time goes (bf16, 128 features, on the device in a graph): 8 requests of 2048 tokens and 32 nodes, 72 MB, 34.6 us.  The first
+// scores are there after 9 us (1.8 us for the lengths of all requests, 2 us for the slots, then the rows, all stages' at once), tiles pass
+// at the rate of memory (6 TB/s), rows go out in 2 us, and the joining kernel begins 2 us behind the last CTA and takes 4.  From two
+// row tiles on the exponentials bound: 1.2 us for 256 rows and 64 keys on an SM.
 #include <algorithm>
 
 #include "common.cuh"
@@ -33,12 +38,8 @@ namespace {
 
 constexpr int kRows = 128;                 // MMA M
 constexpr int kTile = 64;                  // tokens of a tile
-constexpr int kThreads = 384;              // 4 softmax warps, 7 copying warps, one that issues products
-constexpr int kIssueWarp = 11;
-// registers of the groups of 4 warps, of the 384 x 80 that a CTA of two per SM is launched with
-constexpr int kLaunchRegs = 80, kSoftmaxRegs = 128, kOtherRegs = 56;
-static_assert(128 * (kSoftmaxRegs + 2 * kOtherRegs) <= kThreads * kLaunchRegs, "register split");
-constexpr int kStart = 4;                  // units behind every (request, kv head, row tile): what it costs beside its tiles
+constexpr int kSoftmaxRegs = 128;          // registers of the threads that hold rows; the others give back what that takes
+constexpr int kStart = 4;                  // tiles' time that every unit costs beside its tiles
 constexpr int kNoToken = -0x7fffffff;
 constexpr int kParents = 256;              // nodes whose parents are kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
@@ -51,17 +52,16 @@ struct TreeParams {
   void* out;
   float* part_o;     // [CTAs][2][HD / 4][part_rows][4]: lanes, which hold rows, write and read neighbouring addresses
   float* part_lse;   // [CTAs][2][part_rows]
-  int* jobs;         // [CTAs][kJobInts]
+  int* job_rows;     // [CTAs]: rows to join (0: none) of the unit whose last tile the CTA has
+  int4* jobs;        // [CTAs]: first row of q, first head, first CTA of the unit, whether that one has it in its second partial result
   TreeIndex ix;
   const float* sink;
   int64_t q_stride, out_stride, num_slots, kv_tok_stride, kv_head_stride;
-  int hkv, group, tpt, ctas, part_rows, window, chunk;
+  int hkv, group, tpt, unit_nodes, ctas, part_rows, window, chunk;   // tpt: nodes of a row tile
   float scale_log2, cap_in, cap_out;    // cap_out 0: no soft cap
   uint32_t idesc_s, idesc_o;
 };
-// What the CTA with a unit's last tile notes for the joining kernel: rows (0: nothing to join), first row of q, first head, first CTA
-// of the unit, and whether that one has it in its second partial result
-constexpr int kJobInts = 8;
+constexpr int kJobInts = 5;
 
 // first position that a node at position i sees
 __device__ __forceinline__ int first_key(const TreeParams& p, int i) {
@@ -75,14 +75,16 @@ __device__ __forceinline__ int edge_of(const TreeParams& p, const Request& r) { 
 __device__ __forceinline__ int tiles_of(const TreeParams& p, const Request& r) {
   return r.nodes == 0 ? 0 : (r.prefix + r.nodes - first_token(p, r) + kTile - 1) / kTile;
 }
-__device__ __forceinline__ int row_tiles(const TreeParams& p, const Request& r) { return (r.nodes + p.tpt - 1) / p.tpt; }
+__device__ __forceinline__ int units_of(const TreeParams& p, const Request& r) { return (r.nodes + p.unit_nodes - 1) / p.unit_nodes; }
 
 __device__ __forceinline__ int ctas_used(const TreeParams& p, int64_t line) {
   const int64_t want = max(line / 4, min(line / 2, static_cast<int64_t>(64)));
   return static_cast<int>(min(static_cast<int64_t>(p.ctas), max(want, static_cast<int64_t>(1))));
 }
+// (A division of 64 bits takes some 500 cycles.)
+__device__ __forceinline__ bool fits_32(int64_t line, int ctas) { return line < (1ll << 31) && line * (ctas + 1) < (1ll << 32); }
 __device__ __forceinline__ int64_t run_begin(int64_t line, int c, int ctas) {
-  if (line < 0xFFFFFFFFll / (ctas + 1)) return static_cast<uint32_t>(line) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
+  if (fits_32(line, ctas)) return static_cast<uint32_t>(line) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
   return line * c / ctas;
 }
 
@@ -141,24 +143,33 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <int NH, bool KV8>
+// R: row tiles that a CTA takes through its keys and values side by side
+template <int NH, bool KV8, int R>
 struct Cfg {
+  static_assert(R == 1 || NH == 2, "two row tiles of 256 features leave no tensor memory for scores; those of 64 are no faster");
+  static constexpr int kSoftmaxWarps = 4 * R, kIssueWarp = R == 1 ? 11 : 19, kThreads = 32 * (kIssueWarp + 1);
   static constexpr int kD = 64 * NH;
   static constexpr int kQBlock = kRows * 128;              // a 64-feature block of Q
-  static constexpr int kQBytes = NH * kQBlock;
+  static constexpr int kQTile = NH * kQBlock, kQBytes = R * kQTile;
   static constexpr int kBlock = kTile * 128;               // a 64-feature block of a stage
   static constexpr int kStage = NH * kBlock;
-  static constexpr int kStages = NH == 1 ? (KV8 ? 6 : 10) : KV8 ? 3 : 5;
+  static constexpr int kStages = (NH == 1 ? (KV8 ? 6 : 10) : KV8 ? 3 : 5) * R;
   // A team of warps copies every kTeams-th item.  Never more teams than stages: a team that waits for the item kStages before its own
   // to be used has seen its item before go to the stage of the one 2 kStages before (a barrier tells a phase from the next, no more).
-  static constexpr int kTeam = KV8 ? 2 : 1, kTeams = KV8 ? 3 : 5;
-  static constexpr int kQWarps = kIssueWarp - 4 - kTeam * kTeams;     // those that are left copy Q
+  static constexpr int kTeam = KV8 ? 2 : 1, kTeams = R == 1 ? (KV8 ? 3 : 5) : KV8 ? 4 : 8;
+  static constexpr int kQWarps = kIssueWarp - kSoftmaxWarps - kTeam * kTeams;     // those that are left copy Q
   static_assert(kTeams <= kStages && kQWarps > 0, "teams");
   static constexpr int kRaw = KV8 ? kTile * kD : 0;        // an item as it is cached, one per team
   static constexpr int kSmem = kQBytes + kStages * kStage + kTeams * kRaw;
-  static constexpr int kPerSm = NH == 4 ? 1 : 2;
+  static constexpr int kPerSm = NH == 4 || R == 2 ? 1 : 2;
+  // registers that a CTA is launched with and what the threads without rows keep; 256 features have one CTA and need no split
+  static constexpr bool kSplit = NH < 4;
+  static constexpr int kLaunchRegs = R == 1 ? 80 : 96, kOtherRegs = R == 1 ? 56 : 72;
+  static_assert(32 * (kSoftmaxWarps * kSoftmaxRegs + (kThreads / 32 - kSoftmaxWarps) * kOtherRegs) <= kThreads * kLaunchRegs, "register split");
   static_assert(kPerSm * (kSmem + 2048) <= 228 * 1024, "1 KB of each CTA is the system's, 1 KB the kernel's variables");
-  static constexpr int kCols = NH == 4 ? 512 : 256;        // two score buffers of 64 columns, then O
+  // tensor memory: two score buffers of 64 columns a row tile, then O of each
+  static constexpr int kScoreCols = R * 2 * kTile, kCols = NH == 4 || R == 2 ? 512 : 256;
+  static_assert(kScoreCols + R * kD <= kCols, "tensor memory");
 };
 
 // Item i of a segment of n tiles, in the order in which the products need them: K0, K1, V0, K2, V1, ..
@@ -169,18 +180,18 @@ __device__ __forceinline__ int item_tile(int i, int n) {
 }
 
 struct Place {          // of a segment
-  int b, hk, rt, t0;
+  int b, hk, u, t0;
   int64_t left;
 };
 
 // FMT: what the caches hold (kKvSame, kKvE4M3, kKvE5M2)
-template <typename T, int NH, int FMT>
-__global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) attn_tree_kernel(const TreeParams p) {
+template <typename T, int NH, int FMT, int R>
+__global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, FMT != kKvSame, R>::kPerSm) attn_tree_kernel(const TreeParams p) {
   constexpr bool KV8 = FMT != kKvSame, kF16 = std::is_same<T, __half>::value;
-  using C = Cfg<NH, KV8>;
-  constexpr int kD = C::kD, kStages = C::kStages;
+  using C = Cfg<NH, KV8, R>;
+  constexpr int kD = C::kD, kStages = C::kStages, kIssueWarp = C::kIssueWarp, kSoft = C::kSoftmaxWarps;
   extern __shared__ __align__(1024) uint8_t tree_smem[];
-  __shared__ uint64_t bars[2 * C::kStages + 8];
+  __shared__ uint64_t bars[2 * C::kStages + 6 + 2 * R];
   __shared__ uint32_t tmem_holder;
   __shared__ int fail_flag, poison;
   __shared__ int16_t parents[kParents];
@@ -193,10 +204,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
   uint64_t* full = bars;                 // [stage] the warps of a team
   uint64_t* empty = full + kStages;      // [stage] tcgen05.commit
   uint64_t* s_full = empty + kStages;    // [buffer] tcgen05.commit: scores of a tile
-  uint64_t* p_full = s_full + 2;         // [buffer] the softmax warps: P is in tensor memory, O rescaled
+  uint64_t* p_full = s_full + 2;         // [buffer][row tile] the softmax warps: P is in tensor memory, O rescaled
   // [buffer] tcgen05.commit: a tile's P V.  A wait tells a phase from the one before it and no more: the scores of tile t, which a
   // thread has seen, were issued behind P V of t - 2, so one barrier would do for neither of the two products that may be out
-  uint64_t* o_done = p_full + 2;
+  uint64_t* o_done = p_full + 2 * R;
   uint64_t* q_full = o_done + 2;         // the warps that copy Q
   uint64_t* q_free = q_full + 1;         // tcgen05.commit: the segment's last scores
 
@@ -212,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
     Request r{};                     // of the first of this lane's requests
     for (int b = last - 1; b >= first; --b) {
       r = request_of(p.ix, b, &bad);
-      if (r.nodes > 0) mine += static_cast<int64_t>(row_tiles(p, r)) * (tiles_of(p, r) + kStart);
+      if (r.nodes > 0) mine += static_cast<int64_t>(units_of(p, r)) * (tiles_of(p, r) + kStart);
     }
     if (bad && blockIdx.x == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
     int64_t incl = mine;
@@ -238,10 +249,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
       for (int b = first; b < last; ++b) {
         if (b > first) r = request_of(p.ix, b, nullptr);
         const int n = r.nodes > 0 ? tiles_of(p, r) + kStart : 0;
-        const int64_t units = static_cast<int64_t>(n) * row_tiles(p, r) * p.hkv;
+        const int64_t units = static_cast<int64_t>(n) * units_of(p, r) * p.hkv;
         if (begin >= at && begin < at + units) {
           const int64_t in = begin - at;
-          const int unit = in < 0x7fffffff ? static_cast<int>(in) / n : static_cast<int>(in / n);    // 64 bits take some 500 cycles
+          const int unit = in < 0x7fffffff ? static_cast<int>(in) / n : static_cast<int>(in / n);
           begin_of[0] = b;
           begin_of[1] = unit;
           begin_of[2] = static_cast<int>(in - static_cast<int64_t>(unit) * n);
@@ -258,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 4);
+        for (int h = 0; h < R; ++h) mbar_init(&p_full[i * R + h], 4);
         mbar_init(&o_done[i], 1);
       }
       mbar_init(q_full, C::kQWarps);
@@ -287,21 +298,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
     w.b = begin_of[0];
     w.t0 = begin_of[2];
     Request r = begin_request;
-    int rts = row_tiles(p, r), n_all = tiles_of(p, r);
-    w.hk = begin_of[1] / rts;
-    w.rt = begin_of[1] - w.hk * rts;
+    int units = units_of(p, r), n_all = tiles_of(p, r);
+    w.hk = begin_of[1] / units;
+    w.u = begin_of[1] - w.hk * units;
     bool first = true;
     while (w.left > 0) {
       if (w.t0 >= n_all) {
         if (n_all > 0) w.left -= n_all + kStart - w.t0;
         w.t0 = 0;
-        if (n_all == 0 || ++w.rt == rts) {
-          w.rt = 0;
+        if (n_all == 0 || ++w.u == units) {
+          w.u = 0;
           if (n_all == 0 || ++w.hk == p.hkv) {
             w.hk = 0;
             if (++w.b >= p.ix.batch) return;
             r = request_of(p.ix, w.b, nullptr);
-            rts = row_tiles(p, r);
+            units = units_of(p, r);
             n_all = tiles_of(p, r);
           }
         }
@@ -320,11 +331,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
   const uint32_t inv_g = (65536u + g - 1) / g;
   auto node_of = [&](int r) { return static_cast<int>((r * inv_g) >> 16); };
 
-  if (warp >= 4) {
-    if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp < 4 + C::kTeams * C::kTeam) {
+  if (warp >= kSoft) {
+    if constexpr (C::kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    if (warp < kSoft + C::kTeams * C::kTeam) {
       // =============================== keys and values ===============================
-      const int team = (warp - 4) / C::kTeam, part = (warp - 4) % C::kTeam;
+      const int team = (warp - kSoft) / C::kTeam, part = (warp - kSoft) % C::kTeam;
       constexpr int kPart = kTile / C::kTeam;            // rows of this warp
       bool bad = false, ok = true;
       uint32_t item0 = 0;                                // items of the segments before
@@ -452,13 +463,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
       segments([&](const Place& w, const Request& r, int, int, bool) {
         if (seg > 0 && !mbar_wait(q_free, (seg - 1) & 1, &fail_flag)) ok = false;
         if (!(ok = __all_sync(0xffffffffu, ok))) return false;
-        const int n0 = w.rt * p.tpt, rows = min(p.tpt, r.nodes - n0) * g;
+        const int n0 = w.u * p.unit_nodes, rows = min(p.unit_nodes, r.nodes - n0) * g, half = p.tpt * g;     // half: rows of a tile
         const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(r.row + n0) * p.q_stride + static_cast<int64_t>(w.hk) * g * kD;
         constexpr int kCh = 8 * NH;               // 16-byte pieces of a row
 #pragma unroll 4
-        for (int c = (warp - 4 - C::kTeams * C::kTeam) * 32 + lane; c < rows * kCh; c += C::kQWarps * 32) {
-          const int row = c / kCh, ch = c % kCh, node = node_of(row);
-          cp16(smem_u32(sQ) + swz(row, ch, C::kQBlock), q + node * p.q_stride + static_cast<int64_t>(row - node * g) * kD + ch * 8, true);
+        for (int c = (warp - kSoft - C::kTeams * C::kTeam) * 32 + lane; c < rows * kCh; c += C::kQWarps * 32) {
+          const int all = c / kCh, ch = c % kCh, h = R > 1 && all >= half ? 1 : 0, row = all - h * half, node = node_of(row) + h * p.tpt;
+          cp16(smem_u32(sQ) + h * C::kQTile + swz(row, ch, C::kQBlock), q + node * p.q_stride + static_cast<int64_t>(all - node * g) * kD + ch * 8,
+               true);
         }
         cp_commit();
         cp_wait<0>();
@@ -481,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         };
         const uint64_t q_desc = umma_desc_k_sw128(smem_u32(sQ)), k_desc0 = umma_desc_k_sw128(smem_u32(ring));
         const uint64_t v_desc0 = umma_desc_mn_sw128(smem_u32(ring), C::kBlock, 1024);
-        const uint32_t idesc_s = p.idesc_s, idesc_o = p.idesc_o, tmem_o = tmem + 2 * kTile;
+        const uint32_t idesc_s = p.idesc_s, idesc_o = p.idesc_o, tmem_o = tmem + C::kScoreCols;
         uint32_t item = 0, seg = 0, tile = 0;      // tile: products of values so far
         segments([&](const Place&, const Request&, int, int n, bool) {
           auto scores = [&](int t) {
@@ -490,9 +502,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
             if (!ok) return;
             const uint64_t k_desc = k_desc0 + st * (C::kStage >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4 * NH; ++kk)
-              umma_f16(tmem + buf * kTile, q_desc + (kk >> 2) * (C::kQBlock >> 4) + (kk & 3) * 2,
-                       k_desc + (kk >> 2) * (C::kBlock >> 4) + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
+            for (int h = 0; h < R; ++h)
+#pragma unroll
+              for (int kk = 0; kk < 4 * NH; ++kk)
+                umma_f16(tmem + (h * 2 + buf) * kTile, q_desc + h * (C::kQTile >> 4) + (kk >> 2) * (C::kQBlock >> 4) + (kk & 3) * 2,
+                         k_desc + (kk >> 2) * (C::kBlock >> 4) + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
             umma_commit(&empty[st]);
             umma_commit(&s_full[buf]);
             if (t == n - 1) umma_commit(q_free);
@@ -504,12 +518,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
           for (int t = 0; t < n && ok; ++t) {
             const uint32_t st = item % kStages, at = tile + t, buf = at & 1;
             wait_on(&full[st], (item / kStages) & 1);
-            wait_on(&p_full[buf], (at >> 1) & 1);
-            if (!ok) break;
             const uint64_t v_desc = v_desc0 + st * (C::kStage >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f16_ts(tmem_o, tmem + buf * kTile + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
+            for (int h = 0; h < R; ++h) {
+              if (ok && !mbar_wait(&p_full[buf * R + h], (at >> 1) & 1, &fail_flag)) ok = false;
+              tc_fence_after_sync();
+              if (!ok) break;
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma_f16_ts(tmem_o + h * kD, tmem + (h * 2 + buf) * kTile + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
+            }
+            if (!ok) break;
             umma_commit(&empty[st]);
             umma_commit(&o_done[buf]);
             ++item;
@@ -524,18 +543,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
     }
   } else {
     // =============================== softmax ===============================
-    if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int row = tid;
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t tmem_o = tmem + 2 * kTile + lane_base;
-    const int row_node = node_of(row);
+    if constexpr (C::kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int half = R > 1 ? warp >> 2 : 0, in_tile = tid & 127;      // row tile and row
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tmem_o = tmem + C::kScoreCols + half * kD + lane_base;
+    const int tile_node = node_of(in_tile), row_node = half * p.tpt + tile_node, row = half * p.tpt * g + in_tile;    // row of the unit
     const bool capped = p.cap_out > 0.f;
     bool ok = true, bad = false;
     uint32_t tile = 0;
     int job_rows = 0, job_row = 0, job_head = 0, job_tiles = 0;
     segments([&](const Place& w, const Request& r, int n_all, int n, bool first) {
-      const int node = w.rt * p.tpt + row_node;
-      const bool valid = row_node < p.tpt && node < r.nodes;
+      const int node = w.u * p.unit_nodes + row_node;
+      const bool valid = tile_node < p.tpt && node < r.nodes;
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       const int key0 = first_token(p, r) + w.t0 * kTile, len = r.prefix + r.nodes;
       const bool bounded = p.window > 0 || p.chunk > 0;
@@ -549,9 +568,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         return up;
       };
       if (masks) {        // parents to shared memory; one that is no earlier node counts as none
-        asm volatile("bar.sync 1, 128;" ::: "memory");          // the segment before has read them
-        for (int i = row; i < min(r.nodes, kParents); i += 128) parents[i] = static_cast<int16_t>(parent_in(i));
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoft) : "memory");          // the segment before has read them
+        for (int i = tid; i < min(r.nodes, kParents); i += 32 * kSoft) parents[i] = static_cast<int16_t>(parent_in(i));
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoft) : "memory");
       }
       auto parent_of = [&](int i) { return i < kParents ? static_cast<int>(parents[i]) : parent_in(i); };
       int pos = r.prefix, low = 0;
@@ -596,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         tc_fence_after_sync();
         if (warp_valid) {
           uint32_t raw[kTile];
-          const uint32_t tmem_s = tmem + buf * kTile + lane_base;
+          const uint32_t tmem_s = tmem + (half * 2 + buf) * kTile + lane_base;
           tmem_ld_32x32(tmem_s, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
           tmem_ld_32x32(tmem_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
           tmem_ld_wait();
@@ -658,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[buf]);
+        if (lane == 0) mbar_arrive(&p_full[buf * R + half]);
       }
       tile += n;
       if (!mbar_wait(&o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1, &fail_flag)) ok = false;
@@ -735,8 +754,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
         if (!whole && valid) p.part_lse[slot * p.part_rows + row] = l == 0.f ? -INFINITY : m_used + log2f(l);
       }
       if (!whole && w.t0 + n == n_all) {        // the unit's last tile: it began in front of this run
-        job_rows = min(p.tpt, r.nodes - w.rt * p.tpt) * g;
-        job_row = r.row + w.rt * p.tpt;
+        job_rows = min(p.unit_nodes, r.nodes - w.u * p.unit_nodes) * g;
+        job_row = r.row + w.u * p.unit_nodes;
         job_head = w.hk * g;
         job_tiles = w.t0;
       }
@@ -745,19 +764,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
     });
     if (!ok) fail_flag = 1;
     if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
-    if (row == 0) {
-      int* job = p.jobs + blockIdx.x * kJobInts;
-      job[0] = ok ? job_rows : 0;
+    if (tid == 0) {
+      p.job_rows[blockIdx.x] = ok ? job_rows : 0;
       if (ok && job_rows > 0) {
         const int64_t line = line_of[2], begin = line_of[0] - job_tiles;
         const int used = ctas_of;
         // the last CTA whose run begins at or before the unit
-        const int c0 = line < 0xFFFFFFFFll / (used + 1) ? static_cast<int>((static_cast<uint32_t>(begin + 1) * used - 1u) / static_cast<uint32_t>(line))
-                                                        : static_cast<int>(((begin + 1) * used - 1) / line);
-        job[1] = job_row;
-        job[2] = job_head;
-        job[3] = c0;
-        job[4] = run_begin(line, c0, used) < begin ? 1 : 0;
+        const int c0 = fits_32(line, used) ? static_cast<int>((static_cast<uint32_t>(begin + 1) * used - 1u) / static_cast<uint32_t>(line))
+                                           : static_cast<int>(((begin + 1) * used - 1) / line);
+        p.jobs[blockIdx.x] = make_int4(job_row, job_head, c0, run_begin(line, c0, used) < begin ? 1 : 0);
       }
     }
   }
@@ -776,37 +791,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<NH, FMT != kKvSame>::kPerSm) att
 }
 
 // Joins the partial results of the units that lie in several CTAs: out = sum_c w_c O_c with w_c = 2^(lse_c - max) / sum; a head's
-// sink is one more term of the sum, without a value.  blockIdx.x is a note; a warp takes 32 rows (a lane each) and 16 features at a time.
-constexpr int kJoinWarps = 4, kJoinParts = 8;
+// sink is one more term of the sum, without a value.  blockIdx.x is a note; a warp takes 32 rows (a lane each) and 16
+// features, and gridDim.y blocks have a warp for every such task of the largest unit.
+constexpr int kJoinWarps = 8, kJoinFeatures = 16;
 template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kJoinWarps) attn_tree_join_kernel(const TreeParams p) {
   pdl_launch_dependents();
   pdl_wait_loads();
-  const int* job = p.jobs + blockIdx.x * kJobInts;
-  const int rows = __ldcg(job), row0 = __ldcg(job + 1), head0 = __ldcg(job + 2), c0 = __ldcg(job + 3), second = __ldcg(job + 4);
+  const int rows = __ldcg(p.job_rows + blockIdx.x);
+  const int4 job = __ldcg(p.jobs + blockIdx.x);           // anything where rows is 0
+  const int row0 = job.x, head0 = job.y, c0 = job.z, second = job.w;
   const int c1 = blockIdx.x, lane = threadIdx.x & 31;
   const int groups = (rows + 31) / 32;
-  for (int task = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); task < groups * (HD / 16); task += kJoinWarps * kJoinParts) {
-    const int r = task % groups * 32 + lane, d = task / groups * 16;
+  for (int task = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); task < groups * (HD / kJoinFeatures); task += kJoinWarps * gridDim.y) {
+    const int r = task % groups * 32 + lane, d = task / groups * kJoinFeatures;
     if (r >= rows) continue;
     const int node = r / p.group, head = head0 + r - node * p.group;
     auto slot = [&](int c) { return static_cast<int64_t>(c) * 2 + (c == c0 ? second : 0); };
     const float sink = p.sink != nullptr ? p.sink[head] * kLog2e : -INFINITY;
     float top = sink;
+#pragma unroll 4
     for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(p.part_lse + slot(c) * p.part_rows + r));
-    float den = p.sink != nullptr ? exp2f(sink - top) : 0.f, acc[16] = {};
+    float den = p.sink != nullptr ? exp2f(sink - top) : 0.f, acc[kJoinFeatures] = {};
 #pragma unroll 2
     for (int c = c0; c <= c1; ++c) {
       const float lse = __ldcg(p.part_lse + slot(c) * p.part_rows + r);
       const float4* from = reinterpret_cast<const float4*>(p.part_o + slot(c) * p.part_rows * HD) + (d / 4) * p.part_rows + r;
-      float4 x[4];
+      float4 x[kJoinFeatures / 4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = __ldcg(from + k * p.part_rows);
+      for (int k = 0; k < kJoinFeatures / 4; ++k) x[k] = __ldcg(from + k * p.part_rows);
       if (lse == -INFINITY) continue;           // saw no key
       const float w = exp2f(lse - top);
       den += w;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kJoinFeatures / 4; ++k) {
         acc[4 * k] = fmaf(w, x[k].x, acc[4 * k]);
         acc[4 * k + 1] = fmaf(w, x[k].y, acc[4 * k + 1]);
         acc[4 * k + 2] = fmaf(w, x[k].z, acc[4 * k + 2]);
@@ -814,60 +832,66 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_tree_join_kernel(const T
       }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    T o[16];
+    __align__(16) T o[kJoinFeatures];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) o[k] = from_f32<T>(acc[k] * inv);
+    for (int k = 0; k < kJoinFeatures; ++k) o[k] = from_f32<T>(acc[k] * inv);
     uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + node) * p.out_stride + static_cast<int64_t>(head) * HD + d);
-    to[0] = reinterpret_cast<const uint4*>(o)[0];
-    to[1] = reinterpret_cast<const uint4*>(o)[1];
+#pragma unroll
+    for (int k = 0; k < kJoinFeatures / 8; ++k) to[k] = reinterpret_cast<const uint4*>(o)[k];
   }
 }
 
-template <typename T, int NH, int FMT>
+template <typename T, int NH, int FMT, int R>
 int launch_one(const TreeParams& p, cudaStream_t s) {
-  using C = Cfg<NH, FMT != kKvSame>;
-  auto kern = attn_tree_kernel<T, NH, FMT>;
+  using C = Cfg<NH, FMT != kKvSame, R>;
+  auto kern = attn_tree_kernel<T, NH, FMT, R>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem) != cudaSuccess) return -3;
-  if constexpr (C::kPerSm == 2) {
+  if constexpr (C::kSplit) {
     // the softmax warps take registers that the others give back: together no more than the kernel is launched with
     static const int regs = [kern] {
       cudaFuncAttributes at{};
       return cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(kern)) == cudaSuccess ? at.numRegs : 0;
     }();
-    if (regs < kLaunchRegs) return -5;
+    if (regs < C::kLaunchRegs) return -5;
   }
-  cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(kThreads), C::kSmem, s, p);
+  cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(C::kThreads), C::kSmem, s, p);
   note_launch();
   if (err != cudaSuccess) return -4;
-  err = launch_pdl(attn_tree_join_kernel<T, 64 * NH>, dim3(p.ctas, kJoinParts), dim3(32 * kJoinWarps), 0, s, p);
+  const int join_parts = ((p.part_rows + 31) / 32 * (C::kD / kJoinFeatures) + kJoinWarps - 1) / kJoinWarps;
+  err = launch_pdl(attn_tree_join_kernel<T, 64 * NH>, dim3(p.ctas, join_parts), dim3(32 * kJoinWarps), 0, s, p);
   note_launch();
   return err == cudaSuccess ? 0 : -4;
 }
-template <typename T, int NH>
+template <typename T, int NH, int R>
 int launch_format(const TreeParams& p, int fmt, cudaStream_t s) {
   switch (fmt) {
-    case kKvSame: return launch_one<T, NH, kKvSame>(p, s);
-    case kKvE4M3: return launch_one<T, NH, kKvE4M3>(p, s);
-    default: return launch_one<T, NH, kKvE5M2>(p, s);
+    case kKvSame: return launch_one<T, NH, kKvSame, R>(p, s);
+    case kKvE4M3: return launch_one<T, NH, kKvE4M3, R>(p, s);
+    default: return launch_one<T, NH, kKvE5M2, R>(p, s);
   }
 }
 template <typename T>
 int launch_type(const TreeParams& p, int head_dim, int fmt, cudaStream_t s) {
   switch (head_dim) {
-    case 64: return launch_format<T, 1>(p, fmt, s);
-    case 128: return launch_format<T, 2>(p, fmt, s);
-    default: return launch_format<T, 4>(p, fmt, s);
+    case 64: return launch_format<T, 1, 1>(p, fmt, s);
+    case 128: return p.unit_nodes > p.tpt ? launch_format<T, 2, 2>(p, fmt, s) : launch_format<T, 2, 1>(p, fmt, s);
+    default: return launch_format<T, 4, 1>(p, fmt, s);
   }
 }
 
 }  // namespace
 
-int tree_ctas(int head_dim, int num_sms) { return head_dim == 256 ? num_sms : 2 * num_sms; }
-int tree_part_rows(int group, int64_t rows) {
-  return static_cast<int>(std::min<int64_t>(kRows / group * group, rows * group));
-}
-int64_t tree_workspace_floats(int head_dim, int group, int64_t rows, int ctas) {
-  return static_cast<int64_t>(ctas) * (2 * tree_part_rows(group, rows) * (head_dim + 1) + kJobInts);
+TreePlan tree_plan(int head_dim, int group, int64_t rows, int64_t batch, int num_sms) {
+  TreePlan plan;
+  // Row tiles that a CTA takes side by side: two where a request has more rows than one tile on average.  Two tiles against one, 16 requests
+  // of 4096 tokens, 8 query heads over a kv head, 128 features: 24 nodes (192 rows) 59.1 / 82.3 us with e4m3 caches, which are widened
+  // half as often, and 59.9 / 62.8 us in bf16; 16 nodes (128 rows) 55.7 / 52.9 and 54.8 / 47.5.  Heads of 64: 54.7 / 54.2 and 50.0 / 53.6 at 24
+  // nodes, 54.0 / 42.3 and 48.8 / 42.0 at 17: always one.
+  plan.row_tiles = head_dim == 128 && rows > batch * (kRows / group) ? 2 : 1;
+  plan.ctas = head_dim == 256 || plan.row_tiles == 2 ? num_sms : 2 * num_sms;
+  plan.part_rows = static_cast<int>(std::min<int64_t>(plan.row_tiles * (kRows / group * group), rows * group));
+  plan.workspace_floats = static_cast<int64_t>(plan.ctas) * (2 * plan.part_rows * (head_dim + 1) + kJobInts) + 4;      // 4: notes on a 16-byte boundary
+  return plan;
 }
 
 int launch_attention_tree(const TreeAttnArgs& a, cudaStream_t s) {
@@ -879,11 +903,12 @@ int launch_attention_tree(const TreeAttnArgs& a, cudaStream_t s) {
   p.k_cache = a.k_cache;
   p.v_cache = a.v_cache;
   p.out = a.out;
-  p.ctas = a.ctas;
-  p.part_rows = tree_part_rows(g, a.index.rows);
+  p.ctas = a.plan.ctas;
+  p.part_rows = a.plan.part_rows;
   p.part_o = a.workspace;
   p.part_lse = p.part_o + static_cast<int64_t>(p.ctas) * 2 * p.part_rows * a.head_dim;
-  p.jobs = reinterpret_cast<int*>(p.part_lse + static_cast<int64_t>(p.ctas) * 2 * p.part_rows);
+  p.jobs = reinterpret_cast<int4*>(p.part_lse + static_cast<int64_t>(p.ctas) * 2 * p.part_rows + (p.ctas * 2 * p.part_rows & 3));
+  p.job_rows = reinterpret_cast<int*>(p.jobs + p.ctas);
   p.ix = a.index;
   p.sink = a.sink;
   p.q_stride = a.q_stride;
@@ -894,6 +919,7 @@ int launch_attention_tree(const TreeAttnArgs& a, cudaStream_t s) {
   p.hkv = a.hkv;
   p.group = g;
   p.tpt = kRows / g;
+  p.unit_nodes = a.plan.row_tiles * p.tpt;
   p.window = a.window > 0 ? a.window : 0;
   p.chunk = a.chunk > 0 ? a.chunk : 0;
   p.scale_log2 = a.scale * kLog2e;

@@ -92,7 +92,7 @@ Tensor attention_tree(const Tensor& q, const Tensor& k_cache, const Tensor& v_ca
   a.hkv = static_cast<int>(k_cache.size(1));
   a.head_dim = static_cast<int>(hd);
   a.kv_fmt = check_caches(k_cache, v_cache, q.scalar_type(), a.hkv, hd, q);
-  CHECK_ARG(a.hkv > 0 && a.hq % a.hkv == 0 && a.hq / a.hkv <= 128, "attention_tree: ", a.hq, " query heads over ", a.hkv, " kv heads");
+  CHECK_ARG(a.hkv > 0 && a.hq > 0 && a.hq % a.hkv == 0 && a.hq / a.hkv <= 128, "attention_tree: ", a.hq, " query heads over ", a.hkv, " kv heads");
   a.q = q.data_ptr();
   a.k_cache = k_cache.data_ptr();
   a.v_cache = v_cache.data_ptr();
@@ -111,9 +111,9 @@ Tensor attention_tree(const Tensor& q, const Tensor& k_cache, const Tensor& v_ca
   a.scale = static_cast<float>(scale);
   a.logit_cap = static_cast<float>(logit_cap);
   a.dt = dtype_of(q);
-  a.ctas = mb200::tree_ctas(a.head_dim, device_state(q.get_device()).num_sms);
+  a.plan = mb200::tree_plan(a.head_dim, a.hq / a.hkv, q.size(0), a.index.batch, device_state(q.get_device()).num_sms);
   // of this call alone: the caching allocator hands it out again in stream order, and a captured graph has its own
-  Tensor ws = torch::empty({mb200::tree_workspace_floats(a.head_dim, a.hq / a.hkv, q.size(0), a.ctas)}, q.options().dtype(torch::kFloat32));
+  Tensor ws = torch::empty({a.plan.workspace_floats}, q.options().dtype(torch::kFloat32));
   a.workspace = ws.data_ptr<float>();
   const int rc = mb200::launch_attention_tree(a, stream_of(q));
   TORCH_CHECK(rc == 0, "mllm_b200 attention_tree: unsupported configuration or launch failure (code ", rc, ")");

@@ -21,6 +21,13 @@ struct TreeIndex {
   int table_rows, table_cols, rows, batch;
 };
 
+// How the rows of a batch are laid over CTAs
+struct TreePlan {
+  int row_tiles, ctas, part_rows;      // row tiles side by side in a CTA; rows of a partial result
+  int64_t workspace_floats;
+};
+TreePlan tree_plan(int head_dim, int group, int64_t rows, int64_t batch, int num_sms);
+
 // attention of the nodes over the cached tokens, their ancestors and themselves (attention_tree.cu)
 struct TreeAttnArgs {
   TreeIndex index;
@@ -28,15 +35,14 @@ struct TreeAttnArgs {
   const void* k_cache;      // row of head h of slot s at s * kv_tok_stride + h * kv_head_stride (elements)
   const void* v_cache;
   void* out;
-  float* workspace;         // tree_workspace_floats
+  float* workspace;         // of the plan's size
   const float* sink;        // [hq] or null
   int64_t q_stride, out_stride, num_slots, kv_tok_stride, kv_head_stride;
-  int hq, hkv, head_dim, window, chunk, kv_fmt, ctas;
+  int hq, hkv, head_dim, window, chunk, kv_fmt;
+  TreePlan plan;
   float scale, logit_cap;
   DType dt;
 };
-int tree_ctas(int head_dim, int num_sms);
-int64_t tree_workspace_floats(int head_dim, int group, int64_t rows, int ctas);
 int launch_attention_tree(const TreeAttnArgs& args, cudaStream_t s);
 
 // per head: norm, rotation by position * inv_freq; queries out, keys and values to the nodes' slots (tree.cu)

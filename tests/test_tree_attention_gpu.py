@@ -43,6 +43,39 @@ def test_long_runs_of_tiles(D, prefix, nodes, hq, hkv):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("cache", [None, torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("prefix,nodes,hq,hkv,kw", [
+    ([500], [33], 4, 1, {}),                                  # one row over a tile
+    ([0, 64], [43, 43], 3, 1, {}),                            # 42 nodes a tile: 126 rows
+    ([700, 0, 100], [64, 64, 64], 8, 2, {}),                  # two full tiles
+    ([200, 3000], [65, 64], 4, 1, {}),                        # a third tile of one node
+    ([900, 10, 0, 77], [150, 1, 0, 9], 4, 2, {}),             # one tree above a tile, the others far below
+    ([300, 129], [70, 40], 16, 2, dict(window=50)),
+    ([300, 129], [70, 40], 16, 2, dict(chunk=64, logit_cap=4.0)),
+    ([1000], [2], 128, 1, {}),                                # a node per tile
+    ([2048] * 8, [48] * 8, 32, 8, {}),
+])
+def test_two_row_tiles_side_by_side(cache, prefix, nodes, hq, hkv, kw):
+    """More rows of a kv head than a tile of 128 holds, on average: a CTA takes two of them through the same keys and values."""
+    c, got = check(dict(prefix=prefix, nodes=nodes, hq=hq, hkv=hkv, D=128, cache=cache, seed=len(nodes)), **kw)
+    again = ops.attention_tree(c["q"], c["k"], c["v"], c["table"], c["req"], c["seq"], c["prefix"], c["start"], c["parents"], c["scale"], **kw)
+    assert torch.equal(got, again)
+
+
+def test_two_row_tiles_with_values_that_are_no_numbers():
+    c = tree_batch([100], [80], 4, 2, 128, trees=[[-1] + list(range(79))])
+    slots = c["table"][int(c["req"][0])].long()
+    c["v"][slots[170]] = float("nan")                        # node 70, seen by those from 70 on
+    c["k"][slots[175]] = float("nan")
+    got = ops.attention_tree(c["q"], c["k"], c["v"], c["table"], c["req"], c["seq"], c["prefix"], c["start"], c["parents"], c["scale"])
+    ops.check_status()
+    assert torch.isnan(got[70:]).all()
+    c["v"][slots[170]] = 0
+    c["k"][slots[175]] = 0
+    want, bound = exact_attention(c, bounds=True)
+    assert ((got[:70].double() - want[:70]).abs() <= bound[:70]).all()
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("kw", [dict(window=1), dict(window=37), dict(window=130), dict(window=5000), dict(chunk=64), dict(chunk=100), dict(chunk=7),
                                 dict(logit_cap=2.5), dict(window=70, logit_cap=30.0)])
