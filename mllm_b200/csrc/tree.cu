@@ -14,6 +14,10 @@ namespace {
 // requests' first rows), the walk to the root (parents of up to 128 nodes in the warp's registers, a shuffle a step) and the slot; angles
 // are formed once per warp, in 64 bits and reduced to one turn, since 32 lose a hundredth of a turn at positions of 10^5.  Results are
 // rounded once, to the type of what they go into.
+//
+// Bound by the chain q_start -> lengths -> parents -> slot -> rows for small batches (8 nodes, 16 + 16 heads of 128: 3.2 us, of which a
+// launch is 2) and by the rows' bytes for large ones (32 trees of 60 nodes, 32 + 16 heads of 128, e4m3 caches, 42 MB: 15.9 us, 2.7 TB/s:
+// a warp's chain is paid for a few rows only).  As many warps a node as fill the card once (hsplit) halve that chain's share.
 // ---------------------------------------------------------------------------
 struct PrologueParams {
   TreeIndex ix;
@@ -197,8 +201,8 @@ __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams
 // storage.  The path rises (path[i] >= i), so a thread that has its 16 bytes of a plane's rows in the order of i reads every row before
 // it is overwritten: rows are read eight at a time, written behind that, and a later read is of a later node than all written so far.
 // Bound by the chain lengths -> path -> table -> rows for few requests, by the rows' bytes for many; a thread goes through the chain once
-// and then through many planes (with a thread per plane and piece, three waves of blocks went through it: 32 requests of 3.5 accepted
-// nodes, 36 layers of 8 heads of 128, 11.9 us).
+// and then through many planes (32 requests of 3.5 accepted
+// nodes, 36 layers of 8 heads of 128: 9.6 us; with a thread per plane and piece, where three waves of blocks went through it, 11.9).
 // ---------------------------------------------------------------------------
 struct CompactParams {
   uint8_t* store;

@@ -66,6 +66,16 @@ def test_draws_over_many_requests(seed):
     compare(args, 5, probs)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [40000, 70001])
+def test_more_requests_than_sms_for_them(V, dtype):
+    """Requests of 8 CTAs each, more than SMs: two CTAs on an SM, and further ones behind them; flat rows among them."""
+    params = [dict(t=1.0, k=(0, 40, 0)[i % 3], p=(0.95, 1.0, 0.8)[i % 3], m=0.0) for i in range(60)]
+    args, _ = batch([3] * 60, V, seed=11, dtype=dtype, params=params)
+    args[0][:9] *= 0.05
+    compare(args, 3)
+
+
 @pytest.mark.parametrize("steps", [1, 2, 9])
 def test_steps(steps):
     args, _ = batch([10, 10, 10], 500, seed=3, width=1, params=[dict(t=0.0, k=0, p=1.0, m=0.0)] * 3)
