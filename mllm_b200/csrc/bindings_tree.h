@@ -131,6 +131,7 @@ Tensor tree_qk_norm_rope_kv_write(const Tensor& qkv, const c10::optional<Tensor>
                                   const Tensor& prefix_lens, const Tensor& q_start, const Tensor& inv_freq, Tensor& k_cache, Tensor& v_cache,
                                   int64_t hq, int64_t hkv, int64_t hd, double eps, const c10::optional<Tensor>& delta) {
   check_rows_type(qkv, "qkv");
+  CHECK_ARG(hq > 0 && hkv > 0, "tree_qk_norm_rope_kv_write: ", hq, " query heads and ", hkv, " key heads");
   CHECK_ARG((hd == 64 || hd == 128 || hd == 256) && qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) == (hq + 2 * hkv) * hd &&
                   qkv.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(qkv.data_ptr()) & 15) == 0,
               "qkv must be [T, (Hq + 2 Hkv) * D], D 64, 128 or 256, rows on 16-byte boundaries");

@@ -66,6 +66,8 @@ def tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, parents, req_to_token, r
     if ops.use_kernels(qkv):        # the binding makes the same checks
         return ops.ext().tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, *args)
     what = "tree_qk_norm_rope_kv_write"
+    if num_q_heads < 1 or num_kv_heads < 1:
+        raise ValueError(f"{what}: {num_q_heads} query heads and {num_kv_heads} key heads")
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (num_q_heads + 2 * num_kv_heads) * head_dim:
         raise ValueError(f"{what}: qkv must be [T, {(num_q_heads + 2 * num_kv_heads) * head_dim}] with unit inner stride")
     _check_caches(what, k_cache, v_cache, num_kv_heads, head_dim, qkv.dtype, qkv.device)
@@ -95,7 +97,7 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
     hkv = k_cache.shape[1]
     _check_caches("attention_tree", k_cache, v_cache, hkv, q.shape[2], q.dtype, q.device)
     _check_index("attention_tree", q.shape[0], q.device, req_to_token, parents, req_pool_indices, seq_lens, prefix_lens, q_start_loc)
-    if hkv == 0 or q.shape[1] % hkv or q.shape[1] > 128 * hkv:
+    if hkv == 0 or q.shape[1] == 0 or q.shape[1] % hkv or q.shape[1] > 128 * hkv:
         raise ValueError(f"attention_tree: {q.shape[1]} query heads over {hkv} key heads")
     if window is not None and window < 0 or chunk is not None and chunk < 0 or (window and chunk):
         raise ValueError("attention_tree: either a sliding window or chunks, of positive lengths")
@@ -126,9 +128,8 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
     [requests, max_steps] int64, the emitted tokens (those of ``path[:, 1:]`` and one more), both -1 behind ``counts`` [requests] int32."""
     ops = _ops()
     if ops.use_kernels(logits):     # the binding makes the same checks
-        f32 = lambda x: x if x is None or x.dtype == torch.float32 else x.float()  # noqa: E731
-        if top_k.dtype != torch.int32:
-            top_k = top_k.to(torch.int32)
+        f32 = lambda x: None if x is None else x.float().contiguous()  # noqa: E731
+        top_k = top_k.to(torch.int32).contiguous()
         return ops.ext().tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, f32(temperature), top_k, f32(top_p), f32(min_p),
                                                  f32(uniform), f32(uniform_final), int(max_steps), draft_probs)
     what = "tree_speculative_sample"
@@ -156,7 +157,8 @@ def tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, co
     """Brings the cache rows of accepted nodes together, in place and in every plane of ``store`` [.., slots, features] (contiguous; a pool's
     storage of all layers): for i below ``counts[b]``, what node ``path[b, i]`` of request b has in its slot goes to the slot of node i.
     ``path`` [requests, steps] and ``counts`` [requests] are those of :func:`tree_speculative_sample`: a path rises from node 0 on, what
-    stands behind ``counts`` is not read.  The request then holds ``prefix_lens + counts`` tokens."""
+    stands behind ``counts`` is not read.  The request then holds ``prefix_lens + counts`` tokens.  A request appears once in a call, and no two
+    nodes share a slot."""
     ops = _ops()
     if ops.use_kernels(store):      # the binding makes the same checks
         return ops.ext().tree_kv_compact(store, req_to_token, req_pool_indices, prefix_lens, path, counts)

@@ -166,6 +166,18 @@ def test_refused_prologue_rows_and_samples():
             ops.tree_speculative_sample(*{**s, **change}.values())
 
 
+def test_refused_numbers_of_heads():
+    c, kw, call = _case("attention")
+    c["q"] = c["q"][:, :0]
+    with pytest.raises(ValueError):
+        call()
+    c, _, _ = _case("prologue")
+    for hq, hkv in ((0, 4), (8, 0), (-4, 6)):       # the width of the rows fits
+        with pytest.raises(ValueError):
+            ops.tree_qk_norm_rope_kv_write(torch.randn(5, 128), None, None, c["parents"], c["table"], c["req"], c["seq"], c["prefix"], c["start"],
+                                           torch.ones(8), c["k"], c["v"], hq, hkv, 16, 1e-6)
+
+
 @pytest.mark.parametrize("preset", ["qwen3-tiny", "llama-tiny", "qwen2-tiny", "qwen3-moe-tiny"])
 def test_rounds_of_a_model(preset):
     r = Round(preset, "cpu", "float32")

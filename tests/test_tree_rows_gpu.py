@@ -103,3 +103,56 @@ def test_rows_of_bad_paths_stay():
     with pytest.raises(RuntimeError, match="out of range"):
         ops.check_status()
     assert torch.equal(store, before)
+
+
+def test_refusals_of_device_tensors():
+    """What the binding refuses before anything is launched."""
+    c = tree_batch([4, 2], [3, 2], 4, 2, 64)
+    ix = (c["parents"], c["table"], c["req"], c["seq"], c["prefix"], c["start"])
+    inv, qkv, n0 = torch.ones(32, device="cuda"), torch.zeros(5, 512, device="cuda", dtype=torch.bfloat16), ops.launch_count()
+
+    def prologue(qkv=qkv, ix=ix, inv=inv, k=c["k"], v=c["v"], hq=4, hkv=2, hd=64, gain=None, delta=None):
+        ops.tree_qk_norm_rope_kv_write(qkv, gain, None, *ix, inv, k, v, hq, hkv, hd, 1e-6, delta)
+
+    def attention(q=c["q"], k=c["k"], v=c["v"], ix=ix, **kw):
+        ops.attention_tree(q, k, v, *ix[1:], ix[0], 1.0, **kw)
+
+    changed = lambda i, x: ix[:i] + (x,) + ix[i + 1:]  # noqa: E731
+    short = changed(3, c["seq"][:1]), changed(0, c["parents"].long()), changed(1, c["table"].t()), changed(2, c["req"].cpu())
+    calls = [lambda x=x: prologue(ix=x) for x in short] + [lambda x=x: attention(ix=x) for x in short]
+    calls += [lambda: prologue(qkv=qkv.float()), lambda: prologue(qkv=qkv[:, :448]), lambda: prologue(hq=0, hkv=4), lambda: prologue(hq=8, hkv=0),
+              lambda: prologue(hd=32), lambda: prologue(inv=inv[:5]), lambda: prologue(inv=inv.double()), lambda: prologue(k=c["k"][:, :1]),
+              lambda: prologue(k=c["k"].half()), lambda: prologue(gain=torch.ones(64, device="cuda")), lambda: prologue(delta=inv[:2]),
+              lambda: attention(q=c["q"][:, :0]), lambda: attention(q=c["q"][:, :3]), lambda: attention(q=c["q"].float()),
+              lambda: attention(q=c["q"][..., :32]), lambda: attention(k=c["k"].half()), lambda: attention(v=c["v"][:-1]),
+              lambda: attention(window=-1), lambda: attention(window=3, chunk=3), lambda: attention(sink=inv[:3]),
+              lambda: attention(out=torch.empty_like(c["q"]).half())]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    rows = dict(store=torch.zeros(2, 9, 4, device="cuda"), table=ints([[1, 2, 3, 4]]), req=ints([0]), prefix=ints([0]), path=ints([[0, 2]]), counts=ints([2]))
+    calls += [lambda x=x: ops.tree_kv_compact(*{**rows, **x}.values())
+              for x in (dict(store=torch.zeros(2, 9, 3, device="cuda")), dict(path=ints([0, 2])), dict(path=ints([[0, 2]]).long()),
+                        dict(counts=ints([2, 2])), dict(prefix=ints([0]).cpu()))]
+    f = lambda *n: torch.zeros(n, device="cuda")  # noqa: E731
+    s = dict(logits=f(3, 8), tokens=f(3).long(), parents=ints([-1, 0, 0]), lens=ints([3]), start=ints([0]), t=f(1), k=ints([0]), p=f(1), m=None, u=f(3),
+             uf=f(1), steps=3, draft=None)
+    calls += [lambda x=x: ops.tree_speculative_sample(*{**s, **x}.values())
+              for x in (dict(logits=f(8, 3).t()), dict(logits=f(3, 8).double()), dict(logits=f(3, 0)), dict(tokens=f(3)), dict(parents=ints([-1, 0])),
+                        dict(lens=ints([3, 1])), dict(t=f(2)), dict(u=f(2)), dict(uf=f(3)), dict(steps=0), dict(draft=f(3, 7)),
+                        dict(draft=f(3, 8).double()), dict(m=f(2)), dict(u=f(3).cpu()))]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    assert ops.launch_count() == n0
+
+
+def test_parameters_for_all_requests_at_once():
+    """Expanded vectors, other types."""
+    g = torch.Generator().manual_seed(1)
+    logits, u = torch.randn(4, 50, generator=g).cuda(), torch.rand(4, generator=g).cuda()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    fixed = (logits, torch.tensor([1, 2, 3, 4], device="cuda"), ints([-1, 0, -1, 0]), ints([2, 2]), ints([0, 2]))
+    one = lambda x, t=torch.float32: torch.tensor([x], dtype=t, device="cuda").expand(2)  # noqa: E731
+    a = ops.tree_speculative_sample(*fixed, one(0.5, torch.float64), one(9, torch.int64), one(0.75), one(0.0), u, u[:2], 2)
+    b = ops.tree_speculative_sample(*fixed, one(0.5).contiguous(), ints([9, 9]), one(0.75).contiguous(), None, u, u[:2], 2)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
