@@ -39,7 +39,6 @@ namespace {
 
 constexpr int kRows = 128;                 // MMA M
 constexpr int kTile = 64;                  // tokens of a tile
-constexpr int kSoftmaxRegs = 128;          // registers of the threads that hold rows; the others give back what that takes
 constexpr int kStart = 4;                  // tiles' time that every unit costs beside its tiles
 constexpr int kNoToken = -0x7fffffff;
 constexpr int kParents = 256;              // nodes whose parents are kept in shared memory
@@ -163,9 +162,9 @@ struct Cfg {
   static constexpr int kRaw = KV8 ? kTile * kD : 0;        // an item as it is cached, one per team
   static constexpr int kSmem = kQBytes + kStages * kStage + kTeams * kRaw;
   static constexpr int kPerSm = NH == 4 || R == 2 ? 1 : 2;
-  // registers that a CTA is launched with and what the threads without rows keep; 256 features have one CTA and need no split
+  // registers that a CTA is launched with, those of the threads that hold rows, and what the others keep; 256 features have one CTA and need no split
   static constexpr bool kSplit = NH < 4;
-  static constexpr int kLaunchRegs = R == 1 ? 80 : 96, kOtherRegs = R == 1 ? 56 : 72;
+  static constexpr int kLaunchRegs = R == 1 ? 80 : 96, kSoftmaxRegs = 128, kOtherRegs = R == 1 ? 56 : 72;
   static_assert(32 * (kSoftmaxWarps * kSoftmaxRegs + (kThreads / 32 - kSoftmaxWarps) * kOtherRegs) <= kThreads * kLaunchRegs, "register split");
   static_assert(kPerSm * (kSmem + 2048) <= 228 * 1024, "1 KB of each CTA is the system's, 1 KB the kernel's variables");
   // tensor memory: two score buffers of 64 columns a row tile, then O of each
@@ -368,8 +367,8 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
         for (; i < items; i += C::kTeams) {
           const uint32_t item = item0 + i, st = item % kStages;
           const uint32_t stage = smem_u32(ring) + st * C::kStage, raw = smem_u32(ring) + kStages * C::kStage + team * C::kRaw;
-          auto wait_free = [&]() {
-            if (item >= kStages && !mbar_wait(&empty[st], (item / kStages - 1) & 1, &fail_flag)) ok = false;
+          auto wait_free = [&]() {       // asleep in between: warps that poll take issue slots from the softmax (e4m3, 16 nodes: 52.9 -> 49.6 us)
+            if (item >= kStages && !mbar_wait_relaxed(&empty[st], (item / kStages - 1) & 1, 20)) ok = false;
             return ok = __all_sync(0xffffffffu, ok);
           };
           if (!KV8 && !wait_free()) return false;
@@ -462,7 +461,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
       bool ok = true;
       uint32_t seg = 0;
       segments([&](const Place& w, const Request& r, int, int, bool) {
-        if (seg > 0 && !mbar_wait(q_free, (seg - 1) & 1, &fail_flag)) ok = false;
+        if (seg > 0 && !mbar_wait_relaxed(q_free, (seg - 1) & 1)) ok = false;
         if (!(ok = __all_sync(0xffffffffu, ok))) return false;
         const int n0 = w.u * p.unit_nodes, rows = min(p.unit_nodes, r.nodes - n0) * g, half = p.tpt * g;     // half: rows of a tile
         const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(r.row + n0) * p.q_stride + static_cast<int64_t>(w.hk) * g * kD;
@@ -544,7 +543,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
     }
   } else {
     // =============================== softmax ===============================
-    if constexpr (C::kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    if constexpr (C::kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
     const int half = R > 1 ? warp >> 2 : 0, in_tile = tid & 127;      // row tile and row
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tmem_o = tmem + C::kScoreCols + half * kD + lane_base;
@@ -885,9 +884,9 @@ int launch_type(const TreeParams& p, int head_dim, int fmt, cudaStream_t s) {
 TreePlan tree_plan(int head_dim, int group, int64_t rows, int64_t batch, int num_sms) {
   TreePlan plan;
   // Row tiles that a CTA takes side by side: two where a request has more rows than one tile on average.  Two tiles against one, 16 requests
-  // of 4096 tokens, 8 query heads over a kv head, 128 features: 24 nodes (192 rows) 59.1 / 82.3 us with e4m3 caches, which are widened
-  // half as often, and 59.9 / 62.8 us in bf16; 16 nodes (128 rows) 55.7 / 52.9 and 54.8 / 47.5.  Heads of 64: 54.7 / 54.2 and 50.0 / 53.6 at 24
-  // nodes, 54.0 / 42.3 and 48.8 / 42.0 at 17: always one.
+  // of 4096 tokens, 8 query heads over a kv head, 128 features: 24 nodes (192 rows) 59.1 / 76.5 us with e4m3 caches, which are widened
+  // half as often, and 58.4 / 62.5 us in bf16; 17 nodes 56.8 / 58.9 and 55.5 / 51.9; 16 nodes (128 rows) 56.0 / 49.6 and 54.1 / 47.2.  Heads of
+  // 64: 54.7 / 54.2 and 50.0 / 53.6 at 24 nodes, 54.0 / 42.3 and 48.8 / 42.0 at 17: always one.
   plan.row_tiles = head_dim == 128 && rows > batch * (kRows / group) ? 2 : 1;
   plan.ctas = head_dim == 256 || plan.row_tiles == 2 ? num_sms : 2 * num_sms;
   plan.part_rows = static_cast<int>(std::min<int64_t>(plan.row_tiles * (kRows / group * group), rows * group));

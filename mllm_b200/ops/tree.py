@@ -128,8 +128,9 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
     [requests, max_steps] int64, the emitted tokens (those of ``path[:, 1:]`` and one more), both -1 behind ``counts`` [requests] int32."""
     ops = _ops()
     if ops.use_kernels(logits):     # the binding makes the same checks
-        f32 = lambda x: None if x is None else x.float().contiguous()  # noqa: E731
-        top_k = top_k.to(torch.int32).contiguous()
+        f32 = lambda x: x if x is None or x.dtype == torch.float32 and x.is_contiguous() else x.float().contiguous()  # noqa: E731
+        if top_k.dtype != torch.int32 or not top_k.is_contiguous():
+            top_k = top_k.to(torch.int32).contiguous()
         return ops.ext().tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, f32(temperature), top_k, f32(top_p), f32(min_p),
                                                  f32(uniform), f32(uniform_final), int(max_steps), draft_probs)
     what = "tree_speculative_sample"
