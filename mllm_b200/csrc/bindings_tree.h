@@ -124,6 +124,7 @@ void check_gain(const c10::optional<Tensor>& g, const Tensor& like, int64_t n, c
   if (!g.has_value()) return;
   CHECK_ARG(g->device() == like.device() && g->scalar_type() == like.scalar_type() && g->is_contiguous() && g->numel() == n, "mllm_b200: ",
               name, " must be a contiguous vector of ", n, " elements like the rows");
+  CHECK_ARG((reinterpret_cast<uintptr_t>(g->data_ptr()) & 15) == 0, "mllm_b200: ", name, " must begin on a 16-byte boundary");
 }
 
 Tensor tree_qk_norm_rope_kv_write(const Tensor& qkv, const c10::optional<Tensor>& q_gain, const c10::optional<Tensor>& k_gain,
