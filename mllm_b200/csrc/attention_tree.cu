@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
   using C = Cfg<NH, KV8, R>;
   constexpr int kD = C::kD, kStages = C::kStages, kIssueWarp = C::kIssueWarp, kSoft = C::kSoftmaxWarps;
   extern __shared__ __align__(1024) uint8_t tree_smem[];
-  __shared__ uint64_t bars[2 * C::kStages + 6 + 2 * R];
+  __shared__ uint64_t bars[2 * C::kStages + 7 + 2 * R];
   __shared__ uint32_t tmem_holder;
   __shared__ int fail_flag, poison;
   __shared__ int16_t parents[kParents];
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
   uint64_t* o_done = p_full + 2 * R;
   uint64_t* q_full = o_done + 2;         // the warps that copy Q
   uint64_t* q_free = q_full + 1;         // tcgen05.commit: the segment's last scores
+  uint64_t* soft = q_free + 1;           // the softmax warps among themselves; not a named barrier, which would wait for a warp that gave up
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait_loads();
@@ -274,6 +275,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
       }
       mbar_init(q_full, C::kQWarps);
       mbar_init(q_free, 1);
+      mbar_init(soft, kSoft);
       fence_barrier_init();
     }
     __syncwarp();
@@ -550,7 +552,13 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
     const int tile_node = node_of(in_tile), row_node = half * p.tpt + tile_node, row = half * p.tpt * g + in_tile;    // row of the unit
     const bool capped = p.cap_out > 0.f;
     bool ok = true, bad = false;
-    uint32_t tile = 0;
+    uint32_t tile = 0, met = 0;
+    auto meet = [&]() {        // of all softmax warps; false where one has given up
+      __syncwarp();
+      if (lane == 0) mbar_arrive(soft);
+      if (!mbar_wait(soft, met++ & 1, &fail_flag)) ok = false;
+      return ok = __all_sync(0xffffffffu, ok);
+    };
     int job_rows = 0, job_row = 0, job_head = 0, job_tiles = 0;
     segments([&](const Place& w, const Request& r, int n_all, int n, bool first) {
       const int node = w.u * p.unit_nodes + row_node;
@@ -568,9 +576,9 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
         return up;
       };
       if (masks) {        // parents to shared memory; one that is no earlier node counts as none
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoft) : "memory");          // the segment before has read them
+        if (!meet()) return false;          // the segment before has read them
         for (int i = tid; i < min(r.nodes, kParents); i += 32 * kSoft) parents[i] = static_cast<int16_t>(parent_in(i));
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoft) : "memory");
+        if (!meet()) return false;
       }
       auto parent_of = [&](int i) { return i < kParents ? static_cast<int>(parents[i]) : parent_in(i); };
       int pos = r.prefix, low = 0;
