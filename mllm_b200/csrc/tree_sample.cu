@@ -105,22 +105,29 @@ __device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xo
 
 // The weight e of a token: above 2^-12 in 64 bits, below in 32.
 struct Scale {
-  float mx, c_hi, c_lo;     // log2(e) / T as two floats
+  // A largest logit of infinity: infinite logits have weight 1, all others none.  Differences are then taken from the largest finite
+  // number, with both parts of the factor 1: log2_of gives infinity for infinite logits, which no sum of loops over tokens has to look for.
+  float mx, off, c_hi, c_lo;     // largest logit; it, or the largest finite number; log2(e) / T as two floats
   double inv_t, mx_d;
+  __device__ __forceinline__ Scale(float largest, float temp) : mx(largest), off(fminf(largest, 3.402823466e38f)), inv_t(1.0 / static_cast<double>(temp)), mx_d(largest) {
+    const double c = 1.4426950408889634 * inv_t;
+    c_hi = mx == off ? static_cast<float>(c) : 1.f;
+    c_lo = mx == off ? static_cast<float>(c - static_cast<double>(c_hi)) : 1.f;
+  }
   __device__ __forceinline__ float log2_of(float x) const {
-    const float d = fmaxf(x - mx, -1e30f);      // a value that is no number, or minus infinity: no weight
+    const float d = fmaxf(x - off, -1e30f);      // a value that is no number, or minus infinity: no weight
     return fmaf(d, c_hi, d * c_lo);
   }
   __device__ __forceinline__ double large(float x) const { return x == mx ? 1.0 : exp((static_cast<double>(x) - mx_d) * inv_t); }
   __device__ __forceinline__ double operator()(float x) const {
     if (!(x == x)) return 0.0;
     const float t = log2_of(x);
-    return t > -12.f || x == mx ? large(x) : static_cast<double>(fast_exp2(t));
+    return t > -12.f ? large(x) : static_cast<double>(fast_exp2(t));
   }
   // adds it to a sum of two parts, for loops over all tokens
   __device__ __forceinline__ void add(float x, double& big, float& small) const {
     const float t = log2_of(x);
-    if (t > -12.f || x == mx) big += large(x);
+    if (t > -12.f) big += large(x);
     else small += fast_exp2(t);
   }
 };
@@ -416,13 +423,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) tree_sample_kernel(const Sam
       continue;
     }
 
-    Scale w;
-    w.mx = mx;
-    w.mx_d = mx;
-    w.inv_t = 1.0 / static_cast<double>(temp);
-    const double c = 1.4426950408889634 * w.inv_t;
-    w.c_hi = static_cast<float>(c);
-    w.c_lo = static_cast<float>(c - static_cast<double>(w.c_hi));
+    const Scale w(mx, temp);
     const int groups = (n + 7) / 8;          // of eight tokens; minus infinity behind the last token
     auto eight = [&](int i, float (&x)[8]) {
       if constexpr (sizeof(T) == 2) {
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) tree_sample_kernel(const Sam
             float test[kMore], small[kMore] = {};
             double sums[kMore] = {}, none = 0.0, none2 = 0.0;
 #pragma unroll
-            for (int j = 0; j < kMore; ++j) test[j] = (j + 1) * step < span ? Keys<T>::value(at + (j + 1) * step) : INFINITY;
+            for (int j = 0; j < kMore; ++j) test[j] = (j + 1) * step < span ? Keys<T>::value(at + (j + 1) * step) : NAN;
             for (int i = tid; i < groups; i += kThreads) {
               float x[8], x_top = -INFINITY;
               eight(i, x);

@@ -1,0 +1,60 @@
+"""Verification of drafted token trees where logits are infinite, absent or equal, and where most of the mass lies in small weights."""
+import pytest
+import torch
+
+from mllm_b200 import ops
+from mllm_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+INF, NAN = float("inf"), float("nan")
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def both(logits, tokens, parents, u, u_final, draft=None, t=1.0, k=0, p=1.0, m=0.0, steps=3):
+    """One tree; the kernel's answer, which has to be the statement's."""
+    f = lambda x: torch.tensor(x, device="cuda", dtype=torch.float32)  # noqa: E731
+    args = (logits, torch.tensor(tokens, device="cuda"), ints(parents), ints([len(tokens)]), ints([0]), f([t]), ints([k]), f([p]), f([m]), f(u),
+            f([u_final]), steps, draft)
+    got = ops.tree_speculative_sample(*args)
+    ops.check_status()
+    want = ref.tree_speculative_sample(*args)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)), (got, want)
+    n = int(got[2])
+    return got[0][0, :n].tolist(), got[1][0, :n].tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kw", [dict(), dict(m=0.5), dict(t=0.5), dict(k=5), dict(p=0.9), dict(k=1), dict(t=30.0)])
+def test_two_infinite_logits_share_the_mass(dtype, kw):
+    V = 20000
+    logits = torch.randn(2, V, generator=torch.Generator().manual_seed(0)).cuda().to(dtype)
+    logits[0, [70, 15000]] = INF
+    logits[0, 71] = torch.finfo(dtype).max
+    logits[1, 3] = 60.0
+    # a picked candidate: taken below a half (what comes behind it is for the statement to say: a temperature of 30 leaves row 1 flat)
+    path, out = both(logits, [0, 15000], [-1, 0], [0, 0.49], 0.2, **kw)
+    assert path == [0, 1] and out[0] == 15000
+    assert both(logits, [0, 15000], [-1, 0], [0, 0.51], 0.2, **kw) == ([0], [70])
+    assert both(logits, [0, 71], [-1, 0], [0, 0.0], 0.6, **kw) == ([0], [15000])
+    # a drawn one: taken below 0.5 / 0.8, and p - q leaves the other token
+    q = torch.zeros(2, V, device="cuda")
+    q[0, 70], q[0, 9] = 0.8, 0.2
+    path, out = both(logits, [0, 70], [-1, 0], [0, 0.62], 0.2, q, **kw)
+    assert path == [0, 1] and out[0] == 70
+    assert both(logits, [0, 70], [-1, 0], [0, 0.63], 0.2, q, **kw) == ([0], [15000])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kw", [dict(), dict(p=0.7), dict(k=4500), dict(k=4500, p=0.7), dict(k=12, p=0.1)])
+def test_more_infinite_logits_than_are_sorted(dtype, kw):
+    V, n = 40000, 5000
+    logits = torch.randn(2, V, generator=torch.Generator().manual_seed(1)).cuda().to(dtype)
+    places = torch.randperm(V, generator=torch.Generator().manual_seed(2))[:n].sort().values
+    logits[0, places.cuda()] = INF
+    token = int(places[n // 2])
+    assert both(logits, [0, token], [-1, 0], [0, 1.5 / n], 0.5, **kw)[0] == [0]
+    assert both(logits, [0, token], [-1, 0], [0, 0.5 / n], 0.5, **kw)[1][0] == token
+    assert both(logits[:1], [0], [-1], [0], 10.5 / n, steps=1, **kw) == ([0], [int(places[10])])
