@@ -85,10 +85,11 @@ __device__ __forceinline__ uint32_t ld_cluster32(uint32_t a) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
-// order of floats as order of whole numbers; a value that is no number is below all others
+// Order of floats as order of whole numbers; a value that is no number counts as minus infinity, and zeros are alike.
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x);
-  return x != x ? 0u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  if (x != x) return 0x007fffffu;
+  return x == 0.f ? 0x80000000u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 // The same for values of T: numbers without the bits that T does not have, and back.
 template <typename T>

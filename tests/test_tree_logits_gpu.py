@@ -58,3 +58,34 @@ def test_more_infinite_logits_than_are_sorted(dtype, kw):
     assert both(logits, [0, token], [-1, 0], [0, 1.5 / n], 0.5, **kw)[0] == [0]
     assert both(logits, [0, token], [-1, 0], [0, 0.5 / n], 0.5, **kw)[1][0] == token
     assert both(logits[:1], [0], [-1], [0], 10.5 / n, steps=1, **kw) == ([0], [int(places[10])])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("t", [0.0, 1.0])
+def test_rows_without_a_finite_logit_give_their_first_token(dtype, t):
+    V = 17000
+    for fill, other, places in ((NAN, -INF, range(1, V)), (-INF, NAN, range(1, 9000)), (-INF, NAN, [0]), (NAN, NAN, [0]), (NAN, -INF, [V - 1])):
+        logits = torch.full((2, V), fill, device="cuda", dtype=dtype)
+        logits[:, list(places)] = other
+        for kw in (dict(), dict(k=7), dict(p=0.5)):
+            assert both(logits, [0, 0], [-1, 0], [0, 0.5], 0.9, t=t, **kw) == ([0, 1], [0, 0])
+            assert both(logits, [0, 1], [-1, 0], [0, 0.5], 0.9, t=t, **kw) == ([0], [0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_zeros_of_both_signs_are_a_tie(dtype):
+    V = 17000
+    logits = torch.full((1, V), -1.0, device="cuda", dtype=dtype)
+    logits[0, 9001], logits[0, 40] = 0.0, -0.0
+    assert both(logits, [0], [-1], [0], 0.9, t=0.0) == ([0], [40])
+    logits[0, 5] = 0.0
+    assert both(logits, [0], [-1], [0], 0.9, t=0.0) == ([0], [5])
+    # a cut at the zeros keeps all of them
+    for kw in (dict(k=1), dict(k=2), dict(p=0.0), dict(m=1.0)):
+        for u, token in ((0.3, 5), (0.5, 40), (0.9, 9001)):
+            assert both(logits, [0], [-1], [0], u, t=0.2, **kw) == ([0], [token])
+    # a flat row of zeros: more than are sorted
+    logits[0, ::2] = -0.0
+    logits[0, 1::2] = 0.0
+    for kw in (dict(k=1), dict(k=6000), dict(p=0.5), dict(m=1.0)):
+        assert both(logits, [0], [-1], [0], 0.25, **kw) == ([0], [V // 4])
