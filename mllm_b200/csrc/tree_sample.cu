@@ -687,10 +687,23 @@ __global__ void __launch_bounds__(kThreads, PER_SM) tree_sample_kernel(const Sam
       }
     }
 
-    // What eight kept tokens have left after k rejections (with probabilities), added to `sum`.  In 64 bits where the weight or the
-    // draft's probability is above 2^-12.
+    // What a kept token has left after k rejections with probabilities, added to a sum of two parts: in 64 bits where the weight or the
+    // draft's probability is above 2^-12.  The sums and the draw share it: a thread that has mass has a token.
+    auto add_left = [&](float x, float q, int k, double& big, float& small) {
+      const float t = w.log2_of(x);
+      if (t > -12.f || q > 2.44140625e-4f) {
+        double v = w(x);
+        for (int j = 0; j < k && v > 0.0; ++j) v = fmax(v * sh.scale[j] - q, 0.0);
+        big += v;
+      } else {
+        float v = fast_exp2(t);
+        for (int j = 0; j < k && v > 0.f; ++j) v = fmaxf(fmaf(v, static_cast<float>(sh.scale[j]), -q), 0.f);
+        small += v;
+      }
+    };
     const float* draft = p.draft != nullptr ? p.draft + row * p.draft_stride + v0 : nullptr;
     const bool wide = (reinterpret_cast<uintptr_t>(draft) & 15) == 0;
+    // of eight tokens, added to `sum`
     auto left_of_eight = [&](int g, int k, double& sum) {
       float x[8], x_top = -INFINITY;
       eight(g, x);
@@ -707,19 +720,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) tree_sample_kernel(const Sam
       }
       float small = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!(x[e] >= x_cut)) continue;
-        const float t = w.log2_of(x[e]);
-        if (t > -12.f || q[e] > 2.44140625e-4f) {
-          double v = w(x[e]);
-          for (int j = 0; j < k && v > 0.0; ++j) v = fmax(v * sh.scale[j] - q[e], 0.0);
-          sum += v;
-        } else {
-          float v = fast_exp2(t);
-          for (int j = 0; j < k && v > 0.f; ++j) v = fmaxf(fmaf(v, static_cast<float>(sh.scale[j]), -q[e]), 0.f);
-          small += v;
-        }
-      }
+      for (int e = 0; e < 8; ++e)
+        if (x[e] >= x_cut) add_left(x[e], q[e], k, sum, small);
       sum += static_cast<double>(small);
     };
 
@@ -790,17 +792,15 @@ __global__ void __launch_bounds__(kThreads, PER_SM) tree_sample_kernel(const Sam
       auto weight = [&](int i) {
         const float x = to_f32(xs[i]);
         if (!(x >= x_cut)) return 0.0;
-        double v = w(x);
         if (draft != nullptr) {
-          if (rejected > 0) {
-            const double q = __ldcg(draft + i);
-            for (int j = 0; j < rejected && v > 0.0; ++j) v = fmax(v * sh.scale[j] - q, 0.0);
-          }
-        } else {
-          for (int k = 0; k < rejected; ++k)
-            if (sh.removed[k] == v0 + i) v = 0.0;
+          double big = 0.0;
+          float small = 0.f;
+          add_left(x, rejected > 0 ? __ldcg(draft + i) : 0.f, rejected, big, small);
+          return big + small;
         }
-        return v;
+        for (int k = 0; k < rejected; ++k)
+          if (sh.removed[k] == v0 + i) return 0.0;
+        return w(x);
       };
       // neighbouring tokens, a thread's share of them
       const int per = (groups + kThreads - 1) / kThreads, g0 = min(groups, tid * per), g1 = min(groups, g0 + per);
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) tree_sample_kernel(const Sam
               }
             }
           }
-          p.out[static_cast<int64_t>(b) * p.steps + count] = v0 + (pick >= 0 ? pick : last);
+          p.out[static_cast<int64_t>(b) * p.steps + count] = last < 0 ? first_best : v0 + (pick >= 0 ? pick : last);
         }
       } else if (winner < 0 && rank == 0 && tid == 0) {
         p.out[static_cast<int64_t>(b) * p.steps + count] = first_best;      // nothing left to draw from

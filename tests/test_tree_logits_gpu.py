@@ -89,3 +89,26 @@ def test_zeros_of_both_signs_are_a_tie(dtype):
     logits[0, 1::2] = 0.0
     for kw in (dict(k=1), dict(k=6000), dict(p=0.5), dict(m=1.0)):
         assert both(logits, [0], [-1], [0], 0.25, **kw) == ([0], [V // 4])
+
+
+def test_a_draft_that_is_the_target_up_to_rounding():
+    """Every candidate refused, and what p - q leaves is rounding alone: whatever is emitted is a token that the filters keep."""
+    n, V = 20000, 24
+    g = torch.Generator().manual_seed(9)
+    logits = torch.full((n, V), -INF)
+    places = torch.stack([torch.randperm(V, generator=g)[:3] for _ in range(n)])
+    values = torch.cat([torch.zeros(n, 1), -9.0 - 4.0 * torch.rand(n, 2, generator=g)], dim=1)
+    logits.scatter_(1, places, values)
+    q = torch.softmax(logits.double(), dim=-1).float()
+    first = places[:, :1]
+    q.scatter_(1, first, torch.nextafter(q.gather(1, first), torch.ones(n, 1)))        # refused by the largest random number below 1
+    two = lambda t: t.repeat_interleave(2, dim=0).contiguous().cuda()  # noqa: E731
+    ones = torch.ones(n, device="cuda")
+    u = torch.full((2 * n,), 1 - 2 ** -24, device="cuda")
+    path, out, counts = ops.tree_speculative_sample(
+        two(logits), two(first[:, 0]), ints([-1, 0]).repeat(n), ints([2]).repeat(n), 2 * torch.arange(n, dtype=torch.int32, device="cuda"), ones,
+        ints([0]).repeat(n), ones, None, u, torch.rand(n, generator=g).cuda(), 2, two(q))
+    ops.check_status()
+    emitted = out[:, 0].cpu()
+    assert (emitted >= 0).all() and (emitted < V).all()
+    assert torch.isfinite(logits.gather(1, emitted[:, None])).all()
