@@ -504,10 +504,14 @@ __global__ void __launch_bounds__(kThreads, PER_SM) tree_sample_kernel(const Sam
         bound = from;
       } else if (cut_p) {
         // the mass above some levels: the highest that holds what top_p wants is a better bound
+        // (which tokens a full list lacks, and the order of a list, are left to chance: from the row itself then, and of whole
+        // multiples of 2^-40, whose sums are exact in any order)
         double above[kMore] = {}, none = 0.0, none2 = 0.0;
-        for (int i = tid; i < min(sh.list_n, kList); i += kThreads) {
-          const float x = list[i];
-          const double v = w(x);
+        const bool in_list = sh.list_n <= kList;
+        for (int i = tid; i < (in_list ? sh.list_n : n); i += kThreads) {
+          const float x = in_list ? list[i] : to_f32(xs[i]);
+          if (!(x >= mx - kMore * kLevelStep * temp)) continue;
+          const double v = floor(w(x) * 0x1p40) * 0x1p-40;
 #pragma unroll
           for (int l = 0; l < kMore; ++l)
             if (x >= mx - (l + 1) * kLevelStep * temp) above[l] += v;

@@ -112,3 +112,22 @@ def test_a_draft_that_is_the_target_up_to_rounding():
     emitted = out[:, 0].cpu()
     assert (emitted >= 0).all() and (emitted < V).all()
     assert torch.isfinite(logits.gather(1, emitted[:, None])).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_lists_that_overflow_give_the_same_walk_every_time(dtype):
+    """More tokens within reach of top-p's first guess than a list holds, mass in all of them; random numbers near borders."""
+    B, V = 48, 60000
+    g = torch.Generator().manual_seed(3)
+    logits = (12 * torch.rand(B, V, generator=g)).cuda().to(dtype)
+    logits[::3, :200] += 3
+    f = lambda x: torch.tensor(x, device="cuda", dtype=torch.float32)  # noqa: E731
+    args = (logits, torch.zeros(B, dtype=torch.int64, device="cuda"), ints([-1] * B), ints([1] * B), torch.arange(B, dtype=torch.int32, device="cuda"),
+            f([1.0] * B), ints([(0, 9000)[i % 2] for i in range(B)]), f([0.3 + 0.69 * i / B for i in range(B)]), None, f([0.0] * B),
+            torch.rand(B, generator=g).cuda(), 1)
+    first = ops.tree_speculative_sample(*args)
+    want = ref.tree_speculative_sample(*args)
+    assert all(torch.equal(a, b) for a, b in zip(first, want))
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(first, ops.tree_speculative_sample(*args)))
+    ops.check_status()
