@@ -21,6 +21,7 @@
 //   * the first four warps (eight) hold a row per thread: online maximum and sum in fp32, P over S in place.  Masks are 64-bit words per
 //     row and tile, made only in tiles that hold tree nodes or a window's edge: cached part by comparison, tree part by a walk to the
 //     root over parents in shared memory.
+// A token whose slot lies outside the cache is nowhere visible; a row that sees no token at all is zero.
 // A value that is no number must not reach rows that do not see it (0 x NaN): in masked tiles the warps that copied V set such elements to
 // zero, and they are added at the end to the rows that see them.
 //
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
   extern __shared__ __align__(1024) uint8_t tree_smem[];
   __shared__ uint64_t bars[2 * C::kStages + 7 + 2 * R];
   __shared__ uint32_t tmem_holder;
-  __shared__ int fail_flag, poison;
+  __shared__ int fail_flag, poison, holes;
   __shared__ int16_t parents[kParents];
   __shared__ int begin_of[3];
   __shared__ Request begin_request;
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
       ctas_of = used;
       fail_flag = 0;
       poison = 0;
+      holes = 0;
     }
     int64_t at = (incl - mine) * p.hkv;
     if (begin < end && begin >= at && begin < incl * p.hkv) {
@@ -448,6 +450,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
           }
           if (KV8 || look) fence_proxy_async_smem();
           if (found) poison = 1;            // for the rest of the run: the rows' ends look for themselves
+          if (bad) holes = 1;               // likewise, the softmax warps at every tile
           __syncwarp();
           if (lane == 0) mbar_arrive(&full[st]);
         }
@@ -612,6 +615,18 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
         return m;
       };
 
+      // rare: bit c: token col0 + c has a slot
+      auto present = [&](int col0) -> uint64_t {
+        uint64_t m = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int tok = col0 + 32 * h + lane;
+          const int s = tok < len ? __ldcg(p.ix.req_to_token + static_cast<int64_t>(r.table) * p.ix.table_stride + tok) : -1;
+          m |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, s >= 0 && s < p.num_slots)) << (32 * h);
+        }
+        return m;
+      };
+
       float m_used = -INFINITY;   // maximum in use for the exponent (log2 domain)
       uint64_t sums[4] = {0, 0, 0, 0};      // pairs of fp32
       for (int t = 0; t < n; ++t) {
@@ -634,8 +649,10 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
             for (int c = 0; c < kTile; ++c)
               raw[c] = __float_as_uint(p.cap_out * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(raw[c]) * p.cap_in))));
           }
-          if (masked) {
-            const uint64_t vis = visible(col0);
+          const bool gaps = __any_sync(0xffffffffu, holes != 0);
+          if (masked || gaps) {
+            uint64_t vis = masked ? visible(col0) : ~0ull;
+            if (gaps) vis &= present(col0);
 #pragma unroll
             for (int c = 0; c < kTile; ++c) raw[c] = (vis >> c) & 1 ? raw[c] : __float_as_uint(-INFINITY);
           }
@@ -697,7 +714,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
       const int head = w.hk * g + row - row_node * g;
       const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
       float l = both.x + both.y;
-      if (whole && p.sink != nullptr && valid) l += exp2f(p.sink[head] * kLog2e - m_used);
+      if (whole && p.sink != nullptr && valid && m_used > -INFINITY) l += exp2f(p.sink[head] * kLog2e - m_used);
       const float inv = l == 0.f ? 0.f : 1.f / l;       // 0: no key seen.  A sum that is no number shows
       const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1);
       if (masks && poison != 0) {       // rare: every masked tile's values once more, for those that are no numbers
@@ -820,7 +837,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_tree_join_kernel(const T
     float top = sink;
 #pragma unroll 4
     for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(p.part_lse + slot(c) * p.part_rows + r));
-    float den = p.sink != nullptr ? exp2f(sink - top) : 0.f, acc[kJoinFeatures] = {};
+    float den = sink > -INFINITY ? exp2f(sink - top) : 0.f, acc[kJoinFeatures] = {};
 #pragma unroll 2
     for (int c = c0; c <= c1; ++c) {
       const float lse = __ldcg(p.part_lse + slot(c) * p.part_rows + r);

@@ -87,7 +87,8 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
     """Attention of drafted nodes ``q`` [T, Hq, D] (heads of a node contiguous): each sees the cached tokens, its ancestors and itself.
     ``window``, ``logit_cap``, ``sink`` and ``chunk`` as for :func:`mllm_b200.ops.attention_prefill`, by positions: siblings share theirs.
     Heads of 64, 128 and 256 features, 16-bit, over caches of their type or of unscaled 8-bit floats.  Rows of ``out`` that belong to no
-    request keep what they hold.  A value in the cache that is no number reaches the nodes that see it and no others."""
+    request keep what they hold.  A value in the cache that is no number reaches the nodes that see it and no others.  On the GPU a token whose slot
+    lies outside the cache is seen by none, and a node that sees nothing has a row of zeros."""
     ops = _ops()
     if ops.use_kernels(q):          # the binding makes the same checks
         return ops.ext().attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents,
