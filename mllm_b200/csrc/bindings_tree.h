@@ -1,6 +1,8 @@
 // PyTorch binding of the kernels for drafted token trees, part of the module of latent attention.
 #pragma once
 
+#include <cfloat>
+
 #include "bindings_common.h"
 #include "tree.h"
 
@@ -78,6 +80,8 @@ Tensor attention_tree(const Tensor& q, const Tensor& k_cache, const Tensor& v_ca
   CHECK_ARG(hd == 64 || hd == 128 || hd == 256, "attention_tree: heads of 64, 128 or 256 features, not ", hd);
   CHECK_ARG(window >= 0 && chunk >= 0 && (window == 0 || chunk == 0) && window < (1 << 30) && chunk < (1 << 30),
             "attention_tree: either a sliding window or chunks, of positive lengths");
+  // a row's maximum is taken before its scores are scaled, and a score of minus infinity has to stay one
+  CHECK_ARG(scale >= FLT_MIN && scale <= FLT_MAX, "attention_tree: scale must be positive and finite, not ", scale);
   Tensor out = given.has_value() ? *given : torch::empty(q.sizes(), q.options());
   CHECK_ARG(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1 &&
                 out.stride(1) == hd && out.stride(0) % 8 == 0,

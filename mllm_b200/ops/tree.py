@@ -85,7 +85,7 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
                    out: Optional[torch.Tensor] = None, window: Optional[int] = None, logit_cap: float = 0.0,
                    sink: Optional[torch.Tensor] = None, chunk: Optional[int] = None) -> torch.Tensor:
     """Attention of drafted nodes ``q`` [T, Hq, D] (heads of a node contiguous): each sees the cached tokens, its ancestors and itself.
-    ``window``, ``logit_cap``, ``sink`` and ``chunk`` as for :func:`mllm_b200.ops.attention_prefill`, by positions: siblings share theirs.
+    ``scale`` is positive; ``window``, ``logit_cap``, ``sink`` and ``chunk`` as for :func:`mllm_b200.ops.attention_prefill`, by positions: siblings share theirs.
     Heads of 64, 128 and 256 features, 16-bit, over caches of their type or of unscaled 8-bit floats.  Rows of ``out`` that belong to no
     request keep what they hold.  A value in the cache that is no number reaches the nodes that see it and no others.  On the GPU a token whose slot
     lies outside the cache is seen by none, and a node that sees nothing has a row of zeros."""
@@ -102,6 +102,8 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
         raise ValueError(f"attention_tree: {q.shape[1]} query heads over {hkv} key heads")
     if window is not None and window < 0 or chunk is not None and chunk < 0 or (window and chunk):
         raise ValueError("attention_tree: either a sliding window or chunks, of positive lengths")
+    if not torch.finfo(torch.float32).tiny <= scale <= torch.finfo(torch.float32).max:
+        raise ValueError(f"attention_tree: scale must be positive and finite, not {scale}")
     if sink is not None and (sink.dtype != torch.float32 or sink.shape != (q.shape[1],) or sink.device != q.device):
         raise ValueError(f"attention_tree: sink must be fp32 [{q.shape[1]}] on {q.device}")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1

@@ -1,4 +1,5 @@
-"""Drafted token trees on the GPU: operands that the binding refuses because the kernels could not read them."""
+"""Drafted token trees on the GPU: operands that the binding refuses because the kernels could not read them,
+and numbers that they are not made for."""
 import pytest
 import torch
 
@@ -30,3 +31,20 @@ def test_weights_off_16_byte_boundaries_are_refused(D, which, shift):
     gains[which] = buffer[8:]           # 16 bytes on
     call()
     ops.check_status()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), 1e-42, 1e39])
+def test_scales_that_are_not_positive_are_refused(scale):
+    c = tree_batch([70, 2], [3, 2], 4, 2, 64)
+    args = (c["q"], c["k"], c["v"], c["table"], c["req"], c["seq"], c["prefix"], c["start"], c["parents"])
+    before = ops.launch_count()
+    with pytest.raises(ValueError, match="scale"):
+        ops.attention_tree(*args, scale)
+    assert ops.launch_count() == before
+    # the smallest that is taken: all weights alike
+    got = ops.attention_tree(*args, 2.0 ** -126)
+    ops.check_status()
+    slots = c["table"][int(c["req"][0]), :71].long()
+    want = c["v"][slots].double().mean(0).repeat_interleave(2, dim=0)
+    half = torch.finfo(torch.bfloat16).eps / 2       # weights are 1, sums of 71 in 32 bits, one rounding
+    assert ((got[0].double() - want).abs() <= half * want.abs() + c["v"][slots].double().abs().mean(0).repeat_interleave(2, dim=0) * 71 * 2 ** -24).all()
