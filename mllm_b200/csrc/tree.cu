@@ -82,7 +82,11 @@ __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams
     }
   }
   if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
-  if (b < 0) return;            // a row of no request
+  if (b < 0) {                  // a row of no request: zeros
+    for (int h = part * kHeads + lane / kLanes; h < p.hq; h += step)
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.hq + h) * D + at) = make_uint4(0, 0, 0, 0);
+    return;
+  }
   const int node = t - r.row;
   const int slot = __ldcg(p.ix.req_to_token + r.table * p.ix.table_stride + r.prefix + node);
   const int delta = p.delta != nullptr ? __ldcg(p.delta + b) : 0;

@@ -59,7 +59,8 @@ def tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, parents, req_to_token, r
     Query and key heads are divided by their root mean square and multiplied by ``q_weight`` / ``k_weight`` [D] (None: left as they are), then
     the first ``2 * inv_freq.numel()`` features turn (feature i with the one half of them on) by ``inv_freq`` (fp32) times the node's
     position: cached tokens, ancestors, and ``position_delta`` [requests] int32 where text positions do not count from 0.  Heads of 64, 128
-    and 256 features on the GPU, a multiple of 16 of them rotated; rows and weights begin on 16-byte boundaries there.  ``qkv`` is left as it is; results are rounded once."""
+    and 256 features on the GPU, a multiple of 16 of them rotated; rows and weights begin on 16-byte boundaries there.  ``qkv`` is left as it is; results are rounded once; queries of rows
+    that belong to no request are zero."""
     args = (parents, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, inv_freq, k_cache, v_cache, num_q_heads, num_kv_heads,
             head_dim, float(eps), position_delta)
     ops = _ops()
