@@ -580,6 +580,9 @@ class ModelRunner:
         returns the logits of every node.  For models whose layers are all :class:`RadixAttention` (``draft_trees``)."""
         if not getattr(self.model, "draft_trees", False):
             raise ValueError(f"{type(self.model).__name__} does not run drafted token trees")
+        if ops.use_kernels(input_ids) and not ops.tree_kernels_cover(self.head_dim, self.kv_cache_dtype, self.dtype):
+            raise ValueError(f"drafted token trees run on heads of 64, 128 or 256 features in 16 bits, over caches of their type or of 8-bit floats; "
+                             f"here are {self.head_dim} features in {self.dtype} over {self.kv_cache_dtype}")
         if len(tree_lens_cpu) != len(prefix_lens_cpu) or sum(tree_lens_cpu) != input_ids.shape[0] or parents.shape != input_ids.shape:
             raise ValueError("a tree batch has a tree length and a prefix length per request, and a parent per node")
         tree, prefix = (torch.tensor(x, dtype=torch.int32).to(self.device, non_blocking=True) for x in (tree_lens_cpu, prefix_lens_cpu))

@@ -1497,4 +1497,4 @@ def top_k_top_p_min_p_sample(logits, temperature, top_k, top_p, min_p, uniform) 
 
 
 # drafted token trees
-from .tree import attention_tree, tree_kv_compact, tree_qk_norm_rope_kv_write, tree_speculative_sample  # noqa: E402,F401
+from .tree import attention_tree, tree_kernels_cover, tree_kv_compact, tree_qk_norm_rope_kv_write, tree_speculative_sample  # noqa: E402,F401

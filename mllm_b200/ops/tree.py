@@ -35,6 +35,13 @@ def _ops():
     return _front
 
 
+def tree_kernels_cover(head_dim: int, cache_dtype, act_dtype) -> bool:
+    """Whether :func:`tree_qk_norm_rope_kv_write` and :func:`attention_tree` have kernels for such heads, rows and caches; on the GPU they refuse
+    others."""
+    return (head_dim in (64, 128, 256) and act_dtype in (torch.bfloat16, torch.float16)
+            and cache_dtype in (act_dtype, torch.float8_e4m3fn, torch.float8_e5m2))
+
+
 def _check_index(what: str, rows: int, device, req_to_token, parents, *per_request) -> None:
     """Shapes, types and devices of the index tensors of a batch of trees."""
     if req_to_token.dim() != 2 or req_to_token.dtype != torch.int32 or req_to_token.stride(1) != 1 or req_to_token.device != device:
