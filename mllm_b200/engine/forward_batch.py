@@ -49,6 +49,7 @@ class ForwardBatch:
     extend_prefix_lens_cpu: Optional[List[int]] = None
     max_extend_len: int = 0
     # drafted token trees: the node that each row's node continues (see ops.attention_tree); the rows are new tokens of an extend batch
+    # (out_cache_loc has the nodes' slots; positions go on by rows, a node's own is that of its depth)
     tree_parents: Optional[torch.Tensor] = None        # [T] int32
     # rows of input_ids whose logits are wanted (None: the last row of each request)
     logit_rows: Optional[torch.Tensor] = None

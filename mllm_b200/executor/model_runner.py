@@ -585,9 +585,16 @@ class ModelRunner:
                              f"here are {self.head_dim} features in {self.dtype} over {self.kv_cache_dtype}")
         if len(tree_lens_cpu) != len(prefix_lens_cpu) or sum(tree_lens_cpu) != input_ids.shape[0] or parents.shape != input_ids.shape:
             raise ValueError("a tree batch has a tree length and a prefix length per request, and a parent per node")
+        table = self.req_to_token_pool.req_to_token
+        if req_pool_indices.numel() != len(tree_lens_cpu) or any(n < 0 or p < 0 or p + n > table.shape[1] for n, p in zip(tree_lens_cpu, prefix_lens_cpu)):
+            raise ValueError(f"a tree batch has a row of the request table per request, which has room for {table.shape[1]} tokens")
         tree, prefix = (torch.tensor(x, dtype=torch.int32).to(self.device, non_blocking=True) for x in (tree_lens_cpu, prefix_lens_cpu))
         rows = torch.arange(input_ids.shape[0], device=self.device)
-        return self.prepare_forward_batch_extend(input_ids, req_pool_indices, tree + prefix, tree, prefix, rows, list(tree_lens_cpu),
+        # the nodes' slots, for layers that go by them (a request outside the table is found, and recorded, by those that do not)
+        place = torch.tensor([(b, p + j) for b, (n, p) in enumerate(zip(tree_lens_cpu, prefix_lens_cpu)) for j in range(n)],
+                             dtype=torch.int64).view(-1, 2).to(self.device, non_blocking=True)
+        loc = table[req_pool_indices.long().clamp(0, table.shape[0] - 1)[place[:, 0]], place[:, 1]].to(torch.int64)
+        return self.prepare_forward_batch_extend(input_ids, req_pool_indices, tree + prefix, tree, prefix, loc, list(tree_lens_cpu),
                                                  list(prefix_lens_cpu), tree_parents=parents.to(torch.int32).contiguous(), logit_rows=rows, **extra)
 
     # ------------------------------------------------------------------ forward / sample

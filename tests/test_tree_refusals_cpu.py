@@ -36,3 +36,13 @@ def test_models_without_kernels_for_trees_are_refused_when_the_batch_is_made(mon
         else:
             with pytest.raises(ValueError, match=str(dim)):
                 make()
+
+
+def test_batches_outside_the_request_table_are_refused():
+    mr = Round("qwen3-tiny", "cpu", "float32").mr
+    room = mr.req_to_token_pool.req_to_token.shape[1]
+    ids, parents, one = torch.zeros(2, dtype=torch.int64), torch.tensor([-1, 0], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    mr.prepare_forward_batch_tree(ids, parents, one, [2], [room - 2])
+    for rows, lens, prefix in ((one, [2], [room - 1]), (one, [2], [-1]), (one.repeat(2), [2], [3]), (one.repeat(2), [3, -1], [3, 3])):
+        with pytest.raises(ValueError, match="table"):
+            mr.prepare_forward_batch_tree(ids, parents, rows, lens, prefix)
