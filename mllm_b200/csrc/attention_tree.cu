@@ -352,8 +352,8 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
           int2 s = make_int2(kNoToken, kNoToken);
           if (i < items) {
             const int tok = base + item_tile(i, n) * kTile + lane;
-            if (tok < len) s.x = __ldcg(rtt + tok);
-            if (kPart > 32 && tok + 32 < len) s.y = __ldcg(rtt + tok + 32);
+            if (tok < len) s.x = max(__ldcg(rtt + tok), -1);          // no number of the table is taken for kNoToken
+            if (kPart > 32 && tok + 32 < len) s.y = max(__ldcg(rtt + tok + 32), -1);
           }
           return s;
         };

@@ -74,3 +74,11 @@ def test_nodes_that_see_nothing(D, sink):
     spoil(c, 0, [0, 1])             # node 2 sees itself
     spoil(c, 2, list(range(203)))
     run(c, sink=None if sink is None else torch.full((4,), sink, device="cuda"))
+
+
+@pytest.mark.parametrize("slot", [-2 ** 31, -2 ** 31 + 1, -2 ** 31 + 2, -2])
+@pytest.mark.parametrize("cache", [None, torch.float8_e4m3fn])
+def test_any_negative_slot(slot, cache):
+    c = tree_batch([130], [5], 4, 2, 128, cache=cache)
+    c["table"][int(c["req"][0]), [2, 40, 100, 132]] = slot
+    run(c)
