@@ -147,7 +147,7 @@ __device__ __forceinline__ void cp_wait() {
 // R: row tiles that a CTA takes through its keys and values side by side
 template <int NH, bool KV8, int R>
 struct Cfg {
-  static_assert(R == 1 || NH == 2, "two row tiles of 256 features leave no tensor memory for scores; those of 64 are no faster");
+  static_assert(R == 1 || NH == 2, "two row tiles of 256 features leave no tensor memory for scores; those of 64 lose more below 1.5 tiles than they win");
   static constexpr int kSoftmaxWarps = 4 * R, kIssueWarp = R == 1 ? 11 : 19, kThreads = 32 * (kIssueWarp + 1);
   static constexpr int kD = 64 * NH;
   static constexpr int kQBlock = kRows * 128;              // a 64-feature block of Q
@@ -910,8 +910,9 @@ TreePlan tree_plan(int head_dim, int group, int64_t rows, int64_t batch, int num
   TreePlan plan;
   // Row tiles that a CTA takes side by side: two where a request has more rows than one tile on average.  Two tiles against one, 16 requests
   // of 4096 tokens, 8 query heads over a kv head, 128 features: 24 nodes (192 rows) 59.1 / 76.5 us with e4m3 caches, which are widened
-  // half as often, and 58.4 / 62.5 us in bf16; 17 nodes 56.8 / 58.9 and 55.5 / 51.9; 16 nodes (128 rows) 56.0 / 49.6 and 54.1 / 47.2.  Heads of
-  // 64: 54.7 / 54.2 and 50.0 / 53.6 at 24 nodes, 54.0 / 42.3 and 48.8 / 42.0 at 17: always one.
+  // half as often, and 58.4 / 62.5 us in bf16; 17 nodes (136 rows) 56.8 / 58.9 and 55.5 / 51.9; 16 nodes (128 rows) 56.0 / 49.6 and 54.1 / 47.2.
+  // So with 16-bit caches the rule loses 7 % just above one tile and wins as much at one and a half; where that turns is not measured.
+  // Heads of 64: 54.7 / 54.2 and 50.0 / 53.6 at 24 nodes, 54.0 / 42.3 and 48.8 / 42.0 at 17: always one.
   plan.row_tiles = head_dim == 128 && rows > batch * (kRows / group) ? 2 : 1;
   plan.ctas = head_dim == 256 || plan.row_tiles == 2 ? num_sms : 2 * num_sms;
   plan.part_rows = static_cast<int>(std::min<int64_t>(plan.row_tiles * (kRows / group * group), rows * group));

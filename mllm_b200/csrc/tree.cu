@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(128) tree_prologue_kernel(const PrologueParams
 // it is overwritten: rows are read eight at a time, written behind that, and a later read is of a later node than all written so far.
 // Bound by the chain lengths -> path -> table -> rows for few requests, by the rows' bytes for many; a thread goes through the chain once
 // and then through many planes (32 requests of 3.5 accepted
-// nodes, 36 layers of 8 heads of 128: 9.6 us; with a thread per plane and piece, where three waves of blocks went through it, 11.9).
+// nodes, 36 layers of 8 heads of 128: 8.4 us; with a thread per plane and piece, where three waves of blocks went through it, 11.9).
 // ---------------------------------------------------------------------------
 struct CompactParams {
   uint8_t* store;

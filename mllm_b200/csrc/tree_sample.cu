@@ -4,7 +4,7 @@
 //   e_i = exp((l_i - max l) / T),   kept = {i: e_i >= the k-th largest, >= the smallest whose strictly larger mass is below top_p * sum e,
 //   >= min_p}  (ties are kept),   p = e / sum over kept.
 // The node's children are looked at in the order of their numbers: child c with token x is taken if u_c q(x) < p(x); otherwise
-// p <- max(p - q, 0) / sum, where q is the distribution that the children were drawn from, or all of x (candidates without
+// p <- max(p - q, 0) / sum, where q is the distribution that the children were drawn from, each by itself, or all of x (candidates without
 // probabilities).  Without a child that is taken the walk ends with the first token whose running sum of p, in the order of the ids,
 // passes u * sum p.  The emitted tokens are distributed as the target's own samples, whatever the draft.
 //
@@ -14,12 +14,15 @@
 // warps' maxima for top-k, a level that holds the wanted mass for top-p, min_p itself) leaves a few tokens, which every CTA collects and
 // sorts for itself.  Where more than kList are left (flat distributions) the cut is closed in on, seven parts of its range an exchange.
 //
-// A step of a small batch takes some 9 us, nearly all of it latency: five exchanges of 1 to 1.5 us, the row (0.3 MB over 8 SMs), one way
-// through it in shared memory.  On the device: 1 request of 8 nodes, 151936 tokens 54 us; 8 of 16 nodes with draft probabilities 72; 32 of 24
-// nodes, 128256 tokens, two CTAs on an SM, 140.
+// A step of a small batch takes some 9 us, nearly all of it latency: five exchanges of 1 to 1.5 us (two or three more where top-p has to
+// look twice), the row (0.3 MB over 8 SMs), one way through it in shared memory.  Steps and filters follow from the random numbers: on the
+// device 1 request of 8 nodes, 151936 tokens takes 31 to 70 us; 8 of 16 nodes with draft probabilities 65 to 80; 32 of 24 nodes, 128256 tokens, two
+// CTAs on an SM, 90 to 137, once 174.
 //
-// Whole tokens hang on sums: e is taken in 64 bits where it is above 2^-12 and sums are joined in 64 bits, so that the border of a token
-// is off by some 10^-9 of the whole.
+// Whole tokens hang on sums: e is taken in 64 bits where it is above 2^-12, and threads' sums are joined in 64 bits.  Smaller ones are 32-bit
+// (fp64 exponentials of a whole vocabulary would bound the kernel): off by less than 2^-19 each, 2^-22 from the exponential and half a step of
+// an argument of up to 32, twice; a thread adds them up in 32 bits, a rounding a term.  So a token's border is off by some 10^-9 of the whole
+// where the mass is in few tokens, and by less than 2^-18 of the mass below 2^-12 (vocabularies of 151936) where it is in many.
 #include <algorithm>
 #include <type_traits>
 
@@ -952,7 +955,7 @@ int launch_tree_sample(const TreeSampleArgs& a, cudaStream_t s) {
   p.steps = a.steps;
   // CTAs per request: no more than 8192 tokens each, up to 8 (16 requests, 32000 tokens: 57 us; 16384 each 109, 4096 each 56; 8000 tokens: 53 / 53 /
   // 63).  Where all do not have an SM of their own, two share one, with half the registers (32 requests, 128256 tokens: 140 us; fewer CTAs
-  // a request instead 168; with registers for two everywhere 1 request takes 57 us instead of 54.5).
+  // a request instead 168; with registers for two everywhere 1 request took 57 us instead of 54.5).
   const int item = a.dt == kF32 ? 4 : 2;
   int cluster = 1;
   while (cluster < kMaxCluster && cluster * 8192 < a.vocab) cluster *= 2;

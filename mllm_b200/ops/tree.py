@@ -129,11 +129,11 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
     At a node the distribution p is that of :func:`mllm_b200.ops.top_k_top_p_min_p_sample` (temperature up to 1e-6: the most likely token;
     ``top_k`` below 1 and ``top_p`` of 1 and more do not filter; every filter looks at the whole distribution, and ties at a cut are kept).
     The node's children, in order, up to 64 of them: child c with token x is taken if ``uniform[c] * q(x) < p(x)``, otherwise
-    ``p <- max(p - q, 0)``, scaled to 1 (left as it is where nothing remains).  q is row ``draft_probs[node]``, the distribution that the
-    children were drawn from one by one, or without ``draft_probs`` all of x: candidates that were picked, not drawn.  Where no child is
+    ``p <- max(p - q, 0)``, scaled to 1 (left as it is where nothing remains).  q is row ``draft_probs[node]``, the distribution that each of
+    the node's children was drawn from, independently of the others (with replacement), or without ``draft_probs`` all of x: candidates that were picked, not drawn.  Where no child is
     taken, or ``max_steps`` nodes are reached, the walk ends with the first token whose running sum of p in the order of the ids passes
-    ``uniform_final[b]``.  Random numbers are from [0, 1).  A logit that is no number counts as minus infinity, and a row without a finite
-    logit gives its first token.
+    ``uniform_final[b]``.  Random numbers are from [0, 1).  A logit that is no number counts as minus infinity, a row without a finite
+    logit gives its first token, and infinite logits share the mass.
 
     Returns ``path`` [requests, max_steps] int32, the nodes of the walk from node 0 on (whose cache rows are now valid), ``tokens``
     [requests, max_steps] int64, the emitted tokens (those of ``path[:, 1:]`` and one more), both -1 behind ``counts`` [requests] int32."""
