@@ -113,7 +113,8 @@ struct Scale {
   // number, with both parts of the factor 1: log2_of gives infinity for infinite logits, which no sum of loops over tokens has to look for.
   float mx, off, c_hi, c_lo;     // largest logit; it, or the largest finite number; log2(e) / T as two floats
   double inv_t, mx_d;
-  __device__ __forceinline__ Scale(float largest, float temp) : mx(largest), off(fminf(largest, 3.402823466e38f)), inv_t(1.0 / static_cast<double>(temp)), mx_d(largest) {
+  __device__ __forceinline__ Scale(float largest, float temp)
+      : mx(largest), off(fminf(largest, 3.402823466e38f)), inv_t(1.0 / static_cast<double>(temp)), mx_d(largest) {
     const double c = 1.4426950408889634 * inv_t;
     c_hi = mx == off ? static_cast<float>(c) : 1.f;
     c_lo = mx == off ? static_cast<float>(c - static_cast<double>(c_hi)) : 1.f;

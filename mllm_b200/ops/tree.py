@@ -66,8 +66,8 @@ def tree_qk_norm_rope_kv_write(qkv, q_weight, k_weight, parents, req_to_token, r
     Query and key heads are divided by their root mean square and multiplied by ``q_weight`` / ``k_weight`` [D] (None: left as they are), then
     the first ``2 * inv_freq.numel()`` features turn (feature i with the one half of them on) by ``inv_freq`` (fp32) times the node's
     position: cached tokens, ancestors, and ``position_delta`` [requests] int32 where text positions do not count from 0.  Heads of 64, 128
-    and 256 features on the GPU, a multiple of 16 of them rotated; rows and weights begin on 16-byte boundaries there.  ``qkv`` is left as it is; results are rounded once; queries of rows
-    that belong to no request are zero."""
+    and 256 features on the GPU, a multiple of 16 of them rotated; rows and weights begin on 16-byte boundaries there.  ``qkv`` is left as it
+    is; results are rounded once; queries of rows that belong to no request are zero."""
     args = (parents, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, inv_freq, k_cache, v_cache, num_q_heads, num_kv_heads,
             head_dim, float(eps), position_delta)
     ops = _ops()
@@ -93,8 +93,8 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
                    out: Optional[torch.Tensor] = None, window: Optional[int] = None, logit_cap: float = 0.0,
                    sink: Optional[torch.Tensor] = None, chunk: Optional[int] = None) -> torch.Tensor:
     """Attention of drafted nodes ``q`` [T, Hq, D] (heads of a node contiguous): each sees the cached tokens, its ancestors and itself.
-    ``scale`` is positive; ``window``, ``logit_cap``, ``sink`` and ``chunk`` as for :func:`mllm_b200.ops.attention_prefill`, by positions: siblings share theirs.
-    Heads of 64, 128 and 256 features, 16-bit, over caches of their type or of unscaled 8-bit floats.  Rows of ``out`` that belong to no
+    ``scale`` is positive; ``window``, ``logit_cap``, ``sink`` and ``chunk`` as for :func:`mllm_b200.ops.attention_prefill`, by positions:
+    siblings share theirs.  Heads of 64, 128 and 256 features, 16-bit, over caches of their type or of unscaled 8-bit floats.  Rows of ``out`` that belong to no
     request keep what they hold.  A value in the cache that is no number reaches the nodes that see it and no others.  On the GPU a token whose slot
     lies outside the cache is seen by none, and a node that sees nothing has a row of zeros."""
     ops = _ops()
@@ -130,8 +130,8 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
     ``top_k`` below 1 and ``top_p`` of 1 and more do not filter; every filter looks at the whole distribution, and ties at a cut are kept).
     The node's children, in order, up to 64 of them: child c with token x is taken if ``uniform[c] * q(x) < p(x)``, otherwise
     ``p <- max(p - q, 0)``, scaled to 1 (left as it is where nothing remains).  q is row ``draft_probs[node]``, the distribution that each of
-    the node's children was drawn from, independently of the others (with replacement), or without ``draft_probs`` all of x: candidates that were picked, not drawn.  Where no child is
-    taken, or ``max_steps`` nodes are reached, the walk ends with the first token whose running sum of p in the order of the ids passes
+    the node's children was drawn from, independently of the others (with replacement), or without ``draft_probs`` all of x: candidates that
+    were picked, not drawn.  Where no child is taken, or ``max_steps`` nodes are reached, the walk ends with the first token whose running sum of p in the order of the ids passes
     ``uniform_final[b]``.  Random numbers are from [0, 1).  A logit that is no number counts as minus infinity, a row without a finite
     logit gives its first token, and infinite logits share the mass.
 
