@@ -94,9 +94,9 @@ def attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens
                    sink: Optional[torch.Tensor] = None, chunk: Optional[int] = None) -> torch.Tensor:
     """Attention of drafted nodes ``q`` [T, Hq, D] (heads of a node contiguous): each sees the cached tokens, its ancestors and itself.
     ``scale`` is positive; ``window``, ``logit_cap``, ``sink`` and ``chunk`` as for :func:`mllm_b200.ops.attention_prefill`, by positions:
-    siblings share theirs.  Heads of 64, 128 and 256 features, 16-bit, over caches of their type or of unscaled 8-bit floats.  Rows of ``out`` that belong to no
-    request keep what they hold.  A value in the cache that is no number reaches the nodes that see it and no others.  On the GPU a token whose slot
-    lies outside the cache is seen by none, and a node that sees nothing has a row of zeros."""
+    siblings share theirs.  Heads of 64, 128 and 256 features, 16-bit, over caches of their type or of unscaled 8-bit
+    floats.  Rows of ``out`` that belong to no request keep what they hold.  A value in the cache that is no number reaches the nodes that see it and
+    no others.  On the GPU a token whose slot lies outside the cache is seen by none, and a node that sees nothing has a row of zeros."""
     ops = _ops()
     if ops.use_kernels(q):          # the binding makes the same checks
         return ops.ext().attention_tree(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, parents,
@@ -131,9 +131,9 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
     The node's children, in order, up to 64 of them: child c with token x is taken if ``uniform[c] * q(x) < p(x)``, otherwise
     ``p <- max(p - q, 0)``, scaled to 1 (left as it is where nothing remains).  q is row ``draft_probs[node]``, the distribution that each of
     the node's children was drawn from, independently of the others (with replacement), or without ``draft_probs`` all of x: candidates that
-    were picked, not drawn.  Where no child is taken, or ``max_steps`` nodes are reached, the walk ends with the first token whose running sum of p in the order of the ids passes
-    ``uniform_final[b]``.  Random numbers are from [0, 1).  A logit that is no number counts as minus infinity, a row without a finite
-    logit gives its first token, and infinite logits share the mass.
+    were picked, not drawn.  Where no child is taken, or ``max_steps`` nodes are reached, the walk ends with the first token whose running sum of
+    p in the order of the ids passes ``uniform_final[b]``.  Random numbers are from [0, 1).  A logit that is no number counts as minus infinity,
+    a row without a finite logit gives its first token, and infinite logits share the mass.
 
     Returns ``path`` [requests, max_steps] int32, the nodes of the walk from node 0 on (whose cache rows are now valid), ``tokens``
     [requests, max_steps] int64, the emitted tokens (those of ``path[:, 1:]`` and one more), both -1 behind ``counts`` [requests] int32."""
