@@ -193,6 +193,8 @@ void tree_kv_compact(Tensor& store, const Tensor& req_to_token, const Tensor& re
   for (const Tensor* t : {&req_to_token, &req_pool_indices, &prefix_lens, &path, &counts})
     CHECK_ARG(t->device() == store.device(), "mllm_b200: tensors on different devices");
   if (store.numel() == 0 || batch == 0) return;
+  const int64_t planes = store.numel() / (store.size(-2) * store.size(-1));
+  CHECK_ARG(planes * (row / 16) < (int64_t(1) << 31) - (int64_t(1) << 24), "tree_kv_compact: ", planes, " planes of rows of ", row, " bytes are too many");
   c10::cuda::CUDAGuard g(store.device());
   mb200::TreeCompactArgs a{};
   a.store = store.data_ptr();
@@ -208,7 +210,7 @@ void tree_kv_compact(Tensor& store, const Tensor& req_to_token, const Tensor& re
   a.steps = static_cast<int>(path.size(1));
   a.table_rows = static_cast<int>(req_to_token.size(0));
   a.table_cols = static_cast<int>(req_to_token.size(1));
-  a.planes = static_cast<int>(store.numel() / (store.size(-2) * store.size(-1)));
+  a.planes = static_cast<int>(planes);
   a.row_bytes = static_cast<int>(row);
   const int rc = mb200::launch_tree_compact(a, stream_of(store));
   TORCH_CHECK(rc == 0, "mllm_b200 tree_kv_compact: unsupported configuration or launch failure (code ", rc, ")");

@@ -48,3 +48,15 @@ def test_scales_that_are_not_positive_are_refused(scale):
     want = c["v"][slots].double().mean(0).repeat_interleave(2, dim=0)
     half = torch.finfo(torch.bfloat16).eps / 2       # weights are 1, sums of 71 in 32 bits, one rounding
     assert ((got[0].double() - want).abs() <= half * want.abs() + c["v"][slots].double().abs().mean(0).repeat_interleave(2, dim=0) * 71 * 2 ** -24).all()
+
+
+def test_more_planes_than_the_kernel_counts_are_refused():
+    """They were a negative number of planes, and nothing was moved.  (Memory that nobody touches.)"""
+    store = torch.empty((2 ** 31, 1, 8), device="cuda", dtype=torch.bfloat16)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    before = ops.launch_count()
+    with pytest.raises(ValueError, match="too many"):
+        ops.tree_kv_compact(store, ints([[0, 0, 0]]), ints([0]), ints([0]), ints([[0, 2]]), ints([2]))
+    assert ops.launch_count() == before
+    del store
+    torch.cuda.empty_cache()
