@@ -97,13 +97,13 @@ def draw(rng):
         if last == 0:
             context = _log_int(rng, 1, min(3000, math.isqrt(14_000_000_000 // (requests * width))))
         else:
-            context = _log_int(rng, 1, min(32000 // requests, 25000 * 1024 // (requests * kv * dim), 8_000_000_000 // (requests * last * width)))
+            context = _log_int(rng, 1, min(32000 // requests, 20000 * 1024 // (requests * kv * dim), 8_000_000_000 // (requests * last * width)))
         return _prompt(None, requests=requests, context=context, new=context if last == 0 or rng.random() < 0.5 else min(context, 500), last=last,
                        spread=spread, heads=kv * group, kv=kv, dim=dim, page=page, cache=cache, dtype=dtype, add=rng.random() < 0.3,
                        cap=rng.choice([0.0, 0.0, 30.0]), sink=rng.random() < 0.25)
     layers, requests = rng.randint(1, 36), _log_int(rng, 1, 8)
     if op == "select":
-        context = _log_int(rng, 1, min(30000, 13_500_000 // (layers * requests * kv)))
+        context = _log_int(rng, 1, min(30000, 11_500_000 // (layers * requests * kv)))
         return _select(None, layers=layers, requests=requests, context=context, spread=spread, kv=kv, keep=round(rng.uniform(0.05, 1.0), 2),
                        pool=rng.choice([1, 1, 5, 7, 13]), first=rng.choice([0, 4, 9]), recent=rng.choice([0, 1, 32, 64]))
     context = _log_int(rng, 1, min(30000, 140_000_000 // (layers * requests * kv * dim)))
