@@ -1498,3 +1498,5 @@ def top_k_top_p_min_p_sample(logits, temperature, top_k, top_p, min_p, uniform) 
 
 # drafted token trees
 from .tree import attention_tree, tree_kernels_cover, tree_kv_compact, tree_qk_norm_rope_kv_write, tree_speculative_sample  # noqa: E402,F401
+# shortening of cached requests
+from .evict import attention_decode_weights, attention_prefill_weights, cache_evict, cache_select, cache_weights_cover  # noqa: E402,F401

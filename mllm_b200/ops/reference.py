@@ -1089,3 +1089,91 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
             out[b, step] = passed[0, 0] if passed.numel() else torch.nonzero(p > 0)[-1, 0]
             break
     return path.to(logits.device), out.to(logits.device), counts.to(logits.device)
+
+
+def _cached_weights(q, k_cache, slots, place, scale: float, logit_cap: float, sink) -> torch.Tensor:
+    """[W, Hq, L] softmax weights of queries ``q`` [W, Hq, D] at cache indices ``place`` over the cached tokens ``slots`` up to theirs."""
+    hkv, work = k_cache.shape[1], torch.float64 if q.dtype == torch.float64 else torch.float32
+    keys = k_cache[slots].to(work)
+    s = torch.einsum("wkgd,lkd->wkgl", q.to(work).view(q.shape[0], hkv, -1, q.shape[2]), keys).reshape(q.shape[0], q.shape[1], -1) * scale
+    if logit_cap:
+        s = logit_cap * torch.tanh(s / logit_cap)
+    s = s.masked_fill(torch.arange(slots.numel(), device=q.device) > place[:, None, None], float("-inf"))
+    if sink is not None:
+        s = torch.cat([s, sink.to(work).view(1, -1, 1).expand(s.shape[0], -1, 1)], dim=-1)
+    return torch.softmax(s, dim=-1)[..., :slots.numel()]
+
+
+def attention_decode_weights(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, scale: float, sums, decay=1.0, out=None, logit_cap=0.0,
+                             sink=None) -> torch.Tensor:
+    out = torch.empty_like(q) if out is None else out
+    hkv = k_cache.shape[1]
+    for b in range(q.shape[0]):
+        n, row = int(seq_lens[b]), int(req_pool_indices[b])
+        if n <= 0:
+            out[b] = 0
+            continue
+        slots = req_to_token[row, :n].long()
+        w = _cached_weights(q[b:b + 1], k_cache, slots, torch.tensor([n - 1], device=q.device), scale, logit_cap, sink)[0].view(hkv, -1, n)
+        out[b] = torch.einsum("kgl,lkd->kgd", w, v_cache[slots].to(w.dtype)).reshape(q.shape[1:]).to(out.dtype)
+        add = w.sum(1).to(sums.dtype)
+        sums[row, :, :n - 1] = (decay * sums[row, :, :n - 1] if decay else 0.0) + add[:, :-1]
+        sums[row, :, n - 1] = add[:, -1]
+    return out
+
+
+def attention_prefill_weights(q, k_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, scale: float, sums, last=0, add=False,
+                              logit_cap=0.0, sink=None) -> None:
+    hkv = k_cache.shape[1]
+    for b in range(req_pool_indices.numel()):
+        n, prefix, row, start = int(seq_lens[b]), int(prefix_lens[b]), int(req_pool_indices[b]), int(q_start_loc[b])
+        new = n - prefix
+        if n <= 0 or new <= 0:
+            continue
+        slots, total = req_to_token[row, :n].long(), 0.0
+        look = min(last, new) if last else new
+        for at in range(new - look, new, 256):        # some queries at a time
+            end = min(at + 256, new)
+            w = _cached_weights(q[start + at:start + end], k_cache, slots, torch.arange(prefix + at, prefix + end, device=q.device), scale, logit_cap, sink)
+            total = total + w.view(end - at, hkv, -1, n).sum((0, 2))
+        if add:
+            total[:, :prefix] += sums[row, :, :prefix]
+        sums[row, :, :n] = total.to(sums.dtype)
+
+
+def cache_select(sums, req_pool_indices, seq_lens, budgets, max_budget: int, first=4, recent=32, pool=1):
+    layers, batch, hkv = sums.shape[0], req_pool_indices.numel(), sums.shape[2]
+    keep = torch.full((layers, batch, hkv, max_budget), -1, dtype=torch.int32, device=sums.device)
+    counts = torch.zeros(batch, dtype=torch.int32, device=sums.device)
+    for b in range(batch):
+        n = int(seq_lens[b])
+        count = max(0, min(n, int(budgets[b]), max_budget))
+        counts[b] = count
+        if count == 0:
+            continue
+        x = sums[:, int(req_pool_indices[b]), :, :n]
+        x = torch.where(torch.isnan(x), float("-inf"), x)
+        side = torch.nn.functional.pad(x, (pool // 2, pool // 2), value=float("-inf"))
+        score = side.unfold(-1, pool, 1).amax(-1)
+        end = min(recent, count)
+        begin = min(first, count - end)
+        middle = torch.sort(score[..., begin:n - end], dim=-1, descending=True, stable=True).indices[..., :count - begin - end] + begin
+        fixed = torch.cat([torch.arange(begin, device=x.device), torch.arange(n - end, n, device=x.device)])
+        keep[:, b, :, :count] = torch.cat([middle, fixed.expand(layers, hkv, -1)], dim=-1).sort(dim=-1).values.to(torch.int32)
+    return keep, counts
+
+
+def cache_evict(store, sums, req_to_token, req_pool_indices, keep, counts) -> None:
+    for b in range(req_pool_indices.numel()):
+        n, row = int(counts[b]), int(req_pool_indices[b])
+        if n <= 0:
+            continue
+        slots = req_to_token[row].long()
+        for layer in range(store.shape[0]):
+            for head in range(store.shape[2]):
+                kept = keep[layer, b, head, :n].long()
+                if bool((kept < torch.arange(n, device=kept.device)).any()):
+                    raise ValueError("cache_evict: a kept token's index is smaller than its place")
+                store[layer, :, head, slots[:n]] = store[layer, :, head, slots[kept]]
+                if sums is not None:
+                    sums[layer, row, head, :n] = sums[layer, row, head, kept]
