@@ -4,8 +4,7 @@ The extensions live under ``mllm_b200/csrc``:
 
 * ``mllm_b200_C``    — the sm_100a CUDA kernels of every decoder plus their PyTorch binding;
 * ``mllm_b200_R``    — gated delta rule;
-* ``mllm_b200_A``    — latent attention, drafted token trees (speculative decoding);
-* ``mllm_b200_K``    — attention weights per cached token, selection and eviction (requests shortened in the cache);
+* ``mllm_b200_A``    — latent attention, drafted token trees (speculative decoding), cached requests that are shortened;
 * ``mllm_b200_L``    — lightning attention (linear attention with a fixed decay per head);
 * ``mllm_b200_E``    — mixtures of experts;
 * ``mllm_b200_X``    — 4-bit weights, vision towers, tensor- and expert-parallel exchange;
@@ -61,13 +60,9 @@ EXTENSIONS: Dict[str, Dict[str, List[str]]] = {
         "cuda": True,
     },
     "mllm_b200_A": {
-        "sources": ["bindings_latent.cpp", "runtime.cu", "latent.cu", "attention_tree.cu", "tree.cu", "tree_sample.cu"],
-        "headers": _COMMON + ["bindings_tree.h", "tree.h", "tree.cuh"],
-        "cuda": True,
-    },
-    "mllm_b200_K": {
-        "sources": ["bindings_evict.cpp", "runtime.cu", "weights_decode.cu", "weights_prompt.cu", "evict.cu"],
-        "headers": _COMMON + ["evict.h", "evict.cuh"],
+        "sources": ["bindings_latent.cpp", "runtime.cu", "latent.cu", "attention_tree.cu", "tree.cu", "tree_sample.cu",
+                    "weights_decode.cu", "weights_prompt.cu", "evict.cu"],
+        "headers": _COMMON + ["bindings_tree.h", "tree.h", "tree.cuh", "bindings_evict.h", "evict.h", "evict.cuh"],
         "cuda": True,
     },
     "mllm_b200_L": {

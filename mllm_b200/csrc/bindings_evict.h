@@ -1,11 +1,11 @@
-// PyTorch binding of the kernels that shorten requests in the paged cache (module mllm_b200_K).
+// PyTorch binding of the kernels that shorten requests in the paged cache, part of the module of latent attention.
+#pragma once
+
 #include <cfloat>
 
 #include "bindings_common.h"
+#include "bindings_tree.h"      // CHECK_ARG
 #include "evict.h"
-
-// Refusals are ValueErrors, as they are for CPU tensors
-#define CHECK_ARG(...) TORCH_CHECK_VALUE(__VA_ARGS__)
 
 namespace {
 
@@ -254,12 +254,3 @@ void cache_evict(const Tensor& store, const c10::optional<Tensor>& sums, const T
 }
 
 }  // namespace
-
-PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("attention_decode_weights", &attention_decode_weights);
-  m.def("attention_prefill_weights", &attention_prefill_weights);
-  m.def("cache_select", &cache_select);
-  m.def("cache_evict", &cache_evict);
-  m.def("read_status", &read_status);
-  m.def("launch_count", &launch_count);
-}

@@ -1,5 +1,6 @@
 // PyTorch binding of latent attention (module mllm_b200_A).
 #include "bindings_common.h"
+#include "bindings_evict.h"
 #include "bindings_tree.h"
 
 namespace {
@@ -212,6 +213,10 @@ void latent_attention(const Tensor& q, const Tensor& cache, const Tensor& req_to
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("attention_decode_weights", &attention_decode_weights);
+  m.def("attention_prefill_weights", &attention_prefill_weights);
+  m.def("cache_select", &cache_select);
+  m.def("cache_evict", &cache_evict);
   m.def("attention_tree", &attention_tree);
   m.def("tree_qk_norm_rope_kv_write", &tree_qk_norm_rope_kv_write);
   m.def("tree_speculative_sample", &tree_speculative_sample);
