@@ -63,7 +63,7 @@ bool weights_prompt_covers(int head_dim, int group);
 int64_t weights_prompt_floats(const WeightsPromptArgs& args);
 int launch_weights_prompt(const WeightsPromptArgs& args, cudaStream_t s);
 
-// which tokens stay: the last ones, the first ones, the largest sums (evict.cu)
+// which tokens stay: the last ones, the first ones, the largest sums (cache_select.cu)
 struct CacheSelectArgs {
   CacheIndex index;
   const float* sums;        // [layers][rows][hkv][tokens], the strides below
