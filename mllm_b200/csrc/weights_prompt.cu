@@ -8,14 +8,17 @@
 //
 // A row's normaliser needs all of its scores, a token's sum needs all normalisers: two passes over the keys, each a product and one
 // exponential per (row, token).  Keeping the exponentials would take more memory traffic (4 bytes each, twice) than making them again.
-//   * Rows are (query, head of the group) pairs; RT tiles of 128 make a block.  Both passes hold a block in shared memory and let copying
-//     warps bring keys by slot into a ring of 128-token stages in the operand layout.  A step is KT stages: RT * KT = 2, 256 score columns in
-//     tensor memory, two buffers (heads of 256: one stage, 128 columns).
-//   * First pass: S = Q K^T, a row per lane.  16 warps, four to every 32 lanes of tensor memory, take a quarter of the columns each, with a
-//     maximum and sum of their own; they join at the block's end.  Units (request, kv head, block) times steps form one line, dealt evenly to the
-//     CTAs; a block's normaliser is written out, or a partial one per CTA.
-//   * Second pass: S^T = K Q^T, a token per lane: its sum over the rows is a sum in a thread, and no two CTAs have the same token, so nothing
-//     depends on their order.  Tokens are dealt by what they cost: the blocks that see them.
+//   * Rows are (query, head of the group) pairs; RT tiles of 128 make a block.  A CTA holds one operand, the block, in shared memory, and copying
+//     warps bring the other through a ring of 128-row stages in the operand layout, keys by slot.  A step is KT stages: RT * KT = 2, 256 score
+//     columns in tensor memory, two buffers (heads of 256: one stage, 128 columns).
+//   * First pass: S = Q K^T, blocks of rows, a row per lane.  16 warps, four to every 32 lanes of tensor memory, take a quarter of the columns
+//     each, with a maximum and sum of their own; they join at the block's end.  Units (request, kv head, block) times steps form one line, dealt
+//     evenly to the CTAs; a row's normaliser is written out, or a partial one per CTA.
+//   * Second pass: S^T = K Q^T, a token per lane: its sum over the rows is a sum in a thread.  Where the observed rows fit a block or two they
+//     stay in shared memory and keys go by; tokens are dealt by what they cost, the blocks that see them, and no two CTAs have the same
+//     token.  Where there are more rows, 256 tokens are the block and rows go by, in a line as in the first pass; a third kernel adds up the parts
+//     of blocks that were cut.  Nothing depends on the order of CTAs.
+//   * A CTA's first block is brought by the computing warps, which have nothing else to do then, later ones by a warp of its own.
 // What bounds it is the exponentials, 16 per cycle and SM; products take half their time.
 #include <algorithm>
 
@@ -32,8 +35,6 @@ constexpr int kStart = 2;                  // steps' time that every unit of the
 constexpr int kChunk = 8;                  // steps whose sums wait in shared memory
 constexpr int kNoToken = -0x7fffffff;
 constexpr int kCompute = 16;               // warps
-constexpr int kThreads = 32 * (kCompute + 8), kIssueWarp = kCompute + 7;
-
 struct PromptParams {
   CacheIndex ix;
   WeightSums sums;
@@ -42,10 +43,13 @@ struct PromptParams {
   const void* q;
   const void* k_cache;
   float* lse;        // [rows of q][hq]: normalisers of blocks that lie in one CTA
-  float* part;       // [CTAs][2][block rows]
+  float* part;       // [CTAs][2][block rows] of the first pass
+  float* part_sum;   // the same of tokens, where rows go by
+  int4* jobs;        // [CTAs] of units of tokens that end in the CTA and began in another: kv head and request, block, first CTA and its place
   const float* sink;
   int64_t q_stride, num_slots, kv_tok_stride, kv_head_stride;
   int rows, hkv, group, last, ctas;
+  uint32_t inv_group;      // of 16 bits: quotients of numbers below 320, exactly
   bool add;
   float scale_log2, cap_in, cap_out;     // a scaled score x becomes cap_out tanh(x cap_in ln 2 / 2); cap_out 0: no soft cap
 };
@@ -71,59 +75,81 @@ __device__ __forceinline__ Observed observed_of(const PromptParams& p, int b) {
   return o;
 }
 
-template <int NH, bool KV8, int R>
+template <int NH, bool KV8, int R, int PASS>
 struct Cfg {
   static constexpr int RT = R, KT = NH == 4 ? 1 : 2 / R;
+  static_assert(PASS != 3 || KT == 1, "rows go by one stage a step");
   static constexpr int kD = 64 * NH;
   static constexpr int kRows = RT * kTileRows;               // of a block
   static constexpr int kStepKeys = KT * 128;
   static constexpr int kCols = RT * KT * 128, kWarpCols = kCols / 4;
-  static constexpr int kQBlock = kRows * 128, kQBytes = NH * kQBlock;      // 64 features of a block's rows
-  static constexpr int kKBlock = 128 * 128, kStage = NH * kKBlock;
+  static constexpr int kBlock = kRows * 128, kBlockBytes = NH * kBlock;    // 64 features of a block's rows
+  static constexpr int kPiece = 128 * 128, kStage = NH * kPiece;
   static constexpr int kStages = NH == 4 ? 2 : NH == 2 ? (R == 2 ? 4 : 5) : 6;
-  static constexpr int kTeam = KV8 || NH == 4 ? 2 : 1, kTeams = kTeam == 2 ? 2 : 4;     // warps that copy a stage; every kTeams-th each
-  static constexpr int kQWarps = 7 - kTeam * kTeams;
-  static constexpr int kSmem = kQBytes + kStages * kStage;
+  // Warps: those that compute, that copy stages (kCopying of them, every kCopying-th stage each), one that copies blocks, one that issues
+  // products.  8-bit keys are widened on the way, which takes more of them.
+  static constexpr int kCopy = KV8 ? 6 : 2, kCopying = kCopy < kStages ? kCopy : kStages;
+  static constexpr int kBlockWarp = kCompute + kCopy, kIssueWarp = kBlockWarp + 1, kThreads = 32 * (kIssueWarp + 1);
+  // Registers: those of a launch, of the computing threads, of the others.  A quarter of the warps share 16384, four computing ones each.
+  static constexpr int kLaunchRegs = KV8 ? 80 : 96, kComputeRegs = KV8 ? 88 : 104, kOtherRegs = 64;
+  static_assert(4 * kComputeRegs + (kCopy + 2) / 4 * kOtherRegs <= (4 + (kCopy + 2) / 4) * kLaunchRegs && (kCopy + 2) % 4 == 0, "register split");
+  static constexpr int kSmem = kBlockBytes + kStages * kStage;
   static constexpr int kGroups = 4 / KT;                     // parts of a token's sum
-  static_assert(kTeams <= kStages && kQWarps > 0 && 2 * kCols <= 512, "teams, tensor memory");
+  // Normalisers and factors of rows: of the last blocks, or of the stages.  A place is written anew behind the last product of the block in
+  // front, or of the stage kStages before.  That product was issued when the scores of two steps before had been read, so that the computing
+  // warps were through with the step before those.
+  static constexpr int kRing = PASS == 3 ? kStages + 3 : 4, kRingRows = PASS == 3 ? 128 : kRows;
+  static_assert(2 * kCols <= 512, "tensor memory");
 };
 
-// What both passes do with a batch, from its numbers on.  Blocks of a request: rows r = j * group + h.
-template <typename C>
+// What the passes do with a request.  Rows r = j * group + h, in blocks of kRows.
+template <typename C, int PASS>
 struct Work {
   Observed o;
-  int rows, blocks, steps;       // steps: of the second pass
-  __device__ __forceinline__ void set(const PromptParams& p, int b) {
-    o = observed_of(p, b);
+  int rows, blocks, units;       // units: blocks of rows, or (third kind) of tokens
+  __device__ __forceinline__ void set(const PromptParams& p, const Observed& with) {
+    o = with;
     rows = o.look * p.group;
     blocks = (rows + C::kRows - 1) / C::kRows;
-    steps = o.look > 0 ? (o.len + C::kStepKeys - 1) / C::kStepKeys : 0;
+    units = PASS == 3 ? (rows > 0 ? (o.len + C::kRows - 1) / C::kRows : 0) : blocks;
   }
+  __device__ __forceinline__ int least() const { return o.len - o.look; }        // place of the first row
   __device__ __forceinline__ int rows_of(int block) const { return min(C::kRows, rows - block * C::kRows); }
-  // largest place of a block's rows
-  __device__ __forceinline__ int top_of(const PromptParams& p, int block) const {
-    return o.len - o.look + (min(rows, (block + 1) * C::kRows) - 1) / p.group;
+  // steps of the first pass: up to the largest place of a block's rows
+  __device__ __forceinline__ int steps1(const PromptParams& p, int block) const {
+    return (least() + (min(rows, (block + 1) * C::kRows) - 1) / p.group) / C::kStepKeys + 1;
   }
-  __device__ __forceinline__ int steps_of(const PromptParams& p, int block) const { return top_of(p, block) / C::kStepKeys + 1; }
-  // first block that sees a step of the second pass
+  // first tile of rows that sees a block of tokens
+  __device__ __forceinline__ int first_tile(const PromptParams& p, int block) const {
+    const int j = block * C::kRows - least();
+    return j > 0 ? j * p.group / kTileRows : 0;
+  }
+  __device__ __forceinline__ int steps_of(const PromptParams& p, int unit) const {
+    return PASS == 3 ? (rows + kTileRows - 1) / kTileRows - first_tile(p, unit) : steps1(p, unit);
+  }
+  // of the second pass: steps, first block that sees one, steps from the first one on that all blocks see
+  __device__ __forceinline__ int steps() const { return rows > 0 ? (o.len + C::kStepKeys - 1) / C::kStepKeys : 0; }
   __device__ __forceinline__ int first_block(const PromptParams& p, int step) const {
-    const int j = step * C::kStepKeys - (o.len - o.look);
+    const int j = step * C::kStepKeys - least();
     return j > 0 ? j * p.group / C::kRows : 0;
   }
-  // steps, from the first one on, that all blocks see
-  __device__ __forceinline__ int common(const PromptParams& p) const {
-    return min(steps, (o.len - o.look + (C::kRows - 1) / p.group) / C::kStepKeys + 1);
-  }
-  __device__ __forceinline__ int64_t cost1(const PromptParams& p) const {      // of one kv head
+  __device__ __forceinline__ int common(const PromptParams& p) const { return min(steps(), (least() + (C::kRows - 1) / p.group) / C::kStepKeys + 1); }
+  // of one kv head, on the first pass's line and on this one's
+  __device__ __forceinline__ int64_t cost1(const PromptParams& p) const {
     int64_t n = 0;
-    for (int i = 0; i < blocks; ++i) n += steps_of(p, i) + kStart;
+    for (int i = 0; i < blocks; ++i) n += steps1(p, i) + kStart;
     return n;
   }
-  __device__ __forceinline__ int64_t cost2(const PromptParams& p) const {
-    if (blocks == 0) return 0;
-    const int all = common(p);
-    int64_t n = static_cast<int64_t>(all) * blocks;
-    for (int t = all; t < steps; ++t) n += blocks - first_block(p, t);
+  __device__ __forceinline__ int64_t cost(const PromptParams& p) const {
+    int64_t n = 0;
+    if (PASS == 2) {
+      if (blocks == 0) return 0;
+      const int all = common(p), every = steps();
+      n = static_cast<int64_t>(all) * blocks;
+      for (int t = all; t < every; ++t) n += blocks - first_block(p, t);
+    } else {
+      for (int i = 0; i < units; ++i) n += steps_of(p, i) + kStart;
+    }
     return n;
   }
 };
@@ -131,23 +157,35 @@ struct Work {
 // Steps t0 .. t0 + n - 1 of a block
 struct Item {
   int b, hk, block, t0, n;
-  bool load, release;    // the block's queries are not in shared memory yet; the next item, if any, loads others
-  bool first;            // the item begins the CTA's run (first pass)
+  bool load, release;    // the block is not in shared memory yet; the next item, if any, loads another
+  bool first;            // the item begins the CTA's run (not in the second pass)
   bool flush;            // last block over these steps (second pass)
   int chunk;             // steps whose sums wait (second pass)
-  int64_t at;            // where the unit begins on the first pass's line
+  int64_t at;            // where the unit begins: on the first pass's line (second pass), on its own (else)
 };
 
+// CTAs that share a line of units and where CTA c's run begins
 __device__ __forceinline__ int used_ctas(const PromptParams& p, int64_t line) {
   return static_cast<int>(min(static_cast<int64_t>(p.ctas), max(line / 2, static_cast<int64_t>(1))));
 }
-__device__ __forceinline__ int64_t run_begin(int64_t line, int c, int ctas) { return line * c / ctas; }
+// (A division of 64 bits takes some 500 cycles.)
+__device__ __forceinline__ bool fits_32(int64_t line, int ctas) { return line < (1ll << 31) && line * (ctas + 1) < (1ll << 32); }
+__device__ __forceinline__ int64_t run_begin(int64_t line, int c, int ctas) {
+  if (fits_32(line, ctas)) return static_cast<uint32_t>(line) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
+  return line * c / ctas;
+}
+// the last CTA whose run begins at or before x
+__device__ __forceinline__ int owner_of(int64_t line, int64_t x, int ctas) {
+  if (fits_32(line, ctas)) return min(ctas - 1, static_cast<int>((static_cast<uint32_t>(x + 1) * ctas - 1u) / static_cast<uint32_t>(line)));
+  return static_cast<int>(min(static_cast<int64_t>(ctas) - 1, ((x + 1) * ctas - 1) / line));
+}
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
   const int sz = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }       // all but the newest group
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -185,33 +223,35 @@ __device__ __forceinline__ uint32_t swz(int row, int ch, int block) {
   return (ch >> 3) * block + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
 }
 
-// PASS 1: normalisers; 2: sums.  FMT: what the cache holds (kKvSame, kKvE4M3, kKvE5M2)
+// PASS 1: normalisers; 2: sums, blocks of rows; 3: sums, blocks of tokens.  FMT: what the cache holds (kKvSame, kKvE4M3, kKvE5M2)
 template <typename T, int NH, int FMT, int R, int PASS>
-__global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const PromptParams p) {
+__global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1) weights_prompt_kernel(const PromptParams p) {
   constexpr bool KV8 = FMT != kKvSame;
   constexpr bool kScaled = KV8 && !std::is_same<T, __half>::value;      // bf16 queries become fp16, scaled by a power of two per row
-  using C = Cfg<NH, KV8, R>;
-  constexpr int kD = C::kD, kStages = C::kStages, KT = C::KT;
+  using C = Cfg<NH, KV8, R, PASS>;
+  using W = Work<C, PASS>;
+  constexpr int kD = C::kD, kStages = C::kStages, KT = C::KT, kRing = C::kRing, kIssueWarp = C::kIssueWarp;
   extern __shared__ __align__(1024) uint8_t prompt_smem[];
-  __shared__ uint64_t bars[2 * kStages + 10];
+  __shared__ uint64_t bars[2 * kStages + 8 + kRing];
   __shared__ uint32_t tmem_holder;
   __shared__ int fail_flag, holes;
-  __shared__ int begin_b;
-  __shared__ int64_t begin_at, begin_at1, line_of[3];       // places of the first request's first unit; run, length of the run, line of the first pass
-  __shared__ int used_of;                                   // CTAs of the first pass
-  __shared__ __align__(16) float neg_lse[3][C::kRows];      // -normaliser of the rows (second pass)
-  __shared__ __align__(16) float row_mul[3][kScaled ? C::kRows : 4];
-  __shared__ __align__(16) float cells[kChunk * 512];       // first pass: 2 x [4][128] maxima and sums; second: [parts][tokens]
-  uint8_t* sQ = prompt_smem;
-  uint8_t* ring = sQ + C::kQBytes;
+  __shared__ int begin_of[2], used_of;                      // request and kv head of the run's first unit; CTAs of the first pass
+  __shared__ Observed begin_request;
+  __shared__ int64_t begin_rest, begin_at1, line_of[4];     // steps in front of the run; first pass's place of the request; run, its end, both lines
+  __shared__ __align__(16) float neg_lse[kRing][C::kRingRows];      // -normaliser of rows (sums)
+  __shared__ __align__(16) float row_mul[kRing][kScaled ? C::kRingRows : 4];
+  __shared__ __align__(16) float cells[kChunk * 512];       // second pass: [parts][tokens]; else 2 x [4][128] maxima and sums
+  uint8_t* sBlock = prompt_smem;
+  uint8_t* ring = sBlock + C::kBlockBytes;
   uint64_t* full = bars;                 // [stage] the warps of a team
   uint64_t* empty = full + kStages;      // [stage] tcgen05.commit
   uint64_t* s_full = empty + kStages;    // [buffer] tcgen05.commit
   uint64_t* s_free = s_full + 2;         // [buffer] the computing warps have read the scores
-  uint64_t* q_full = s_free + 2;         // the warps that copy queries
-  uint64_t* q_free = q_full + 1;         // tcgen05.commit: the last scores of a block
-  uint64_t* l_full = q_free + 1;         // [3] the same warps, for the computing ones
-  uint64_t* met_bar = l_full + 3;        // the computing warps among themselves
+  uint64_t* b_first = s_free + 2;        // the computing warps: the first block
+  uint64_t* b_full = b_first + 1;        // the warp that copies blocks: the others
+  uint64_t* b_free = b_full + 1;         // tcgen05.commit: the last scores of a block
+  uint64_t* met_bar = b_free + 1;        // the computing warps among themselves
+  uint64_t* l_full = met_bar + 1;        // [ring] who writes normalisers and factors (not of the first block)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = p.group;
   pdl_wait_loads();
@@ -220,65 +260,81 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
   if (warp == 0) {
     const int per = (p.ix.batch + 31) / 32;
     const int first = min(p.ix.batch, lane * per), last = min(p.ix.batch, first + per);
-    int64_t mine1 = 0, mine2 = 0;
+    int64_t mine1 = 0, mine = 0;
     bool bad = false;
-    Work<C> w;
-    for (int b = first; b < last; ++b) {
-      w.set(p, b);
+    W w;
+    int64_t c1 = 0, c = 0;                // of one kv head of this lane's first request
+    for (int b = last - 1; b >= first; --b) {
+      w.set(p, observed_of(p, b));
       bad = bad || w.o.bad;
-      mine1 += w.cost1(p) * p.hkv;
-      if (PASS == 2) mine2 += w.cost2(p) * p.hkv;
+      c = w.cost(p);
+      c1 = PASS == 1 ? c : w.cost1(p);
+      mine += c * p.hkv;
+      mine1 += c1 * p.hkv;
     }
     if (PASS == 1 && bad && blockIdx.x == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
-    int64_t incl1 = mine1, incl2 = mine2;
+    int64_t incl1 = mine1, incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v1 = __shfl_up_sync(0xffffffffu, incl1, o), v2 = __shfl_up_sync(0xffffffffu, incl2, o);
-      if (lane >= o) {
-        incl1 += v1;
-        incl2 += v2;
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+      if (PASS != 1) {
+        const int64_t v1 = __shfl_up_sync(0xffffffffu, incl1, o);
+        if (lane >= o) incl1 += v1;
       }
     }
-    const int64_t line1 = __shfl_sync(0xffffffffu, incl1, 31), line = PASS == 1 ? line1 : __shfl_sync(0xffffffffu, incl2, 31);
-    const int used1 = used_ctas(p, line1), used = PASS == 1 ? used1 : static_cast<int>(min(static_cast<int64_t>(p.ctas), max(line, static_cast<int64_t>(1))));
-    const int c = blockIdx.x;
-    const int64_t begin = c < used ? run_begin(line, c, used) : line, end = c < used ? run_begin(line, c + 1, used) : line;
+    if (PASS == 1) incl1 = incl;
+    const int64_t line1 = __shfl_sync(0xffffffffu, incl1, 31), line = __shfl_sync(0xffffffffu, incl, 31);
+    // the second pass has no cost beside its steps
+    const int used = PASS == 2 ? static_cast<int>(min(static_cast<int64_t>(p.ctas), max(line, static_cast<int64_t>(1)))) : used_ctas(p, line);
+    const int cta = blockIdx.x;
+    const int64_t begin = cta < used ? run_begin(line, cta, used) : line, end = cta < used ? run_begin(line, cta + 1, used) : line;
     if (lane == 0) {
       line_of[0] = begin;
       line_of[1] = end;
       line_of[2] = line1;
-      used_of = used1;
+      line_of[3] = line;
+      used_of = used_ctas(p, line1);
       fail_flag = 0;
       holes = 0;
+      if (PASS == 1) p.jobs[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
-    int64_t at = PASS == 1 ? incl1 - mine1 : incl2 - mine2, at1 = incl1 - mine1;
-    if (begin < end && begin >= at && begin < (PASS == 1 ? incl1 : incl2)) {
+    int64_t at = incl - mine, at1 = incl1 - mine1;
+    if (begin < end && begin >= at && begin < incl) {
       for (int b = first; b < last; ++b) {
-        w.set(p, b);
-        const int64_t n1 = w.cost1(p) * p.hkv, n = PASS == 1 ? n1 : w.cost2(p) * p.hkv;
-        if (begin >= at && begin < at + n) {
-          begin_b = b;
-          begin_at = at;
+        if (b > first) {
+          w.set(p, observed_of(p, b));
+          c = w.cost(p);
+          c1 = PASS == 1 ? c : w.cost1(p);
+        }
+        if (begin >= at && begin < at + c * p.hkv) {
+          const int64_t in = begin - at;
+          const int hk = c < (1ll << 31) && in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(c) : static_cast<int>(in / c);
+          begin_of[0] = b;
+          begin_of[1] = hk;
+          begin_request = w.o;
+          begin_rest = in - hk * c;
           begin_at1 = at1;
         }
-        at += n;
-        at1 += n1;
+        at += c * p.hkv;
+        at1 += c1 * p.hkv;
       }
     }
   } else if (warp == kIssueWarp) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(&full[i], C::kTeam);
+        mbar_init(&full[i], 1);
         mbar_init(&empty[i], 1);
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
         mbar_init(&s_free[i], kCompute);
       }
-      mbar_init(q_full, C::kQWarps);
-      mbar_init(q_free, 1);
-      for (int i = 0; i < 3; ++i) mbar_init(&l_full[i], C::kQWarps);
+      mbar_init(b_first, kCompute);
+      mbar_init(b_full, 1);
+      mbar_init(b_free, 1);
       mbar_init(met_bar, kCompute);
+      for (int i = 0; i < kRing; ++i) mbar_init(&l_full[i], 1);
       fence_barrier_init();
     }
     __syncwarp();
@@ -296,62 +352,66 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
 
   // Calls fn(request's numbers, item) for every item of the run; all roles walk the same way.
   auto items = [&](auto&& fn) {
-    const int64_t begin = line_of[0], end = aligned ? line_of[1] : line_of[0];
-    if (begin >= end) return;
-    Work<C> w;
+    int64_t pos = line_of[0];
+    const int64_t end = aligned ? line_of[1] : pos;
+    if (pos >= end) return;
+    W w;
     Item it;
-    it.b = begin_b;
-    w.set(p, it.b);
-    int64_t request_at = begin_at, at1 = begin_at1;        // of the request on this pass's and on the first pass's line
-    int64_t unit = PASS == 1 ? w.cost1(p) : w.cost2(p), unit1 = PASS == 1 ? unit : w.cost1(p);
-    it.hk = static_cast<int>((begin - request_at) / unit);
-    int64_t pos = begin, rest = begin - request_at - it.hk * unit;
+    it.b = begin_of[0];
+    it.hk = begin_of[1];
+    w.set(p, begin_request);
+    int64_t rest = begin_rest;
     it.block = 0;
     it.first = true;
     it.flush = false;
     it.chunk = 0;
-    int64_t block_at = 0;
     int t = 0;
-    if (PASS == 1) {
-      while (rest >= w.steps_of(p, it.block) + kStart) {
-        const int n = w.steps_of(p, it.block++) + kStart;
-        rest -= n;
-        block_at += n;
+    auto next_request = [&]() {
+      do {
+        if (++it.b >= p.ix.batch) return false;
+        w.set(p, observed_of(p, it.b));
+      } while (w.units == 0);
+      return true;
+    };
+    if (PASS != 2) {
+      int all = w.steps_of(p, 0);
+      while (rest >= all + kStart) {
+        rest -= all + kStart;
+        all = w.steps_of(p, ++it.block);
       }
       t = static_cast<int>(rest);
-      while (pos < end) {
-        const int all = w.steps_of(p, it.block), n = static_cast<int>(min(static_cast<int64_t>(all - t), end - pos));
+      while (true) {
+        const int n = static_cast<int>(min(static_cast<int64_t>(all - t), end - pos));
         if (n > 0) {
           it.t0 = t;
           it.n = n;
           it.load = it.release = true;
-          it.at = 0;
+          it.at = pos - t;
           if (!fn(w, it)) return;
-          it.first = false;
           pos += n;
           t += n;
         }
         if (pos >= end) return;
         pos += all + kStart - t;
+        if (pos >= end) return;
         it.first = false;
         t = 0;
-        if (++it.block == w.blocks) {
+        if (++it.block == w.units) {
           it.block = 0;
           if (++it.hk == p.hkv) {
             it.hk = 0;
-            do {
-              if (++it.b >= p.ix.batch) return;
-              w.set(p, it.b);
-            } while (w.blocks == 0);
+            if (!next_request()) return;
           }
         }
+        all = w.steps_of(p, it.block);
       }
     } else {
       // the first step that begins at or behind the run's begin
+      int64_t at1 = begin_at1, unit1 = w.cost1(p);        // of the request on the first pass's line
       const int all = w.common(p);
       const int64_t level = static_cast<int64_t>(all) * w.blocks;
       if (rest <= level) {
-        t = static_cast<int>((rest + w.blocks - 1) / w.blocks);
+        t = w.blocks == 1 ? static_cast<int>(rest) : static_cast<int>((rest + w.blocks - 1) / w.blocks);
         pos += static_cast<int64_t>(t) * w.blocks - rest;
       } else {
         t = all;
@@ -361,33 +421,31 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
       }
       int loaded = -1;        // the block whose queries are there
       while (pos < end) {
-        if (t >= w.steps) {
+        const int steps = w.steps();
+        if (t >= steps) {
           t = 0;
           loaded = -1;
           if (++it.hk == p.hkv) {
             it.hk = 0;
             at1 += unit1 * p.hkv;
-            do {
-              if (++it.b >= p.ix.batch) return;
-              w.set(p, it.b);
-            } while (w.blocks == 0);
+            if (!next_request()) return;
             unit1 = w.cost1(p);
           }
           continue;
         }
         int n = 0;
-        while (n < kChunk && t + n < w.steps && pos < end) pos += w.blocks - w.first_block(p, t + n++);
+        while (n < kChunk && t + n < steps && pos < end) pos += w.blocks - w.first_block(p, t + n++);
         it.t0 = t;
         it.chunk = n;
         it.block = w.first_block(p, t);
         int64_t off = 0;
-        for (int i = 0; i < it.block; ++i) off += w.steps_of(p, i) + kStart;
+        for (int i = 0; i < it.block; ++i) off += w.steps1(p, i) + kStart;
         for (; it.block < w.blocks; ++it.block) {
-          const int mine = w.steps_of(p, it.block);
+          const int mine = w.steps1(p, it.block);
           it.n = min(n, mine - t);
           it.load = loaded != it.block;
           it.flush = it.block == w.blocks - 1;
-          it.release = !it.flush || t + n >= w.steps || pos >= end || w.first_block(p, t + n) != it.block;
+          it.release = !it.flush || t + n >= steps || pos >= end || w.first_block(p, t + n) != it.block;
           it.at = at1 + it.hk * unit1 + off;
           loaded = it.block;
           if (!fn(w, it)) return;
@@ -398,204 +456,292 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
     }
   };
 
-  if (warp >= kCompute && warp < kCompute + C::kTeam * C::kTeams) {
-    // =============================== keys ===============================
-    const int team = (warp - kCompute) / C::kTeam, part = (warp - kCompute) % C::kTeam;
-    constexpr int kPart = 128 / C::kTeam;              // rows of this warp
-    constexpr int kCh = KV8 ? 4 * NH : 8 * NH;         // 16-byte pieces of a cached row
-    constexpr int kRowsPer = 32 / kCh;                 // rows of a warp's copy
-    using Elem = typename std::conditional<KV8, uint8_t, uint16_t>::type;
-    bool bad = false, ok = true;
-    uint32_t stage0 = 0;                               // stages of the items before
-    items([&](const Work<C>& w, const Item& it) {
-      const int* rtt = p.ix.req_to_token + static_cast<int64_t>(w.o.row) * p.ix.table_stride;
-      const int base = it.t0 * C::kStepKeys + part * kPart, stages = it.n * KT;
-      struct Slots {
-        int s[kPart / 32];
-      };
-      // slots of tokens lane, lane + 32, .. of this warp's rows of stage i
-      auto slots_of = [&](int i) {
-        Slots s;
-#pragma unroll
-        for (int k = 0; k < kPart / 32; ++k) {
-          const int tok = base + i * 128 + k * 32 + lane;
-          s.s[k] = i < stages && tok < w.o.len ? max(__ldcg(rtt + tok), -1) : kNoToken;      // no number of the table is taken for kNoToken
-        }
-        return s;
-      };
-      const int ch = lane % kCh, r0 = lane / kCh;
-      const Elem* from = static_cast<const Elem*>(p.k_cache) + it.hk * p.kv_head_stride + ch * (16 / sizeof(Elem));
-      int i = (team + C::kTeams - static_cast<int>(stage0 % C::kTeams)) % C::kTeams;
-      Slots next = slots_of(i);
-      for (; i < stages; i += C::kTeams) {
-        const uint32_t n = stage0 + i, st = n % kStages, stage = smem_u32(ring) + st * C::kStage;
-        Slots s = next;
-#pragma unroll
-        for (int k = 0; k < kPart / 32; ++k)
-          if (s.s[k] < 0 || s.s[k] >= p.num_slots) {
-            bad = bad || s.s[k] != kNoToken;
-            s.s[k] = -1;
-          }
-        next = slots_of(i + C::kTeams);
-        if (n >= kStages && !mbar_wait_relaxed(&empty[st], (n / kStages - 1) & 1, 20)) ok = false;
-        if (!(ok = __all_sync(0xffffffffu, ok))) return false;
-        if constexpr (!KV8) {
-#pragma unroll
-          for (int k = 0; k < kPart / kRowsPer; ++k) {
-            const int row = k * kRowsPer + r0;
-            const int rs = __shfl_sync(0xffffffffu, s.s[k * kRowsPer / 32], row & 31);
-            cp16(stage + swz(part * kPart + row, ch, C::kKBlock), from + max(rs, 0) * p.kv_tok_stride, rs >= 0);
-          }
-          cp_commit();
-          cp_wait_all();
-        } else {
-          constexpr int kBatch = 8;
-          static_assert(kPart / kRowsPer % kBatch == 0, "batches of rows");
-          auto widen = [&](uint32_t two) -> uint32_t {     // two 8-bit values -> two fp16, exactly
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), FMT == kKvE5M2 ? __NV_E5M2 : __NV_E4M3);
-            return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
-          };
-#pragma unroll
-          for (int k0 = 0; k0 < kPart / kRowsPer; k0 += kBatch) {
-            uint4 x[kBatch];
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int row = (k0 + k) * kRowsPer + r0;
-              const int rs = __shfl_sync(0xffffffffu, s.s[(k0 + k) * kRowsPer / 32], row & 31);
-              x[k] = rs >= 0 ? __ldcg(reinterpret_cast<const uint4*>(from + rs * p.kv_tok_stride)) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int row = part * kPart + (k0 + k) * kRowsPer + r0;
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t a = h ? x[k].z : x[k].x, b = h ? x[k].w : x[k].y;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + swz(row, ch * 2 + h, C::kKBlock)), "r"(widen(a)),
-                             "r"(widen(a >> 16)), "r"(widen(b)), "r"(widen(b >> 16))
-                             : "memory");
-              }
-            }
-          }
-          fence_proxy_async_smem();
-        }
-        if (bad) holes = 1;               // the computing warps look at every step
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[st]);
+  // ---- what is copied, by one warp or several ----
+  using Elem = typename std::conditional<KV8, uint8_t, uint16_t>::type;
+  constexpr int kKeyPieces = KV8 ? 4 * NH : 8 * NH, kKeyRows = 32 / kKeyPieces;      // 16-byte pieces of a cached row; rows of a warp's copy
+  auto widen = [&](uint32_t two) -> uint32_t {     // two 8-bit values -> two fp16, exactly
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), FMT == kKvE5M2 ? __NV_E5M2 : __NV_E4M3);
+    return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+  };
+  // 32 rows of keys whose slots the lanes have (-1: zeros), to rows row0 .. of a tile with blocks of `block` bytes
+  auto copy_keys = [&](const Elem* head, int slot, uint32_t dst, int row0, int block) {
+    const int ch = lane % kKeyPieces, r0 = lane / kKeyPieces;
+    const Elem* from = head + ch * (16 / sizeof(Elem));
+    if constexpr (!KV8) {
+#pragma unroll 4
+      for (int k = 0; k < kKeyPieces; ++k) {
+        const int row = k * kKeyRows + r0, rs = __shfl_sync(0xffffffffu, slot, row);
+        cp16(dst + swz(row0 + row, ch, block), from + max(rs, 0) * p.kv_tok_stride, rs >= 0);
       }
-      stage0 += stages;
-      return true;
-    });
-    if (!ok) fail_flag = 1;
-    if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
-  } else if (warp >= kCompute && warp < kIssueWarp) {
-    // =============================== queries, and in the second pass the rows' normalisers ===============================
-    const int me = warp - kCompute - C::kTeam * C::kTeams;
-    bool ok = true;
-    uint32_t loads = 0;
-    items([&](const Work<C>& w, const Item& it) {
-      if (!it.load) return true;
-      if (loads > 0 && !mbar_wait_relaxed(q_free, (loads - 1) & 1)) ok = false;
-      if (!(ok = __all_sync(0xffffffffu, ok))) return false;
-      const int rows = w.rows_of(it.block), row0 = it.block * C::kRows;
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(w.o.first) * p.q_stride + static_cast<int64_t>(it.hk) * g * kD;
-      constexpr int kCh = 8 * NH;               // 16-byte pieces of a row
-      if constexpr (!kScaled) {
-        for (int c = me * 32 + lane; c < rows * kCh; c += C::kQWarps * 32) {
-          const int row = c / kCh, ch = c % kCh, j = (row0 + row) / g;
-          cp16(smem_u32(sQ) + swz(row, ch, C::kQBlock), q + j * p.q_stride + static_cast<int64_t>(row0 + row - j * g) * kD + ch * 8, true);
+    } else {
+      constexpr int kBatch = kKeyPieces < 8 ? kKeyPieces : 8;
+#pragma unroll 1
+      for (int k0 = 0; k0 < kKeyPieces; k0 += kBatch) {
+        uint4 x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int rs = __shfl_sync(0xffffffffu, slot, (k0 + k) * kKeyRows + r0);
+          x[k] = rs >= 0 ? __ldcg(reinterpret_cast<const uint4*>(from + rs * p.kv_tok_stride)) : make_uint4(0, 0, 0, 0);
         }
-        cp_commit();
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int row = row0 + (k0 + k) * kKeyRows + r0;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a = h ? x[k].z : x[k].x, b = h ? x[k].w : x[k].y;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + swz(row, ch * 2 + h, block)), "r"(widen(a)), "r"(widen(a >> 16)),
+                         "r"(widen(b)), "r"(widen(b >> 16))
+                         : "memory");
+          }
+        }
+      }
+    }
+  };
+  // n rows of queries from row r0 of the request on, every `step`-th 32 pieces from the `me`-th on
+  auto copy_queries = [&](const W& w, int hk, int r0, int n, uint32_t dst, int block, float* muls, int me, int step) {
+    const int j0 = r0 / g, h0 = r0 - j0 * g;
+    const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(w.o.first + j0) * p.q_stride + static_cast<int64_t>(hk) * g * kD;
+    constexpr int kCh = 8 * NH, kRowsPer = 32 / kCh;          // 16-byte pieces of a row
+    const int ch = lane % kCh;
+#pragma unroll 4
+    for (int row = me * kRowsPer + lane / kCh; row < (n + kRowsPer - 1) / kRowsPer * kRowsPer; row += step * kRowsPer) {
+      const int x = h0 + row, j = (x * p.inv_group) >> 16;
+      const uint16_t* from = q + j * p.q_stride + static_cast<int64_t>(x - j * g) * kD + ch * 8;
+      if constexpr (!kScaled) {
+        if (row < n) cp16(dst + swz(row, ch, block), from, true);
       } else {
         // the largest of a row gets an exponent of 14: what is 2^-25 times smaller than that goes below fp16's last place
-        constexpr int kLanes = kCh < 32 ? kCh : 32;
-        for (int c0 = me * 32; c0 < rows * kCh; c0 += C::kQWarps * 32) {
-          const int c = c0 + lane, row = c / kCh, ch = c % kCh;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (row < rows) {
-            const int j = (row0 + row) / g;
-            x = __ldcg(reinterpret_cast<const uint4*>(q + j * p.q_stride + static_cast<int64_t>(row0 + row - j * g) * kD + ch * 8));
-          }
-          uint32_t v[4] = {x.x, x.y, x.z, x.w};
-          float top = 0.f;
+        uint4 y = make_uint4(0, 0, 0, 0);
+        if (row < n) y = __ldcg(reinterpret_cast<const uint4*>(from));
+        uint32_t v[4] = {y.x, y.y, y.z, y.w};
+        float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack_bf16x2(v[i]);
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-#pragma unroll
-          for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int raise = top > 0.f ? min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126) : 0;
-          const float by = __uint_as_float((raise + 127) << 23);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack_bf16x2(v[i]);
-            const __half2 y = __floats2half2_rn(f.x * by, f.y * by);
-            v[i] = *reinterpret_cast<const uint32_t*>(&y);
-          }
-          if (row < rows) {
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(sQ) + swz(row, ch, C::kQBlock)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
-                         : "memory");
-            if (ch == 0) row_mul[loads % 3][row] = p.scale_log2 * __uint_as_float((127 - raise) << 23);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack_bf16x2(v[i]);
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
+#pragma unroll
+        for (int o = 1; o < kCh; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int raise = top > 0.f ? min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126) : 0;
+        const float by = __uint_as_float((raise + 127) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack_bf16x2(v[i]);
+          const __half2 z = __floats2half2_rn(f.x * by, f.y * by);
+          v[i] = *reinterpret_cast<const uint32_t*>(&z);
+        }
+        if (row < n) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + swz(row, ch, block)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+          if (ch == 0) muls[row] = p.scale_log2 * __uint_as_float((127 - raise) << 23);
+        }
+      }
+    }
+  };
+  // -normaliser of row r of the request, whose block begins at `at` on the first pass's line and has n steps
+  struct Parts {
+    int c0, c1, second;       // the first CTA has the block in its second place
+  };
+  auto parts_of = [&](int64_t at, int n) {
+    const int64_t line = line_of[2];
+    Parts x;
+    x.c0 = owner_of(line, at, used_of);
+    x.c1 = owner_of(line, at + n - 1, used_of);
+    x.second = run_begin(line, x.c0, used_of) < at ? 1 : 0;
+    return x;
+  };
+  auto normaliser = [&](const W& w, int hk, int r, const Parts& x) -> float {
+    const int j = r / g, head = hk * g + r - j * g;
+    float lse;
+    if (x.c0 == x.c1) {
+      lse = __ldcg(p.lse + static_cast<int64_t>(w.o.first + j) * p.hkv * g + head);
+    } else {
+      const int row = r % C::kRows;
+      auto part = [&](int c) { return __ldcg(p.part + (static_cast<int64_t>(c) * 2 + (c == x.c0 ? x.second : 0)) * C::kRows + row); };
+      float top = -INFINITY;
+#pragma unroll 8
+      for (int c = x.c0; c <= x.c1; ++c) top = fmaxf(top, part(c));
+      const bool none = top == -INFINITY;
+      const float sink = p.sink != nullptr ? __ldcg(p.sink + head) * kLog2e : -INFINITY;
+      top = fmaxf(top, sink);
+      float sum = p.sink != nullptr ? exp2f(sink - top) : 0.f;
+#pragma unroll 8
+      for (int c = x.c0; c <= x.c1; ++c) {
+        const float v = part(c);
+        sum += v == -INFINITY ? 0.f : exp2f(v - top);
+      }
+      lse = none && sum == sum ? -INFINITY : top + log2f(sum);
+    }
+    return lse == -INFINITY ? -INFINITY : -lse;       // nothing seen: no weights
+  };
+  // an item's block, by warps `me` of `all`, and in the second pass its rows' normalisers; true where a token's slot lies outside the cache
+  auto load_block = [&](const W& w, const Item& it, int held, int me, int all) {
+    bool bad = false;
+    if constexpr (PASS == 3) {
+      const Elem* head = static_cast<const Elem*>(p.k_cache) + it.hk * p.kv_head_stride;
+      const int* rtt = p.ix.req_to_token + static_cast<int64_t>(w.o.row) * p.ix.table_stride;
+      for (int row0 = me * 32; row0 < C::kRows; row0 += all * 32) {
+        const int tok = it.block * C::kRows + row0 + lane;
+        int s = tok < w.o.len ? __ldcg(rtt + tok) : -1;
+        if (s < 0 || s >= p.num_slots) {
+          bad = bad || tok < w.o.len;
+          s = -1;
+        }
+        copy_keys(head, s, smem_u32(sBlock), row0, C::kBlock);
+      }
+    } else {
+      const int rows = w.rows_of(it.block);
+      copy_queries(w, it.hk, it.block * C::kRows, rows, smem_u32(sBlock), C::kBlock, row_mul[held], me, all);
+      if (PASS == 2) {
+        const Parts x = parts_of(it.at, w.steps1(p, it.block));
+        for (int row = me * 32 + lane; row < rows; row += all * 32) neg_lse[held][row] = normaliser(w, it.hk, it.block * C::kRows + row, x);
+      }
+    }
+    cp_commit();
+    cp_wait_all();
+    fence_proxy_async_smem();
+    if (bad) holes = 1;               // the computing warps look at every step
+    __syncwarp();
+    return bad;
+  };
+
+  if (warp >= kCompute) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    if (warp < C::kBlockWarp) {
+      // =============================== stages ===============================
+      constexpr int kWarps = C::kCopying;
+      const int me = warp - kCompute;
+      bool bad = false, ok = true;
+      uint32_t stage0 = 0;                               // stages of the items before
+      // A stage may be on its way while the one before is waited for, unless its place waits for that one's products
+      constexpr bool kTwo = !KV8 && kStages > kWarps;
+      int pending = -1;                                  // the place of a stage that has not been waited for
+      auto arrived = [&](int place) {
         fence_proxy_async_smem();
-      }
-      if constexpr (PASS == 2) {
-        const int n = w.steps_of(p, it.block), used = used_of;
-        const int64_t line = line_of[2];
-        // the last CTA whose run begins at or before x
-        auto owner = [&](int64_t x) { return static_cast<int>(min(static_cast<int64_t>(used) - 1, ((x + 1) * used - 1) / line)); };
-        const int c0 = owner(it.at), c1 = owner(it.at + n - 1);
-        const int second = run_begin(line, c0, used) < it.at ? 1 : 0;      // the first CTA has the block in its second place
-        for (int row = me * 32 + lane; row < rows; row += C::kQWarps * 32) {
-          const int j = (row0 + row) / g, head = it.hk * g + row0 + row - j * g;
-          float lse;
-          if (c0 == c1) {
-            lse = __ldcg(p.lse + static_cast<int64_t>(w.o.first + j) * p.hkv * g + head);
-          } else {
-            auto part = [&](int c) { return __ldcg(p.part + (static_cast<int64_t>(c) * 2 + (c == c0 ? second : 0)) * C::kRows + row); };
-            float top = -INFINITY;
-#pragma unroll 8
-            for (int c = c0; c <= c1; ++c) top = fmaxf(top, part(c));
-            const bool none = top == -INFINITY;
-            const float sink = p.sink != nullptr ? __ldcg(p.sink + head) * kLog2e : -INFINITY;
-            top = fmaxf(top, sink);
-            float sum = p.sink != nullptr ? exp2f(sink - top) : 0.f;
-#pragma unroll 8
-            for (int c = c0; c <= c1; ++c) {
-              const float v = part(c);
-              sum += v == -INFINITY ? 0.f : exp2f(v - top);
+        if (bad) holes = 1;               // the computing warps look at every step
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[place]);
+      };
+      items([&](const W& w, const Item& it) {
+        const int stages = it.n * KT;
+        int i = me < kWarps ? (me + kWarps - static_cast<int>(stage0 % kWarps)) % kWarps : stages;
+        auto wait_free = [&](uint32_t n) {       // asleep in between: warps that poll take issue slots from the computing ones
+          if (n >= kStages && !mbar_wait_relaxed(&empty[n % kStages], (n / kStages - 1) & 1, 20)) ok = false;
+          return ok = __all_sync(0xffffffffu, ok);
+        };
+        if constexpr (PASS == 3) {
+          const int tile0 = w.first_tile(p, it.block) + it.t0;
+          // the block of the first pass that a tile of rows lies in, and where it begins on that line
+          int block = tile0 * kTileRows / C::kRows;
+          int64_t at = begin_at1;
+          {
+            W v;
+            for (int b = begin_of[0]; b < it.b; ++b) {
+              v.set(p, observed_of(p, b));
+              at += v.cost1(p) * p.hkv;
             }
-            lse = none && sum == sum ? -INFINITY : top + log2f(sum);
+            at += w.cost1(p) * it.hk;
           }
-          neg_lse[loads % 3][row] = lse == -INFINITY ? -INFINITY : -lse;       // nothing seen: no weights
+          for (int b = 0; b < block; ++b) at += w.steps1(p, b) + kStart;
+          for (; i < stages; i += kWarps) {
+            const uint32_t n = stage0 + i;
+            if (!wait_free(n)) return false;
+            const int r0 = (tile0 + i) * kTileRows, rows = min(kTileRows, w.rows - r0);
+            for (; (block + 1) * C::kRows <= r0; ++block) at += w.steps1(p, block) + kStart;
+            const uint32_t held = n % kRing;
+            copy_queries(w, it.hk, r0, rows, smem_u32(ring) + n % kStages * C::kStage, C::kPiece, row_mul[held], 0, 1);
+            cp_commit();
+            const Parts x = parts_of(at, w.steps1(p, block));
+            for (int row = lane; row < rows; row += 32) neg_lse[held][row] = normaliser(w, it.hk, r0 + row, x);
+            cp_wait_all();
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&full[n % kStages]);
+              mbar_arrive(&l_full[held]);
+            }
+          }
+        } else {
+          const int* rtt = p.ix.req_to_token + static_cast<int64_t>(w.o.row) * p.ix.table_stride;
+          const int base = it.t0 * C::kStepKeys;
+          const Elem* head = static_cast<const Elem*>(p.k_cache) + it.hk * p.kv_head_stride;
+          int next[4];          // slots of a stage's tokens lane, lane + 32, ..
+          auto look = [&](int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int tok = base + i * 128 + k * 32 + lane;
+              next[k] = i < stages && tok < w.o.len ? max(__ldcg(rtt + tok), -1) : kNoToken;      // no number of the table is taken for kNoToken
+            }
+          };
+          look(i);
+          for (; i < stages; i += kWarps) {
+            const uint32_t n = stage0 + i, stage = smem_u32(ring) + n % kStages * C::kStage;
+            int s[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              s[k] = next[k];
+              if (s[k] < 0 || s[k] >= p.num_slots) {
+                bad = bad || s[k] != kNoToken;
+                s[k] = -1;
+              }
+            }
+            look(i + kWarps);
+            if (!wait_free(n)) return false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) copy_keys(head, s[k], stage, k * 32, C::kPiece);
+            cp_commit();
+            if (kTwo) {
+              if (pending >= 0) {
+                cp_wait_one();
+                arrived(pending);
+              }
+              pending = n % kStages;
+            } else {
+              cp_wait_all();
+              arrived(n % kStages);
+            }
+          }
         }
-      }
-      if constexpr (!kScaled) cp_wait_all();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(q_full);
-        mbar_arrive(&l_full[loads % 3]);
-      }
-      ++loads;
-      return true;
-    });
-    if (!ok) fail_flag = 1;
-  } else if (warp == kIssueWarp) {
-    if (elect_one()) {
+        stage0 += stages;
+        return true;
+      });
+      cp_wait_all();
+      if (pending >= 0) arrived(pending);
+      if (!ok) fail_flag = 1;
+      if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
+    } else if (warp == C::kBlockWarp) {
+      // =============================== blocks behind the first ===============================
+      bool bad = false, ok = true;
+      uint32_t loads = 0;
+      items([&](const W& w, const Item& it) {
+        if (!it.load) return true;
+        if (loads > 0) {
+          if (!mbar_wait_relaxed(b_free, (loads - 1) & 1)) ok = false;
+          if (!(ok = __all_sync(0xffffffffu, ok))) return false;
+          bad = load_block(w, it, loads % kRing, 0, 1) || bad;
+          if (lane == 0) {
+            mbar_arrive(b_full);
+            if (PASS != 3) mbar_arrive(&l_full[loads % kRing]);
+          }
+        }
+        ++loads;
+        return true;
+      });
+      if (!ok) fail_flag = 1;
+      if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
+    } else if (elect_one()) {
       // =============================== products ===============================
       bool ok = true;
-      const uint64_t q_desc = umma_desc_k_sw128(smem_u32(sQ)), k_desc0 = umma_desc_k_sw128(smem_u32(ring));
+      const uint64_t b_desc = umma_desc_k_sw128(smem_u32(sBlock)), r_desc0 = umma_desc_k_sw128(smem_u32(ring));
       const uint32_t fmt = KV8 || std::is_same<T, __half>::value ? 0u : 1u;
       uint32_t stage = 0, step = 0, loads = 0;
-      items([&](const Work<C>& w, const Item& it) {
+      items([&](const W& w, const Item& it) {
         if (it.load) {
-          if (ok && !mbar_wait(q_full, loads & 1, &fail_flag)) ok = false;
+          if (ok && !mbar_wait(loads == 0 ? b_first : b_full, loads == 0 ? 0 : (loads - 1) & 1, &fail_flag)) ok = false;
           ++loads;
         }
-        const int rows = w.rows_of(it.block);
-        // first pass: N is the 128 tokens of a stage; second: the block's rows
-        const uint32_t idesc = umma_idesc(128, PASS == 1 ? 128 : (rows + 15) / 16 * 16, 1, fmt, fmt, 0, 0);
+        // lanes are the block's rows, a tile at a time, over the stage's 128; in the second pass the stage's over the block's
+        const int rows = PASS == 3 ? min(C::kRows, w.o.len - it.block * C::kRows) : w.rows_of(it.block);
+        const uint32_t idesc = umma_idesc(128, PASS == 2 ? (rows + 15) / 16 * 16 : 128, 1, fmt, fmt, 0, 0);
         for (int t = 0; t < it.n && ok; ++t, ++step) {
           const uint32_t buf = step & 1;
           if (step >= 2 && !mbar_wait(&s_free[buf], ((step >> 1) - 1) & 1, &fail_flag)) ok = false;
@@ -604,18 +750,18 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
             const uint32_t st = stage % kStages;
             if (ok && !mbar_wait(&full[st], (stage / kStages) & 1, &fail_flag)) ok = false;
             if (!ok) break;
-            fence_proxy_async_smem();       // copies by cp.async were made in the generic proxy
+            fence_proxy_async_smem();       // copies were made in the generic proxy
             tc_fence_after_sync();
-            const uint64_t k_desc = k_desc0 + st * (C::kStage >> 4);
+            const uint64_t r_desc = r_desc0 + st * (C::kStage >> 4);
             const uint32_t to = tmem + buf * C::kCols + kt * 128;
 #pragma unroll
-            for (int h = 0; h < (PASS == 1 ? C::RT : 1); ++h) {
+            for (int h = 0; h < (PASS == 2 ? 1 : C::RT); ++h) {
               if (h * kTileRows >= rows) break;
 #pragma unroll
               for (int kk = 0; kk < 4 * NH; ++kk) {
-                const uint64_t a = q_desc + (kk >> 2) * (C::kQBlock >> 4) + h * (kTileRows * 128 >> 4) + (kk & 3) * 2;
-                const uint64_t k = k_desc + (kk >> 2) * (C::kKBlock >> 4) + (kk & 3) * 2;
-                umma_f16(to + h * 128, PASS == 1 ? a : k, PASS == 1 ? k : a, idesc, kk > 0 ? 1u : 0u);
+                const uint64_t b = b_desc + (kk >> 2) * (C::kBlock >> 4) + h * (kTileRows * 128 >> 4) + (kk & 3) * 2;
+                const uint64_t r = r_desc + (kk >> 2) * (C::kPiece >> 4) + (kk & 3) * 2;
+                umma_f16(to + h * 128, PASS == 2 ? r : b, PASS == 2 ? b : r, idesc, kk > 0 ? 1u : 0u);
               }
             }
             umma_commit(&empty[st]);
@@ -623,18 +769,19 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
           if (!ok) break;
           umma_commit(&s_full[buf]);
         }
-        if (ok && it.release) umma_commit(q_free);
+        if (ok && it.release) umma_commit(b_free);
         return ok;
       });
       if (!ok) fail_flag = 1;
     }
   } else {
     // =============================== scores ===============================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kComputeRegs));
     const int quarter = warp >> 2, in_tile = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool capped = p.cap_out > 0.f;
     constexpr int kWarpCols = C::kWarpCols;
-    bool ok = true;
+    bool ok = true, bad = false;
     uint32_t step = 0, loads = 0, met = 0, turn = 0;
     auto meet = [&]() {        // of all computing warps; false where one has given up
       __syncwarp();
@@ -648,23 +795,72 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
       tc_fence_after_sync();
       return ok;
     };
-    auto scores_read = [&]() {
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[step & 1]);
+    // 32 of a quarter's columns of this step (none where `any` is false); behind the last of them the buffer is free
+    uint32_t raw[32];
+    auto read_scores = [&](int half, bool any) {
+      if (any) {
+        tmem_ld_32x32(tmem + lanes + (step & 1) * C::kCols + quarter * kWarpCols + half, raw);
+        tmem_ld_wait();
+      }
+      if (half == kWarpCols - 32) {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[step & 1]);
+      }
+    };
+    auto gaps = [&]() { return *const_cast<const volatile int*>(&holes) != 0; };
+    auto slot_inside = [&](const W& w, int token) {
+      const int s = token < w.o.len ? __ldcg(p.ix.req_to_token + static_cast<int64_t>(w.o.row) * p.ix.table_stride + token) : -1;
+      return s >= 0 && s < p.num_slots;
     };
     // cap tanh(x / cap), in the log2 domain; tanh(y) = 1 - 2 / (1 + e^(2 y))
     auto cap = [&](uint32_t x, float mul) { return __float_as_uint(p.cap_out * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(x) * mul * p.cap_in)))); };
-
-    items([&](const Work<C>& w, const Item& it) {
-      const int rows = w.rows_of(it.block), row0 = it.block * C::kRows, least = w.o.len - w.o.look;
-      if (it.load) ++loads;
-      const int held = (loads - 1) % 3;
-      if (PASS == 2 || kScaled) {
-        if (it.load && !mbar_wait(&l_full[held], ((loads - 1) / 3) & 1, &fail_flag)) ok = false;
-        if (!(ok = __all_sync(0xffffffffu, ok))) return false;
+    // What a token gets of 32 rows: columns from `low` up to `high` alone where masked
+    auto weights = [&](const float* neg, const float* muls, bool masked, int low, int high, uint64_t (&sums)[4]) {
+      if (capped) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) raw[c] = cap(raw[c], kScaled ? muls[c] : p.scale_log2);
       }
+      const float same = capped ? 1.f : p.scale_log2;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 n4 = *reinterpret_cast<const float4*>(neg + 4 * i);
+        float4 m4 = make_float4(same, same, same, same);
+        if (kScaled && !capped) m4 = *reinterpret_cast<const float4*>(muls + 4 * i);
+        const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), pair_of(m4.x, m4.y), pair_of(n4.x, n4.y)));
+        const float2 y = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), pair_of(m4.z, m4.w), pair_of(n4.z, n4.w)));
+        float e[4] = {ex2(x.x), ex2(x.y), ex2(y.x), ex2(y.y)};
+        if (masked) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e[k] = 4 * i + k >= low && 4 * i + k < high ? e[k] : 0.f;
+        }
+        sums[(2 * i) & 3] = add2(sums[(2 * i) & 3], pair_of(e[0], e[1]));
+        sums[(2 * i + 1) & 3] = add2(sums[(2 * i + 1) & 3], pair_of(e[2], e[3]));
+      }
+    };
+    auto total = [&](const uint64_t (&sums)[4]) {
+      const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+      return both.x + both.y;
+    };
+
+    items([&](const W& w, const Item& it) {
+      const int least = w.least();
+      if (it.load) {
+        const int held = loads % kRing;
+        if (loads == 0) {
+          bad = load_block(w, it, 0, warp, kCompute);
+          if (lane == 0) mbar_arrive(b_first);
+          if ((PASS == 2 || (PASS == 1 && kScaled)) && !mbar_wait(b_first, 0, &fail_flag)) ok = false;
+        } else if (PASS == 2 || (PASS == 1 && kScaled)) {
+          // (the first block's place was not written by the warp that arrives here)
+          if (!mbar_wait(&l_full[held], (held == 0 ? loads / kRing - 1 : loads / kRing) & 1, &fail_flag)) ok = false;
+        }
+        if (!(ok = __all_sync(0xffffffffu, ok))) return false;
+        ++loads;
+      }
+      const int held = (loads - 1) % kRing;
       if constexpr (PASS == 1) {
+        const int rows = w.rows_of(it.block), row0 = it.block * C::kRows;
         const int row = (C::RT == 2 ? (quarter >> 1) * 128 : 0) + in_tile, col0 = quarter * kWarpCols % C::kStepKeys;
         const bool valid = row < rows, any = __any_sync(0xffffffffu, valid);
         const int place = least + (row0 + min(row, rows - 1)) / g, sure = least + row0 / g;       // sure: what all rows of the block see
@@ -675,37 +871,31 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
         uint64_t sums[4] = {0, 0, 0, 0};      // pairs of fp32
         for (int t = 0; t < it.n; ++t, ++step) {
           if (!wait_scores()) return false;
-#pragma unroll
-          for (int half = 0; half < kWarpCols / 32; ++half) {
-            uint32_t raw[32];
-            if (any) {
-              tmem_ld_32x32(tmem + lanes + (step & 1) * C::kCols + quarter * kWarpCols + half * 32, raw);
-              tmem_ld_wait();
-            }
-            if (half == kWarpCols / 32 - 1) scores_read();
+#pragma unroll 1
+          for (int half = 0; half < kWarpCols; half += 32) {
+            read_scores(half, any);
             if (!any) continue;
-            const int key = (it.t0 + t) * C::kStepKeys + col0 + half * 32;
+            const int key = (it.t0 + t) * C::kStepKeys + col0 + half;
             float by = mul;
             if (capped) {
               by = 1.f;
 #pragma unroll
               for (int c = 0; c < 32; ++c) raw[c] = cap(raw[c], mul);
             }
-            const bool gaps = __any_sync(0xffffffffu, *const_cast<const volatile int*>(&holes) != 0);
-            if (key + 31 > sure || gaps) {
+            const bool rare = __any_sync(0xffffffffu, gaps());
+            if (key + 31 > sure || rare) {
               const int seen = place + 1 - key;          // columns in front
               uint32_t there = 0xffffffffu;
-              if (gaps) {      // rare: tokens whose slots lie outside the cache
-                const int s = key + lane < w.o.len ? __ldcg(p.ix.req_to_token + static_cast<int64_t>(w.o.row) * p.ix.table_stride + key + lane) : -1;
-                there = __ballot_sync(0xffffffffu, s >= 0 && s < p.num_slots);
-              }
+              if (rare) there = __ballot_sync(0xffffffffu, slot_inside(w, key + lane));        // tokens whose slots lie outside the cache
 #pragma unroll
               for (int c = 0; c < 32; ++c) raw[c] = c < seen && ((there >> c) & 1) ? raw[c] : __float_as_uint(-INFINITY);
             }
-            float mx[2] = {fmaxf(__uint_as_float(raw[0]), __uint_as_float(raw[1])), fmaxf(__uint_as_float(raw[2]), __uint_as_float(raw[3]))};
+            float mx[4];
 #pragma unroll
-            for (int c = 4; c < 32; c += 2) mx[(c >> 1) & 1] = max3(mx[(c >> 1) & 1], __uint_as_float(raw[c]), __uint_as_float(raw[c + 1]));
-            const float top = fmaxf(mx[0], mx[1]) * by;
+            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+#pragma unroll
+            for (int c = 8; c < 32; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(raw[c]), __uint_as_float(raw[c + 1]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * by;
             if (top > m + kRescaleThreshold) {        // the first tile raises; so does one behind tiles of minus infinity
               const float f = m == -INFINITY ? 0.f : exp2f(m - top);
 #pragma unroll
@@ -722,9 +912,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
           }
         }
         // ---- the quarters' maxima and sums meet ----
-        const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
         float2* parts = reinterpret_cast<float2*>(cells) + (turn++ & 1) * 512;
-        parts[quarter * 128 + in_tile] = make_float2(m, both.x + both.y);
+        parts[quarter * 128 + in_tile] = make_float2(m, total(sums));
         if (!meet()) return false;
         if (tid < rows) {
           const int tile = C::RT == 2 ? tid >> 7 : 0;
@@ -739,10 +928,9 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
           const bool none = top == -INFINITY;
 #pragma unroll
           for (int i = 0; i < kParts; ++i) sum += x[i].x == -INFINITY ? x[i].y : x[i].y * exp2f(x[i].x - top);       // no score: 0, or no number
-          const bool whole = it.t0 == 0 && it.n == w.steps_of(p, it.block);
-          const int j = (row0 + tid) / g, head = it.hk * g + row0 + tid - j * g;
           float lse = none && sum == 0.f ? -INFINITY : top + log2f(sum);
-          if (whole) {
+          if (it.t0 == 0 && it.n == w.steps1(p, it.block)) {
+            const int j = (row0 + tid) / g, head = it.hk * g + row0 + tid - j * g;
             if (p.sink != nullptr && lse != -INFINITY) {
               const float sink = __ldcg(p.sink + head) * kLog2e, at = fmaxf(top, sink);
               lse = at + log2f(sum * exp2f(top - at) + exp2f(sink - at));
@@ -752,7 +940,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
             p.part[(static_cast<int64_t>(blockIdx.x) * 2 + (it.first ? 0 : 1)) * C::kRows + tid] = lse;
           }
         }
-      } else {
+      } else if constexpr (PASS == 2) {
+        const int rows = w.rows_of(it.block), row0 = it.block * C::kRows;
         const int kt = C::RT == 1 && KT == 2 ? quarter >> 1 : 0, group = KT == 2 ? quarter & 1 : quarter;       // stage and part of the columns
         const int col0 = group * kWarpCols, chunk_keys = it.chunk * C::kStepKeys;
         const float* neg = neg_lse[held] + col0;
@@ -760,54 +949,22 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
         for (int t = 0; t < it.n; ++t, ++step) {
           const int token = (it.t0 + t) * C::kStepKeys + kt * 128 + in_tile;
           // this token is seen by the block's rows from `low` on
-          const int low = token > least ? min(static_cast<int64_t>(token - least) * g - row0, static_cast<int64_t>(C::kRows)) : 0;
+          const int low = token > least ? static_cast<int>(min(static_cast<int64_t>(token - least) * g - row0, static_cast<int64_t>(C::kRows))) : 0;
           uint64_t sums[4] = {0, 0, 0, 0};
           if (!wait_scores()) return false;
-#pragma unroll
-          for (int half = 0; half < kWarpCols / 32; ++half) {
-            uint32_t raw[32];
-            const int col = col0 + half * 32;
-            const bool any = col < rows;
-            if (any) {
-              tmem_ld_32x32(tmem + lanes + (step & 1) * C::kCols + quarter * kWarpCols + half * 32, raw);
-              tmem_ld_wait();
-            }
-            if (half == kWarpCols / 32 - 1) scores_read();
-            if (!any) continue;
-            if (capped) {
-#pragma unroll
-              for (int c = 0; c < 32; ++c) raw[c] = cap(raw[c], kScaled ? muls[half * 32 + c] : p.scale_log2);
-            }
-            auto add_up = [&](auto masked) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 n4 = *reinterpret_cast<const float4*>(neg + half * 32 + 4 * i);
-                float4 m4 = make_float4(p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2);
-                if (kScaled) m4 = *reinterpret_cast<const float4*>(muls + half * 32 + 4 * i);
-                if (capped) m4 = make_float4(1.f, 1.f, 1.f, 1.f);
-                const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), pair_of(m4.x, m4.y), pair_of(n4.x, n4.y)));
-                const float2 y = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), pair_of(m4.z, m4.w), pair_of(n4.z, n4.w)));
-                float e[4] = {ex2(x.x), ex2(x.y), ex2(y.x), ex2(y.y)};
-                if constexpr (decltype(masked)::value) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) e[k] = col + 4 * i + k >= low && col + 4 * i + k < rows ? e[k] : 0.f;
-                }
-                sums[(2 * i) & 3] = add2(sums[(2 * i) & 3], pair_of(e[0], e[1]));
-                sums[(2 * i + 1) & 3] = add2(sums[(2 * i + 1) & 3], pair_of(e[2], e[3]));
-              }
-            };
+#pragma unroll 1
+          for (int half = 0; half < kWarpCols; half += 32) {
+            const int col = col0 + half;
+            read_scores(half, col < rows);
+            if (col >= rows) continue;
             if (col + 32 > rows || __any_sync(0xffffffffu, low > col)) {
-              add_up(std::true_type());
+              weights(neg + half, muls + (kScaled ? half : 0), true, low - col, rows - col, sums);
             } else {
-              add_up(std::false_type());
+              weights(neg + half, muls + (kScaled ? half : 0), false, 0, 32, sums);
             }
           }
-          const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-          float sum = both.x + both.y;
-          if (*const_cast<const volatile int*>(&holes) != 0) {       // rare: a token whose slot lies outside the cache is not seen
-            const int s = token < w.o.len ? __ldcg(p.ix.req_to_token + static_cast<int64_t>(w.o.row) * p.ix.table_stride + token) : -1;
-            if (s < 0 || s >= p.num_slots) sum = 0.f;
-          }
+          float sum = total(sums);
+          if (gaps() && !slot_inside(w, token)) sum = 0.f;       // rare: a token whose slot lies outside the cache is not seen
           float* cell = cells + group * chunk_keys + t * C::kStepKeys + kt * 128 + in_tile;
           *cell = w.first_block(p, it.t0 + t) == it.block ? sum : *cell + sum;
         }
@@ -824,10 +981,62 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
           }
           if (!meet()) return false;
         }
+      } else {
+        const int tile = C::RT == 2 ? quarter >> 1 : 0, col0 = quarter * kWarpCols % 128;
+        const int token = it.block * C::kRows + tile * 128 + in_tile, tile0 = w.first_tile(p, it.block) + it.t0;
+        const bool any = __any_sync(0xffffffffu, token < w.o.len);
+        float all = 0.f;
+        for (int t = 0; t < it.n; ++t, ++step) {
+          const uint32_t place = step % kRing;
+          if (!mbar_wait(&l_full[place], (step / kRing) & 1, &fail_flag)) ok = false;
+          if (!wait_scores()) return false;
+          const int r0 = (tile0 + t) * kTileRows + col0, rows = w.rows - r0;
+          // this token is seen by the rows from `low` on
+          const int low = token > least ? static_cast<int>(min(static_cast<int64_t>(token - least) * g - r0, static_cast<int64_t>(128))) : 0;
+          uint64_t sums[4] = {0, 0, 0, 0};
+#pragma unroll 1
+          for (int half = 0; half < kWarpCols; half += 32) {
+            read_scores(half, any && half < rows);
+            if (!any || half >= rows) continue;
+            const float* neg = neg_lse[place] + col0 + half;
+            const float* muls = row_mul[place] + (kScaled ? col0 + half : 0);
+            if (half + 32 > rows || __any_sync(0xffffffffu, low > half)) {
+              weights(neg, muls, true, low - half, rows - half, sums);
+            } else {
+              weights(neg, muls, false, 0, 32, sums);
+            }
+          }
+          all += total(sums);
+        }
+        if (gaps() && !slot_inside(w, token)) all = 0.f;       // rare: a token whose slot lies outside the cache is not seen
+        float* parts = cells + (turn++ & 1) * 512;
+        parts[quarter * 128 + in_tile] = all;
+        if (!meet()) return false;
+        constexpr int kParts = C::RT == 2 ? 2 : 4;
+        const int steps = w.steps_of(p, it.block), at = it.block * C::kRows + tid;
+        const bool whole = it.t0 == 0 && it.n == steps;
+        if (tid < C::kRows && at < w.o.len) {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) sum += parts[((tid >> 7) * kParts + i) * 128 + (tid & 127)];
+          if (whole) {
+            float* to = p.sums.data + w.o.row * p.sums.row_stride + it.hk * p.sums.head_stride + at;
+            *to = p.add && at < w.o.prefix ? __ldcg(to) + sum : sum;
+          } else {
+            p.part_sum[(static_cast<int64_t>(blockIdx.x) * 2 + (it.first ? 0 : 1)) * C::kRows + tid] = sum;
+          }
+        }
+        // the unit's last step: it began in front of this run
+        if (tid == 0 && !whole && it.t0 + it.n == steps) {
+          const int64_t line = line_of[3];
+          const int used = used_ctas(p, line), c0 = owner_of(line, it.at, used);
+          p.jobs[blockIdx.x] = make_int4(it.b, it.hk, it.block, c0 * 2 + (run_begin(line, c0, used) < it.at ? 1 : 0));
+        }
       }
       return true;
     });
     if (!ok) fail_flag = 1;
+    if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
   }
 
   tc_fence_before_sync();
@@ -843,48 +1052,83 @@ __global__ void __launch_bounds__(kThreads, 1) weights_prompt_kernel(const Promp
   }
 }
 
-template <typename T, int NH, int FMT, int R>
-int launch_one(const PromptParams& p, cudaStream_t s) {
-  using C = Cfg<NH, FMT != kKvSame, R>;
-  auto first = weights_prompt_kernel<T, NH, FMT, R, 1>;
-  auto second = weights_prompt_kernel<T, NH, FMT, R, 2>;
-  if (ensure_dynamic_smem(reinterpret_cast<const void*>(first), C::kSmem) != cudaSuccess) return -3;
-  if (ensure_dynamic_smem(reinterpret_cast<const void*>(second), C::kSmem) != cudaSuccess) return -3;
-  cudaError_t err = launch_pdl(first, dim3(p.ctas), dim3(kThreads), C::kSmem, s, p);
-  note_launch();
-  if (err != cudaSuccess) return -4;
-  err = launch_pdl(second, dim3(p.ctas), dim3(kThreads), C::kSmem, s, p);
+// Adds up the parts of blocks of tokens that were cut, in the order of the CTAs; a block per CTA of the kernel above, whose note says what
+// ends there (request -1: nothing).
+__global__ void __launch_bounds__(256) prompt_parts_kernel(const PromptParams p, int block_rows) {
+  pdl_wait_loads();
+  pdl_launch_dependents();
+  const int4 job = __ldcg(p.jobs + blockIdx.x);
+  if (job.x < 0) return;
+  const Observed o = observed_of(p, job.x);
+  const int token = job.z * block_rows + threadIdx.x;
+  if (static_cast<int>(threadIdx.x) >= block_rows || token >= o.len) return;
+  float sum = __ldcg(p.part_sum + static_cast<int64_t>(job.w) * block_rows + threadIdx.x);
+#pragma unroll 4
+  for (int c = job.w / 2 + 1; c <= static_cast<int>(blockIdx.x); ++c) sum += __ldcg(p.part_sum + static_cast<int64_t>(c) * 2 * block_rows + threadIdx.x);
+  float* to = p.sums.data + o.row * p.sums.row_stride + job.y * p.sums.head_stride + token;
+  *to = p.add && token < o.prefix ? __ldcg(to) + sum : sum;
+}
+
+template <typename T, int NH, int FMT, int R, int PASS>
+int launch_pass(const PromptParams& p, cudaStream_t s) {
+  using C = Cfg<NH, FMT != kKvSame, R, PASS>;
+  auto kern = weights_prompt_kernel<T, NH, FMT, R, PASS>;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem) != cudaSuccess) return -3;
+  // the computing warps take registers that the others give back: together no more than the kernel is launched with
+  static const int regs = [kern] {
+    cudaFuncAttributes at{};
+    return cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(kern)) == cudaSuccess ? at.numRegs : 0;
+  }();
+  if (regs < C::kLaunchRegs) return -5;
+  const cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(C::kThreads), C::kSmem, s, p);
   note_launch();
   return err == cudaSuccess ? 0 : -4;
 }
+template <typename T, int NH, int FMT, int R>
+int launch_one(const PromptParams& p, bool rows_go_by, cudaStream_t s) {
+  int rc = launch_pass<T, NH, FMT, R, 1>(p, s);
+  if (rc != 0) return rc;
+  if constexpr (R == 2 || NH == 4) {
+    if (rows_go_by) {
+      rc = launch_pass<T, NH, FMT, R, 3>(p, s);
+      if (rc != 0) return rc;
+      const cudaError_t err = launch_pdl(prompt_parts_kernel, dim3(p.ctas), dim3(256), 0, s, p, R * kTileRows);
+      note_launch();
+      return err == cudaSuccess ? 0 : -4;
+    }
+  }
+  return launch_pass<T, NH, FMT, R, 2>(p, s);
+}
 template <typename T, int NH, int R>
-int launch_format(const PromptParams& p, int fmt, cudaStream_t s) {
+int launch_format(const PromptParams& p, int fmt, bool rows_go_by, cudaStream_t s) {
   switch (fmt) {
-    case kKvSame: return launch_one<T, NH, kKvSame, R>(p, s);
-    case kKvE4M3: return launch_one<T, NH, kKvE4M3, R>(p, s);
-    default: return launch_one<T, NH, kKvE5M2, R>(p, s);
+    case kKvSame: return launch_one<T, NH, kKvSame, R>(p, rows_go_by, s);
+    case kKvE4M3: return launch_one<T, NH, kKvE4M3, R>(p, rows_go_by, s);
+    default: return launch_one<T, NH, kKvE5M2, R>(p, rows_go_by, s);
   }
 }
 template <typename T>
-int launch_type(const PromptParams& p, int head_dim, int fmt, int tiles, cudaStream_t s) {
+int launch_type(const PromptParams& p, int head_dim, int fmt, int tiles, bool rows_go_by, cudaStream_t s) {
   switch (head_dim) {
-    case 64: return tiles == 2 ? launch_format<T, 1, 2>(p, fmt, s) : launch_format<T, 1, 1>(p, fmt, s);
-    case 128: return tiles == 2 ? launch_format<T, 2, 2>(p, fmt, s) : launch_format<T, 2, 1>(p, fmt, s);
-    default: return launch_format<T, 4, 1>(p, fmt, s);
+    case 64: return tiles == 2 ? launch_format<T, 1, 2>(p, fmt, rows_go_by, s) : launch_format<T, 1, 1>(p, fmt, rows_go_by, s);
+    case 128: return tiles == 2 ? launch_format<T, 2, 2>(p, fmt, rows_go_by, s) : launch_format<T, 2, 1>(p, fmt, rows_go_by, s);
+    default: return launch_format<T, 4, 1>(p, fmt, rows_go_by, s);
   }
 }
 
-// Row tiles of a block: two where a request has more observed rows than one tile holds, on average; 256 features leave no room for two.
-int row_tiles(const WeightsPromptArgs& a) {
-  const int64_t each = a.rows / std::max(1, a.index.batch), look = a.last > 0 ? std::min<int64_t>(a.last, each) : each;
-  return a.head_dim <= 128 && look * (a.hq / a.hkv) > kTileRows ? 2 : 1;
+// observed rows of a request and kv head, on average over the batch
+int64_t rows_each(const WeightsPromptArgs& a) {
+  const int64_t each = a.rows / std::max(1, a.index.batch);
+  return (a.last > 0 ? std::min<int64_t>(a.last, each) : each) * (a.hq / a.hkv);
 }
+// Row tiles of a block: two where a request has more observed rows than one tile holds; 256 features leave no room for two.
+int row_tiles(const WeightsPromptArgs& a) { return a.head_dim <= 128 && rows_each(a) > kTileRows ? 2 : 1; }
 
 }  // namespace
 
 bool weights_prompt_covers(int head_dim, int group) { return (head_dim == 64 || head_dim == 128 || head_dim == 256) && group >= 1 && group <= 32; }
 
-int64_t weights_prompt_floats(const WeightsPromptArgs& a) { return a.rows * a.hq + static_cast<int64_t>(a.num_sms) * 2 * row_tiles(a) * kTileRows; }
+int64_t weights_prompt_floats(const WeightsPromptArgs& a) { return a.rows * a.hq + static_cast<int64_t>(a.num_sms) * (4 * row_tiles(a) * kTileRows + 4) + 4; }
 
 int launch_weights_prompt(const WeightsPromptArgs& a, cudaStream_t s) {
   if (a.hkv <= 0 || a.hq % a.hkv != 0 || !weights_prompt_covers(a.head_dim, a.hq / a.hkv)) return -1;
@@ -896,8 +1140,11 @@ int launch_weights_prompt(const WeightsPromptArgs& a, cudaStream_t s) {
   p.q_start = a.q_start;
   p.q = a.q;
   p.k_cache = a.k_cache;
-  p.lse = a.workspace;
-  p.part = a.workspace + a.rows * a.hq;
+  p.ctas = a.num_sms;
+  p.jobs = reinterpret_cast<int4*>(a.workspace);       // on a 16-byte boundary
+  p.lse = a.workspace + 4 * p.ctas;
+  p.part = p.lse + a.rows * a.hq;
+  p.part_sum = p.part + static_cast<int64_t>(p.ctas) * 2 * row_tiles(a) * kTileRows;
   p.sink = a.sink;
   p.q_stride = a.q_stride;
   p.num_slots = a.num_slots;
@@ -907,14 +1154,17 @@ int launch_weights_prompt(const WeightsPromptArgs& a, cudaStream_t s) {
   p.hkv = a.hkv;
   p.group = a.hq / a.hkv;
   p.last = a.last;
-  p.ctas = a.num_sms;
+  p.inv_group = (65536 + p.group - 1) / p.group;
   p.add = a.add;
   p.scale_log2 = a.scale * kLog2e;
   if (a.logit_cap > 0.f) {
     p.cap_in = 2.f / a.logit_cap;
     p.cap_out = a.logit_cap * kLog2e;
   }
-  return a.dt == kF16 ? launch_type<__half>(p, a.head_dim, a.kv_fmt, row_tiles(a), s) : launch_type<__nv_bfloat16>(p, a.head_dim, a.kv_fmt, row_tiles(a), s);
+  const int tiles = row_tiles(a);
+  const bool rows_go_by = rows_each(a) > 2 * tiles * kTileRows;
+  return a.dt == kF16 ? launch_type<__half>(p, a.head_dim, a.kv_fmt, tiles, rows_go_by, s)
+                      : launch_type<__nv_bfloat16>(p, a.head_dim, a.kv_fmt, tiles, rows_go_by, s);
 }
 
 }  // namespace mb200
