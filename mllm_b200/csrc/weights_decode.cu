@@ -34,6 +34,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kWarpTokens = 16;
 constexpr int kTile = kWarps * kWarpTokens;   // tokens of a tile
 constexpr int kNoToken = -0x7fffffff;
+constexpr int kSums = 4;                      // sums of a thread that are on their way while the normalisers are made
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleThreshold = 8.0f;     // the running maximum is raised when a score passes it by 2^8
 
@@ -91,10 +92,16 @@ __device__ __forceinline__ int ctas_used(int ctas, int64_t line) {
   const int64_t want = max(line / 4, min(line / 2, static_cast<int64_t>(64)));
   return static_cast<int>(min(static_cast<int64_t>(ctas), max(want, static_cast<int64_t>(1))));
 }
+// (A division of 64 bits takes some 500 cycles of the chain in front of the first copy.)
+__device__ __forceinline__ bool fits_32(int64_t line, int ctas) { return line < (1ll << 31) && line * (ctas + 1) < (1ll << 32); }
 __device__ __forceinline__ int64_t run_begin(int64_t line, int c, int ctas) {
-  // a division of 64 bits takes some 500 cycles of the chain in front of the first copy
-  if (line < 0xFFFFFFFFll / (ctas + 1)) return static_cast<uint32_t>(line) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
+  if (fits_32(line, ctas)) return static_cast<uint32_t>(line) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
   return line * c / ctas;
+}
+// the last CTA whose run begins at or before x
+__device__ __forceinline__ int owner_of(int64_t line, int64_t x, int ctas) {
+  if (fits_32(line, ctas)) return min(ctas - 1, static_cast<int>((static_cast<uint32_t>(x + 1) * ctas - 1u) / static_cast<uint32_t>(line)));
+  return static_cast<int>(min(static_cast<int64_t>(ctas) - 1, ((x + 1) * ctas - 1) / line));
 }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
@@ -227,16 +234,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT, FMT>::kPerSm) weights_de
           s = -1;
         }
         const uint32_t dst = ring_addr + (t % C::kStages) * (2 * C::kTensorBytes);
-        constexpr int kRowsPerPass = 32 / C::kChunks;
+        constexpr int kRowsPerPass = 32 / C::kChunks, kPasses = kWarpTokens / kRowsPerPass;
         const int ch = lane % C::kChunks, r0 = lane / C::kChunks;
+        int rs[kPasses];          // slots first, then copies: a copy does not wait for its own
 #pragma unroll
-        for (int i = 0; i < kWarpTokens / kRowsPerPass; ++i) {
-          const int row = i * kRowsPerPass + r0;
-          const int rs = __shfl_sync(0xffffffffu, s, row);
-          const int64_t off = static_cast<int64_t>(max(rs, 0)) * p.kv_tok_stride + ch * (16 / C::kItem);
-          const uint32_t to = dst + C::at(row, ch);
-          cp16_l2(to, kbase + off, rs >= 0);
-          cp16_l2(to + C::kTensorBytes, vbase + off, rs >= 0);
+        for (int i = 0; i < kPasses; ++i) rs[i] = __shfl_sync(0xffffffffu, s, i * kRowsPerPass + r0);
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          const int64_t off = static_cast<int64_t>(max(rs[i], 0)) * p.kv_tok_stride + ch * (16 / C::kItem);
+          const uint32_t to = dst + C::at(i * kRowsPerPass + r0, ch);
+          cp16_l2(to, kbase + off, rs[i] >= 0);
+          cp16_l2(to + C::kTensorBytes, vbase + off, rs[i] >= 0);
         }
       }
       cp_commit();
@@ -528,7 +536,7 @@ __global__ void __launch_bounds__(kThreads) weights_join_kernel(const DecodePara
   __shared__ int warp_sums[kWarps];
   __shared__ int mine[2];       // units in front of the request, and its tiles
   __shared__ int start[3];
-  __shared__ float weight[kThreads];
+  __shared__ __align__(16) float weight[kThreads];
   pdl_launch_dependents();
   const int g = p.group, hq = p.hkv * g, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool joins = static_cast<int>(blockIdx.x) < hq * p.ix.batch;
@@ -537,8 +545,7 @@ __global__ void __launch_bounds__(kThreads) weights_join_kernel(const DecodePara
   int before = scan_units(p, warp_sums, first, last, total);       // the lengths were complete when the first kernel began
   const int64_t line = static_cast<int64_t>(total) * p.hkv;
   const int used = ctas_used(p.ctas, line);
-  // the last CTA whose run begins at or before x
-  auto owner = [&](int64_t x) { return static_cast<int>(min(static_cast<int64_t>(used) - 1, ((x + 1) * used - 1) / line)); };
+  auto owner = [&](int64_t x) { return owner_of(line, x, used); };
 
   if (joins) {
     const int b = b_join;
@@ -598,8 +605,10 @@ __global__ void __launch_bounds__(kThreads) weights_join_kernel(const DecodePara
 
   // ---- weights ----
   const int c = blockIdx.x - hq * p.ix.batch;
-  const int64_t run0 = run_begin(line, c, p.weight_ctas);
-  int64_t left = run_begin(line, c + 1, p.weight_ctas) - run0;
+  const int shared = static_cast<int>(min(static_cast<int64_t>(p.weight_ctas), max(line, static_cast<int64_t>(1))));
+  if (c >= shared) return;
+  const int64_t run0 = run_begin(line, c, shared);
+  int64_t left = run_begin(line, c + 1, shared) - run0;
   if (left <= 0) return;
   {
     int64_t at = static_cast<int64_t>(before) * p.hkv;
@@ -617,49 +626,78 @@ __global__ void __launch_bounds__(kThreads) weights_join_kernel(const DecodePara
   __syncthreads();
   int b = start[0], hk = start[1], t0 = start[2];
   int64_t pair0 = run0 - t0;         // where the pair begins on the line
-  pdl_wait_loads();
+  bool waited = false;
   while (left > 0 && b < p.ix.batch) {
     const Cached r = cached_of(p.ix, b);
     const int n_all = tiles_of(r.len), n = static_cast<int>(min(static_cast<int64_t>(max(n_all - t0, 0)), left));
     if (n > 0) {
       const int c0 = owner(pair0), c1 = owner(pair0 + n_all - 1);
       const int first_slot = c0 * 2 + (run_begin(line, c0, used) < pair0 ? 1 : 0);
+      const int64_t pair = static_cast<int64_t>(b) * p.hkv + hk;
+      const float* scores = p.scores + pair * p.ix.table_cols * g;
+      float* sums = p.sums.data + r.row * p.sums.row_stride + hk * p.sums.head_stride;
+      const int begin = t0 * kTile, end = min(r.len, (t0 + n) * kTile);
+      // the sums so far are nothing that the first kernel writes
+      float old[kSums];
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) {
+        const int tok = begin + k * kThreads + static_cast<int>(threadIdx.x);
+        old[k] = tok < end && tok < r.len - 1 && p.decay != 0.f ? p.decay * __ldcg(sums + tok) : 0.f;
+      }
+      if (!waited) pdl_wait_loads();
+      waited = true;
       __syncthreads();
       for (int h = warp; h < g; h += kWarps) {         // the heads' normalisers
         float lse;
         if (c0 == c1) {
-          lse = __ldcg(p.whole_lse + (static_cast<int64_t>(b) * p.hkv + hk) * g + h);
+          lse = __ldcg(p.whole_lse + pair * g + h);
         } else {
           auto part = [&](int i) { return __ldcg(p.part_lse + static_cast<int64_t>(i == c0 ? first_slot : i * 2) * g + h).y; };
-          float top = -INFINITY;
-          for (int i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, part(i));
-          top = warp_max(top);
-          const bool none = top == -INFINITY;
-          const float sink = p.sink != nullptr ? p.sink[hk * g + h] * kLog2e : -INFINITY;
-          top = fmaxf(top, sink);
-          float all = 0.f;
+          const float sink = p.sink != nullptr ? __ldcg(p.sink + hk * g + h) * kLog2e : -INFINITY;
+          float top = -INFINITY, all = 0.f;
           for (int i = c0 + lane; i <= c1; i += 32) {
-            const float v = part(i);
-            all += v == -INFINITY ? 0.f : exp2f(v - top);
+            const float v = part(i), most = fmaxf(top, v);
+            if (most > -INFINITY) {
+              all = (top == -INFINITY ? all : all * exp2f(top - most)) + (v == -INFINITY ? 0.f : exp2f(v - most));
+              top = most;
+            } else {
+              all += v == v ? 0.f : v;
+            }
           }
-          all = warp_sum(all) + (p.sink != nullptr ? exp2f(sink - top) : 0.f);
-          lse = none ? -INFINITY : top + log2f(all);
+          const float most = warp_max(top);
+          const bool none = most == -INFINITY;
+          const float over = fmaxf(most, sink);
+          all = warp_sum(top == -INFINITY ? all : all * exp2f(top - over));
+          lse = none && all == 0.f ? -INFINITY : over + log2f(all + (p.sink != nullptr ? exp2f(sink - over) : 0.f));
         }
         if (lane == 0) weight[h] = lse;
       }
       __syncthreads();
-      const float* scores = p.scores + (static_cast<int64_t>(b) * p.hkv + hk) * p.ix.table_cols * g;
-      float* sums = p.sums.data + r.row * p.sums.row_stride + hk * p.sums.head_stride;
-      const int end = min(r.len, (t0 + n) * kTile);
-      for (int tok = t0 * kTile + threadIdx.x; tok < end; tok += kThreads) {
-        const float old = tok < r.len - 1 && p.decay != 0.f ? p.decay * __ldcg(sums + tok) : 0.f;
+      // scores of a token and its heads lie side by side
+      auto add_up = [&](int tok) {
+        const float* s = scores + static_cast<int64_t>(tok) * g;
         float add = 0.f;
-        for (int h = 0; h < g; ++h) {
-          const float lse = weight[h];
-          add += lse == -INFINITY ? 0.f : exp2f(__ldcg(scores + static_cast<int64_t>(tok) * g + h) - lse);
+        if ((g & 3) == 0) {
+          for (int h = 0; h < g; h += 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(s + h)), l = *reinterpret_cast<const float4*>(&weight[h]);
+            add += (l.x == -INFINITY ? 0.f : fast_exp2(v.x - l.x)) + (l.y == -INFINITY ? 0.f : fast_exp2(v.y - l.y)) +
+                   (l.z == -INFINITY ? 0.f : fast_exp2(v.z - l.z)) + (l.w == -INFINITY ? 0.f : fast_exp2(v.w - l.w));
+          }
+        } else {
+          for (int h = 0; h < g; ++h) {
+            const float l = weight[h];
+            add += l == -INFINITY ? 0.f : fast_exp2(__ldcg(s + h) - l);
+          }
         }
-        sums[tok] = old + add;
+        return add;
+      };
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) {
+        const int tok = begin + k * kThreads + static_cast<int>(threadIdx.x);
+        if (tok < end) sums[tok] = old[k] + add_up(tok);
       }
+      for (int tok = begin + kSums * kThreads + static_cast<int>(threadIdx.x); tok < end; tok += kThreads)
+        sums[tok] = (tok < r.len - 1 && p.decay != 0.f ? p.decay * __ldcg(sums + tok) : 0.f) + add_up(tok);
     }
     left -= n;
     t0 += n;
@@ -715,7 +753,7 @@ bool weights_decode_covers(int head_dim, int group) {
 
 int64_t weights_decode_floats(const WeightsDecodeArgs& a) {
   const int64_t group = a.hq / a.hkv, parts = static_cast<int64_t>(stream_ctas(a)) * 2 * group;
-  return parts * (a.head_dim + 2) + static_cast<int64_t>(a.index.batch) * a.hq * (1 + static_cast<int64_t>(a.index.table_cols));
+  return parts * (a.head_dim + 2) + 4 + static_cast<int64_t>(a.index.batch) * a.hq * (1 + static_cast<int64_t>(a.index.table_cols));
 }
 
 int launch_weights_decode(const WeightsDecodeArgs& a, cudaStream_t s) {
@@ -731,11 +769,11 @@ int launch_weights_decode(const WeightsDecodeArgs& a, cudaStream_t s) {
   p.group = a.hq / a.hkv;
   p.hkv = a.hkv;
   p.ctas = stream_ctas(a);
-  p.weight_ctas = 4 * a.num_sms;
+  p.weight_ctas = 8 * a.num_sms;
   const int64_t parts = static_cast<int64_t>(p.ctas) * 2 * p.group;
   p.part_o = a.workspace;
   p.part_lse = reinterpret_cast<float2*>(a.workspace + parts * a.head_dim);
-  p.scores = a.workspace + parts * (a.head_dim + 2);
+  p.scores = a.workspace + (parts * (a.head_dim + 2) + 3) / 4 * 4;      // on a 16-byte boundary
   p.whole_lse = p.scores + static_cast<int64_t>(a.index.batch) * a.hq * a.index.table_cols;
   p.sink = a.sink;
   p.q_stride = a.q_stride;

@@ -29,7 +29,7 @@ namespace mb200 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescaleThreshold = 8.0f;  // the running maximum is raised when a score passes it by 2^8
+constexpr float kLargest = 1e30f;          // a sum of exponentials that is not below this gets a new maximum
 constexpr int kTileRows = 128;             // MMA M
 constexpr int kStart = 2;                  // steps' time that every unit of the first pass costs beside its steps
 constexpr int kChunk = 8;                  // steps whose sums wait in shared memory
@@ -50,9 +50,17 @@ struct PromptParams {
   int64_t q_stride, num_slots, kv_tok_stride, kv_head_stride;
   int rows, hkv, group, last, ctas;
   uint32_t inv_group;      // of 16 bits: quotients of numbers below 320, exactly
+  uint32_t inv_group32;    // floor(2^32 / group), 2^32 - 1 for 1
   bool add;
   float scale_log2, cap_in, cap_out;     // a scaled score x becomes cap_out tanh(x cap_in ln 2 / 2); cap_out 0: no soft cap
 };
+
+// n / group, n >= 0: the quotient by the reciprocal is too small by one at most
+__device__ __forceinline__ int by_group(const PromptParams& p, int n) {
+  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(n), p.inv_group32));
+  if (n - q * p.group >= p.group) ++q;
+  return q;
+}
 
 struct Observed {
   int len, row, prefix, first, look;      // tokens; row of the table; cached before; row of q of the first observed query; observed ones
@@ -87,11 +95,11 @@ struct Cfg {
   static constexpr int kPiece = 128 * 128, kStage = NH * kPiece;
   static constexpr int kStages = NH == 4 ? 2 : NH == 2 ? (R == 2 ? 4 : 5) : 6;
   // Warps: those that compute, that copy stages (kCopying of them, every kCopying-th stage each), one that copies blocks, one that issues
-  // products.  8-bit keys are widened on the way, which takes more of them.
-  static constexpr int kCopy = KV8 ? 6 : 2, kCopying = kCopy < kStages ? kCopy : kStages;
+  // products.
+  static constexpr int kCopy = 6, kCopying = kCopy < kStages ? kCopy : kStages;
   static constexpr int kBlockWarp = kCompute + kCopy, kIssueWarp = kBlockWarp + 1, kThreads = 32 * (kIssueWarp + 1);
   // Registers: those of a launch, of the computing threads, of the others.  A quarter of the warps share 16384, four computing ones each.
-  static constexpr int kLaunchRegs = KV8 ? 80 : 96, kComputeRegs = KV8 ? 88 : 104, kOtherRegs = 64;
+  static constexpr int kLaunchRegs = 80, kComputeRegs = 88, kOtherRegs = 64;
   static_assert(4 * kComputeRegs + (kCopy + 2) / 4 * kOtherRegs <= (4 + (kCopy + 2) / 4) * kLaunchRegs && (kCopy + 2) % 4 == 0, "register split");
   static constexpr int kSmem = kBlockBytes + kStages * kStage;
   static constexpr int kGroups = 4 / KT;                     // parts of a token's sum
@@ -117,7 +125,7 @@ struct Work {
   __device__ __forceinline__ int rows_of(int block) const { return min(C::kRows, rows - block * C::kRows); }
   // steps of the first pass: up to the largest place of a block's rows
   __device__ __forceinline__ int steps1(const PromptParams& p, int block) const {
-    return (least() + (min(rows, (block + 1) * C::kRows) - 1) / p.group) / C::kStepKeys + 1;
+    return (least() + by_group(p, min(rows, (block + 1) * C::kRows) - 1)) / C::kStepKeys + 1;
   }
   // first tile of rows that sees a block of tokens
   __device__ __forceinline__ int first_tile(const PromptParams& p, int block) const {
@@ -133,7 +141,7 @@ struct Work {
     const int j = step * C::kStepKeys - least();
     return j > 0 ? j * p.group / C::kRows : 0;
   }
-  __device__ __forceinline__ int common(const PromptParams& p) const { return min(steps(), (least() + (C::kRows - 1) / p.group) / C::kStepKeys + 1); }
+  __device__ __forceinline__ int common(const PromptParams& p) const { return min(steps(), (least() + by_group(p, C::kRows - 1)) / C::kStepKeys + 1); }
   // of one kv head, on the first pass's line and on this one's
   __device__ __forceinline__ int64_t cost1(const PromptParams& p) const {
     int64_t n = 0;
@@ -192,6 +200,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // two 32-bit operations an instruction
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
   uint64_t r;
@@ -237,7 +250,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
   __shared__ int fail_flag, holes;
   __shared__ int begin_of[2], used_of;                      // request and kv head of the run's first unit; CTAs of the first pass
   __shared__ Observed begin_request;
-  __shared__ int64_t begin_rest, begin_at1, line_of[4];     // steps in front of the run; first pass's place of the request; run, its end, both lines
+  __shared__ int64_t begin_rest, begin_at1, begin_unit1, line_of[4];     // steps in front of the run; request and kv head on the first pass's line; run, its end, both lines
   __shared__ __align__(16) float neg_lse[kRing][C::kRingRows];      // -normaliser of rows (sums)
   __shared__ __align__(16) float row_mul[kRing][kScaled ? C::kRingRows : 4];
   __shared__ __align__(16) float cells[kChunk * 512];       // second pass: [parts][tokens]; else 2 x [4][128] maxima and sums
@@ -315,6 +328,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           begin_request = w.o;
           begin_rest = in - hk * c;
           begin_at1 = at1;
+          begin_unit1 = c1;
         }
         at += c * p.hkv;
         at1 += c1 * p.hkv;
@@ -407,15 +421,16 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
       }
     } else {
       // the first step that begins at or behind the run's begin
-      int64_t at1 = begin_at1, unit1 = w.cost1(p);        // of the request on the first pass's line
+      int64_t at1 = begin_at1, unit1 = begin_unit1;        // of the request on the first pass's line
       const int all = w.common(p);
       const int64_t level = static_cast<int64_t>(all) * w.blocks;
-      if (rest <= level) {
-        t = w.blocks == 1 ? static_cast<int>(rest) : static_cast<int>((rest + w.blocks - 1) / w.blocks);
+      if (rest <= level && level < (1ll << 31)) {
+        t = w.blocks == 1 ? static_cast<int>(rest) : static_cast<int>((static_cast<uint32_t>(rest) + w.blocks - 1) / w.blocks);
         pos += static_cast<int64_t>(t) * w.blocks - rest;
       } else {
-        t = all;
-        int64_t x = level;
+        const bool behind = rest > level;
+        t = behind ? all : 0;
+        int64_t x = behind ? level : 0;
         while (x < rest) x += w.blocks - w.first_block(p, t++);
         pos += x - rest;
       }
@@ -463,26 +478,38 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), FMT == kKvE5M2 ? __NV_E5M2 : __NV_E4M3);
     return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
   };
-  // 32 rows of keys whose slots the lanes have (-1: zeros), to rows row0 .. of a tile with blocks of `block` bytes
+  // 32 rows of keys whose slots the lanes have, to rows row0 .. of a tile with blocks of `block` bytes.  What stands for a token that is none, or
+  // whose slot lies outside the cache, is some other row: its scores are left out where they are read.
   auto copy_keys = [&](const Elem* head, int slot, uint32_t dst, int row0, int block) {
     const int ch = lane % kKeyPieces, r0 = lane / kKeyPieces;
     const Elem* from = head + ch * (16 / sizeof(Elem));
     if constexpr (!KV8) {
-#pragma unroll 4
-      for (int k = 0; k < kKeyPieces; ++k) {
-        const int row = k * kKeyRows + r0, rs = __shfl_sync(0xffffffffu, slot, row);
-        cp16(dst + swz(row0 + row, ch, block), from + max(rs, 0) * p.kv_tok_stride, rs >= 0);
+      // a copy is a slot, an address and the copy itself: one warp has to keep up with the products
+      uint32_t at[8 / kKeyRows];
+#pragma unroll
+      for (int k = 0; k < 8 / kKeyRows; ++k) at[k] = dst + swz(row0 + k * kKeyRows + r0, ch, block) - k * kKeyRows * 128;
+      constexpr int kBatch = 8;          // slots first, then copies: one after the other a copy waits for its slot, 64 cycles each
+#pragma unroll
+      for (int k0 = 0; k0 < kKeyPieces; k0 += kBatch) {
+        int rs[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) rs[k] = __shfl_sync(0xffffffffu, slot, (k0 + k) * kKeyRows + r0);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(at[(k0 + k) % (8 / kKeyRows)] + (k0 + k) * kKeyRows * 128),
+                       "l"(from + rs[k] * p.kv_tok_stride)
+                       : "memory");
       }
     } else {
       constexpr int kBatch = kKeyPieces < 8 ? kKeyPieces : 8;
 #pragma unroll 1
       for (int k0 = 0; k0 < kKeyPieces; k0 += kBatch) {
         uint4 x[kBatch];
+        int rs[kBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const int rs = __shfl_sync(0xffffffffu, slot, (k0 + k) * kKeyRows + r0);
-          x[k] = rs >= 0 ? __ldcg(reinterpret_cast<const uint4*>(from + rs * p.kv_tok_stride)) : make_uint4(0, 0, 0, 0);
-        }
+        for (int k = 0; k < kBatch; ++k) rs[k] = __shfl_sync(0xffffffffu, slot, (k0 + k) * kKeyRows + r0);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) x[k] = __ldcg(reinterpret_cast<const uint4*>(from + rs[k] * p.kv_tok_stride));
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const int row = row0 + (k0 + k) * kKeyRows + r0;
@@ -499,7 +526,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
   };
   // n rows of queries from row r0 of the request on, every `step`-th 32 pieces from the `me`-th on
   auto copy_queries = [&](const W& w, int hk, int r0, int n, uint32_t dst, int block, float* muls, int me, int step) {
-    const int j0 = r0 / g, h0 = r0 - j0 * g;
+    const int j0 = by_group(p, r0), h0 = r0 - j0 * g;
     const uint16_t* q = static_cast<const uint16_t*>(p.q) + static_cast<int64_t>(w.o.first + j0) * p.q_stride + static_cast<int64_t>(hk) * g * kD;
     constexpr int kCh = 8 * NH, kRowsPer = 32 / kCh;          // 16-byte pieces of a row
     const int ch = lane % kCh;
@@ -549,27 +576,41 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
     x.second = run_begin(line, x.c0, used_of) < at ? 1 : 0;
     return x;
   };
-  auto normaliser = [&](const W& w, int hk, int r, const Parts& x) -> float {
-    const int j = r / g, head = hk * g + r - j * g;
+  // (`of` neighbouring lanes share a row's parts, and whole warps call)
+  auto normaliser = [&](const W& w, int hk, int r, const Parts& x, int sub, int of) -> float {
+    const int j = by_group(p, r), head = hk * g + r - j * g;
     float lse;
     if (x.c0 == x.c1) {
       lse = __ldcg(p.lse + static_cast<int64_t>(w.o.first + j) * p.hkv * g + head);
     } else {
-      const int row = r % C::kRows;
-      auto part = [&](int c) { return __ldcg(p.part + (static_cast<int64_t>(c) * 2 + (c == x.c0 ? x.second : 0)) * C::kRows + row); };
-      float top = -INFINITY;
-#pragma unroll 8
-      for (int c = x.c0; c <= x.c1; ++c) top = fmaxf(top, part(c));
-      const bool none = top == -INFINITY;
+      const float* part = p.part + r % C::kRows;
       const float sink = p.sink != nullptr ? __ldcg(p.sink + head) * kLog2e : -INFINITY;
-      top = fmaxf(top, sink);
-      float sum = p.sink != nullptr ? exp2f(sink - top) : 0.f;
-#pragma unroll 8
-      for (int c = x.c0; c <= x.c1; ++c) {
-        const float v = part(c);
-        sum += v == -INFINITY ? 0.f : exp2f(v - top);
+      float top = -INFINITY, sum = 0.f;
+      for (int c = x.c0 + sub; c <= x.c1; c += 4 * of) {
+        float v[4], most = top;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int at = c + k * of;
+          v[k] = at <= x.c1 ? __ldcg(part + (static_cast<int64_t>(at) * 2 + (at == x.c0 ? x.second : 0)) * C::kRows) : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) most = fmaxf(most, v[k]);
+        if (most > -INFINITY) sum = top == -INFINITY ? sum : sum * ex2(top - most);      // 0, or no number, in front of the first
+        top = most;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += v[k] == -INFINITY ? 0.f : ex2(v[k] - top);
       }
-      lse = none && sum == sum ? -INFINITY : top + log2f(sum);
+      for (int o = 1; o < of; o <<= 1) {
+        const float t = __shfl_xor_sync(0xffffffffu, top, o), s = __shfl_xor_sync(0xffffffffu, sum, o), most = fmaxf(top, t);
+        sum = (top == -INFINITY ? sum : sum * ex2(top - most)) + (t == -INFINITY ? s : s * ex2(t - most));
+        top = most;
+      }
+      if (top == -INFINITY && sum == 0.f) {
+        lse = -INFINITY;
+      } else {
+        const float most = fmaxf(top, sink);
+        lse = most + lg2((top == -INFINITY ? sum : sum * ex2(top - most)) + (p.sink != nullptr ? ex2(sink - most) : 0.f));
+      }
     }
     return lse == -INFINITY ? -INFINITY : -lse;       // nothing seen: no weights
   };
@@ -584,16 +625,21 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
         int s = tok < w.o.len ? __ldcg(rtt + tok) : -1;
         if (s < 0 || s >= p.num_slots) {
           bad = bad || tok < w.o.len;
-          s = -1;
+          s = 0;
         }
-        copy_keys(head, s, smem_u32(sBlock), row0, C::kBlock);
+        if (p.num_slots > 0) copy_keys(head, s, smem_u32(sBlock), row0, C::kBlock);
       }
     } else {
       const int rows = w.rows_of(it.block);
       copy_queries(w, it.hk, it.block * C::kRows, rows, smem_u32(sBlock), C::kBlock, row_mul[held], me, all);
       if (PASS == 2) {
         const Parts x = parts_of(it.at, w.steps1(p, it.block));
-        for (int row = me * 32 + lane; row < rows; row += all * 32) neg_lse[held][row] = normaliser(w, it.hk, it.block * C::kRows + row, x);
+        const int of = all * 32 > C::kRows ? all * 32 / C::kRows : 1, log2_of = 31 - __clz(of);
+        for (int row0 = me * 32 >> log2_of; row0 < rows; row0 += all * 32 >> log2_of) {
+          const int row = row0 + (lane >> log2_of);
+          const float v = normaliser(w, it.hk, it.block * C::kRows + min(row, rows - 1), x, lane & (of - 1), of);
+          if (row < rows) neg_lse[held][row] = v;
+        }
       }
     }
     cp_commit();
@@ -651,7 +697,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
             copy_queries(w, it.hk, r0, rows, smem_u32(ring) + n % kStages * C::kStage, C::kPiece, row_mul[held], 0, 1);
             cp_commit();
             const Parts x = parts_of(at, w.steps1(p, block));
-            for (int row = lane; row < rows; row += 32) neg_lse[held][row] = normaliser(w, it.hk, r0 + row, x);
+            for (int row = lane; row < kTileRows; row += 32) neg_lse[held][row] = normaliser(w, it.hk, r0 + min(row, rows - 1), x, 0, 1);
             cp_wait_all();
             fence_proxy_async_smem();
             __syncwarp();
@@ -681,13 +727,18 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
               s[k] = next[k];
               if (s[k] < 0 || s[k] >= p.num_slots) {
                 bad = bad || s[k] != kNoToken;
-                s[k] = -1;
+                s[k] = 0;
               }
             }
             look(i + kWarps);
             if (!wait_free(n)) return false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) copy_keys(head, s[k], stage, k * 32, C::kPiece);
+#pragma unroll 1
+            for (int k = 0; k < 4 && p.num_slots > 0; ++k) {
+              copy_keys(head, s[0], stage, k * 32, C::kPiece);
+              s[0] = s[1];
+              s[1] = s[2];
+              s[2] = s[3];
+            }
             cp_commit();
             if (kTwo) {
               if (pending >= 0) {
@@ -795,18 +846,28 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
       tc_fence_after_sync();
       return ok;
     };
-    // 32 of a quarter's columns of this step (none where `any` is false); behind the last of them the buffer is free
-    uint32_t raw[32];
-    auto read_scores = [&](int half, bool any) {
-      if (any) {
-        tmem_ld_32x32(tmem + lanes + (step & 1) * C::kCols + quarter * kWarpCols + half, raw);
-        tmem_ld_wait();
+    // A quarter's columns of this step, 32 at a time; behind the last the buffer is free.  use(first column, scores).  One copy of the code: what
+    // the warps run has to stay in the instruction caches.
+    auto columns = [&](int count, auto&& use) {
+      const uint32_t from = tmem + lanes + (step & 1) * C::kCols + quarter * kWarpCols;
+#pragma unroll 1
+      for (int c = 0; c < kWarpCols; c += 32) {
+        uint32_t raw[32];
+        if (c < count) {
+          tmem_ld_32x32(from + c, raw);
+          tmem_ld_wait();
+        }
+        if (c + 32 == kWarpCols) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[step & 1]);
+        }
+        if (c < count) use(c, raw);
       }
-      if (half == kWarpCols - 32) {
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[step & 1]);
-      }
+    };
+    auto total = [&](const uint64_t (&sums)[4]) {
+      const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+      return both.x + both.y;
     };
     auto gaps = [&]() { return *const_cast<const volatile int*>(&holes) != 0; };
     auto slot_inside = [&](const W& w, int token) {
@@ -815,13 +876,23 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
     };
     // cap tanh(x / cap), in the log2 domain; tanh(y) = 1 - 2 / (1 + e^(2 y))
     auto cap = [&](uint32_t x, float mul) { return __float_as_uint(p.cap_out * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(x) * mul * p.cap_in)))); };
-    // What a token gets of 32 rows: columns from `low` up to `high` alone where masked
-    auto weights = [&](const float* neg, const float* muls, bool masked, int low, int high, uint64_t (&sums)[4]) {
+    // What a token gets of 32 rows: of those from `low` up to `high` alone where masked
+    auto weights = [&](uint32_t (&raw)[32], const float* neg, const float* muls, bool masked, int low, int high, uint64_t (&sums)[4]) {
       if (capped) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) raw[c] = cap(raw[c], kScaled ? muls[c] : p.scale_log2);
       }
       const float same = capped ? 1.f : p.scale_log2;
+      if (masked) {
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float e = ex2(fmaf(__uint_as_float(raw[c]), kScaled && !capped ? muls[c] : same, neg[c]));
+          sum += c >= low && c < high ? e : 0.f;
+        }
+        sums[0] = add2(sums[0], pair_of(sum, 0.f));
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float4 n4 = *reinterpret_cast<const float4*>(neg + 4 * i);
@@ -829,18 +900,9 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
         if (kScaled && !capped) m4 = *reinterpret_cast<const float4*>(muls + 4 * i);
         const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), pair_of(m4.x, m4.y), pair_of(n4.x, n4.y)));
         const float2 y = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), pair_of(m4.z, m4.w), pair_of(n4.z, n4.w)));
-        float e[4] = {ex2(x.x), ex2(x.y), ex2(y.x), ex2(y.y)};
-        if (masked) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) e[k] = 4 * i + k >= low && 4 * i + k < high ? e[k] : 0.f;
-        }
-        sums[(2 * i) & 3] = add2(sums[(2 * i) & 3], pair_of(e[0], e[1]));
-        sums[(2 * i + 1) & 3] = add2(sums[(2 * i + 1) & 3], pair_of(e[2], e[3]));
+        sums[(2 * i) & 3] = add2(sums[(2 * i) & 3], pair_of(ex2(x.x), ex2(x.y)));
+        sums[(2 * i + 1) & 3] = add2(sums[(2 * i + 1) & 3], pair_of(ex2(y.x), ex2(y.y)));
       }
-    };
-    auto total = [&](const uint64_t (&sums)[4]) {
-      const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-      return both.x + both.y;
     };
 
     items([&](const W& w, const Item& it) {
@@ -863,7 +925,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
         const int rows = w.rows_of(it.block), row0 = it.block * C::kRows;
         const int row = (C::RT == 2 ? (quarter >> 1) * 128 : 0) + in_tile, col0 = quarter * kWarpCols % C::kStepKeys;
         const bool valid = row < rows, any = __any_sync(0xffffffffu, valid);
-        const int place = least + (row0 + min(row, rows - 1)) / g, sure = least + row0 / g;       // sure: what all rows of the block see
+        const int place = least + by_group(p, row0 + min(row, rows - 1)), sure = least + by_group(p, row0);       // sure: what all rows of the block see
         float mul = p.scale_log2;
         if constexpr (kScaled)
           if (valid) mul = row_mul[held][row];
@@ -871,45 +933,54 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
         uint64_t sums[4] = {0, 0, 0, 0};      // pairs of fp32
         for (int t = 0; t < it.n; ++t, ++step) {
           if (!wait_scores()) return false;
-#pragma unroll 1
-          for (int half = 0; half < kWarpCols; half += 32) {
-            read_scores(half, any);
-            if (!any) continue;
-            const int key = (it.t0 + t) * C::kStepKeys + col0 + half;
+          const int key0 = (it.t0 + t) * C::kStepKeys + col0;
+          const bool rare = gaps(), plain = key0 + kWarpCols - 1 <= sure && !rare;
+          columns(any ? kWarpCols : 0, [&](int col, uint32_t (&raw)[32]) {
+            const int key = key0 + col;
             float by = mul;
             if (capped) {
               by = 1.f;
 #pragma unroll
               for (int c = 0; c < 32; ++c) raw[c] = cap(raw[c], mul);
             }
-            const bool rare = __any_sync(0xffffffffu, gaps());
-            if (key + 31 > sure || rare) {
+            if (!plain) {
               const int seen = place + 1 - key;          // columns in front
-              uint32_t there = 0xffffffffu;
-              if (rare) there = __ballot_sync(0xffffffffu, slot_inside(w, key + lane));        // tokens whose slots lie outside the cache
+              uint32_t there = seen >= 32 ? 0xffffffffu : seen > 0 ? (1u << seen) - 1 : 0u;
+              if (__any_sync(0xffffffffu, rare)) there &= __ballot_sync(0xffffffffu, slot_inside(w, key + lane));        // tokens whose slots lie outside the cache
 #pragma unroll
-              for (int c = 0; c < 32; ++c) raw[c] = c < seen && ((there >> c) & 1) ? raw[c] : __float_as_uint(-INFINITY);
+              for (int c = 0; c < 32; ++c) raw[c] = (there >> c) & 1 ? raw[c] : __float_as_uint(-INFINITY);
             }
-            float mx[4];
+            // The maximum of the first scores serves until a sum gets large: fp32 has the range.  (A sum that is no number raises it every time.)
+            bool raise = m == -INFINITY, raised = false;
+            while (true) {
+              if (raise) {
+                float mx[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+                for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
 #pragma unroll
-            for (int c = 8; c < 32; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(raw[c]), __uint_as_float(raw[c + 1]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * by;
-            if (top > m + kRescaleThreshold) {        // the first tile raises; so does one behind tiles of minus infinity
-              const float f = m == -INFINITY ? 0.f : exp2f(m - top);
+                for (int c = 8; c < 32; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(raw[c]), __uint_as_float(raw[c + 1]));
+                const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * by, m);
+                const float f = m == -INFINITY ? 1.f : ex2(m - top);      // 0, or no number, in front of the first
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sums[i] = m == -INFINITY ? sums[i] : fma2(sums[i], pair_of(f, f), 0);
-              m = top;
+                for (int i = 0; i < 4; ++i) sums[i] = fma2(sums[i], pair_of(f, f), 0);
+                m = top;
+                raised = true;
+              }
+              const float neg = m == -INFINITY ? 0.f : -m;
+              const uint64_t by2 = pair_of(by, by), neg2 = pair_of(neg, neg);
+              uint64_t now[4] = {sums[0], sums[1], sums[2], sums[3]};
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), by2, neg2));
+                now[i & 3] = add2(now[i & 3], pair_of(ex2(x.x), ex2(x.y)));
+              }
+              raise = !raised && !(total(now) < kLargest);
+              if (raise) continue;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sums[i] = now[i];
+              break;
             }
-            const float neg = m == -INFINITY ? 0.f : -m;
-            const uint64_t by2 = pair_of(by, by), neg2 = pair_of(neg, neg);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), by2, neg2));
-              sums[i & 3] = add2(sums[i & 3], pair_of(ex2(x.x), ex2(x.y)));
-            }
-          }
+          });
         }
         // ---- the quarters' maxima and sums meet ----
         float2* parts = reinterpret_cast<float2*>(cells) + (turn++ & 1) * 512;
@@ -927,13 +998,13 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           }
           const bool none = top == -INFINITY;
 #pragma unroll
-          for (int i = 0; i < kParts; ++i) sum += x[i].x == -INFINITY ? x[i].y : x[i].y * exp2f(x[i].x - top);       // no score: 0, or no number
-          float lse = none && sum == 0.f ? -INFINITY : top + log2f(sum);
+          for (int i = 0; i < kParts; ++i) sum += x[i].x == -INFINITY ? x[i].y : x[i].y * ex2(x[i].x - top);       // no score: 0, or no number
+          float lse = none && sum == 0.f ? -INFINITY : top + lg2(sum);
           if (it.t0 == 0 && it.n == w.steps1(p, it.block)) {
-            const int j = (row0 + tid) / g, head = it.hk * g + row0 + tid - j * g;
+            const int j = by_group(p, row0 + tid), head = it.hk * g + row0 + tid - j * g;
             if (p.sink != nullptr && lse != -INFINITY) {
               const float sink = __ldcg(p.sink + head) * kLog2e, at = fmaxf(top, sink);
-              lse = at + log2f(sum * exp2f(top - at) + exp2f(sink - at));
+              lse = at + lg2(sum * ex2(top - at) + ex2(sink - at));
             }
             p.lse[static_cast<int64_t>(w.o.first + j) * p.hkv * g + head] = lse;
           } else {
@@ -950,23 +1021,17 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           const int token = (it.t0 + t) * C::kStepKeys + kt * 128 + in_tile;
           // this token is seen by the block's rows from `low` on
           const int low = token > least ? static_cast<int>(min(static_cast<int64_t>(token - least) * g - row0, static_cast<int64_t>(C::kRows))) : 0;
+          const bool plain = (it.t0 + t + 1) * C::kStepKeys - 1 <= least;       // all rows see all of the step's tokens
           uint64_t sums[4] = {0, 0, 0, 0};
           if (!wait_scores()) return false;
-#pragma unroll 1
-          for (int half = 0; half < kWarpCols; half += 32) {
-            const int col = col0 + half;
-            read_scores(half, col < rows);
-            if (col >= rows) continue;
-            if (col + 32 > rows || __any_sync(0xffffffffu, low > col)) {
-              weights(neg + half, muls + (kScaled ? half : 0), true, low - col, rows - col, sums);
-            } else {
-              weights(neg + half, muls + (kScaled ? half : 0), false, 0, 32, sums);
-            }
-          }
+          columns(rows - col0, [&](int at, uint32_t (&raw)[32]) {
+            const int col = col0 + at;
+            weights(raw, neg + at, muls + (kScaled ? at : 0), col + 32 > rows || !plain, low - col, rows - col, sums);
+          });
           float sum = total(sums);
           if (gaps() && !slot_inside(w, token)) sum = 0.f;       // rare: a token whose slot lies outside the cache is not seen
           float* cell = cells + group * chunk_keys + t * C::kStepKeys + kt * 128 + in_tile;
-          *cell = w.first_block(p, it.t0 + t) == it.block ? sum : *cell + sum;
+          *cell = it.block == 0 || w.first_block(p, it.t0 + t) == it.block ? sum : *cell + sum;
         }
         if (it.flush) {
           if (!meet()) return false;
@@ -993,19 +1058,14 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           const int r0 = (tile0 + t) * kTileRows + col0, rows = w.rows - r0;
           // this token is seen by the rows from `low` on
           const int low = token > least ? static_cast<int>(min(static_cast<int64_t>(token - least) * g - r0, static_cast<int64_t>(128))) : 0;
+          // all of the stage's rows see all of the block's tokens
+          const bool plain = static_cast<int64_t>((it.block + 1) * C::kRows - 1 - least) * g <= (tile0 + t) * kTileRows;
           uint64_t sums[4] = {0, 0, 0, 0};
-#pragma unroll 1
-          for (int half = 0; half < kWarpCols; half += 32) {
-            read_scores(half, any && half < rows);
-            if (!any || half >= rows) continue;
-            const float* neg = neg_lse[place] + col0 + half;
-            const float* muls = row_mul[place] + (kScaled ? col0 + half : 0);
-            if (half + 32 > rows || __any_sync(0xffffffffu, low > half)) {
-              weights(neg, muls, true, low - half, rows - half, sums);
-            } else {
-              weights(neg, muls, false, 0, 32, sums);
-            }
-          }
+          columns(any ? rows : 0, [&](int at, uint32_t (&raw)[32]) {
+            const float* neg = neg_lse[place] + col0 + at;
+            const float* muls = row_mul[place] + (kScaled ? col0 + at : 0);
+            weights(raw, neg, muls, at + 32 > rows || !plain, low - at, rows - at, sums);
+          });
           all += total(sums);
         }
         if (gaps() && !slot_inside(w, token)) all = 0.f;       // rare: a token whose slot lies outside the cache is not seen
@@ -1155,6 +1215,7 @@ int launch_weights_prompt(const WeightsPromptArgs& a, cudaStream_t s) {
   p.group = a.hq / a.hkv;
   p.last = a.last;
   p.inv_group = (65536 + p.group - 1) / p.group;
+  p.inv_group32 = static_cast<uint32_t>(p.group == 1 ? 0xffffffffull : (1ull << 32) / p.group);
   p.add = a.add;
   p.scale_log2 = a.scale * kLog2e;
   if (a.logit_cap > 0.f) {
