@@ -52,6 +52,7 @@ struct DecodeParams {
   const float* sink;
   int64_t q_stride, out_stride, num_slots, kv_tok_stride, kv_head_stride;
   int hkv, group, ctas, weight_ctas;
+  int join_heads, joins;     // query heads that a CTA joins, and how many CTAs a pair has for that
   float scale_log2, cap_pre, cap_post, decay;   // cap_post 0: no soft cap
 };
 
@@ -132,7 +133,8 @@ struct Cfg {
   static constexpr int kPart = NT * 8 * kOutStride * 4;          // a warp's partial result, where its ring was
   static constexpr int kRingBytes = kRing > kPart ? kRing : kPart;
   static constexpr int kSmem = kWarps * kRingBytes + 128;
-  static constexpr int kPerSm = HD == 256 ? 1 : 2;
+  // three where the rings are small: 8-bit rows, which are widened on the way to the products, and heads of 64
+  static constexpr int kPerSm = HD == 256 ? 1 : kRow <= 128 && NT == 1 ? 3 : 2;
   static_assert(kOutStride % 4 == 0 && kRingBytes % 128 == 0, "partial results are read four values at a time, rings begin on 128 bytes");
   static_assert(kPerSm * (kSmem + 4096) <= 227 * 1024, "shared memory");
   // 16-byte piece `ch` of row `row`: eight rows of one piece lie in eight different bank groups
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT, FMT>::kPerSm) weights_de
   if (__any_sync(0xffffffffu, bad) && lane == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
 }
 
-// The second kernel.  Its first hq * batch CTAs join the partial results of a query head that lies in several CTAs:
+// The second kernel.  Its first CTAs join the partial results of pairs that lie in several CTAs, some query heads each:
 // out = sum_c w_c O_c, w_c = 2^(lse_c - max) / sum.  The others take equal runs of the line of tiles and turn scores into weights.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads) weights_join_kernel(const DecodeParams p) {
@@ -538,9 +540,8 @@ __global__ void __launch_bounds__(kThreads) weights_join_kernel(const DecodePara
   __shared__ int start[3];
   __shared__ __align__(16) float weight[kThreads];
   pdl_launch_dependents();
-  const int g = p.group, hq = p.hkv * g, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool joins = static_cast<int>(blockIdx.x) < hq * p.ix.batch;
-  const int head = blockIdx.x % hq, b_join = blockIdx.x / hq;
+  const int g = p.group, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, all_joins = p.joins * p.hkv * p.ix.batch;
+  const bool joins = static_cast<int>(blockIdx.x) < all_joins;
   int first, last, total;
   int before = scan_units(p, warp_sums, first, last, total);       // the lengths were complete when the first kernel began
   const int64_t line = static_cast<int64_t>(total) * p.hkv;
@@ -548,63 +549,67 @@ __global__ void __launch_bounds__(kThreads) weights_join_kernel(const DecodePara
   auto owner = [&](int64_t x) { return owner_of(line, x, used); };
 
   if (joins) {
-    const int b = b_join;
+    const int which = blockIdx.x / p.joins, b = which / p.hkv, hk = which - b * p.hkv;
+    const int h0 = (blockIdx.x - which * p.joins) * p.join_heads, h1 = min(g, h0 + p.join_heads);
     if (b >= first && b < last) {
       for (int r = first; r < b; ++r) before += units_of(p, r);
       mine[0] = before;
       mine[1] = tiles_of(cached_of(p.ix, b).len);
     }
     __syncthreads();
-    const int n = mine[1], hk = head / g, h = head % g;
+    const int n = mine[1];
     const int64_t begin = static_cast<int64_t>(mine[0]) * p.hkv + static_cast<int64_t>(hk) * (n + kStart);
-    T* out = static_cast<T*>(p.out) + b * p.out_stride + static_cast<int64_t>(head) * HD;
     const int c0 = n > 0 ? owner(begin) : 0, c1 = n > 0 ? owner(begin + n - 1) : 0;
     // the first of the pair's CTAs has it in its second slot where its run begins with another pair; the others in their first
     const int first_slot = c0 * 2 + (n > 0 && run_begin(line, c0, used) < begin ? 1 : 0);
-    auto slot = [&](int c) { return static_cast<int64_t>(c == c0 ? first_slot : c * 2) * g + h; };
     pdl_wait_loads();
-    if (n == 0) {
-      for (int d = threadIdx.x; d < HD; d += kThreads) out[d] = from_f32<T>(0.f);
-      return;
-    }
-    if (c0 == c1) return;         // one CTA had all of it and has written the output
-    const float sink = p.sink != nullptr ? p.sink[head] * kLog2e : -INFINITY;
+    if (n > 0 && c0 == c1) return;         // one CTA had all of it and has written the output
     constexpr int kPer = (HD + kThreads - 1) / kThreads;
-    float top = -INFINITY;
-    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(p.part_lse + slot(c)).x);
-    top = warp_max(top);
-    const bool none = top == -INFINITY;
-    top = fmaxf(top, sink);
-    float den = p.sink != nullptr ? exp2f(sink - top) : 0.f, acc[kPer] = {};
-    for (int at = c0; at <= c1; at += kThreads) {
-      const int m = min(kThreads, c1 + 1 - at);
-      __syncthreads();
-      if (static_cast<int>(threadIdx.x) < m) {
-        const float lse = __ldcg(p.part_lse + slot(at + threadIdx.x)).x;
-        weight[threadIdx.x] = lse == -INFINITY ? 0.f : exp2f(lse - top);
+    for (int h = h0; h < h1; ++h) {
+      const int head = hk * g + h;
+      T* out = static_cast<T*>(p.out) + b * p.out_stride + static_cast<int64_t>(head) * HD;
+      auto slot = [&](int c) { return static_cast<int64_t>(c == c0 ? first_slot : c * 2) * g + h; };
+      if (n == 0) {
+        for (int d = threadIdx.x; d < HD; d += kThreads) out[d] = from_f32<T>(0.f);
+        continue;
       }
-      __syncthreads();
+      const float sink = p.sink != nullptr ? __ldcg(p.sink + head) * kLog2e : -INFINITY;
+      float top = -INFINITY;
+      for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(p.part_lse + slot(c)).x);
+      top = warp_max(top);
+      top = fmaxf(top, sink);
+      // no key seen: 0, beside a sink too; a part that is no number shows
+      float den = sink > -INFINITY ? exp2f(sink - top) : 0.f, acc[kPer] = {};
+      for (int at = c0; at <= c1; at += kThreads) {
+        const int m = min(kThreads, c1 + 1 - at);
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < m) {
+          const float lse = __ldcg(p.part_lse + slot(at + threadIdx.x)).x;
+          weight[threadIdx.x] = lse == -INFINITY ? 0.f : exp2f(lse - top);
+        }
+        __syncthreads();
 #pragma unroll 8
-      for (int i = 0; i < m; ++i) {
-        const float w = weight[i];
-        den += w;
+        for (int i = 0; i < m; ++i) {
+          const float w = weight[i];
+          den += w;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-          const int d = threadIdx.x + k * kThreads;
-          if (d < HD) acc[k] += w * __ldcg(p.part_o + slot(at + i) * HD + d);
+          for (int k = 0; k < kPer; ++k) {
+            const int d = threadIdx.x + k * kThreads;
+            if (d < HD) acc[k] += w * __ldcg(p.part_o + slot(at + i) * HD + d);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int d = threadIdx.x + k * kThreads;
-      if (d < HD) out[d] = from_f32<T>(none || den == 0.f ? 0.f : acc[k] / den);
+      for (int k = 0; k < kPer; ++k) {
+        const int d = threadIdx.x + k * kThreads;
+        if (d < HD) out[d] = from_f32<T>(den == 0.f ? 0.f : acc[k] / den);
+      }
     }
     return;
   }
 
   // ---- weights ----
-  const int c = blockIdx.x - hq * p.ix.batch;
+  const int c = blockIdx.x - all_joins;
   const int shared = static_cast<int>(min(static_cast<int64_t>(p.weight_ctas), max(line, static_cast<int64_t>(1))));
   if (c >= shared) return;
   const int64_t run0 = run_begin(line, c, shared);
@@ -722,7 +727,7 @@ int launch_one(const DecodeParams& p, cudaStream_t s) {
   cudaError_t err = launch_pdl(kern, dim3(p.ctas), dim3(kThreads), C::kSmem, s, p);
   note_launch();
   if (err != cudaSuccess) return -4;
-  err = launch_pdl(weights_join_kernel<T, HD>, dim3(p.hkv * p.group * p.ix.batch + p.weight_ctas), dim3(kThreads), 0, s, p);
+  err = launch_pdl(weights_join_kernel<T, HD>, dim3(p.joins * p.hkv * p.ix.batch + p.weight_ctas), dim3(kThreads), 0, s, p);
   note_launch();
   return err == cudaSuccess ? 0 : -4;
 }
@@ -742,7 +747,11 @@ int launch_format(const DecodeParams& p, int fmt, cudaStream_t s) {
   }
 }
 
-int stream_ctas(const WeightsDecodeArgs& a) { return a.head_dim == 256 ? a.num_sms : 2 * a.num_sms; }
+// as many as run at once (Cfg's kPerSm)
+int stream_ctas(const WeightsDecodeArgs& a) {
+  const int row = a.head_dim * (a.kv_fmt == kKvSame ? 2 : 1);
+  return (a.head_dim == 256 ? 1 : row <= 128 && a.hq / a.hkv <= 8 ? 3 : 2) * a.num_sms;
+}
 
 }  // namespace
 
@@ -770,6 +779,10 @@ int launch_weights_decode(const WeightsDecodeArgs& a, cudaStream_t s) {
   p.hkv = a.hkv;
   p.ctas = stream_ctas(a);
   p.weight_ctas = 8 * a.num_sms;
+  // a CTA joins several heads where there are more heads than two per SM
+  const int64_t heads = static_cast<int64_t>(a.index.batch) * a.hq;
+  p.join_heads = static_cast<int>(std::min<int64_t>(p.group, std::max<int64_t>(1, heads / (2 * a.num_sms))));
+  p.joins = (p.group + p.join_heads - 1) / p.join_heads;
   const int64_t parts = static_cast<int64_t>(p.ctas) * 2 * p.group;
   p.part_o = a.workspace;
   p.part_lse = reinterpret_cast<float2*>(a.workspace + parts * a.head_dim);

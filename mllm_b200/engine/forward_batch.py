@@ -51,6 +51,12 @@ class ForwardBatch:
     # drafted token trees: the node that each row's node continues (see ops.attention_tree); the rows are new tokens of an extend batch
     # (out_cache_loc has the nodes' slots; positions go on by rows, a node's own is that of its depth)
     tree_parents: Optional[torch.Tensor] = None        # [T] int32
+    # sums of attention weights per cached token, of all layers (KVPool.make_weight_sums, ops.attention_decode_weights): decode steps add their
+    # weights, faded by weight_decay; prompts set or add those of their last weight_last queries (0: of all)
+    weight_sums: Optional[torch.Tensor] = None         # [layers, request rows, kv heads, tokens] fp32
+    weight_last: int = 0
+    weight_add: bool = False
+    weight_decay: float = 1.0
     # rows of input_ids whose logits are wanted (None: the last row of each request)
     logit_rows: Optional[torch.Tensor] = None
     # multimodal

@@ -109,7 +109,8 @@ class CudaGraphRunner:
         logger.info("captured %d decode graphs (batch sizes %s)", len(self.graphs), self.batch_sizes)
 
     def can_run(self, fb: ForwardBatch) -> bool:
-        return fb.forward_mode.is_decode() and fb.batch_size <= self.batch_sizes[-1] and bool(self.graphs)
+        return (fb.forward_mode.is_decode() and fb.batch_size <= self.batch_sizes[-1] and bool(self.graphs)
+                and getattr(fb, "weight_sums", None) is None)
 
     def captured_size_for(self, raw: int) -> Optional[int]:
         """The captured batch size a batch of ``raw`` rows would replay, or None when none is large enough."""

@@ -526,17 +526,19 @@ class ModelRunner:
         self, input_ids: torch.Tensor, req_pool_indices: torch.Tensor, seq_lens: torch.Tensor,
         extend_seq_lens: torch.Tensor, extend_prefix_lens: torch.Tensor, out_cache_loc: torch.Tensor,
         extend_seq_lens_cpu: Optional[List[int]] = None, extend_prefix_lens_cpu: Optional[List[int]] = None,
-        **extra,
+        first_positions_cpu: Optional[List[int]] = None, **extra,
     ) -> ForwardBatch:
         """Batch of new tokens (after optional cached prefixes). Passing the ``*_cpu`` lists avoids
-        a device->host sync."""
+        a device->host sync.  ``first_positions_cpu``: position of each request's first new token where it is not the number of
+        cached ones (requests that were shortened).  ``weight_sums`` and what belongs to it: see :meth:`evict_cache`."""
+        self._check_weight_sums(extra)
         if extend_seq_lens_cpu is None:
             extend_seq_lens_cpu = extend_seq_lens.tolist()
         if extend_prefix_lens_cpu is None:
             extend_prefix_lens_cpu = extend_prefix_lens.tolist()
         bs = len(extend_seq_lens_cpu)
         starts, pos_parts, acc = [], [], 0
-        for n, p in zip(extend_seq_lens_cpu, extend_prefix_lens_cpu):
+        for n, p in zip(extend_seq_lens_cpu, first_positions_cpu if first_positions_cpu is not None else extend_prefix_lens_cpu):
             starts.append(acc)
             pos_parts.append(torch.arange(p, p + n, dtype=torch.int64))
             acc += n
@@ -558,14 +560,16 @@ class ModelRunner:
 
     def prepare_forward_batch_decode(
         self, input_ids: torch.Tensor, req_pool_indices: torch.Tensor, seq_lens: torch.Tensor,
-        out_cache_loc: torch.Tensor, max_seq_len: Optional[int] = None, **extra,
+        out_cache_loc: torch.Tensor, max_seq_len: Optional[int] = None, positions: Optional[torch.Tensor] = None, **extra,
     ) -> ForwardBatch:
-        """One new token per request; ``seq_lens`` already counts it. No host sync."""
+        """One new token per request; ``seq_lens`` already counts it. No host sync.  ``positions``: where they are not
+        ``seq_lens - 1`` (requests that were shortened).  ``weight_sums``, ``weight_decay``: see :meth:`evict_cache`."""
+        self._check_weight_sums(extra)
         bs = input_ids.shape[0]
         return ForwardBatch(
             forward_mode=ForwardMode.DECODE, batch_size=bs, input_ids=input_ids,
             req_pool_indices=req_pool_indices.to(torch.int32), seq_lens=seq_lens.to(torch.int32),
-            out_cache_loc=out_cache_loc, positions=(seq_lens - 1).to(torch.int64),
+            out_cache_loc=out_cache_loc, positions=(seq_lens - 1 if positions is None else positions).to(torch.int64),
             max_seq_len=int(max_seq_len if max_seq_len is not None else self.context_len),
             req_to_token_pool=self.req_to_token_pool, token_to_kv_pool=self.token_to_kv_pool,
             attn_backend=self.attn_backend, **extra,
@@ -596,6 +600,34 @@ class ModelRunner:
         loc = table[req_pool_indices.long().clamp(0, table.shape[0] - 1)[place[:, 0]], place[:, 1]].to(torch.int64)
         return self.prepare_forward_batch_extend(input_ids, req_pool_indices, tree + prefix, tree, prefix, loc, list(tree_lens_cpu),
                                                  list(prefix_lens_cpu), tree_parents=parents.to(torch.int32).contiguous(), logit_rows=rows, **extra)
+
+    def _check_weight_sums(self, extra: dict) -> None:
+        sums = extra.get("weight_sums")
+        if sums is None:
+            return
+        if not getattr(self.model, "draft_trees", False):        # every layer that mixes tokens is a RadixAttention
+            raise ValueError(f"{type(self.model).__name__} does not add up attention weights")
+        if any(getattr(m, "sliding_window", None) for m in self.model.modules()):
+            raise ValueError("layers with a sliding window do not add up attention weights")
+        group = self.num_attention_heads // self.num_kv_heads
+        if sums.is_cuda and ops.use_kernels(sums) and not ops.cache_weights_cover(self.head_dim, group, self.kv_cache_dtype, self.dtype):
+            raise ValueError(f"attention weights are added up for heads of 64, 128 or 256 features in 16 bits, over caches of their type or of 8-bit floats; "
+                             f"here are {self.head_dim} features in {self.dtype} over {self.kv_cache_dtype}")
+        if sums.dim() != 4 or sums.shape[0] != self.token_to_kv_pool.layer_num:
+            raise ValueError(f"sums of attention weights are [{self.token_to_kv_pool.layer_num} layers, rows, heads, tokens]")
+
+    def evict_cache(self, weight_sums: torch.Tensor, req_pool_indices: torch.Tensor, seq_lens: torch.Tensor, budgets: torch.Tensor, max_budget: int,
+                    first: int = 4, recent: int = 32, pool: int = 1) -> torch.Tensor:
+        """Shortens requests in the cache to ``budgets`` tokens (int32, at most ``max_budget``): every kv head of every layer keeps the last
+        ``recent`` tokens, the first ``first`` and those with the largest sums (:func:`ops.cache_select`).  ``weight_sums`` come from
+        ``token_to_kv_pool.make_weight_sums(rows of the request table, tokens)`` and grow in the batches that are made with them
+        (``weight_sums=``, and ``weight_last=``, ``weight_add=`` for prompts, ``weight_decay=`` for decode steps).  Returns the requests' new lengths, int32
+        on the device: their slots behind those are free to be given back, and their next tokens' positions go on from what they were
+        (``positions=``, ``first_positions_cpu=``).  Requests whose slots others share, the prefix cache's among them, cannot be shortened."""
+        keep, counts = ops.cache_select(weight_sums, req_pool_indices.to(torch.int32).contiguous(), seq_lens.to(torch.int32).contiguous(),
+                                        budgets.to(torch.int32).contiguous(), max_budget, first=first, recent=recent, pool=pool)
+        self.token_to_kv_pool.evict(weight_sums, self.req_to_token_pool.req_to_token, req_pool_indices.to(torch.int32).contiguous(), keep, counts)
+        return counts
 
     # ------------------------------------------------------------------ forward / sample
     @torch.no_grad()

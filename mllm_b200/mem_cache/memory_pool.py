@@ -103,6 +103,16 @@ class KVPool:
 
         tree_kv_compact(self.store, req_to_token, req_pool_indices, prefix_lens, path, counts)
 
+    def make_weight_sums(self, rows: int, tokens: int) -> torch.Tensor:
+        """Sums of attention weights per cached token for ``rows`` rows of a request table and up to ``tokens`` tokens each, all zero."""
+        return torch.zeros((self.layer_num, rows, self.kv_heads, tokens), dtype=torch.float32, device=self.device)
+
+    def evict(self, sums, req_to_token, req_pool_indices, keep, counts) -> None:
+        """Moves the rows of the tokens that stay, and their sums, to the front, in all layers (see :func:`ops.cache_evict`)."""
+        from ..ops import cache_evict
+
+        cache_evict(self.store, sums, req_to_token, req_pool_indices, keep, counts)
+
     def clear(self) -> None:
         self.store.zero_()
 

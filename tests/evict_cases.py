@@ -147,3 +147,95 @@ def plain_select(sums, req, lens, budgets, width, first, recent, pool):
                     stay.add(i)
                 keep[layer, b, head, :count] = torch.tensor(sorted(stay), dtype=torch.int32)
     return keep, torch.tensor(counts, dtype=torch.int32)
+
+
+class Shortened:
+    """A tiny model whose requests are shortened while they are decoded."""
+
+    def __init__(self, preset, device, dtype, kv_cache_dtype="auto"):
+        from mllm_b200.configs import ServerConfig
+        from mllm_b200.executor import ModelRunner
+
+        self.mr = ModelRunner(ServerConfig(model_path=f"preset:{preset}", dtype=dtype, max_running_requests=8, max_total_tokens=4096),
+                              kv_cache_dtype=kv_cache_dtype, device=device)
+        self.mr.initialize()
+        self.dev = torch.device(device)
+
+    def ints(self, x):
+        return torch.tensor(x, dtype=torch.int32, device=self.dev)
+
+    def start(self, prompts, **kw):
+        mr = self.mr
+        rows = mr.req_to_token_pool.alloc(len(prompts))
+        table, lens = mr.req_to_token_pool.req_to_token, [len(p) for p in prompts]
+        locs = [mr.token_to_kv_pool_allocator.alloc(n) for n in lens]
+        for r, loc in zip(rows, locs):
+            table[r, :len(loc)] = loc.to(torch.int32)
+        fb = mr.prepare_forward_batch_extend(torch.tensor([t for p in prompts for t in p], device=self.dev), self.ints(rows), self.ints(lens), self.ints(lens),
+                                             self.ints([0] * len(rows)), torch.cat(locs), lens, [0] * len(rows), **kw)
+        return rows, mr.forward(fb).next_token_logits.clone()
+
+    def step(self, rows, lens, positions, tokens, **kw):
+        """The next token of every request, whose cache has ``lens`` tokens."""
+        mr = self.mr
+        locs = torch.cat([mr.token_to_kv_pool_allocator.alloc(1) for _ in rows])
+        table = mr.req_to_token_pool.req_to_token
+        for r, n, loc in zip(rows, lens, locs.tolist()):
+            table[r, n] = loc
+        fb = mr.prepare_forward_batch_decode(torch.tensor(tokens, device=self.dev), self.ints(rows), self.ints([n + 1 for n in lens]), locs,
+                                             max_seq_len=max(lens) + 1, positions=self.ints(positions), **kw)
+        return mr.forward(fb).next_token_logits.clone()        # (a captured step has its logits in one place)
+
+    def free(self, rows):
+        for r in rows:
+            self.mr.req_to_token_pool.free(r)
+
+    def check(self, close):
+        from mllm_b200 import ops
+
+        g = random.Random(5)
+        mr, prompts = self.mr, [[g.randrange(self.mr.vocab_size) for _ in range(n)] for n in (50, 23, 4)]
+        tokens = [[g.randrange(mr.vocab_size) for _ in prompts] for _ in range(4)]
+        table = mr.req_to_token_pool.req_to_token
+        sums = mr.token_to_kv_pool.make_weight_sums(table.shape[0], 80)
+        lens = [len(p) for p in prompts]
+        # nothing is dropped: as if nothing had been asked for
+        plain, want = self.start(prompts)
+        want = [want] + [self.step(plain, [n + i for n in lens], [n + i for n in lens], tokens[i]) for i in range(2)]
+        rows, got = self.start(prompts, weight_sums=sums, weight_last=8)
+        close(got, want[0])
+        heads = mr.model.model.layers[0].self_attn.attn.num_heads
+        mass = sums[:, rows].sum((2, 3))
+        torch.testing.assert_close(mass, torch.tensor([min(n, 8) * heads for n in lens], device=self.dev).float().expand_as(mass), rtol=1e-4, atol=1e-4)
+        now = mr.evict_cache(sums, self.ints(rows), self.ints(lens), self.ints([80, 23, 4]), 80)
+        assert now.tolist() == lens
+        close(self.step(rows, lens, lens, tokens[0], weight_sums=sums), want[1])
+        close(self.step(rows, [n + 1 for n in lens], [n + 1 for n in lens], tokens[1], weight_sums=sums, weight_decay=0.9), want[2])
+        # and now it is: what is left is attended to as any cache is, at the positions that the tokens have in the text
+        here = [n + 2 for n in lens]
+        now = mr.evict_cache(sums, self.ints(rows), self.ints(here), self.ints([20, 12, 80]), 80, first=2, recent=5, pool=3)
+        assert now.tolist() == [20, 12, 6]
+        store, table_now = mr.token_to_kv_pool.store.clone(), table.clone()
+        a = self.step(rows, now.tolist(), here, tokens[2], weight_sums=sums)
+        mr.token_to_kv_pool.store.copy_(store)
+        table.copy_(table_now)
+        close(a, self.step(rows, now.tolist(), here, tokens[2]))
+        # the dropped tokens matter to the requests that lost some, and to no other
+        full = self.step(plain, here, here, tokens[2])
+        assert (a[0].float() - full[0].float()).abs().max() > 1e-3 and (a[1].float() - full[1].float()).abs().max() > 1e-3
+        close(a[2], full[2])
+        # new text behind a shortened request
+        n = [x + 1 for x in now.tolist()]
+        locs = [mr.token_to_kv_pool_allocator.alloc(3) for _ in rows]
+        for r, at, loc in zip(rows, n, locs):
+            table[r, at:at + 3] = loc.to(torch.int32)
+        fb = mr.prepare_forward_batch_extend(torch.tensor([1, 2, 3] * 3, device=self.dev), self.ints(rows), self.ints([x + 3 for x in n]), self.ints([3] * 3),
+                                             self.ints(n), torch.cat(locs), [3] * 3, n, first_positions_cpu=[x + 1 for x in here], weight_sums=sums, weight_add=True)
+        assert fb.positions.tolist() == [x + 1 + i for x in here for i in range(3)]
+        before = sums.clone()
+        assert torch.isfinite(mr.forward(fb).next_token_logits).all()
+        added = (sums - before)[:, rows[0], :, :n[0]]
+        assert (added >= 0).all() and (added.sum((1, 2)) > 0).all()
+        ops.check_status()
+        self.free(rows)
+        self.free(plain)

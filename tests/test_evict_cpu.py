@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from evict_cases import cached_batch, exact_decode, exact_prompt, plain_select
+from evict_cases import Shortened, cached_batch, exact_decode, exact_prompt, plain_select
 from mllm_b200 import ops
 
 
@@ -130,3 +130,23 @@ def test_kernels_cover():
     assert ops.cache_weights_cover(128, 32, bf, bf) and ops.cache_weights_cover(256, 16, torch.float8_e5m2, fp)
     assert not ops.cache_weights_cover(256, 17, bf, bf) and not ops.cache_weights_cover(96, 4, bf, bf) and not ops.cache_weights_cover(64, 4, fp, bf)
     assert not ops.cache_weights_cover(64, 4, torch.float32, torch.float32)
+
+
+@pytest.mark.parametrize("preset", ["qwen3-tiny", "llama-tiny", "qwen2-tiny", "qwen3-moe-tiny"])
+def test_shortened_requests_of_a_model(preset):
+    Shortened(preset, "cpu", "float32").check(lambda a, b: torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4))
+
+
+def test_models_with_other_layers_keep_no_sums():
+    s = Shortened("qwen3.5-tiny", "cpu", "float32")
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="attention weights"):
+        s.mr.prepare_forward_batch_decode(one.long(), one, one + 1, one.long(), weight_sums=torch.zeros(1, 1, 1, 1))
+    s = Shortened("qwen3-tiny", "cpu", "float32")
+    with pytest.raises(ValueError, match="layers"):
+        s.mr.prepare_forward_batch_decode(one.long(), one, one + 1, one.long(), weight_sums=torch.zeros(1, 1, 1, 1))
+    for m in s.mr.model.modules():
+        if hasattr(m, "sliding_window"):
+            m.sliding_window = 16
+    with pytest.raises(ValueError, match="sliding window"):
+        s.mr.prepare_forward_batch_decode(one.long(), one, one + 1, one.long(), weight_sums=s.mr.token_to_kv_pool.make_weight_sums(2, 8))

@@ -3,7 +3,7 @@ moved rows exactly; lengths around the tiles, odd groups, slots in any order, 8-
 import pytest
 import torch
 
-from evict_cases import cached_batch, exact_decode, exact_prompt, plain_select
+from evict_cases import Shortened, cached_batch, exact_decode, exact_prompt, plain_select
 from mllm_b200 import ops
 from mllm_b200.ops import reference as ref
 
@@ -150,6 +150,18 @@ def test_decode_values_that_are_no_numbers():
     assert torch.isnan(got[1, 2:]).all() and not torch.isnan(got[1, :2]).any() and not torch.isnan(got[[0, 2]]).any()
     row = int(c["req"][1])
     assert torch.isnan(c["sums"][row, 1, :100]).all() and not torch.isnan(c["sums"][row, 0]).any() and not torch.isnan(c["sums"][row, 1, 100:]).any()
+
+
+def test_decode_values_that_are_no_numbers_in_pairs_of_many_parts():
+    c = cached_batch([9000, 50], 4, 2, 128, seed=15)
+    slots = c["table"][int(c["req"][0])].long()
+    c["k"][slots[:9000], 0] = float("nan")       # every part of the first kv head
+    c["v"][slots[8000], 1] = float("inf")        # one part of the second
+    got = decode(c, sink=c["sink"])
+    ops.check_status()
+    assert torch.isnan(got[0, :2]).all() and torch.isinf(got[0, 2:]).all() and not torch.isnan(got[1]).any()
+    row = int(c["req"][0])
+    assert torch.isnan(c["sums"][row, 0, :9000]).all() and not torch.isnan(c["sums"][row, 1]).any()
 
 
 def test_decode_scores_of_minus_infinity():
@@ -553,3 +565,18 @@ def test_refusals_on_the_device():
         decode(cached_batch([40], 4, 2, 96))
     with pytest.raises(ValueError):
         decode(dict(cached_batch([40], 4, 2, 64), req=torch.zeros(1, dtype=torch.int32)))
+
+
+@pytest.mark.parametrize("preset", ["qwen3-tiny", "llama-tiny", "qwen3-moe-tiny"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_shortened_requests_of_a_model(preset, dtype):
+    # both sides round some 12 tensors per layer to the activation type, half a step each, in two layers
+    bound = 2 * 2 * 12 * torch.finfo(getattr(torch, dtype)).eps / 2
+    before = ops.launch_count()
+
+    def close(a, b):
+        off = ((a.double() - b.double()).norm() / b.double().norm()).item()
+        assert off <= bound, (off, bound)
+
+    Shortened(preset, "cuda:0", dtype).check(close)
+    assert ops.launch_count() > before
