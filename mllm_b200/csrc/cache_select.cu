@@ -237,9 +237,9 @@ __device__ __forceinline__ void select_list(const CacheSelectArgs& a, int* keep,
       want = still;
       const int there = found;
       if (there == want || pass == 2) {
-        // Nothing is left to tell them apart, or all of them stay: then what has more in its open digits is above `top`, the rest its equals
-        top = prefix;
-        if (there == want) want = 0x7fffffff;
+        // Nothing is left to tell them apart, or all of them stay: those with this prefix and any digits behind it
+        top = prefix - (there == want ? 1 : 0);
+        want = there == want ? 0 : want;
         break;
       }
       if (pass == 0) {
@@ -247,12 +247,18 @@ __device__ __forceinline__ void select_list(const CacheSelectArgs& a, int* keep,
         for (int p0 = 8 * tid; p0 < all; p0 += 8 * kThreads) {
           uint32_t v[8];
           get(p0, v);
+          int mine = 0;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if ((v[k] ^ prefix) < 1u << 21) {
-              const int at = atomicAdd(&collected, 1);
-              if (at < kEquals) equals[at] = v[k];
-            }
+          for (int k = 0; k < 8; ++k) mine += (v[k] ^ prefix) < 1u << 21 ? 1 : 0;
+          if (mine != 0) {
+            int at = atomicAdd(&collected, mine);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if ((v[k] ^ prefix) < 1u << 21) {
+                if (at < kEquals) equals[at] = v[k];
+                ++at;
+              }
+          }
         }
         __syncthreads();
         listed = collected <= kEquals;
@@ -275,8 +281,9 @@ __device__ __forceinline__ void select_list(const CacheSelectArgs& a, int* keep,
             same += few[i] == v;
           }
           if (above < want && want <= above + same) {       // the same for all equals
-            chosen = v;
-            still = want - above;
+            const bool all = want == above + same;
+            chosen = v - (all ? 1 : 0);
+            still = all ? 0 : want - above;
           }
         }
         __syncthreads();
@@ -286,7 +293,7 @@ __device__ __forceinline__ void select_list(const CacheSelectArgs& a, int* keep,
       }
     }
   }
-  // ---- indices: what is above `top`, of its equals the first `want`, and the tokens that stay in any case ----
+  // ---- indices: what is above `top`, of its equals the first `want` (0: none of them), and the tokens that stay in any case ----
   auto classify = [&](int p0, uint32_t& above, uint32_t& equal) {
     above = equal = 0;
     if (p0 >= all) return;
@@ -294,10 +301,10 @@ __device__ __forceinline__ void select_list(const CacheSelectArgs& a, int* keep,
       uint32_t v[8];
       get(p0, v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        above |= v[k] > top ? 1u << k : 0u;
-        equal |= v[k] == top ? 1u << k : 0u;
-      }
+      for (int k = 0; k < 8; ++k) above |= v[k] > top ? 1u << k : 0u;
+      if (want > 0)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) equal |= v[k] == top ? 1u << k : 0u;
     }
     if (p0 + shift0 < max(first, lo) || p0 + shift0 + 8 > min(end, hi)) above |= between(p0, lo, min(first, hi)) | between(p0, max(end, lo), hi);
   };
@@ -352,7 +359,10 @@ __device__ __forceinline__ void select_list(const CacheSelectArgs& a, int* keep,
       int left = max(0, want - my_equal);
       for (uint32_t e = equal; e != 0 && left > 0; e &= e - 1, --left) stay |= e & -e;
     }
-    for (uint32_t e = stay; e != 0; e &= e - 1) keep[to++] = p0 + shift0 + __ffs(e) - 1;
+    int* at = keep + to;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (stay >> k & 1) *at++ = p0 + shift0 + k;
     above_before += total & 0xffff;
     equal_before += total >> 16;
   }
