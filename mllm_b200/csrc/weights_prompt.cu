@@ -94,13 +94,13 @@ struct Cfg {
   static constexpr int kBlock = kRows * 128, kBlockBytes = NH * kBlock;    // 64 features of a block's rows
   static constexpr int kPiece = 128 * 128, kStage = NH * kPiece;
   static constexpr int kStages = NH == 4 ? 2 : NH == 2 ? (R == 2 ? 4 : 5) : 6;
-  // Warps: those that compute, that copy stages (kCopying of them, every kCopying-th stage each), one that copies blocks, one that issues
-  // products.
-  static constexpr int kCopy = 6, kCopying = kCopy < kStages ? kCopy : kStages;
-  static constexpr int kBlockWarp = kCompute + kCopy, kIssueWarp = kBlockWarp + 1, kThreads = 32 * (kIssueWarp + 1);
+  // Warps: those that compute, that copy stages (kCopying of them, every kCopying-th stage each), one that walks through the CTA's run, one that
+  // copies blocks, one that issues products.
+  static constexpr int kCopy = 5, kCopying = kCopy < kStages ? kCopy : kStages;
+  static constexpr int kWalkWarp = kCompute + kCopy, kBlockWarp = kWalkWarp + 1, kIssueWarp = kBlockWarp + 1, kThreads = 32 * (kIssueWarp + 1);
   // Registers: those of a launch, of the computing threads, of the others.  A quarter of the warps share 16384, four computing ones each.
   static constexpr int kLaunchRegs = 80, kComputeRegs = 88, kOtherRegs = 64;
-  static_assert(4 * kComputeRegs + (kCopy + 2) / 4 * kOtherRegs <= (4 + (kCopy + 2) / 4) * kLaunchRegs && (kCopy + 2) % 4 == 0, "register split");
+  static_assert(4 * kComputeRegs + (kCopy + 3) / 4 * kOtherRegs <= (4 + (kCopy + 3) / 4) * kLaunchRegs && (kCopy + 3) % 4 == 0, "register split");
   static constexpr int kSmem = kBlockBytes + kStages * kStage;
   static constexpr int kGroups = 4 / KT;                     // parts of a token's sum
   // Normalisers and factors of rows: of the last blocks, or of the stages.  A place is written anew behind the last product of the block in
@@ -170,7 +170,13 @@ struct Item {
   bool flush;            // last block over these steps (second pass)
   int chunk;             // steps whose sums wait (second pass)
   int64_t at;            // where the unit begins: on the first pass's line (second pass), on its own (else)
+  int64_t at1;           // where the request's and kv head's units begin on the first pass's line (blocks of tokens)
 };
+struct Record {
+  Observed o;
+  Item it;               // n 0: the run's end
+};
+constexpr int kItems = 4;      // items that the walking warp is ahead
 
 // CTAs that share a line of units and where CTA c's run begins
 __device__ __forceinline__ int used_ctas(const PromptParams& p, int64_t line) {
@@ -205,27 +211,6 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// two 32-bit operations an instruction
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 halves_of(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -245,12 +230,12 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
   using W = Work<C, PASS>;
   constexpr int kD = C::kD, kStages = C::kStages, KT = C::KT, kRing = C::kRing, kIssueWarp = C::kIssueWarp;
   extern __shared__ __align__(1024) uint8_t prompt_smem[];
-  __shared__ uint64_t bars[2 * kStages + 8 + kRing];
+  __shared__ uint64_t bars[2 * kStages + 8 + kRing + 2 * kItems];
   __shared__ uint32_t tmem_holder;
   __shared__ int fail_flag, holes;
-  __shared__ int begin_of[2], used_of;                      // request and kv head of the run's first unit; CTAs of the first pass
-  __shared__ Observed begin_request;
-  __shared__ int64_t begin_rest, begin_at1, begin_unit1, line_of[4];     // steps in front of the run; request and kv head on the first pass's line; run, its end, both lines
+  __shared__ int used_of;                                   // CTAs of the first pass
+  __shared__ int64_t line_of[2];                            // lines of the first pass and of this one
+  __shared__ Record records[kItems];
   __shared__ __align__(16) float neg_lse[kRing][C::kRingRows];      // -normaliser of rows (sums)
   __shared__ __align__(16) float row_mul[kRing][kScaled ? C::kRingRows : 4];
   __shared__ __align__(16) float cells[kChunk * 512];       // second pass: [parts][tokens]; else 2 x [4][128] maxima and sums
@@ -265,17 +250,22 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
   uint64_t* b_free = b_full + 1;         // tcgen05.commit: the last scores of a block
   uint64_t* met_bar = b_free + 1;        // the computing warps among themselves
   uint64_t* l_full = met_bar + 1;        // [ring] who writes normalisers and factors (not of the first block)
+  uint64_t* r_full = l_full + kRing;     // [record] the walking warp
+  uint64_t* r_free = r_full + kItems;    // [record] all others: computing, copying and issuing warps
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = p.group;
   pdl_wait_loads();
 
-  // ---- where this CTA's run begins ----
-  if (warp == 0) {
+  // ---- where this CTA's run begins: what one lane of the walking warp goes on with ----
+  W w;
+  Item it{};
+  int64_t pos = 0, end = 0, rest = 0, at1 = 0, unit1 = 0;      // on this pass's line; behind the unit's first; on the first pass's line
+  bool walks = false;
+  if (warp == C::kWalkWarp) {
     const int per = (p.ix.batch + 31) / 32;
     const int first = min(p.ix.batch, lane * per), last = min(p.ix.batch, first + per);
     int64_t mine1 = 0, mine = 0;
     bool bad = false;
-    W w;
     int64_t c1 = 0, c = 0;                // of one kv head of this lane's first request
     for (int b = last - 1; b >= first; --b) {
       w.set(p, observed_of(p, b));
@@ -301,39 +291,39 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
     // the second pass has no cost beside its steps
     const int used = PASS == 2 ? static_cast<int>(min(static_cast<int64_t>(p.ctas), max(line, static_cast<int64_t>(1)))) : used_ctas(p, line);
     const int cta = blockIdx.x;
-    const int64_t begin = cta < used ? run_begin(line, cta, used) : line, end = cta < used ? run_begin(line, cta + 1, used) : line;
+    pos = cta < used ? run_begin(line, cta, used) : line;
+    end = cta < used ? run_begin(line, cta + 1, used) : line;
     if (lane == 0) {
-      line_of[0] = begin;
-      line_of[1] = end;
-      line_of[2] = line1;
-      line_of[3] = line;
+      line_of[0] = line1;
+      line_of[1] = line;
       used_of = used_ctas(p, line1);
       fail_flag = 0;
       holes = 0;
       if (PASS == 1) p.jobs[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
-    int64_t at = incl - mine, at1 = incl1 - mine1;
-    if (begin < end && begin >= at && begin < incl) {
+    int64_t at = incl - mine;
+    at1 = incl1 - mine1;
+    if (pos < end && pos >= at && pos < incl) {
       for (int b = first; b < last; ++b) {
         if (b > first) {
           w.set(p, observed_of(p, b));
           c = w.cost(p);
           c1 = PASS == 1 ? c : w.cost1(p);
         }
-        if (begin >= at && begin < at + c * p.hkv) {
-          const int64_t in = begin - at;
-          const int hk = c < (1ll << 31) && in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(c) : static_cast<int>(in / c);
-          begin_of[0] = b;
-          begin_of[1] = hk;
-          begin_request = w.o;
-          begin_rest = in - hk * c;
-          begin_at1 = at1;
-          begin_unit1 = c1;
+        if (pos < at + c * p.hkv) {
+          const int64_t in = pos - at;
+          it.b = b;
+          it.hk = c < (1ll << 31) && in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(c) : static_cast<int>(in / c);
+          rest = in - it.hk * c;
+          unit1 = c1;
+          walks = true;
+          break;
         }
         at += c * p.hkv;
         at1 += c1 * p.hkv;
       }
     }
+    if (pos >= end) walks = lane == 0;
   } else if (warp == kIssueWarp) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
@@ -349,6 +339,10 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
       mbar_init(b_free, 1);
       mbar_init(met_bar, kCompute);
       for (int i = 0; i < kRing; ++i) mbar_init(&l_full[i], 1);
+      for (int i = 0; i < kItems; ++i) {
+        mbar_init(&r_full[i], 1);
+        mbar_init(&r_free[i], kCompute + C::kCopying + 2);
+      }
       fence_barrier_init();
     }
     __syncwarp();
@@ -364,110 +358,23 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
   const bool aligned = (smem_u32(prompt_smem) & 1023) == 0;      // the swizzle counts from 1 KB boundaries
   if (!aligned && tid == 0 && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusPipelineTimeout);
 
-  // Calls fn(request's numbers, item) for every item of the run; all roles walk the same way.
-  auto items = [&](auto&& fn) {
-    int64_t pos = line_of[0];
-    const int64_t end = aligned ? line_of[1] : pos;
-    if (pos >= end) return;
-    W w;
-    Item it;
-    it.b = begin_of[0];
-    it.hk = begin_of[1];
-    w.set(p, begin_request);
-    int64_t rest = begin_rest;
-    it.block = 0;
-    it.first = true;
-    it.flush = false;
-    it.chunk = 0;
-    int t = 0;
-    auto next_request = [&]() {
-      do {
-        if (++it.b >= p.ix.batch) return false;
-        w.set(p, observed_of(p, it.b));
-      } while (w.units == 0);
-      return true;
-    };
-    if (PASS != 2) {
-      int all = w.steps_of(p, 0);
-      while (rest >= all + kStart) {
-        rest -= all + kStart;
-        all = w.steps_of(p, ++it.block);
+  // Calls fn(request's numbers, item) for every item of the run
+  auto items = [&](bool one, auto&& fn) {      // one: of a warp that is one thread
+    for (uint32_t i = 0;; ++i) {
+      bool there = mbar_wait(&r_full[i % kItems], (i / kItems) & 1, &fail_flag);
+      if (!one) there = __all_sync(0xffffffffu, there);
+      if (!there) {
+        fail_flag = 1;
+        return;
       }
-      t = static_cast<int>(rest);
-      while (true) {
-        const int n = static_cast<int>(min(static_cast<int64_t>(all - t), end - pos));
-        if (n > 0) {
-          it.t0 = t;
-          it.n = n;
-          it.load = it.release = true;
-          it.at = pos - t;
-          if (!fn(w, it)) return;
-          pos += n;
-          t += n;
-        }
-        if (pos >= end) return;
-        pos += all + kStart - t;
-        if (pos >= end) return;
-        it.first = false;
-        t = 0;
-        if (++it.block == w.units) {
-          it.block = 0;
-          if (++it.hk == p.hkv) {
-            it.hk = 0;
-            if (!next_request()) return;
-          }
-        }
-        all = w.steps_of(p, it.block);
-      }
-    } else {
-      // the first step that begins at or behind the run's begin
-      int64_t at1 = begin_at1, unit1 = begin_unit1;        // of the request on the first pass's line
-      const int all = w.common(p);
-      const int64_t level = static_cast<int64_t>(all) * w.blocks;
-      if (rest <= level && level < (1ll << 31)) {
-        t = w.blocks == 1 ? static_cast<int>(rest) : static_cast<int>((static_cast<uint32_t>(rest) + w.blocks - 1) / w.blocks);
-        pos += static_cast<int64_t>(t) * w.blocks - rest;
-      } else {
-        const bool behind = rest > level;
-        t = behind ? all : 0;
-        int64_t x = behind ? level : 0;
-        while (x < rest) x += w.blocks - w.first_block(p, t++);
-        pos += x - rest;
-      }
-      int loaded = -1;        // the block whose queries are there
-      while (pos < end) {
-        const int steps = w.steps();
-        if (t >= steps) {
-          t = 0;
-          loaded = -1;
-          if (++it.hk == p.hkv) {
-            it.hk = 0;
-            at1 += unit1 * p.hkv;
-            if (!next_request()) return;
-            unit1 = w.cost1(p);
-          }
-          continue;
-        }
-        int n = 0;
-        while (n < kChunk && t + n < steps && pos < end) pos += w.blocks - w.first_block(p, t + n++);
-        it.t0 = t;
-        it.chunk = n;
-        it.block = w.first_block(p, t);
-        int64_t off = 0;
-        for (int i = 0; i < it.block; ++i) off += w.steps1(p, i) + kStart;
-        for (; it.block < w.blocks; ++it.block) {
-          const int mine = w.steps1(p, it.block);
-          it.n = min(n, mine - t);
-          it.load = loaded != it.block;
-          it.flush = it.block == w.blocks - 1;
-          it.release = !it.flush || t + n >= steps || pos >= end || w.first_block(p, t + n) != it.block;
-          it.at = at1 + it.hk * unit1 + off;
-          loaded = it.block;
-          if (!fn(w, it)) return;
-          off += mine + kStart;
-        }
-        t += n;
-      }
+      const Record& r = records[i % kItems];
+      const Item now = r.it;
+      if (now.n == 0) return;
+      W v;
+      v.set(p, r.o);
+      if (!fn(v, now)) return;
+      if (!one) __syncwarp();
+      if (one || lane == 0) mbar_arrive(&r_free[i % kItems]);
     }
   };
 
@@ -569,7 +476,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
     int c0, c1, second;       // the first CTA has the block in its second place
   };
   auto parts_of = [&](int64_t at, int n) {
-    const int64_t line = line_of[2];
+    const int64_t line = line_of[0];
     Parts x;
     x.c0 = owner_of(line, at, used_of);
     x.c1 = owner_of(line, at + n - 1, used_of);
@@ -652,7 +559,123 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
 
   if (warp >= kCompute) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-    if (warp < C::kBlockWarp) {
+    if (warp == C::kWalkWarp) {
+      // =============================== the run ===============================
+      if (walks) {
+        uint32_t count = 0;
+        bool ok = true;
+        auto put = [&]() {
+          const uint32_t place = count % kItems;
+          if (count >= kItems && !mbar_wait(&r_free[place], (count / kItems - 1) & 1, &fail_flag)) ok = false;
+          if (!ok) return false;
+          records[place].o = w.o;
+          records[place].it = it;
+          mbar_arrive(&r_full[place]);
+          ++count;
+          return true;
+        };
+        auto next_request = [&]() {
+          do {
+            if (++it.b >= p.ix.batch) return false;
+            w.set(p, observed_of(p, it.b));
+          } while (w.units == 0);
+          return true;
+        };
+        auto walk = [&]() {
+          if (!aligned || pos >= end) return;
+          it.first = true;
+          int t = 0;
+          if (PASS != 2) {
+            int all = w.steps_of(p, 0);
+            while (rest >= all + kStart) {
+              rest -= all + kStart;
+              all = w.steps_of(p, ++it.block);
+            }
+            t = static_cast<int>(rest);
+            while (true) {
+              const int n = static_cast<int>(min(static_cast<int64_t>(all - t), end - pos));
+              if (n > 0) {
+                it.t0 = t;
+                it.n = n;
+                it.load = it.release = true;
+                it.at = pos - t;
+                it.at1 = at1 + it.hk * unit1;
+                if (!put()) return;
+                pos += n;
+                t += n;
+              }
+              if (pos >= end) return;
+              pos += all + kStart - t;
+              if (pos >= end) return;
+              it.first = false;
+              t = 0;
+              if (++it.block == w.units) {
+                it.block = 0;
+                if (++it.hk == p.hkv) {
+                  it.hk = 0;
+                  at1 += unit1 * p.hkv;
+                  if (!next_request()) return;
+                  if (PASS == 3) unit1 = w.cost1(p);
+                }
+              }
+              all = w.steps_of(p, it.block);
+            }
+          } else {
+            // the first step that begins at or behind the run's begin
+            const int all = w.common(p);
+            const int64_t level = static_cast<int64_t>(all) * w.blocks;
+            if (rest <= level && level < (1ll << 31)) {
+              t = w.blocks == 1 ? static_cast<int>(rest) : static_cast<int>((static_cast<uint32_t>(rest) + w.blocks - 1) / w.blocks);
+              pos += static_cast<int64_t>(t) * w.blocks - rest;
+            } else {
+              const bool behind = rest > level;
+              t = behind ? all : 0;
+              int64_t x = behind ? level : 0;
+              while (x < rest) x += w.blocks - w.first_block(p, t++);
+              pos += x - rest;
+            }
+            int loaded = -1;        // the block whose queries are there
+            while (pos < end) {
+              const int steps = w.steps();
+              if (t >= steps) {
+                t = 0;
+                loaded = -1;
+                if (++it.hk == p.hkv) {
+                  it.hk = 0;
+                  at1 += unit1 * p.hkv;
+                  if (!next_request()) return;
+                  unit1 = w.cost1(p);
+                }
+                continue;
+              }
+              int n = 0;
+              while (n < kChunk && t + n < steps && pos < end) pos += w.blocks - w.first_block(p, t + n++);
+              it.t0 = t;
+              it.chunk = n;
+              it.block = w.first_block(p, t);
+              int64_t off = 0;
+              for (int i = 0; i < it.block; ++i) off += w.steps1(p, i) + kStart;
+              for (; it.block < w.blocks; ++it.block) {
+                const int mine = w.steps1(p, it.block);
+                it.n = min(n, mine - t);
+                it.load = loaded != it.block;
+                it.flush = it.block == w.blocks - 1;
+                it.release = !it.flush || t + n >= steps || pos >= end || w.first_block(p, t + n) != it.block;
+                it.at = at1 + it.hk * unit1 + off;
+                loaded = it.block;
+                if (!put()) return;
+                off += mine + kStart;
+              }
+              t += n;
+            }
+          }
+        };
+        walk();
+        it.n = 0;
+        if (ok) put();
+        if (!ok) fail_flag = 1;
+      }
+    } else if (warp < C::kWalkWarp) {
       // =============================== stages ===============================
       constexpr int kWarps = C::kCopying;
       const int me = warp - kCompute;
@@ -667,9 +690,9 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[place]);
       };
-      items([&](const W& w, const Item& it) {
+      if (me < kWarps) items(false, [&](const W& w, const Item& it) {
         const int stages = it.n * KT;
-        int i = me < kWarps ? (me + kWarps - static_cast<int>(stage0 % kWarps)) % kWarps : stages;
+        int i = (me + kWarps - static_cast<int>(stage0 % kWarps)) % kWarps;
         auto wait_free = [&](uint32_t n) {       // asleep in between: warps that poll take issue slots from the computing ones
           if (n >= kStages && !mbar_wait_relaxed(&empty[n % kStages], (n / kStages - 1) & 1, 20)) ok = false;
           return ok = __all_sync(0xffffffffu, ok);
@@ -678,15 +701,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           const int tile0 = w.first_tile(p, it.block) + it.t0;
           // the block of the first pass that a tile of rows lies in, and where it begins on that line
           int block = tile0 * kTileRows / C::kRows;
-          int64_t at = begin_at1;
-          {
-            W v;
-            for (int b = begin_of[0]; b < it.b; ++b) {
-              v.set(p, observed_of(p, b));
-              at += v.cost1(p) * p.hkv;
-            }
-            at += w.cost1(p) * it.hk;
-          }
+          int64_t at = it.at1;
           for (int b = 0; b < block; ++b) at += w.steps1(p, b) + kStart;
           for (; i < stages; i += kWarps) {
             const uint32_t n = stage0 + i;
@@ -763,7 +778,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
       // =============================== blocks behind the first ===============================
       bool bad = false, ok = true;
       uint32_t loads = 0;
-      items([&](const W& w, const Item& it) {
+      items(false, [&](const W& w, const Item& it) {
         if (!it.load) return true;
         if (loads > 0) {
           if (!mbar_wait_relaxed(b_free, (loads - 1) & 1)) ok = false;
@@ -785,7 +800,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
       const uint64_t b_desc = umma_desc_k_sw128(smem_u32(sBlock)), r_desc0 = umma_desc_k_sw128(smem_u32(ring));
       const uint32_t fmt = KV8 || std::is_same<T, __half>::value ? 0u : 1u;
       uint32_t stage = 0, step = 0, loads = 0;
-      items([&](const W& w, const Item& it) {
+      items(true, [&](const W& w, const Item& it) {
         if (it.load) {
           if (ok && !mbar_wait(loads == 0 ? b_first : b_full, loads == 0 ? 0 : (loads - 1) & 1, &fail_flag)) ok = false;
           ++loads;
@@ -846,12 +861,11 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
       tc_fence_after_sync();
       return ok;
     };
-    // A quarter's columns of this step, 32 at a time; behind the last the buffer is free.  use(first column, scores).  One copy of the code: what
-    // the warps run has to stay in the instruction caches.
+    // A quarter's columns of this step, 32 at a time; behind the last the buffer is free.  use(first column, scores).  Steps without masks and
+    // caps have a loop of their own: with the code for the others in between a step takes a third longer.
     auto columns = [&](int count, auto&& use) {
       const uint32_t from = tmem + lanes + (step & 1) * C::kCols + quarter * kWarpCols;
-#pragma unroll 1
-      for (int c = 0; c < kWarpCols; c += 32) {
+      auto some = [&](int c) {
         uint32_t raw[32];
         if (c < count) {
           tmem_ld_32x32(from + c, raw);
@@ -863,12 +877,11 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           if (lane == 0) mbar_arrive(&s_free[step & 1]);
         }
         if (c < count) use(c, raw);
-      }
+      };
+#pragma unroll
+      for (int c = 0; c < kWarpCols; c += 32) some(c);
     };
-    auto total = [&](const uint64_t (&sums)[4]) {
-      const float2 both = halves_of(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-      return both.x + both.y;
-    };
+    auto total = [&](const float (&sums)[4]) { return (sums[0] + sums[1]) + (sums[2] + sums[3]); };
     auto gaps = [&]() { return *const_cast<const volatile int*>(&holes) != 0; };
     auto slot_inside = [&](const W& w, int token) {
       const int s = token < w.o.len ? __ldcg(p.ix.req_to_token + static_cast<int64_t>(w.o.row) * p.ix.table_stride + token) : -1;
@@ -876,36 +889,37 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
     };
     // cap tanh(x / cap), in the log2 domain; tanh(y) = 1 - 2 / (1 + e^(2 y))
     auto cap = [&](uint32_t x, float mul) { return __float_as_uint(p.cap_out * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(x) * mul * p.cap_in)))); };
-    // What a token gets of 32 rows: of those from `low` up to `high` alone where masked
-    auto weights = [&](uint32_t (&raw)[32], const float* neg, const float* muls, bool masked, int low, int high, uint64_t (&sums)[4]) {
-      if (capped) {
+    // What a token gets of 32 rows; where masks or caps are, of those from `low` up to `high`
+    auto weights = [&](auto plain, uint32_t (&raw)[32], const float* neg, const float* muls, int low, int high, float (&sums)[4]) {
+      constexpr bool kPlain = decltype(plain)::value;
+      if (!kPlain && capped) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) raw[c] = cap(raw[c], kScaled ? muls[c] : p.scale_log2);
       }
-      const float same = capped ? 1.f : p.scale_log2;
-      if (masked) {
+      const float same = !kPlain && capped ? 1.f : p.scale_log2;
+      if (!kPlain) {
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
           const float e = ex2(fmaf(__uint_as_float(raw[c]), kScaled && !capped ? muls[c] : same, neg[c]));
           sum += c >= low && c < high ? e : 0.f;
         }
-        sums[0] = add2(sums[0], pair_of(sum, 0.f));
+        sums[0] += sum;
         return;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float4 n4 = *reinterpret_cast<const float4*>(neg + 4 * i);
         float4 m4 = make_float4(same, same, same, same);
-        if (kScaled && !capped) m4 = *reinterpret_cast<const float4*>(muls + 4 * i);
-        const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), pair_of(m4.x, m4.y), pair_of(n4.x, n4.y)));
-        const float2 y = halves_of(fma2(pair_of(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), pair_of(m4.z, m4.w), pair_of(n4.z, n4.w)));
-        sums[(2 * i) & 3] = add2(sums[(2 * i) & 3], pair_of(ex2(x.x), ex2(x.y)));
-        sums[(2 * i + 1) & 3] = add2(sums[(2 * i + 1) & 3], pair_of(ex2(y.x), ex2(y.y)));
+        if (kScaled) m4 = *reinterpret_cast<const float4*>(muls + 4 * i);
+        sums[0] += ex2(fmaf(__uint_as_float(raw[4 * i]), m4.x, n4.x));
+        sums[1] += ex2(fmaf(__uint_as_float(raw[4 * i + 1]), m4.y, n4.y));
+        sums[2] += ex2(fmaf(__uint_as_float(raw[4 * i + 2]), m4.z, n4.z));
+        sums[3] += ex2(fmaf(__uint_as_float(raw[4 * i + 3]), m4.w, n4.w));
       }
     };
 
-    items([&](const W& w, const Item& it) {
+    items(false, [&](const W& w, const Item& it) {
       const int least = w.least();
       if (it.load) {
         const int held = loads % kRing;
@@ -930,20 +944,20 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
         if constexpr (kScaled)
           if (valid) mul = row_mul[held][row];
         float m = -INFINITY;
-        uint64_t sums[4] = {0, 0, 0, 0};      // pairs of fp32
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
         for (int t = 0; t < it.n; ++t, ++step) {
           if (!wait_scores()) return false;
           const int key0 = (it.t0 + t) * C::kStepKeys + col0;
-          const bool rare = gaps(), plain = key0 + kWarpCols - 1 <= sure && !rare;
-          columns(any ? kWarpCols : 0, [&](int col, uint32_t (&raw)[32]) {
+          const bool rare = gaps(), plain = key0 + kWarpCols - 1 <= sure && !rare && !capped;
+          auto add_up = [&](auto tag, int col, uint32_t (&raw)[32]) {
+            constexpr bool kPlain = decltype(tag)::value;
             const int key = key0 + col;
-            float by = mul;
-            if (capped) {
-              by = 1.f;
+            const float by = !kPlain && capped ? 1.f : mul;
+            if (!kPlain && capped) {
 #pragma unroll
               for (int c = 0; c < 32; ++c) raw[c] = cap(raw[c], mul);
             }
-            if (!plain) {
+            if (!kPlain) {
               const int seen = place + 1 - key;          // columns in front
               uint32_t there = seen >= 32 ? 0xffffffffu : seen > 0 ? (1u << seen) - 1 : 0u;
               if (__any_sync(0xffffffffu, rare)) there &= __ballot_sync(0xffffffffu, slot_inside(w, key + lane));        // tokens whose slots lie outside the cache
@@ -962,23 +976,26 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
                 const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * by, m);
                 const float f = m == -INFINITY ? 1.f : ex2(m - top);      // 0, or no number, in front of the first
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sums[i] = fma2(sums[i], pair_of(f, f), 0);
+                for (int i = 0; i < 4; ++i) sums[i] *= f;
                 m = top;
                 raised = true;
               }
               const float neg = m == -INFINITY ? 0.f : -m;
-              const uint64_t by2 = pair_of(by, by), neg2 = pair_of(neg, neg);
-              uint64_t now[4] = {sums[0], sums[1], sums[2], sums[3]};
+              float now[4] = {sums[0], sums[1], sums[2], sums[3]};
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 x = halves_of(fma2(pair_of(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), by2, neg2));
-                now[i & 3] = add2(now[i & 3], pair_of(ex2(x.x), ex2(x.y)));
-              }
+              for (int c = 0; c < 32; ++c) now[c & 3] += ex2(fmaf(__uint_as_float(raw[c]), by, neg));
               raise = !raised && !(total(now) < kLargest);
               if (raise) continue;
 #pragma unroll
               for (int i = 0; i < 4; ++i) sums[i] = now[i];
               break;
+            }
+          };
+          columns(any ? kWarpCols : 0, [&](int col, uint32_t (&raw)[32]) {
+            if (__builtin_expect(plain, 1)) {
+              add_up(std::true_type(), col, raw);
+            } else {
+              add_up(std::false_type(), col, raw);
             }
           });
         }
@@ -1021,12 +1038,16 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           const int token = (it.t0 + t) * C::kStepKeys + kt * 128 + in_tile;
           // this token is seen by the block's rows from `low` on
           const int low = token > least ? static_cast<int>(min(static_cast<int64_t>(token - least) * g - row0, static_cast<int64_t>(C::kRows))) : 0;
-          const bool plain = (it.t0 + t + 1) * C::kStepKeys - 1 <= least;       // all rows see all of the step's tokens
-          uint64_t sums[4] = {0, 0, 0, 0};
+          // all rows see all of the step's tokens, and this warp's columns are rows
+          const bool plain = (it.t0 + t + 1) * C::kStepKeys - 1 <= least && (col0 >= rows || col0 + kWarpCols <= rows) && !capped;
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};
           if (!wait_scores()) return false;
           columns(rows - col0, [&](int at, uint32_t (&raw)[32]) {
-            const int col = col0 + at;
-            weights(raw, neg + at, muls + (kScaled ? at : 0), col + 32 > rows || !plain, low - col, rows - col, sums);
+            if (__builtin_expect(plain, 1)) {
+              weights(std::true_type(), raw, neg + at, muls + (kScaled ? at : 0), 0, 32, sums);
+            } else {
+              weights(std::false_type(), raw, neg + at, muls + (kScaled ? at : 0), low - col0 - at, rows - col0 - at, sums);
+            }
           });
           float sum = total(sums);
           if (gaps() && !slot_inside(w, token)) sum = 0.f;       // rare: a token whose slot lies outside the cache is not seen
@@ -1059,12 +1080,16 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
           // this token is seen by the rows from `low` on
           const int low = token > least ? static_cast<int>(min(static_cast<int64_t>(token - least) * g - r0, static_cast<int64_t>(128))) : 0;
           // all of the stage's rows see all of the block's tokens
-          const bool plain = static_cast<int64_t>((it.block + 1) * C::kRows - 1 - least) * g <= (tile0 + t) * kTileRows;
-          uint64_t sums[4] = {0, 0, 0, 0};
+          const bool plain = static_cast<int64_t>((it.block + 1) * C::kRows - 1 - least) * g <= (tile0 + t) * kTileRows && (rows <= 0 || rows >= kWarpCols) && !capped;
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};
+          const float* neg = neg_lse[place] + col0;
+          const float* muls = row_mul[place] + (kScaled ? col0 : 0);
           columns(any ? rows : 0, [&](int at, uint32_t (&raw)[32]) {
-            const float* neg = neg_lse[place] + col0 + at;
-            const float* muls = row_mul[place] + (kScaled ? col0 + at : 0);
-            weights(raw, neg, muls, at + 32 > rows || !plain, low - at, rows - at, sums);
+            if (__builtin_expect(plain, 1)) {
+              weights(std::true_type(), raw, neg + at, muls + (kScaled ? at : 0), 0, 32, sums);
+            } else {
+              weights(std::false_type(), raw, neg + at, muls + (kScaled ? at : 0), low - at, rows - at, sums);
+            }
           });
           all += total(sums);
         }
@@ -1088,7 +1113,7 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
         }
         // the unit's last step: it began in front of this run
         if (tid == 0 && !whole && it.t0 + it.n == steps) {
-          const int64_t line = line_of[3];
+          const int64_t line = line_of[1];
           const int used = used_ctas(p, line), c0 = owner_of(line, it.at, used);
           p.jobs[blockIdx.x] = make_int4(it.b, it.hk, it.block, c0 * 2 + (run_begin(line, c0, used) < it.at ? 1 : 0));
         }
