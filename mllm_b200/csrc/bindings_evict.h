@@ -145,7 +145,7 @@ void attention_prefill_weights(const Tensor& q, const Tensor& k_cache, const Ten
   check_sums(what, sums, 3, hkv, q);
   check_scores(what, scale, logit_cap, sink, q);
   CHECK_ARG(last >= 0 && last <= INT32_MAX, what, ": last must be 0 (all new tokens) or positive, not ", last);
-  CHECK_ARG(q.size(0) < (int64_t(1) << 31) && batch < 65536, what, ": too many rows or requests");
+  CHECK_ARG(q.size(0) * q.size(1) < (int64_t(1) << 31) && batch < 65536, what, ": too many rows or requests");
   check_ints(prefix_lens, batch, "prefix_lens", q);
   check_ints(q_start, batch, "q_start_loc", q);
   c10::cuda::CUDAGuard g(q.device());

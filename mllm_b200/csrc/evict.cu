@@ -138,10 +138,11 @@ int launch_cache_evict(const CacheEvictArgs& a, cudaStream_t s) {
   if (lists <= 0 || a.width <= 0) return 0;
   EvictParams p{};
   p.a = a;
-  // Pieces of a row: no more than a warp takes at once, and half as much down to 128 bytes while there are fewer warps than 12 per SM
+  // Pieces of a row: no more than a warp takes at once, and half as much down to 64 bytes while there are fewer warps than 12 per SM (28 layers
+  // of one request, 1200 tokens, 43 % kept: 34.1 us in pieces of 64, 36.3 of 128, some 57 of 256; 36 layers, 4 x 4000 tokens, whole rows, 231)
   p.pieces = 1;
   auto piece = [&] { return ((a.row_bytes + p.pieces - 1) / p.pieces + 15) / 16 * 16; };
-  while (piece() > 512 || (lists * 2 * p.pieces < 12 * a.num_sms && piece() >= 256)) p.pieces *= 2;
+  while (piece() > 512 || (lists * 2 * p.pieces < 12 * a.num_sms && piece() >= 128)) p.pieces *= 2;
   p.piece = piece();
   p.pieces = (a.row_bytes + p.piece - 1) / p.piece;
   while (16 << p.lanes_log2 < p.piece) ++p.lanes_log2;
