@@ -61,7 +61,7 @@ EXTENSIONS: Dict[str, Dict[str, List[str]]] = {
     },
     "mllm_b200_A": {
         "sources": ["bindings_latent.cpp", "runtime.cu", "latent.cu", "attention_tree.cu", "tree.cu", "tree_sample.cu",
-                    "weights_decode.cu", "weights_prompt.cu", "weights_prompt_fp16.cu", "cache_select.cu", "evict.cu"],
+                    "weights_decode.cu", "weights_prompt.cu", "weights_prompt_fp16.cu", "weights_prompt_short.cu", "cache_select.cu", "evict.cu"],
         "headers": _COMMON + ["bindings_tree.h", "tree.h", "tree.cuh", "bindings_evict.h", "evict.h", "evict.cuh", "weights_prompt.cuh"],
         "cuda": True,
     },

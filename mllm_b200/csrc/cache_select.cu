@@ -8,8 +8,10 @@
 // they are few enough every one is compared with every other.  Then a pass over the list, a stretch per warp, keeps what is above the k-th and
 // of its equals the first ones: counts first, then indices.
 //
-// What bounds it is instructions, some 30 per sum; eight neighbours are a thread's, so that scores are made in registers.  Lists that are too few for the SMs, or too long for a block's shared memory, are cut into slices for a cluster of up to 8
-// blocks, which add up histograms and counts through each other's shared memory.
+// What bounds it is instructions, 65 to 90 per sum (2304 lists of up to 8192 sums, a quarter kept, pool 7: 71 us, their bytes take 14);
+// eight neighbours are a thread's, so that scores are made in registers.  Lists that are too few for the SMs, or too long for a block's shared
+// memory, are cut into slices for a cluster of up to 8 blocks, which add up histograms and counts through each other's shared memory
+// (224 lists of 1200 sums: 6.2 us, most of it one wait behind the other).
 #include <algorithm>
 
 #include "common.cuh"

@@ -63,6 +63,8 @@ bool weights_prompt_covers(int head_dim, int group);
 int64_t weights_prompt_floats(const WeightsPromptArgs& args);
 int launch_weights_prompt(const WeightsPromptArgs& args, cudaStream_t s);
 int launch_weights_prompt_fp16(const WeightsPromptArgs& args, cudaStream_t s);
+constexpr int kShortPromptTokens = 256;      // what the kernel for short prompts has room for (weights_prompt_short.cu)
+int launch_weights_prompt_short(const WeightsPromptArgs& args, cudaStream_t s);
 
 // which tokens stay: the last ones, the first ones, the largest sums (cache_select.cu)
 struct CacheSelectArgs {

@@ -66,9 +66,10 @@ class RadixAttention(nn.Module):
             sums = sums[self.layer_id - fb.token_to_kv_pool.layer_offset]
             if self.sliding_window:
                 raise ValueError("a layer with a sliding window has no sums of attention weights: its old tokens are not looked at in any case")
+            table = fb.req_to_token_pool.req_to_token[:, :fb.max_seq_len or None]      # its width is what the kernels provide for
         if sums is not None and fb.forward_mode.is_decode():
-            ops.attention_decode_weights(q, k_cache, v_cache, fb.req_to_token_pool.req_to_token, fb.req_pool_indices, fb.seq_lens, self.scaling,
-                                         sums, decay=fb.weight_decay, out=out, logit_cap=self.logit_cap)
+            ops.attention_decode_weights(q, k_cache, v_cache, table, fb.req_pool_indices, fb.seq_lens, self.scaling, sums,
+                                         decay=fb.weight_decay, out=out, logit_cap=self.logit_cap)
         elif fb.forward_mode.is_decode():
             ops.attention_decode(q, k_cache, v_cache, fb.req_to_token_pool.req_to_token, fb.req_pool_indices,
                                  fb.seq_lens, self.scaling, out=out, max_seq_len=fb.max_seq_len,
@@ -78,9 +79,8 @@ class RadixAttention(nn.Module):
                                   fb.seq_lens, fb.extend_prefix_lens, fb.extend_start_loc, self.scaling, out=out,
                                   max_q_len=fb.max_extend_len, window=self.sliding_window, logit_cap=self.logit_cap)
             if sums is not None:
-                ops.attention_prefill_weights(q, k_cache, fb.req_to_token_pool.req_to_token, fb.req_pool_indices, fb.seq_lens,
-                                              fb.extend_prefix_lens, fb.extend_start_loc, self.scaling, sums, last=fb.weight_last,
-                                              add=fb.weight_add, logit_cap=self.logit_cap)
+                ops.attention_prefill_weights(q, k_cache, table, fb.req_pool_indices, fb.seq_lens, fb.extend_prefix_lens, fb.extend_start_loc,
+                                              self.scaling, sums, last=fb.weight_last, add=fb.weight_add, logit_cap=self.logit_cap)
         return out.view(T, self.num_heads * self.head_dim)
 
     def _forward_tree(self, qkv, q_norm_w, k_norm_w, fb, inv_freq, k_cache, v_cache) -> torch.Tensor:

@@ -228,9 +228,42 @@ def test_prompt_many_tiles(D, lens, new, last, hq, hkv):
     assert torch.equal(c["sums"], once)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("cache", [None, E4, E5])
+@pytest.mark.parametrize("room", [256, 257])
+@pytest.mark.parametrize("lens,new,last", [
+    ([1], [1], 1), ([17], [17], 16), ([130], [2], 8), ([127, 128, 129], [127, 128, 129], 32), ([1, 0, 64, 5], [1, 0, 10, 0], 64), ([256, 33], [200, 33], 20),
+    ([255, 31, 32, 33], [255, 31, 1, 30], 64), ([100] * 30, [100] * 30, 7),
+])
+def test_prompts_around_what_is_short(D, cache, room, lens, new, last):
+    """Tables of 256 tokens and a few rows have a kernel of their own; the same requests in larger tables do not."""
+    check_prompt(cached_batch(lens, 8, 2, D, cache=cache, seed=len(lens) + D, new=new, room=room), last=last)
+
+
+@pytest.mark.parametrize("room", [250, 1000])
+@pytest.mark.parametrize("hq,hkv,D,dtype,cache", [(1, 1, 128, torch.bfloat16, None), (5, 1, 64, torch.float16, None), (7, 7, 128, torch.bfloat16, E4),
+                                                  (32, 1, 128, torch.float16, E5), (12, 3, 256, torch.bfloat16, None), (17, 1, 64, torch.bfloat16, E5)])
+@pytest.mark.parametrize("kw", [dict(add=True), dict(cap=3.0), dict(sink=True), dict(cap=2.0, sink=True, add=True)])
+def test_short_prompts_options(room, hq, hkv, D, dtype, cache, kw):
+    c = cached_batch([200, 64, 1, 90], hq, hkv, D, dtype=dtype, cache=cache, seed=7, new=[100, 64, 1, 30], room=room)
+    kw = dict(kw)
+    check_prompt(c, sink=c["sink"] if kw.pop("sink", False) else None, last=8, **kw)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e30])
+@pytest.mark.parametrize("room", [200, 300])
+def test_prompt_queries_of_extreme_size_over_8_bit_caches(scale, room):
+    c = cached_batch([77, 150], 4, 2, 64, cache=E4, seed=14, new=[20, 30], room=room)
+    c["q"] = (c["q"].float() * scale).to(torch.bfloat16)
+    c["q"][3, 1] = 0
+    c["scale"] = c["scale"] / scale
+    check_prompt(c, last=10)
+
+
+@pytest.mark.parametrize("room", [None, 300])
 @pytest.mark.parametrize("where", ["slot", "row", "length", "rows of q", "prefix"])
-def test_prompt_numbers_outside(where):
-    c = cached_batch([200, 50], 4, 2, 128, seed=11, new=[60, 20])
+def test_prompt_numbers_outside(where, room):
+    c = cached_batch([200, 50], 4, 2, 128, seed=11, new=[60, 20], room=room)
     row, before = int(c["req"][0]), c["sums"].clone()
     if where == "slot":
         c["table"][row, 70] = c["k"].shape[0]
@@ -256,8 +289,9 @@ def test_prompt_numbers_outside(where):
         ops.check_status()
 
 
-def test_prompt_values_that_are_no_numbers():
-    c = cached_batch([100, 90, 64], 4, 2, 128, seed=12, new=[100, 20, 64])
+@pytest.mark.parametrize("room", [None, 300])
+def test_prompt_values_that_are_no_numbers(room):
+    c = cached_batch([100, 90, 64], 4, 2, 128, seed=12, new=[100, 20, 64], room=room)
     c["k"][0] = float("nan")                 # nobody's slot
     check_prompt(c, last=30)
     row = int(c["req"][0])
@@ -267,13 +301,17 @@ def test_prompt_values_that_are_no_numbers():
     ops.check_status()
     assert torch.isnan(c["sums"][row, 1, :100]).all() and not torch.isnan(c["sums"][row, 0]).any()
     assert not torch.isnan(c["sums"][[int(r) for r in c["req"][1:]]]).any()
-    c["q"][70:] = 0                          # those that see it are not looked at
     prompt(c, last=0)
-    assert torch.isnan(c["sums"][row, 1, 80])
+    assert torch.isnan(c["sums"][row, 1, :81]).all()
+    c["k"][slot, 1] = 0
+    c["q"][90, 2] = float("nan")             # a query: what stands behind it does not see it
+    prompt(c, last=12)
+    assert torch.isnan(c["sums"][row, 1, :91]).all() and not torch.isnan(c["sums"][row, 1, 91:]).any() and not torch.isnan(c["sums"][row, 0]).any()
 
 
-def test_prompt_queries_without_a_visible_score():
-    c = cached_batch([70], 4, 1, 64, seed=13, dtype=torch.float16, new=[70])
+@pytest.mark.parametrize("room", [None, 300])
+def test_prompt_queries_without_a_visible_score(room):
+    c = cached_batch([70], 4, 1, 64, seed=13, dtype=torch.float16, new=[70], room=room)
     c["q"][:] = c["q"].abs() + 0.1
     slots = c["table"][int(c["req"][0])].long()
     c["k"][slots[:10]] = float("-inf")       # the first ten queries see nothing
@@ -447,6 +485,27 @@ def test_sums_behind_2_31_elements():
     again, _ = ops.cache_select(small[None], c["req"], c["seq"], i32([90]), 90)
     ops.check_status()
     assert torch.equal(keep, again) and int(counts) == 90
+
+
+@pytest.mark.parametrize("room", [32, 300])
+def test_the_most_requests(room):
+    n, dev = 65535, "cuda"
+    table = torch.zeros((n, room), dtype=torch.int32, device=dev)
+    table[:, 0] = torch.arange(n, device=dev, dtype=torch.int32) % 999
+    k = torch.randn((2, 999, 64), device=dev).to(torch.bfloat16).transpose(0, 1)
+    q = torch.randn((n, 6, 64), device=dev).to(torch.bfloat16)
+    ints = torch.arange(n, device=dev, dtype=torch.int32)
+    one, none = torch.ones_like(ints), torch.zeros_like(ints)
+    sums = torch.zeros((n, 2, room), device=dev)
+    ops.attention_prefill_weights(q, k, table, ints.flip(0).contiguous(), one, none, ints, 0.125, sums, last=1)
+    ops.check_status()
+    assert (sums[:, :, 0] - 3).abs().max() < 1e-5 and (sums[:, :, 1:] == 0).all()
+    ops.attention_decode_weights(q, k, k, table, ints, one, 0.125, sums)
+    ops.check_status()
+    assert (sums[:, :, 0] - 3).abs().max() < 1e-5 and (sums[:, :, 1:] == 0).all()
+    more = torch.zeros(70000, dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError, match="too many"):
+        ops.attention_prefill_weights(q, k, table, more, more, more, more, 0.125, sums, last=1)
 
 
 def round_of(c, p, one, sums, budgets, width):
