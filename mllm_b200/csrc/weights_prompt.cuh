@@ -75,7 +75,7 @@ __device__ __forceinline__ Observed observed_of(const PromptParams& p, int b) {
   o.row = c.row;
   o.bad = c.bad;
   o.prefix = __ldcg(p.prefix_lens + b);
-  const int start = __ldcg(p.q_start + b), n = c.len - o.prefix;
+  const int start = __ldcg(p.q_start + b), n = o.prefix >= 0 ? c.len - o.prefix : 1;
   o.look = c.len > 0 && o.prefix < c.len ? (p.last > 0 ? min(p.last, n) : n) : 0;
   if (o.look > 0 && (o.prefix < 0 || start < 0 || n > p.rows - start)) {
     o.bad = true;

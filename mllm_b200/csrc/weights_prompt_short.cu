@@ -49,15 +49,12 @@ __global__ void __launch_bounds__(kThreads) weights_short_kernel(const ShortPara
   pdl_wait();
   pdl_launch_dependents();
   const Cached c = cached_of(a.index, b);
-  const int prefix = __ldcg(a.prefix_lens + b), start = __ldcg(a.q_start + b), fresh = c.len - prefix;
-  bool bad = c.bad;
-  int look = c.len > 0 && prefix < c.len ? (a.last > 0 ? min(a.last, fresh) : fresh) : 0;
-  if (look > 0 && (prefix < 0 || start < 0 || fresh > a.rows - start)) {
-    bad = true;
-    look = 0;
-  }
+  const int prefix = __ldcg(a.prefix_lens + b), start = __ldcg(a.q_start + b), fresh = prefix >= 0 ? c.len - prefix : 0;
+  const bool any = c.len > 0 && prefix < c.len;       // new rows, and whether they are there
+  const bool bad = c.bad || (any && (prefix < 0 || start < 0 || fresh > a.rows - start));
   if (bad && tid == 0 && hk == 0 && a.index.status != nullptr) atomicExch(a.index.status, kStatusBadIndex);
-  if (look == 0) return;
+  if (bad || !any) return;
+  const int look = a.last > 0 ? min(a.last, fresh) : fresh;
   const int len = c.len, rows = look * g, first = start + fresh - look;
 
   // ---- keys: a thread looks up a token's slot, a warp copies its 32 rows ----

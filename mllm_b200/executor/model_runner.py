@@ -607,6 +607,8 @@ class ModelRunner:
             return
         if not getattr(self.model, "draft_trees", False):        # every layer that mixes tokens is a RadixAttention
             raise ValueError(f"{type(self.model).__name__} does not add up attention weights")
+        if extra.get("tree_parents") is not None:
+            raise ValueError("drafted token trees do not add up attention weights")
         if any(getattr(m, "sliding_window", None) for m in self.model.modules()):
             raise ValueError("layers with a sliding window do not add up attention weights")
         group = self.num_attention_heads // self.num_kv_heads

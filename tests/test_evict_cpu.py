@@ -145,6 +145,8 @@ def test_models_with_other_layers_keep_no_sums():
     s = Shortened("qwen3-tiny", "cpu", "float32")
     with pytest.raises(ValueError, match="layers"):
         s.mr.prepare_forward_batch_decode(one.long(), one, one + 1, one.long(), weight_sums=torch.zeros(1, 1, 1, 1))
+    with pytest.raises(ValueError, match="trees"):
+        s.mr.prepare_forward_batch_tree(one.long(), one - 1, one, [1], [0], weight_sums=s.mr.token_to_kv_pool.make_weight_sums(2, 8))
     for m in s.mr.model.modules():
         if hasattr(m, "sliding_window"):
             m.sliding_window = 16

@@ -261,7 +261,7 @@ def test_prompt_queries_of_extreme_size_over_8_bit_caches(scale, room):
 
 
 @pytest.mark.parametrize("room", [None, 300])
-@pytest.mark.parametrize("where", ["slot", "row", "length", "rows of q", "prefix"])
+@pytest.mark.parametrize("where", ["slot", "row", "length", "rows of q", "prefix", "lowest prefix"])
 def test_prompt_numbers_outside(where, room):
     c = cached_batch([200, 50], 4, 2, 128, seed=11, new=[60, 20], room=room)
     row, before = int(c["req"][0]), c["sums"].clone()
@@ -274,7 +274,7 @@ def test_prompt_numbers_outside(where, room):
     elif where == "rows of q":
         c["start"][0] = 30
     else:
-        c["prefix"][0] = -1
+        c["prefix"][0] = -1 if where == "prefix" else -2 ** 31
     if where != "slot":
         c["new"][0] = 0
         q = c["q"]
