@@ -20,6 +20,10 @@
 //   * Weights are rounded to 16 bits for the product with the values, and the output's normaliser sums the rounded ones, as in plain
 //     decode attention.  The sums of weights have a normaliser of their own from the unrounded ones: a rounded weight that carries most of a
 //     row would be off by 2^-9.
+//
+// What bounds it: memory while the first kernel streams, a start of some 6 us, and what shows of the second kernel (29 requests of about 1900
+// tokens, 32 / 8 heads of 128, fp16: 55.8 us for 229 MB, where the bytes take 35; two chains of products per score save 0.5 us).  8-bit rows
+// are bound by the warps' instructions, widening first of all (32 requests of about 4096, 32 / 4 heads of 128, e4m3: 53.4 us, the bytes take 21).
 #include <algorithm>
 
 #include "common.cuh"
@@ -331,13 +335,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT, FMT>::kPerSm) weights_de
         for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
       const int row = lane & 15;
       if constexpr (FMT == kKvSame) {
+        float s2[4] = {0.f, 0.f, 0.f, 0.f};       // every other product, where the heads make only one chain of them
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           uint32_t a[4];
           ldsm4(a, sk + C::at(row, kk * 2 + (lane >> 4)));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<M>(s[nt], a[0], a[1], a[2], a[3], qf[kk][nt][0], qf[kk][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816<M>(NT == 1 && (kk & 1) ? s2 : s[nt], a[0], a[1], a[2], a[3], qf[kk][nt][0], qf[kk][nt][1]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[0][i] += s2[i];
       } else {
 #pragma unroll
         for (int k2 = 0; k2 < HD / 32; ++k2) {
@@ -778,11 +785,14 @@ int launch_weights_decode(const WeightsDecodeArgs& a, cudaStream_t s) {
   p.group = a.hq / a.hkv;
   p.hkv = a.hkv;
   p.ctas = stream_ctas(a);
-  p.weight_ctas = 8 * a.num_sms;
   // a CTA joins several heads where there are more heads than two per SM
   const int64_t heads = static_cast<int64_t>(a.index.batch) * a.hq;
   p.join_heads = static_cast<int>(std::min<int64_t>(p.group, std::max<int64_t>(1, heads / (2 * a.num_sms))));
   p.joins = (p.group + p.join_heads - 1) / p.join_heads;
+  // No more CTAs than run at once, 9 on an SM, as long as that leaves a few for the weights (29 x 1900, 32 / 8 heads: 8 an SM for the weights
+  // 58.4 us, 6 and 4 56.6; 32 x 4096, 32 / 4 heads, e4m3: 8, 6, 4 an SM 57.4, 53.4, 55.2)
+  const int64_t joining = static_cast<int64_t>(p.joins) * p.hkv * a.index.batch;
+  p.weight_ctas = static_cast<int>(std::min<int64_t>(6 * a.num_sms, std::max<int64_t>(4 * a.num_sms, 9 * a.num_sms - joining)));
   const int64_t parts = static_cast<int64_t>(p.ctas) * 2 * p.group;
   p.part_o = a.workspace;
   p.part_lse = reinterpret_cast<float2*>(a.workspace + parts * a.head_dim);
