@@ -110,9 +110,8 @@ def attention_prefill_weights(q, k_cache, req_to_token, req_pool_indices, seq_le
     (call it behind the prologue; the attention itself is that function's).  Of request b's ``n = seq_lens[b] - prefix_lens[b]`` new rows, from
     ``q_start_loc[b]`` on, the last ``last`` are observed, all of them where that is 0 or more than n.  Every cached token's sum becomes what the
     observed queries behind it and at it give it, all heads of a group; with ``add``, tokens in front of the new ones (index below
-    ``prefix_lens[b]``) keep what they have and get that on top.  A request without new rows is left as it is; no row of ``q`` is two requests'.  Sizes and types as for
-    :func:`attention_decode_weights`; a group has up to 32 heads at each of them, a batch up to 65535
-    requests."""
+    ``prefix_lens[b]``) keep what they have and get that on top.  A request without new rows is left as it is; no row of ``q`` is two requests'.
+    Sizes and types as for :func:`attention_decode_weights`; a group has up to 32 heads at each of them, a batch up to 65535 requests."""
     ops = _ops()
     if ops.use_kernels(q):          # the binding makes the same checks
         return ops.ext().attention_prefill_weights(q, k_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, float(scale), sums,
