@@ -407,6 +407,17 @@ def test_evict(lens, part, D, cache, page):
     assert torch.equal(c["store"].view(torch.uint8), store.view(torch.uint8)) and torch.equal(c["sums"], sums)
 
 
+@pytest.mark.parametrize("layers,D", [(20, 128), (40, 64), (40, 256), (120, 128)])
+def test_evict_many_lists(layers, D):
+    """With more lists rows are moved in larger pieces and shorter runs."""
+    c = cached_batch([1, 70, 300, 129], 2, 2, D, seed=layers, layers=layers)
+    keep, counts = ops.cache_select(c["sums"], c["req"], c["seq"], i32([1, 69, 170, 64]), 170, first=2, recent=5)
+    store, sums = moved(c, keep, counts)
+    ops.cache_evict(c["store"], c["sums"], c["table"], c["req"], keep, counts)
+    ops.check_status()
+    assert torch.equal(c["store"], store) and torch.equal(c["sums"], sums)
+
+
 def test_evict_rows_that_are_read_where_others_are_written():
     """The token dropped stands in front: every row moves by one.  And rows that are kept more than once."""
     c = cached_batch([3000], 1, 1, 128, seed=1, layers=1)
