@@ -686,7 +686,8 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
       const int me = warp - kCompute;
       bool bad = false, ok = true;
       uint32_t stage0 = 0;                               // stages of the items before
-      // A stage may be on its way while the one before is waited for, unless its place waits for that one's products
+      // A stage may be on its way while the one before is waited for, unless its place waits for that one's products.  None outlives its item:
+      // the next record may wait for this item's scores, and those wait for every stage.
       constexpr bool kTwo = !KV8 && kStages > kWarps;
       int pending = -1;                                  // the place of a stage that has not been waited for
       auto arrived = [&](int place) {
@@ -771,12 +772,17 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R, PASS>::kThreads, 1)
               arrived(n % kStages);
             }
           }
+          if (pending >= 0) {
+            cp_wait_all();
+            arrived(pending);
+            pending = -1;
+          }
         }
         stage0 += stages;
         return true;
       });
       cp_wait_all();
-      if (pending >= 0) arrived(pending);
+      if (pending >= 0) arrived(pending);       // of an item that was given up
       if (!ok) fail_flag = 1;
       if (bad && p.ix.status != nullptr) atomicExch(p.ix.status, kStatusBadIndex);
     } else if (warp == C::kBlockWarp) {
