@@ -624,7 +624,8 @@ class ModelRunner:
         ``recent`` tokens, the first ``first`` and those with the largest sums (:func:`ops.cache_select`).  ``weight_sums`` come from
         ``token_to_kv_pool.make_weight_sums(rows of the request table, tokens)`` and grow in the batches that are made with them
         (``weight_sums=``, and ``weight_last=``, ``weight_add=`` for prompts, ``weight_decay=`` for decode steps).  Returns the requests' new lengths, int32
-        on the device: their slots behind those are free to be given back, and their next tokens' positions go on from what they were
+        on the device.  Whole pages behind those are free: ``token_to_kv_pool_allocator.free_behind(slots, length)`` gives them back (``free`` takes
+        the page of every slot it is given, also one with kept tokens).  The next tokens' positions go on from what they were
         (``positions=``, ``first_positions_cpu=``).  Requests whose slots others share, the prefix cache's among them, cannot be shortened."""
         keep, counts = ops.cache_select(weight_sums, req_pool_indices.to(torch.int32).contiguous(), seq_lens.to(torch.int32).contiguous(),
                                         budgets.to(torch.int32).contiguous(), max_budget, first=first, recent=recent, pool=pool)

@@ -279,6 +279,20 @@ class TokenToKVPoolAllocator:
         else:
             self._released.append(pages)
 
+    def free_behind(self, slots, kept: int) -> int:
+        """Gives back what a shortened request does not need: of ``slots``, its slots in the order of its tokens, the first ``kept`` stay, and
+        so does every page that one of them lies in.  Returns how many of the leading slots are the request's still; those behind
+        ``kept`` are for its next tokens."""
+        if isinstance(slots, torch.Tensor):
+            slots = slots.detach().to("cpu", torch.int64).numpy()
+        slots, kept = np.asarray(slots, dtype=np.int64).reshape(-1), int(kept)
+        if not 0 <= kept <= slots.size:
+            raise ValueError(f"a request of {slots.size} slots cannot keep {kept}")
+        pages = slots // self.page_size
+        gone = ~np.isin(pages, pages[:kept])
+        self.free(slots[gone])
+        return int(np.argmax(gone)) if gone.any() else int(slots.size)
+
     # batched frees: collect, then release once
     def free_group_begin(self) -> None:
         self._groups = []

@@ -156,7 +156,8 @@ def cache_evict(store, sums, req_to_token, req_pool_indices, keep, counts) -> No
     """Moves what stays to the front, in place: for i below ``counts[b]``, what the token at cache index ``keep[layer, b, head, i]`` has in ``store``
     [layers, 2, Hkv, slots, features] (contiguous; :class:`mllm_b200.mem_cache.memory_pool.KVPool`'s storage) and in ``sums`` [layers, rows, Hkv,
     tokens] (or None) goes to index i.  ``keep`` and ``counts`` are those of :func:`cache_select`; no index may be smaller than its place, and none
-    is read behind ``counts``.  The request then has ``counts[b]`` tokens, and its slots from there on are free."""
+    is read behind ``counts``.  The request then has ``counts[b]`` tokens, and nothing is kept in its slots from there on (a paged allocator takes
+    pages back: :meth:`mllm_b200.mem_cache.memory_pool.TokenToKVPoolAllocator.free_behind`)."""
     ops = _ops()
     if ops.use_kernels(store):      # the binding makes the same checks
         return ops.ext().cache_evict(store, sums, req_to_token, req_pool_indices, keep, counts)
