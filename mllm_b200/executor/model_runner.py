@@ -145,6 +145,7 @@ class ModelRunner:
         self.quantization_method = quantization_method
         self.kv_cache_dtype_name = kv_cache_dtype
         self.model = None
+        self._window_modules: Optional[list] = None       # see _layers_with_a_window
         self.quant_config = None
         self.req_to_token_pool: Optional[ReqToTokenPool] = None
         self.token_to_kv_pool: Optional[KVPool] = None
@@ -383,6 +384,7 @@ class ModelRunner:
         try:
             with torch.device(self.device):
                 self.model = model_cls(self.hf_config, quant_config=self.quant_config, params_dtype=self.dtype)
+            self._window_modules = None
         finally:
             torch.set_default_dtype(prev)
         if load_format == "dummy" or is_preset:
@@ -531,11 +533,11 @@ class ModelRunner:
         """Batch of new tokens (after optional cached prefixes). Passing the ``*_cpu`` lists avoids
         a device->host sync.  ``first_positions_cpu``: position of each request's first new token where it is not the number of
         cached ones (requests that were shortened).  ``weight_sums`` and what belongs to it: see :meth:`evict_cache`."""
-        self._check_weight_sums(extra)
         if extend_seq_lens_cpu is None:
             extend_seq_lens_cpu = extend_seq_lens.tolist()
         if extend_prefix_lens_cpu is None:
             extend_prefix_lens_cpu = extend_prefix_lens.tolist()
+        self._check_weight_sums(extra, max((n + p for n, p in zip(extend_seq_lens_cpu, extend_prefix_lens_cpu)), default=0))
         bs = len(extend_seq_lens_cpu)
         starts, pos_parts, acc = [], [], 0
         for n, p in zip(extend_seq_lens_cpu, first_positions_cpu if first_positions_cpu is not None else extend_prefix_lens_cpu):
@@ -563,8 +565,9 @@ class ModelRunner:
         out_cache_loc: torch.Tensor, max_seq_len: Optional[int] = None, positions: Optional[torch.Tensor] = None, **extra,
     ) -> ForwardBatch:
         """One new token per request; ``seq_lens`` already counts it. No host sync.  ``positions``: where they are not
-        ``seq_lens - 1`` (requests that were shortened).  ``weight_sums``, ``weight_decay``: see :meth:`evict_cache`."""
-        self._check_weight_sums(extra)
+        ``seq_lens - 1`` (requests that were shortened).  ``weight_sums``, ``weight_decay``: see :meth:`evict_cache`; with them
+        ``max_seq_len``, which no request may pass, is what the kernels provide for, and the sums have to be that wide."""
+        self._check_weight_sums(extra, int(max_seq_len if max_seq_len is not None else self.context_len))
         bs = input_ids.shape[0]
         return ForwardBatch(
             forward_mode=ForwardMode.DECODE, batch_size=bs, input_ids=input_ids,
@@ -601,7 +604,8 @@ class ModelRunner:
         return self.prepare_forward_batch_extend(input_ids, req_pool_indices, tree + prefix, tree, prefix, loc, list(tree_lens_cpu),
                                                  list(prefix_lens_cpu), tree_parents=parents.to(torch.int32).contiguous(), logit_rows=rows, **extra)
 
-    def _check_weight_sums(self, extra: dict) -> None:
+    def _check_weight_sums(self, extra: dict, longest: int) -> None:
+        """``longest``: no request of the batch has more tokens, the new ones included."""
         sums = extra.get("weight_sums")
         if sums is None:
             return
@@ -609,14 +613,24 @@ class ModelRunner:
             raise ValueError(f"{type(self.model).__name__} does not add up attention weights")
         if extra.get("tree_parents") is not None:
             raise ValueError("drafted token trees do not add up attention weights")
-        if any(getattr(m, "sliding_window", None) for m in self.model.modules()):
+        if any(getattr(m, "sliding_window", None) for m in self._layers_with_a_window()):
             raise ValueError("layers with a sliding window do not add up attention weights")
         group = self.num_attention_heads // self.num_kv_heads
         if sums.is_cuda and ops.use_kernels(sums) and not ops.cache_weights_cover(self.head_dim, group, self.kv_cache_dtype, self.dtype):
             raise ValueError(f"attention weights are added up for heads of 64, 128 or 256 features in 16 bits, over caches of their type or of 8-bit floats; "
                              f"here are {self.head_dim} features in {self.dtype} over {self.kv_cache_dtype}")
-        if sums.dim() != 4 or sums.shape[0] != self.token_to_kv_pool.layer_num:
-            raise ValueError(f"sums of attention weights are [{self.token_to_kv_pool.layer_num} layers, rows, heads, tokens]")
+        layers, rows, heads = self.token_to_kv_pool.layer_num, self.req_to_token_pool.req_to_token.shape[0], self.token_to_kv_pool.kv_heads
+        if sums.dim() != 4 or sums.shape[0] != layers or sums.shape[1] < rows or sums.shape[2] != heads:
+            raise ValueError(f"sums of attention weights are [{layers} layers, {rows} rows of the request table, {heads} heads, tokens], not {list(sums.shape)}")
+        if sums.shape[3] < longest:      # the kernels take a request that the sums have no room for as one without tokens
+            raise ValueError(f"sums of attention weights for {sums.shape[3]} tokens, and requests of up to {longest} (max_seq_len=; the context's where "
+                             "it is not given)")
+
+    def _layers_with_a_window(self) -> list:
+        """Modules that may have a sliding window, looked up once: batches are made in every step."""
+        if self._window_modules is None:
+            self._window_modules = [m for m in self.model.modules() if hasattr(m, "sliding_window")]
+        return self._window_modules
 
     def evict_cache(self, weight_sums: torch.Tensor, req_pool_indices: torch.Tensor, seq_lens: torch.Tensor, budgets: torch.Tensor, max_budget: int,
                     first: int = 4, recent: int = 32, pool: int = 1) -> torch.Tensor:
@@ -667,7 +681,7 @@ class ModelRunner:
 
     def shutdown(self) -> None:
         self.cuda_graph_runner = None
-        self.model = None
+        self.model = self._window_modules = None
         self.token_to_kv_pool = None
         self.req_to_token_pool = None
         if self.device.type == "cuda":
