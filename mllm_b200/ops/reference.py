@@ -1092,7 +1092,8 @@ def tree_speculative_sample(logits, tokens, parents, tree_lens, q_start_loc, tem
 
 
 def _cached_weights(q, k_cache, slots, place, scale: float, logit_cap: float, sink) -> torch.Tensor:
-    """[W, Hq, L] softmax weights of queries ``q`` [W, Hq, D] at cache indices ``place`` over the cached tokens ``slots`` up to theirs."""
+    """[W, Hq, L] softmax weights of queries ``q`` [W, Hq, D] at cache indices ``place`` over the cached tokens ``slots`` up to theirs; of a query whose
+    scores are all minus infinity 0."""
     hkv, work = k_cache.shape[1], torch.float64 if q.dtype == torch.float64 else torch.float32
     keys = k_cache[slots].to(work)
     s = torch.einsum("wkgd,lkd->wkgl", q.to(work).view(q.shape[0], hkv, -1, q.shape[2]), keys).reshape(q.shape[0], q.shape[1], -1) * scale
@@ -1101,7 +1102,8 @@ def _cached_weights(q, k_cache, slots, place, scale: float, logit_cap: float, si
     s = s.masked_fill(torch.arange(slots.numel(), device=q.device) > place[:, None, None], float("-inf"))
     if sink is not None:
         s = torch.cat([s, sink.to(work).view(1, -1, 1).expand(s.shape[0], -1, 1)], dim=-1)
-    return torch.softmax(s, dim=-1)[..., :slots.numel()]
+    nothing = s.amax(-1, keepdim=True) == float("-inf")
+    return torch.softmax(s.masked_fill(nothing, 0.0), dim=-1).masked_fill(nothing, 0.0)[..., :slots.numel()]
 
 
 def attention_decode_weights(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, scale: float, sums, decay=1.0, out=None, logit_cap=0.0,
