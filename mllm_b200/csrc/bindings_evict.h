@@ -1,7 +1,10 @@
 // PyTorch binding of the kernels that shorten requests in the paged cache, part of the module of latent attention.
 #pragma once
 
+#include <algorithm>
 #include <cfloat>
+#include <utility>
+#include <vector>
 
 #include "bindings_common.h"
 #include "bindings_tree.h"      // CHECK_ARG
@@ -53,6 +56,27 @@ void check_sums(const char* what, const Tensor& sums, int64_t dims, int64_t head
             what, ": sums must be fp32 [", dims == 4 ? "layers, " : "", "requests, ", heads, ", tokens] with unit inner stride on ", like.device());
 }
 
+// Whether no element of a tensor that is written lies where another does (an expanded tensor's do)
+bool apart(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;       // stride, size
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) == 0) return true;
+    if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+  }
+  std::sort(dims.begin(), dims.end());
+  int64_t span = 1;
+  for (const auto& d : dims) {
+    if (d.first < span) return false;
+    span += d.first * (d.second - 1);
+  }
+  return true;
+}
+
+void check_written_sums(const char* what, const Tensor& sums, int64_t dims, int64_t heads, const Tensor& like) {
+  check_sums(what, sums, dims, heads, like);
+  CHECK_ARG(apart(sums), what, ": sums are written: their rows and heads must not overlap");
+}
+
 void check_queries(const char* what, const Tensor& q, int64_t hkv) {
   CHECK_ARG(q.is_cuda() && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf), what, ": q must be a bf16 or fp16 device tensor");
   CHECK_ARG(q.dim() == 3 && q.stride(2) == 1 && q.stride(1) == q.size(2) && q.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0,
@@ -95,12 +119,13 @@ Tensor attention_decode_weights(const Tensor& q, const Tensor& k_cache, const Te
   CHECK_ARG(q.size(0) == batch, what, ": q has ", q.size(0), " rows for ", batch, " requests");
   CHECK_ARG(mb200::weights_decode_covers(static_cast<int>(hd), static_cast<int>(q.size(1) / hkv)), what, ": ", q.size(1), " heads of ", hd,
             " features over ", hkv, " key heads: heads of 64, 128 or 256 features, groups of up to 32 heads (16 of 256 features)");
-  check_sums(what, sums, 3, hkv, q);
+  check_written_sums(what, sums, 3, hkv, q);
   check_scores(what, scale, logit_cap, sink, q);
   CHECK_ARG(decay >= 0. && decay <= 1., what, ": decay must be from 0 to 1, not ", decay);
   Tensor out = given.has_value() ? *given : torch::empty(q.sizes(), q.options());
-  CHECK_ARG(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1 && out.stride(1) == hd,
-            what, ": out must be like q, heads of a row contiguous");
+  CHECK_ARG(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1 &&
+                out.stride(1) == hd && apart(out),
+            what, ": out must be like q, heads of a row contiguous, rows apart");
   c10::cuda::CUDAGuard g(q.device());
   a.index = cache_index(what, req_to_token, req_pool_indices, seq_lens, sums, q);
   a.sums = {sums.data_ptr<float>(), sums.stride(0), sums.stride(1)};
@@ -142,7 +167,7 @@ void attention_prefill_weights(const Tensor& q, const Tensor& k_cache, const Ten
   const int64_t batch = req_pool_indices.numel(), hd = q.size(2);
   CHECK_ARG(mb200::weights_prompt_covers(static_cast<int>(hd), static_cast<int>(q.size(1) / hkv)), what, ": ", q.size(1), " heads of ", hd,
             " features over ", hkv, " key heads: heads of 64, 128 or 256 features, groups of up to 32 heads");
-  check_sums(what, sums, 3, hkv, q);
+  check_written_sums(what, sums, 3, hkv, q);
   check_scores(what, scale, logit_cap, sink, q);
   CHECK_ARG(last >= 0 && last <= INT32_MAX, what, ": last must be 0 (all new tokens) or positive, not ", last);
   CHECK_ARG(q.size(0) * q.size(1) < (int64_t(1) << 31) && batch < 65536, what, ": too many rows or requests");
@@ -228,7 +253,7 @@ void cache_evict(const Tensor& store, const c10::optional<Tensor>& sums, const T
                 store.size(4) * store.element_size() < (int64_t(1) << 20),
             what, ": too many lists, tokens or slots, or rows too wide");
   if (sums.has_value()) {
-    check_sums(what, *sums, 4, store.size(2), store);
+    check_written_sums(what, *sums, 4, store.size(2), store);
     CHECK_ARG(sums->size(0) == store.size(0), what, ": sums of ", sums->size(0), " layers, and a store of ", store.size(0));
   }
   c10::cuda::CUDAGuard g(store.device());

@@ -60,6 +60,22 @@ def _check_sums(what: str, device, sums, dims: int, heads: int) -> None:
         raise ValueError(f"{what}: sums must be fp32 [{'layers, ' if dims == 4 else ''}requests, {heads}, tokens] with unit inner stride on {device}")
 
 
+def _apart(t) -> bool:
+    """Whether no element of a tensor that is written lies where another does (an expanded tensor's do)."""
+    span = 1
+    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+        if stride < span:
+            return t.numel() == 0
+        span += stride * (size - 1)
+    return True
+
+
+def _check_written_sums(what: str, device, sums, dims: int, heads: int) -> None:
+    _check_sums(what, device, sums, dims, heads)
+    if not _apart(sums):
+        raise ValueError(f"{what}: sums are written: their rows and heads must not overlap")
+
+
 def _check_rows(what: str, q, caches, scale: float, logit_cap: float, sink) -> int:
     """Checks queries, caches and what makes scores of them; the number of kv heads."""
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
@@ -96,11 +112,12 @@ def attention_decode_weights(q, k_cache, v_cache, req_to_token, req_pool_indices
     hkv = _check_rows(what, q, (k_cache, v_cache), scale, logit_cap, sink)
     _check_table(what, q.device, req_to_token)
     _check_ints(what, q.device, q.shape[0], req_pool_indices=req_pool_indices, seq_lens=seq_lens)
-    _check_sums(what, q.device, sums, 3, hkv)
+    _check_written_sums(what, q.device, sums, 3, hkv)
     if not 0.0 <= decay <= 1.0:
         raise ValueError(f"{what}: decay must be from 0 to 1, not {decay}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.stride(1) != out.shape[2]):
-        raise ValueError(f"{what}: out must be like q, with the heads of a row contiguous")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.stride(1) != out.shape[2]
+                            or not _apart(out)):
+        raise ValueError(f"{what}: out must be like q, with the heads of a row contiguous and rows apart")
     return ref.attention_decode_weights(q, k_cache, v_cache, req_to_token, req_pool_indices, seq_lens, scale, sums, decay, out, logit_cap, sink)
 
 
@@ -121,7 +138,7 @@ def attention_prefill_weights(q, k_cache, req_to_token, req_pool_indices, seq_le
     _check_table(what, q.device, req_to_token)
     _check_ints(what, q.device, req_pool_indices.numel(), req_pool_indices=req_pool_indices, seq_lens=seq_lens, prefix_lens=prefix_lens,
                 q_start_loc=q_start_loc)
-    _check_sums(what, q.device, sums, 3, hkv)
+    _check_written_sums(what, q.device, sums, 3, hkv)
     if last < 0:
         raise ValueError(f"{what}: last must be 0 (all new tokens) or positive, not {last}")
     ref.attention_prefill_weights(q, k_cache, req_to_token, req_pool_indices, seq_lens, prefix_lens, q_start_loc, scale, sums, int(last), bool(add),
@@ -171,7 +188,7 @@ def cache_evict(store, sums, req_to_token, req_pool_indices, keep, counts) -> No
             or keep.device != dev):
         raise ValueError(f"{what}: keep must be contiguous int32 [{store.shape[0]}, {batch}, {store.shape[2]}, tokens] on {dev}")
     if sums is not None:
-        _check_sums(what, dev, sums, 4, store.shape[2])
+        _check_written_sums(what, dev, sums, 4, store.shape[2])
         if sums.shape[0] != store.shape[0]:
             raise ValueError(f"{what}: sums of {sums.shape[0]} layers, and a store of {store.shape[0]}")
     ref.cache_evict(store, sums, req_to_token, req_pool_indices, keep, counts)
