@@ -18,7 +18,6 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kLoads = 8;                 // 16-byte pieces of a lane in a run
 constexpr int kSumsPer = 8;               // sums of a lane on their way
-constexpr int kStays = -0x7fffffff - 1;   // in the place of a slot: this row stays where it is
 
 struct EvictParams {
   CacheEvictArgs a;
@@ -90,32 +89,34 @@ __global__ void __launch_bounds__(kThreads, 6) cache_evict_kernel(const EvictPar
     const int i = t * rows + lane;
     return t < runs && lane < rows && i < count ? __ldcg(keep + i) : -1;
   };
+  struct Slots {
+    int from, to;
+    bool moves;          // no slot's value says that a row stays
+  };
   auto slots_of = [&](int t, int k) {
     const int i = t * rows + lane;
-    if (t >= runs || lane >= rows || (k = checked(i, k)) < 0) return make_int2(-1, kStays);
-    return make_int2(__ldcg(rtt + k), __ldcg(rtt + i));
+    if (t >= runs || lane >= rows || (k = checked(i, k)) < 0) return Slots{-1, -1, false};
+    return Slots{__ldcg(rtt + k), __ldcg(rtt + i), true};
   };
   const int row0 = lane >> p.lanes_log2, ch = lane & ((1 << p.lanes_log2) - 1), per = 32 >> p.lanes_log2;     // of every 32 lanes' pieces
   const bool mine = ch * 16 < bytes;
   store += ch * 16;
-  int2 s = slots_of(0, kept(0));
-  int2 next = slots_of(1, kept(1));
+  Slots s = slots_of(0, kept(0));
+  Slots next = slots_of(1, kept(1));
   int k_next = kept(2);
   for (int t = 0; t < runs; ++t) {
-    if (s.y == kStays) {
-      s.x = -1;
-    } else if (s.x < 0 || s.x >= a.num_slots || s.y < 0 || s.y >= a.num_slots) {
+    if (s.moves && (s.from < 0 || s.from >= a.num_slots || s.to < 0 || s.to >= a.num_slots)) {
       bad = true;
-      s.x = s.y = -1;
+      s.from = s.to = -1;
     }
     uint4 x[kLoads];
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       if (u >= p.loads) break;
-      const int from = __shfl_sync(0xffffffffu, s.x, u * per + row0);
+      const int from = __shfl_sync(0xffffffffu, s.from, u * per + row0);
       if (from >= 0 && mine) x[u] = __ldcg(reinterpret_cast<const uint4*>(store + static_cast<int64_t>(from) * a.row_bytes));
     }
-    const int to_slot = s.y;
+    const int to_slot = s.to;
     s = next;
     next = slots_of(t + 2, k_next);
     k_next = kept(t + 3);
