@@ -38,9 +38,9 @@ __global__ void __launch_bounds__(kThreads, 6) cache_evict_kernel(const EvictPar
   const int64_t list = moves ? which / p.pieces / 2 : which;
   const int hk = static_cast<int>(list % a.hkv), b = static_cast<int>(list / a.hkv % a.index.batch);
   const int64_t layer = list / a.hkv / a.index.batch;
-  const int row = __ldcg(a.index.req_pool_indices + b), count = min(__ldcg(a.counts + b), a.width);
+  const int row = __ldcg(a.index.req_pool_indices + b), count = __ldcg(a.counts + b);
   if (count <= 0) return;
-  if (row < 0 || row >= a.index.table_rows || count > a.index.table_cols) {
+  if (row < 0 || row >= a.index.table_rows || count > a.index.table_cols || count > a.width) {
     if (lane == 0 && a.index.status != nullptr) atomicExch(a.index.status, kStatusBadIndex);
     return;
   }
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 6) cache_evict_kernel(const EvictPar
 
 int launch_cache_evict(const CacheEvictArgs& a, cudaStream_t s) {
   const int64_t lists = static_cast<int64_t>(a.layers) * a.index.batch * a.hkv;
-  if (lists <= 0 || a.width <= 0) return 0;
+  if (lists <= 0) return 0;
   EvictParams p{};
   p.a = a;
   // Pieces of a row: no more than a warp takes at once, and half as much down to 64 bytes while there are fewer warps than 12 per SM (28 layers

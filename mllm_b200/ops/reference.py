@@ -1170,6 +1170,8 @@ def cache_evict(store, sums, req_to_token, req_pool_indices, keep, counts) -> No
         n, row = int(counts[b]), int(req_pool_indices[b])
         if n <= 0:
             continue
+        if n > keep.shape[3]:
+            raise ValueError(f"cache_evict: {n} tokens stay and keep has {keep.shape[3]}")
         slots = req_to_token[row].long()
         for layer in range(store.shape[0]):
             for head in range(store.shape[2]):

@@ -35,3 +35,19 @@ def test_moved_rows_whose_slots_are_none(slot, end):
     others = [i for i in range(10) if i != 4]
     moved[:, :, :, slots[others]] = before[:, :, :, slots[[i + 20 for i in others]]]
     assert torch.equal(c["store"], moved)
+
+
+@pytest.mark.parametrize("width", [0, 1, 10, 40])
+def test_more_tokens_stay_than_keep_has(width):
+    """One request's count says more than the list holds: that request stays as it is."""
+    c = cached_batch([50, 45], 2, 2, 64, seed=3, layers=2)
+    store, sums = c["store"].clone(), c["sums"].clone()
+    keep = (torch.arange(width, dtype=torch.int32, device="cuda") + 2).expand(2, 2, 2, width).contiguous()
+    ops.cache_evict(c["store"], c["sums"], c["table"], c["req"], keep, i32(width + 1, width))
+    assert recorded()
+    row = int(c["req"][1])
+    slots = c["table"][row].long()
+    want, total = store.clone(), sums.clone()
+    want[:, :, :, slots[:width]] = store[:, :, :, slots[2:2 + width]]
+    total[:, row, :, :width] = sums[:, row, :, 2:2 + width]
+    assert torch.equal(c["store"], want) and torch.equal(c["sums"], total)
