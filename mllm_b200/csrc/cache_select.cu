@@ -382,10 +382,10 @@ __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectPara
   const int cta = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0, list = blockIdx.x / p.cluster, tid = threadIdx.x;
   const int hk = list % a.hkv, b = list / a.hkv % a.index.batch, layer = list / a.hkv / a.index.batch;
   const Cached r = cached_of(a.index, b);
-  const int n = r.len, budget = __ldcg(a.budgets + b), count = max(0, min(n, min(budget, a.width)));
+  const int n = r.len, count = max(0, min(n, min(__ldcg(a.budgets + b), a.width)));
   if (tid == 0 && cta == 0 && layer == 0 && hk == 0) {
     a.counts[b] = count;
-    if ((r.bad || budget > a.width) && a.index.status != nullptr) atomicExch(a.index.status, kStatusBadIndex);
+    if (r.bad && a.index.status != nullptr) atomicExch(a.index.status, kStatusBadIndex);
   }
   int* keep = a.keep + static_cast<int64_t>(list) * a.width;
   for (int i = count + cta * kThreads + tid; i < a.width; i += p.cluster * kThreads) keep[i] = -1;
