@@ -19,7 +19,8 @@
 //     that is rounded below fp16's last place, far below the fp32 sum's own rounding.
 //   * Weights are rounded to 16 bits for the product with the values, and the output's normaliser sums the rounded ones, as in plain
 //     decode attention.  The sums of weights have a normaliser of their own from the unrounded ones: a rounded weight that carries most of a
-//     row would be off by 2^-9.
+//     row would be off by 2^-9.  fp16 weights are held 2^7 up: fp16's last place is then 2^-32 of a warp's largest weight, and a tail of tens of
+//     thousands of tokens that have less than 2^-25 each is not lost.
 //
 // What bounds it: memory while the first kernel streams, a start of some 6 us, and what shows of the second kernel (29 requests of about 1900
 // tokens, 32 / 8 heads of 128, fp16: 55.8 us for 229 MB, where the bytes take 35; two chains of products per score save 0.5 us).  8-bit rows
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT, FMT>::kPerSm) weights_de
   using C = Cfg<HD, NT, FMT>;
   using M = typename std::conditional<FMT == kKvSame, T, __half>::type;        // type of the products
   using Elem = typename std::conditional<FMT == kKvSame, T, uint8_t>::type;
+  constexpr float kUp = std::is_same<M, __half>::value ? 7.f : 0.f;      // weights are 2^kUp times 2^(score - maximum): 2^15 at most, which fp16 holds
   extern __shared__ uint8_t smem_raw[];
   __shared__ int warp_sums[kWarps];
   __shared__ int start[3];                          // where the run begins: request, kv head, tile
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT, FMT>::kPerSm) weights_de
       }
     }
     float o[HD / 16][NT][4];
-    float m[NT][2], l[NT][2], x[NT][2];     // maximum, sum of the rounded weights, sum of the weights
+    float m[NT][2], l[NT][2], x[NT][2];     // maximum less kUp, sum of the rounded weights, sum of the weights
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT, FMT>::kPerSm) weights_de
           s[nt][i] = ok0 ? s[nt][i] : -INFINITY;
           s[nt][i + 2] = ok1 ? s[nt][i + 2] : -INFINITY;
           const float top = fmaxf(s[nt][i], s[nt][i + 2]);
-          raise = raise || top > m[nt][i] + kRescaleThreshold;   // the first tile always raises
+          raise = raise || top > m[nt][i] + (kRescaleThreshold + kUp);   // the first tile always raises
         }
         // the scores wait for the normaliser
         const int h = nt * 8 + 2 * (lane & 3);
@@ -404,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT, FMT>::kPerSm) weights_de
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float now = fmaxf(m[nt][i], top);
+            const float now = fmaxf(m[nt][i], top - kUp);
             const float f = m[nt][i] == -INFINITY ? 0.f : fast_exp2(m[nt][i] - now);
             m[nt][i] = now;
             l[nt][i] *= f;
