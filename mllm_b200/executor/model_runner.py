@@ -641,6 +641,8 @@ class ModelRunner:
         on the device.  Whole pages behind those are free: ``token_to_kv_pool_allocator.free_behind(slots, length)`` gives them back (``free`` takes
         the page of every slot it is given, also one with kept tokens).  The next tokens' positions go on from what they were
         (``positions=``, ``first_positions_cpu=``).  Requests whose slots others share, the prefix cache's among them, cannot be shortened."""
+        if not hasattr(self.token_to_kv_pool, "evict"):
+            raise ValueError(f"requests in a {type(self.token_to_kv_pool).__name__} cannot be shortened")
         keep, counts = ops.cache_select(weight_sums, req_pool_indices.to(torch.int32).contiguous(), seq_lens.to(torch.int32).contiguous(),
                                         budgets.to(torch.int32).contiguous(), max_budget, first=first, recent=recent, pool=pool)
         self.token_to_kv_pool.evict(weight_sums, self.req_to_token_pool.req_to_token, req_pool_indices.to(torch.int32).contiguous(), keep, counts)

@@ -54,3 +54,10 @@ def test_modules_are_looked_up_once(tiny):
         decode(mr, 3, sums, max_seq_len=3)
     finally:
         mr.model.modules = walk
+
+
+@pytest.mark.parametrize("preset", ["pebulix-tiny", "lufizen-tiny", "kesovik-tiny"])
+def test_caches_that_cannot_be_shortened(preset):
+    mr = Shortened(preset, "cpu", "float32").mr
+    with pytest.raises(ValueError, match="cannot be shortened"):
+        mr.evict_cache(torch.zeros((2, 3, 2, 24)), i32(0), i32(20), i32(10), 10)
