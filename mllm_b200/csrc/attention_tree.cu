@@ -45,6 +45,9 @@ constexpr int kNoToken = -0x7fffffff;
 constexpr int kParents = 256;              // nodes whose parents are kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleThreshold = 8.0f;  // the running maximum is raised when a score passes it by 2^8
+// The quick form of tanh keeps a score to 2^-22 of the cap: at 256 a tenth of what weights are rounded by in 16 bits.  Larger caps have kernels
+// with tanhf, which keeps a score's own places (16 x 4096 tokens, 24 nodes, 32 / 4 heads of 128, e4m3: 102 us and 148).
+constexpr float kFarCap = 256.0f;
 
 struct TreeParams {
   const void* q;
@@ -60,6 +63,7 @@ struct TreeParams {
   int64_t q_stride, out_stride, num_slots, kv_tok_stride, kv_head_stride;
   int hkv, group, tpt, unit_nodes, ctas, part_rows, window, chunk;   // tpt: nodes of a row tile
   float scale_log2, cap_in, cap_out;    // cap_out 0: no soft cap
+  bool far_cap;                         // a soft cap above kFarCap
   uint32_t idesc_s, idesc_o;
 };
 constexpr int kJobInts = 5;
@@ -185,8 +189,8 @@ struct Place {          // of a segment
   int64_t left;
 };
 
-// FMT: what the caches hold (kKvSame, kKvE4M3, kKvE5M2)
-template <typename T, int NH, int FMT, int R>
+// FMT: what the caches hold (kKvSame, kKvE4M3, kKvE5M2); FAR: a soft cap above kFarCap
+template <typename T, int NH, int FMT, int R, bool FAR>
 __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, FMT != kKvSame, R>::kPerSm) attn_tree_kernel(const TreeParams p) {
   constexpr bool KV8 = FMT != kKvSame, kF16 = std::is_same<T, __half>::value;
   using C = Cfg<NH, KV8, R>;
@@ -643,11 +647,12 @@ __global__ void __launch_bounds__(Cfg<NH, FMT != kKvSame, R>::kThreads, Cfg<NH, 
           tmem_ld_32x32(tmem_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
           tmem_ld_wait();
           float mul = p.scale_log2;
-          if (capped) {        // cap tanh(x / cap), in the log2 domain; tanh(y) = 1 - 2 / (1 + e^(2 y))
+          if (FAR || capped) {        // cap tanh(x / cap), in the log2 domain; where the cap is near, tanh(y) = 1 - 2 / (1 + e^(2 y))
             mul = 1.f;
 #pragma unroll
             for (int c = 0; c < kTile; ++c)
-              raw[c] = __float_as_uint(p.cap_out * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(raw[c]) * p.cap_in))));
+              raw[c] = __float_as_uint(p.cap_out * (FAR ? tanhf(__uint_as_float(raw[c]) * p.cap_in)
+                                                        : 1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(raw[c]) * p.cap_in))));
           }
           const bool gaps = __any_sync(0xffffffffu, holes != 0);
           if (masked || gaps) {
@@ -866,10 +871,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_tree_join_kernel(const T
   }
 }
 
-template <typename T, int NH, int FMT, int R>
-int launch_one(const TreeParams& p, cudaStream_t s) {
+template <typename T, int NH, int FMT, int R, bool FAR>
+int launch_far(const TreeParams& p, cudaStream_t s) {
   using C = Cfg<NH, FMT != kKvSame, R>;
-  auto kern = attn_tree_kernel<T, NH, FMT, R>;
+  auto kern = attn_tree_kernel<T, NH, FMT, R, FAR>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem) != cudaSuccess) return -3;
   if constexpr (C::kSplit) {
     // the softmax warps take registers that the others give back: together no more than the kernel is launched with
@@ -886,6 +891,10 @@ int launch_one(const TreeParams& p, cudaStream_t s) {
   err = launch_pdl(attn_tree_join_kernel<T, 64 * NH>, dim3(p.ctas, join_parts), dim3(32 * kJoinWarps), 0, s, p);
   note_launch();
   return err == cudaSuccess ? 0 : -4;
+}
+template <typename T, int NH, int FMT, int R>
+int launch_one(const TreeParams& p, cudaStream_t s) {
+  return p.far_cap ? launch_far<T, NH, FMT, R, true>(p, s) : launch_far<T, NH, FMT, R, false>(p, s);
 }
 template <typename T, int NH, int R>
 int launch_format(const TreeParams& p, int fmt, cudaStream_t s) {
@@ -950,7 +959,8 @@ int launch_attention_tree(const TreeAttnArgs& a, cudaStream_t s) {
   p.chunk = a.chunk > 0 ? a.chunk : 0;
   p.scale_log2 = a.scale * kLog2e;
   if (a.logit_cap > 0.f) {
-    p.cap_in = 2.f * kLog2e * a.scale / a.logit_cap;
+    p.far_cap = a.logit_cap > kFarCap;
+    p.cap_in = p.far_cap ? a.scale / a.logit_cap : 2.f * kLog2e * a.scale / a.logit_cap;
     p.cap_out = a.logit_cap * kLog2e;
   }
   const uint32_t fmt = a.dt == kF16 ? 0u : 1u;
