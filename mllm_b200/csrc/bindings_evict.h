@@ -98,8 +98,9 @@ int cache_format(const char* what, const Tensor& cache, const Tensor& like) {
 }
 
 void check_scores(const char* what, double scale, double cap, const c10::optional<Tensor>& sink, const Tensor& q) {
-  CHECK_ARG(scale >= FLT_MIN && scale <= FLT_MAX, what, ": scale must be positive and finite, not ", scale);
-  CHECK_ARG(cap == 0. || (cap >= FLT_MIN && cap <= FLT_MAX), what, ": logit_cap must be 0 or positive and finite, not ", cap);
+  constexpr double kMost = FLT_MAX / 2;         // times log2 e it is finite still
+  CHECK_ARG(scale >= FLT_MIN && scale <= kMost, what, ": scale must be positive and at most ", kMost, ", not ", scale);
+  CHECK_ARG(cap == 0. || (cap >= FLT_MIN && cap <= kMost), what, ": logit_cap must be 0, or positive and at most ", kMost, ", not ", cap);
   if (sink.has_value())
     CHECK_ARG(sink->device() == q.device() && sink->scalar_type() == at::kFloat && sink->is_contiguous() && sink->dim() == 1 && sink->numel() == q.size(1),
               what, ": sink must be fp32 [", q.size(1), "] on ", q.device());

@@ -87,10 +87,11 @@ def _check_rows(what: str, q, caches, scale: float, logit_cap: float, sink) -> i
     hkv = caches[0].shape[1]
     if hkv == 0 or q.shape[1] == 0 or q.shape[1] % hkv:
         raise ValueError(f"{what}: {q.shape[1]} query heads over {hkv} key heads")
-    if not _FP32.tiny <= scale <= _FP32.max:
-        raise ValueError(f"{what}: scale must be positive and finite, not {scale}")
-    if logit_cap != 0 and not _FP32.tiny <= logit_cap <= _FP32.max:
-        raise ValueError(f"{what}: logit_cap must be 0 or positive and finite, not {logit_cap}")
+    most = _FP32.max / 2        # times log2 e it is finite still
+    if not _FP32.tiny <= scale <= most:
+        raise ValueError(f"{what}: scale must be positive and at most {most:.3g}, not {scale}")
+    if logit_cap != 0 and not _FP32.tiny <= logit_cap <= most:
+        raise ValueError(f"{what}: logit_cap must be 0, or positive and at most {most:.3g}, not {logit_cap}")
     if sink is not None and (sink.dtype != torch.float32 or sink.shape != (q.shape[1],) or not sink.is_contiguous() or sink.device != q.device):
         raise ValueError(f"{what}: sink must be fp32 [{q.shape[1]}] on {q.device}")
     return hkv

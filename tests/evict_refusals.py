@@ -29,3 +29,17 @@ def overlapping(device):
         calls += [(decode(sums=bad), "must not overlap"), (prompt(bad), "must not overlap"), (evict(bad[None].expand(3, -1, -1, -1)), "must not overlap")]
     calls += [(evict(s["sums"][:1].expand(3, -1, -1, -1)), "must not overlap"), (decode(out=c["q"][:1].expand(2, -1, -1)), "out must be")]
     return calls
+
+
+def too_large(device):
+    """Scales and caps that are finite, but not in units of log2."""
+    c = cached_batch([40, 17], 4, 2, 64, dtype=torch.bfloat16, seed=1, device=device)
+    p = cached_batch([40, 17], 4, 2, 64, dtype=torch.bfloat16, seed=1, new=[5, 6], device=device)
+
+    def decode(scale=0.1, cap=0.0):
+        return lambda: ops.attention_decode_weights(c["q"], c["k"], c["v"], c["table"], c["req"], c["seq"], scale, c["sums"], logit_cap=cap)
+
+    def prompt(scale=0.1, cap=0.0):
+        return lambda: ops.attention_prefill_weights(p["q"], p["k"], p["table"], p["req"], p["seq"], p["prefix"], p["start"], scale, p["sums"], logit_cap=cap)
+
+    return [(f(**kw), name) for f in (decode, prompt) for kw, name in ((dict(scale=3e38), "scale"), (dict(cap=3e38), "logit_cap"))]

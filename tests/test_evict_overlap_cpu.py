@@ -3,13 +3,20 @@ import pytest
 import torch
 
 from evict_cases import cached_batch
-from evict_refusals import overlapping
+from evict_refusals import overlapping, too_large
 from mllm_b200 import ops
 
 
 @pytest.mark.parametrize("i", range(len(overlapping("cpu"))))
 def test_refusals(i):
     call, message = overlapping("cpu")[i]
+    with pytest.raises(ValueError, match=message):
+        call()
+
+
+@pytest.mark.parametrize("i", range(len(too_large("cpu"))))
+def test_scales_and_caps_that_are_too_large(i):
+    call, message = too_large("cpu")[i]
     with pytest.raises(ValueError, match=message):
         call()
 

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from evict_cases import cached_batch
-from evict_refusals import overlapping
+from evict_refusals import overlapping, too_large
 from mllm_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -15,6 +15,12 @@ def test_what_lies_on_itself():
         with pytest.raises(ValueError, match=message):
             call()
     assert ops.launch_count() == before
+
+
+def test_scales_and_caps_that_are_too_large():
+    for call, message in too_large("cuda"):
+        with pytest.raises(ValueError, match=message):
+            call()
 
 
 def test_layouts_that_are_taken():
