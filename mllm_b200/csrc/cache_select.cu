@@ -1,6 +1,6 @@
 // Which cached tokens stay.  Of a list of n sums (a layer, a request, a kv head) stay: the last min(recent, count) tokens, of the rest the
 // first min(first, count - those), and of the rest those with the largest scores, where a score is the largest of the `pool` sums around the
-// token and ties go to the lowest index; count = min(n, budget).  The list comes out in ascending order.
+// token, those of the first and last tokens among them, and ties go to the lowest index; count = min(n, budget).  The list comes out in ascending order.
 //
 // A score's bits are turned into a number of 32 bits that rises with it, its rank (NaN is as low as minus infinity, zeros of both signs are
 // one).  The k-th largest is found digit by digit, 11 bits at a time from the top: a histogram in shared memory, its bins added up from
@@ -8,8 +8,9 @@
 // they are few enough every one is compared with every other.  Then a pass over the list, a stretch per warp, keeps what is above the k-th and
 // of its equals the first ones: counts first, then indices.
 //
-// What bounds it is instructions, 65 to 90 per sum (2304 lists of up to 8192 sums, a quarter kept, pool 7: 71 us, their bytes take 14);
-// eight neighbours are a thread's, so that scores are made in registers.  Lists that are too few for the SMs, or too long for a block's shared
+// What bounds it is instructions, 65 to 90 per sum in three passes over shared memory, and the barriers between them, which the warps that
+// shared memory leaves room for (46 %) do not cover: 60 % of the issue slots are used (2304 lists of up to 8192 sums, a quarter kept, pool 7: 71 us,
+// their bytes take 14).  Eight neighbours are a thread's, so that scores are made in registers.  Lists that are too few for the SMs, or too long for a block's shared
 // memory, are cut into slices for a cluster of up to 8 blocks, which add up histograms and counts through each other's shared memory
 // (224 lists of 1200 sums: 6.2 us, most of it one wait behind the other).
 #include <algorithm>

@@ -23,8 +23,9 @@
 //     thousands of tokens that have less than 2^-25 each is not lost.
 //
 // What bounds it: memory while the first kernel streams, a start of some 6 us, and what shows of the second kernel (29 requests of about 1900
-// tokens, 32 / 8 heads of 128, fp16: 55.8 us for 229 MB, where the bytes take 35; two chains of products per score save 0.5 us).  8-bit rows
-// are bound by the warps' instructions, widening first of all (32 requests of about 4096, 32 / 4 heads of 128, e4m3: 53.4 us, the bytes take 21).
+// tokens, 32 / 8 heads of 128, fp16: 56.3 us for 229 MB, where the bytes take 35; two chains of products per score save 0.5 us).  8-bit rows
+// are bound by the latency of a warp's chain - rows, widening, product, exponential, transpose, product - with 12 warps on an SM to cover it: 41 % of
+// the issue slots are used, 50 % of the ALU (32 requests of about 4096, 32 / 4 heads of 128, e4m3: 54.3 us, the bytes take 21).
 #include <algorithm>
 
 #include "common.cuh"

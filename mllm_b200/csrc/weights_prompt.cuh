@@ -19,10 +19,13 @@
 //     token.  Where there are more rows, 256 tokens are the block and rows go by, in a line as in the first pass; a third kernel adds up the parts
 //     of blocks that were cut.  Nothing depends on the order of CTAs.
 //   * A CTA's first block is brought by the computing warps, which have nothing else to do then, later ones by a warp of its own.
-// What bounds it is the exponentials, 16 per cycle and SM; products take half their time.  256 x 128 scores take 2048 cycles of them, and the
-// first pass 2750 in all, the second 3050 (one request of 32000 tokens behind its last 64, 32 / 8 heads of 128: 94 us; 2 x 1500 tokens, all
-// queries: 133).  Where there are few scores, two starts and ends count: 6 us to the first scores, 2.5 to join a block's normalisers from
-// the first pass, 2 at the end (8 x 2048 tokens behind the last 32: 46.5 us).
+// What it costs: 256 x 128 scores take 2048 cycles of exponentials (16 per cycle and SM; products take half of that), and the first pass 2750 in
+// all, the second 3050.  One request of 32000 tokens behind its last 64, 32 / 8 heads of 128, has 13.5 such steps an SM: 40 of its 95 us, starts and
+// ends of the passes some 18, and the rest is not explained; 2 x 1500 tokens, all queries: 132 us, of which steps without masks at these
+// rates would be less than half, and a step is masked for all warps as soon as one score of it is.  Where there are few scores, two starts
+// and ends count: 6 us to the first scores, 2.5 to join a block's normalisers from the first pass, 2 at the end (8 x 2048 tokens behind the
+// last 32: 46.5 us).  Soft caps take the masked steps' loop and a tanhf per score (83, 195 and 250 us), 8-bit rows are widened by the
+// copying warps (the three cases over e4m3: 101, 180 and 605 us; why the last one is so slow was not looked into).
 #pragma once
 
 #include <algorithm>

@@ -151,7 +151,8 @@ def cache_select(sums, req_pool_indices, seq_lens, budgets, max_budget: int, fir
     """Which tokens stay: ``(keep [layers, requests, Hkv, max_budget], counts [requests])``, int32.  ``counts[b]`` is ``budgets[b]``, at most
     ``max_budget`` and the request's ``seq_lens[b]``.  Of every list of ``sums`` [layers, rows, Hkv, tokens] stay the last ``recent`` tokens, then of
     the others the first ``first``, then those with the largest scores until there are ``counts[b]``; a score is the largest of the ``pool`` sums
-    (odd, up to 63) around the token, ties go to the lowest index, NaN counts as minus infinity.  The kept tokens' cache indices rise; behind them
+    (odd, up to 63) around the token (of the request's tokens, the first and the last ones among them, so that the ``pool // 2`` beside those
+    inherit theirs), ties go to the lowest index, NaN counts as minus infinity.  The kept tokens' cache indices rise; behind them
     stands -1."""
     ops = _ops()
     if ops.use_kernels(sums):       # the binding makes the same checks
